@@ -14,9 +14,27 @@
 #include <optional>
 #include <tuple>
 
+#include "bindings_common.h"
 #include "tdc_dwconv.h"
 
 namespace tma_dwconv {
+
+void check_status(int rc, const char* what) {
+  if (rc == TDC_OK) return;
+  if (rc == TDC_ERR_CUDA) {
+    TORCH_CHECK(false, what, ": ", tdc_strerror(rc), ": ",
+                cudaGetErrorString(static_cast<cudaError_t>(tdc_last_cuda_error())));
+  }
+  if (rc == TDC_ERR_TMA_ENCODE) {
+    TORCH_CHECK(false, what, ": ", tdc_strerror(rc), " (CUresult ", tdc_last_cuda_error(), ")");
+  }
+  TORCH_CHECK(false, what, ": ", tdc_strerror(rc), " (status ", rc, ")");
+}
+
+void* stream_of(const torch::Tensor& x) {
+  return static_cast<void*>(at::cuda::getCurrentCUDAStream(x.device().index()).stream());
+}
+
 namespace {
 
 void check_common(const torch::Tensor& x, const torch::Tensor& w) {
@@ -41,22 +59,6 @@ bool check_common_16(const torch::Tensor& x, const torch::Tensor& w, const char*
   TORCH_CHECK(x.is_contiguous() && w.is_contiguous(), xname, "/w must be contiguous");
   TORCH_CHECK(x.device() == w.device(), xname, " and w must be on the same device");
   return x.scalar_type() == torch::kBFloat16;
-}
-
-void check_status(int rc, const char* what) {
-  if (rc == TDC_OK) return;
-  if (rc == TDC_ERR_CUDA) {
-    TORCH_CHECK(false, what, ": ", tdc_strerror(rc), ": ",
-                cudaGetErrorString(static_cast<cudaError_t>(tdc_last_cuda_error())));
-  }
-  if (rc == TDC_ERR_TMA_ENCODE) {
-    TORCH_CHECK(false, what, ": ", tdc_strerror(rc), " (CUresult ", tdc_last_cuda_error(), ")");
-  }
-  TORCH_CHECK(false, what, ": ", tdc_strerror(rc), " (status ", rc, ")");
-}
-
-void* stream_of(const torch::Tensor& x) {
-  return static_cast<void*>(at::cuda::getCurrentCUDAStream(x.device().index()).stream());
 }
 
 void check_ws_args(const torch::Tensor& x, const torch::Tensor& w, int64_t pad) {
@@ -616,4 +618,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("set_wait_timeout_ns", &tma_dwconv::set_wait_timeout_ns,
         "Limit of every pipeline wait of later launches (default 2 s).", pybind11::arg("ns"));
   m.def("consumer_warps", &tma_dwconv::consumer_warps, "Consumer warps per CTA of the ws kernel.");
+  tma_dwconv::bind_sequence(m);
 }

@@ -28,6 +28,7 @@
 #include <vector>
 
 #include "tdc_dwconv.h"
+#include "tdc_host.h"
 #include "tdc_kernels.cuh"
 #include "tdc_wgrad.cuh"
 #include "tdc_dgrad_s2.cuh"
@@ -1687,6 +1688,19 @@ cudaError_t pipe_ready(HostPipe& hp) {
 }
 
 }  // namespace
+
+namespace tdc {
+namespace host {
+
+int cuda_fail(int cuda_error) { return ::cuda_fail(static_cast<cudaError_t>(cuda_error)); }
+
+int prepare_device() {
+  DeviceInfo* info = nullptr;
+  return current_device(&info, nullptr);
+}
+
+}  // namespace host
+}  // namespace tdc
 
 extern "C" {
 

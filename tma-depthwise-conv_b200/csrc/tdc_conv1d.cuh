@@ -1,0 +1,436 @@
+// tdc_conv1d.cuh — causal depthwise convolution over [B, T, C]: forward,
+// gradients and the step of running sequences.
+//
+// The forward moves 4 bytes per element and does 2K flops on them, so it is
+// bound by memory.  A thread owns 8 channels (one 16-byte vector) and slides
+// down a run of rows with the last K-1 inputs in registers, as packed pairs
+// that fma.rn.f32.{f16,bf16} takes without conversion; consecutive threads own
+// consecutive channels, so every access of a warp is whole 128-byte lines and
+// needs no shared memory.  Four rows are loaded ahead of their use.
+#pragma once
+
+#include "tdc_seq_common.cuh"
+
+namespace tdc {
+
+struct Conv1dParams {
+  const void* x;
+  const void* w;
+  const void* bias;
+  const void* init;      // [N, K-1, C] or null
+  void* final_state;     // [N, K-1, C] or null
+  void* y;
+  SeqTable seq;          // seq.n = N
+  int64_t B, T, C;
+  int64_t x_sb, x_st;
+  int64_t runs_per_b;    // runs of `run` rows in each batch row
+  int run;
+  int64_t main_threads;  // B * runs_per_b * C / 8; the threads behind it copy final states
+  // backward
+  const void* dy;
+  int64_t dy_sb, dy_st;
+  const void* dfinal;
+  void* dx;
+  void* dinit;
+  float* partial;        // [groups][K + 1][C]
+  int64_t groups;
+  // step
+  void* state;
+  const void* idx;
+  int64_t slots;
+  bool idx64;
+};
+
+// The sequence that owns row t of batch row b.  covered: rows [lo, hi) belong
+// to sequence n; otherwise no sequence owns rows t .. hi-1.
+struct SeqSpan {
+  int64_t n, lo, hi;
+  bool covered;
+};
+
+__device__ __forceinline__ SeqSpan span_from(const SeqTable& s, int64_t n, int64_t t) {
+  while (n < s.n && s.at(n + 1) <= t) ++n;
+  SeqSpan r;
+  r.n = n;
+  if (n >= s.n) {
+    r.covered = false;
+    r.lo = t;
+    r.hi = s.T;
+    return r;
+  }
+  const int64_t lo = s.at(n);
+  r.covered = lo <= t;
+  r.lo = r.covered ? lo : t;
+  r.hi = r.covered ? s.at(n + 1) : lo;
+  return r;
+}
+
+__device__ __forceinline__ SeqSpan span_at(const SeqTable& s, int64_t b, int64_t t) {
+  if (s.cu == nullptr) return {b, 0, s.T, true};
+  return span_from(s, s.first_ending_after(t), t);
+}
+
+__device__ __forceinline__ uint4 ld16(const void* base, int64_t elem) {
+  return __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + elem));
+}
+__device__ __forceinline__ void st16(void* base, int64_t elem, const uint4& v) {
+  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + elem) = v;
+}
+
+// Row t as an input of sequence s: from x, or for t < lo from the initial
+// state (zeros without one).
+__device__ __forceinline__ uint4 conv_input(const Conv1dParams& p, int taps, const SeqSpan& s,
+                                            int64_t xbase, int64_t t, int64_t c) {
+  if (t >= s.lo) return ld16(p.x, xbase + t * p.x_st + c);
+  const int64_t row = t - s.lo + taps - 1;
+  if (p.init == nullptr || row < 0) return make_uint4(0, 0, 0, 0);
+  return ld16(p.init, (s.n * (taps - 1) + row) * p.C + c);
+}
+
+template <class E, int K>
+__device__ __forceinline__ void conv_dot(float z[8], const uint4 win[K], const uint4 w[K]) {
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    fma2<E>(win[j].x, w[j].x, z[0], z[1]);
+    fma2<E>(win[j].y, w[j].y, z[2], z[3]);
+    fma2<E>(win[j].z, w[j].z, z[4], z[5]);
+    fma2<E>(win[j].w, w[j].w, z[6], z[7]);
+  }
+}
+
+template <class E, int K, bool SILU>
+__global__ void __launch_bounds__(256) conv1d_fwd_kernel(const Conv1dParams p) {
+  const int64_t id = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int64_t vecs = p.C / 8;
+  if (id >= p.main_threads) {
+    // The last K-1 inputs of each sequence, one vector a thread.
+    const int64_t r = id - p.main_threads;
+    if (p.final_state == nullptr || r >= p.seq.n * (K - 1) * vecs) return;
+    const int64_t c = (r % vecs) * 8, j = (r / vecs) % (K - 1), n = r / (vecs * (K - 1));
+    SeqSpan s{n, 0, p.T, true};
+    int64_t xbase = n * p.x_sb;
+    if (p.seq.cu != nullptr) {
+      s.lo = p.seq.at(n);
+      s.hi = max(s.lo, p.seq.at(n + 1));
+      xbase = 0;
+    }
+    const uint4 v = conv_input(p, K, s, xbase, s.hi - (K - 1) + j, c);
+    st16(p.final_state, (n * (K - 1) + j) * p.C + c, v);
+    return;
+  }
+  const int64_t c = (id % vecs) * 8, run = id / vecs;
+  const int64_t b = run / p.runs_per_b, t0 = (run % p.runs_per_b) * p.run;
+  const int64_t t1 = min(t0 + p.run, p.T);
+  const int64_t xbase = b * p.x_sb, ybase = b * p.T * p.C + c;
+  SeqSpan s = span_at(p.seq, b, t0);
+
+  uint4 w[K];
+#pragma unroll
+  for (int j = 0; j < K; ++j) w[j] = ld16(p.w, j * p.C + c);
+  float bias[8] = {};
+  if (p.bias != nullptr) unpack8<E>(ld16(p.bias, c), bias);
+
+  uint4 win[K];  // win[0..K-2]: the inputs before the current row
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j)
+    win[j] = s.covered ? conv_input(p, K, s, xbase, t0 - (K - 1) + j, c) : make_uint4(0, 0, 0, 0);
+
+  for (int64_t t = t0; t < t1; t += 4) {
+    uint4 next[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (t + u < t1) next[u] = ld16(p.x, xbase + (t + u) * p.x_st + c);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (t + u >= t1) break;
+      if (t + u >= s.hi) {  // only in packed batches: the next sequence (or gap) starts here
+        s = span_from(p.seq, s.n, t + u);
+        if (s.covered) {
+#pragma unroll
+          for (int j = 0; j < K - 1; ++j) win[j] = conv_input(p, K, s, xbase, s.lo - (K - 1) + j, c);
+        }
+      }
+      win[K - 1] = next[u];
+      float z[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z[i] = bias[i];
+      conv_dot<E, K>(z, win, w);
+      if constexpr (SILU) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] *= sigmoid_f(z[i]);
+      }
+      st16(p.y, ybase + (t + u) * p.C, s.covered ? pack8<E>(z) : make_uint4(0, 0, 0, 0));
+#pragma unroll
+      for (int j = 0; j < K - 1; ++j) win[j] = win[j + 1];
+    }
+  }
+}
+
+// ---- gradients -----------------------------------------------------------------
+// With dz = dy * act'(z): dx[t] = sum_j w[j] dz[t + K-1-j] within the sequence
+// (plus dfinal where the row is among the sequence's last K-1 inputs), dw[j] =
+// sum_t dz[t] x[t-(K-1)+j], dbias = sum dz.  z is recomputed from x, so the
+// pass reads x and dy and writes dx: bound by memory.  A thread owns VEC
+// channels and a run of rows, recomputes the K-1 values of dz behind the run,
+// and keeps its share of dw and dbias in registers; the runs of a block are
+// added in shared memory and one partial sum per block goes to the workspace,
+// which conv1d_wsum_kernel adds in a fixed order.
+template <class E, int VEC>
+__device__ __forceinline__ void ldv(const void* base, int64_t elem, float f[VEC]) {
+  if constexpr (VEC == 8) {
+    unpack8<E>(ld16(base, elem), f);
+  } else {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + elem));
+    unpack2<E>(v.x, f[0], f[1]);
+    unpack2<E>(v.y, f[2], f[3]);
+  }
+}
+template <class E, int VEC>
+__device__ __forceinline__ void stv(void* base, int64_t elem, const float f[VEC]) {
+  if constexpr (VEC == 8) {
+    st16(base, elem, pack8<E>(f));
+  } else {
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + elem) =
+        make_uint2(pack2_rn<E>(f[0], f[1]), pack2_rn<E>(f[2], f[3]));
+  }
+}
+
+template <class E, int VEC>
+__device__ __forceinline__ void conv_input_v(const Conv1dParams& p, int taps, const SeqSpan& s,
+                                             int64_t xbase, int64_t t, int64_t c, float f[VEC]) {
+  if (t >= s.lo) return ldv<E, VEC>(p.x, xbase + t * p.x_st + c, f);
+  const int64_t row = t - s.lo + taps - 1;
+  if (p.init == nullptr || row < 0) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = 0.f;
+    return;
+  }
+  ldv<E, VEC>(p.init, (s.n * (taps - 1) + row) * p.C + c, f);
+}
+
+// dz of one row from its window of inputs (win[K-1] is the row itself).
+template <class E, int K, int VEC, bool SILU>
+__device__ __forceinline__ void conv_dz(float dz[VEC], const float win[K][VEC],
+                                        const float w[K][VEC], const float bias[VEC],
+                                        const float dy[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    if constexpr (SILU) {
+      float z = bias[i];
+#pragma unroll
+      for (int j = 0; j < K; ++j) z = fmaf(win[j][i], w[j][i], z);
+      const float sg = sigmoid_f(z);
+      dz[i] = dy[i] * sg * fmaf(z, 1.f - sg, 1.f);
+    } else {
+      dz[i] = dy[i];
+    }
+  }
+}
+
+template <class E, int K, int VEC, bool SILU>
+__global__ void __launch_bounds__(256, 2) conv1d_bwd_kernel(const Conv1dParams p) {
+  extern __shared__ float red[];  // [blockDim.y][blockDim.x * VEC]
+  const int64_t c = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * VEC;
+  const int64_t run = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
+  const int64_t b = run / p.runs_per_b;
+  const bool live = c < p.C && b < p.B;
+  float dw[K][VEC] = {}, db[VEC] = {};
+  if (live) {
+    const int64_t t0 = (run % p.runs_per_b) * p.run, t1 = min(t0 + p.run, p.T);
+    const int64_t xbase = b * p.x_sb, dybase = b * p.dy_sb, dxbase = b * p.T * p.C + c;
+    float w[K][VEC], bias[VEC] = {};
+#pragma unroll
+    for (int j = 0; j < K; ++j) ldv<E, VEC>(p.w, j * p.C + c, w[j]);
+    if (p.bias != nullptr) ldv<E, VEC>(p.bias, c, bias);
+    SeqSpan s = span_at(p.seq, b, t0);
+    int64_t a = t0;
+    while (a < t1) {  // the part [a, e) of the run that lies in one sequence (or gap)
+      const int64_t e = min(t1, s.hi);
+      if (!s.covered) {
+        const float zero[VEC] = {};
+        for (int64_t t = a; t < e; ++t) stv<E, VEC>(p.dx, dxbase + t * p.C, zero);
+      } else {
+        float win[K][VEC], q[K][VEC];  // inputs; q[K-1-i] = dz[t - i]
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j) {
+          conv_input_v<E, VEC>(p, K, s, xbase, a - (K - 1) + j, c, win[j]);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) q[j][i] = 0.f;
+        }
+        const int64_t last = min(e + K - 1, s.hi);  // dz is wanted for rows [a, last)
+        for (int64_t t = a; t < e + K - 1; ++t) {
+          if (t < last) {
+            float dyv[VEC];
+            ldv<E, VEC>(p.x, xbase + t * p.x_st + c, win[K - 1]);
+            ldv<E, VEC>(p.dy, dybase + t * p.dy_st + c, dyv);
+            conv_dz<E, K, VEC, SILU>(q[K - 1], win, w, bias, dyv);
+            if (t < e) {
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) {
+                db[i] += q[K - 1][i];
+#pragma unroll
+                for (int j = 0; j < K; ++j) dw[j][i] = fmaf(q[K - 1][i], win[j][i], dw[j][i]);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) q[K - 1][i] = 0.f;
+          }
+          const int64_t to = t - (K - 1);  // the row whose dz window is complete
+          if (to >= a) {
+            float d[VEC] = {};
+            const int64_t f = to + K - 1 - s.hi;  // the row of final_state that it is
+            if (p.dfinal != nullptr && f >= 0)
+              ldv<E, VEC>(p.dfinal, (s.n * (K - 1) + f) * p.C + c, d);
+#pragma unroll
+            for (int j = 0; j < K; ++j)
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) d[i] = fmaf(w[j][i], q[K - 1 - j][i], d[i]);
+            stv<E, VEC>(p.dx, dxbase + to * p.C, d);
+          }
+#pragma unroll
+          for (int j = 0; j < K - 1; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              win[j][i] = win[j + 1][i];
+              q[j][i] = q[j + 1][i];
+            }
+        }
+      }
+      a = e;
+      if (a < t1) s = span_from(p.seq, s.n, a);
+    }
+  }
+  // Add the block's runs, tap by tap (K is the bias).
+  const int width = blockDim.x * VEC;
+#pragma unroll
+  for (int j = 0; j <= K; ++j) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      red[threadIdx.y * width + threadIdx.x * VEC + i] = j < K ? dw[j < K ? j : 0][i] : db[i];
+    __syncthreads();
+    for (int i = threadIdx.y * blockDim.x + threadIdx.x; i < width; i += blockDim.x * blockDim.y) {
+      const int64_t cc = int64_t(blockIdx.y) * width + i;
+      if (cc >= p.C) continue;
+      float sum = 0.f;
+      for (int r = 0; r < int(blockDim.y); ++r) sum += red[r * width + i];
+      p.partial[(int64_t(blockIdx.x) * (K + 1) + j) * p.C + cc] = sum;
+    }
+  }
+}
+
+// dw [K, C] and dbias [C] from the blocks' partial sums, in block order.
+template <class E>
+__global__ void __launch_bounds__(256) conv1d_wsum_kernel(const float* partial, int64_t groups,
+                                                          int64_t taps, int64_t C, void* dw,
+                                                          void* dbias) {
+  // 8 threads a value: each adds every 8th group, then the 8 are added.
+  const int64_t v = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) / 8;
+  const int part = threadIdx.x & 7;
+  const int64_t total = (taps + 1) * C;
+  float sum = 0.f;
+  if (v < total)
+    for (int64_t g = part; g < groups; g += 8) sum += partial[g * total + v];
+  sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+  sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+  sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+  if (v >= total || part != 0) return;
+  if (v < taps * C) store_float<E>(dw, v, sum);
+  else if (dbias != nullptr) store_float<E>(dbias, v - taps * C, sum);
+}
+
+// Gradient of the initial states: row r of sequence n is input t = lo-(K-1)+r,
+// reached by dz[lo .. lo+r].
+template <class E, int K, bool SILU>
+__global__ void __launch_bounds__(128) conv1d_dinit_kernel(const Conv1dParams p) {
+  const int64_t vecs = p.C / 4;
+  const int64_t id = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (id >= p.seq.n * vecs) return;
+  const int64_t c = (id % vecs) * 4, n = id / vecs;
+  SeqSpan s{n, 0, p.T, true};
+  int64_t b = n;
+  if (p.seq.cu != nullptr) {
+    s.lo = p.seq.at(n);
+    s.hi = max(s.lo, p.seq.at(n + 1));
+    b = 0;
+  }
+  const int64_t len = s.hi - s.lo;
+  float w[K][4], bias[4] = {}, win[K][4], d[K - 1][4] = {};
+#pragma unroll
+  for (int j = 0; j < K; ++j) ldv<E, 4>(p.w, j * p.C + c, w[j]);
+  if (p.bias != nullptr) ldv<E, 4>(p.bias, c, bias);
+  if (p.dfinal != nullptr) {  // input r + len of the K-1 + len ones is row r of final_state
+#pragma unroll
+    for (int r = 0; r < K - 1; ++r)
+      if (r >= len) ldv<E, 4>(p.dfinal, (n * (K - 1) + r - len) * p.C + c, d[r]);
+  }
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j)
+    conv_input_v<E, 4>(p, K, s, b * p.x_sb, s.lo - (K - 1) + j, c, win[j]);
+#pragma unroll
+  for (int t = 0; t < K - 1; ++t) {
+    if (t < len) {
+      float dyv[4], dz[4];
+      ldv<E, 4>(p.x, b * p.x_sb + (s.lo + t) * p.x_st + c, win[K - 1]);
+      ldv<E, 4>(p.dy, b * p.dy_sb + (s.lo + t) * p.dy_st + c, dyv);
+      conv_dz<E, K, 4, SILU>(dz, win, w, bias, dyv);
+      // dz[t] reaches inputs t .. t+K-1 through w[0 .. K-1]
+#pragma unroll
+      for (int r = t; r < K - 1; ++r)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[r][i] = fmaf(w[r - t][i], dz[i], d[r][i]);
+#pragma unroll
+      for (int j = 0; j < K - 1; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) win[j][i] = win[j + 1][i];
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < K - 1; ++r) stv<E, 4>(p.dinit, (n * (K - 1) + r) * p.C + c, d[r]);
+}
+
+// ---- running sequences ---------------------------------------------------------
+// One thread takes 8 channels of one request: K-1 state rows in, T inputs
+// through the window, K-1 rows out.  Bound by latency at the usual sizes: all
+// loads of a thread are independent.
+template <class E, int K, bool SILU>
+__global__ void __launch_bounds__(128) conv1d_step_kernel(const Conv1dParams p) {
+  const int64_t b = blockIdx.x;
+  const int64_t c = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * 8;
+  const int64_t slot = slot_of(p.idx, p.idx64, b, p.slots, threadIdx.x, blockDim.x);
+  if (c >= p.C) return;
+  const int64_t ybase = b * p.T * p.C + c;
+  if (slot < 0) {
+    const uint32_t nan2 = nan16<E>() * 0x10001u, fill = slot == -1 ? 0u : nan2;
+    for (int64_t t = 0; t < p.T; ++t) st16(p.y, ybase + t * p.C, make_uint4(fill, fill, fill, fill));
+    return;
+  }
+  uint4 w[K], win[K];
+  const int64_t sbase = slot * (K - 1) * p.C + c;
+#pragma unroll
+  for (int j = 0; j < K; ++j) w[j] = ld16(p.w, j * p.C + c);
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j)
+    win[j] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.state) + sbase + j * p.C);
+  float bias[8] = {};
+  if (p.bias != nullptr) unpack8<E>(ld16(p.bias, c), bias);
+  for (int64_t t = 0; t < p.T; ++t) {
+    win[K - 1] = ld16(p.x, b * p.x_sb + t * p.x_st + c);
+    float z[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] = bias[i];
+    conv_dot<E, K>(z, win, w);
+    if constexpr (SILU) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z[i] *= sigmoid_f(z[i]);
+    }
+    st16(p.y, ybase + t * p.C, pack8<E>(z));
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) win[j] = win[j + 1];
+  }
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j) st16(p.state, sbase + j * p.C, win[j]);
+}
+
+}  // namespace tdc

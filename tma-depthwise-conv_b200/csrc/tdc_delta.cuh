@@ -1,0 +1,1212 @@
+// tdc_delta.cuh — the gated delta rule: chunked forward and gradients with
+// warp matrix instructions, and the recurrence for running sequences.
+//
+// Chunks of C = 64 tokens.  With G the running sum of g in the chunk (fp64),
+// gam = e^G, Gam_ij = e^(G_i - G_j) and w_i = e^(G_63 - G_i):
+//   L = strictly lower part of (K K^T) * Gam      A = L diag(beta)
+//   T = (I + A)^-1                                P = scale * lower(Q K^T) * Gam
+//   X = V - diag(gam) K S,  U = T X,  V' = diag(beta) U
+//   O = scale diag(gam) Q S + P V'                S <- gam_63 S + K^T diag(w) V'
+// delta_prepare makes T and P of all chunks at once; delta_scan walks the
+// chunks of a sequence.  The columns of S (the value channels) do not mix, so
+// a warp keeps 16 of them, as S^T [16 x K], in the accumulators of its matrix
+// instructions for the whole sequence, and every product of the chain
+// (transposed) takes its A operand straight from the accumulators of the one
+// before it: the warps of a block share tiles but never wait for one another's
+// results.
+//
+// Precision: states, decays, sums and all accumulators are fp32.  An fp32
+// operand of a matrix instruction is split into two bf16 parts (16 bits of
+// mantissa or more; fp16 inputs are split as well, exactly), since one bf16
+// rounding (2^-9) at each of the chain's operands would put about 3e-3 on
+// every output, more than the output's own rounding, and the final state is
+// fp32: with the split it is off by 4e-6.
+#pragma once
+
+#include "tdc_seq_common.cuh"
+
+namespace tdc {
+
+constexpr int kChunk = 64;
+constexpr int kLdT = kChunk + 8;     // row of a [64][64] tile in shared memory
+constexpr int kSq = kChunk * kChunk;  // elements of such a tile in the workspace
+
+struct DeltaParams {
+  const void *q, *k, *v, *beta;
+  const float* g;
+  const float* init;      // [N, HV, K, V] or null
+  float* final_state;     // or null
+  void* o;
+  int64_t T;
+  int H, HV, V, group;
+  int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, g_sb, g_st, b_sb, b_st;
+  SeqTable seq;
+  int64_t chunks_per_b;   // batch form: chunks of each sequence
+  int64_t max_chunks;     // chunks, or their upper bound in a packed batch
+  // packed batches: filled by delta_plan
+  int64_t* seq_lo;        // [N + 1] row offsets, not decreasing
+  int64_t* seq_chunk;     // [N + 1] first chunk of each sequence
+  bool beta_f32;
+  float scale;
+  // workspace of all chunks, [chunk][HV] each
+  __nv_bfloat16* tm;      // [2][64][64]: T, high parts and remainders
+  __nv_bfloat16* pm;      // [2][64][64]: P
+  float* coef;            // [3][64]: gam, w, beta
+  // gradients
+  __nv_bfloat16* um;      // [2][V][64]: U^T
+  __nv_bfloat16* xm;      // [2][V][64]: dX^T
+  __nv_bfloat16* sm;      // [2][V][K]: S^T before the chunk
+  __nv_bfloat16* dm;      // [2][V][K]: dS^T behind the chunk
+  const void* d_o;
+  int64_t do_sb, do_st, do_sh;
+  const float* dfinal;
+  void *dq, *dk, *dv, *dbeta;
+  float *dg, *dinit;
+};
+
+// Where chunk c of the batch lies.
+struct ChunkAt {
+  int64_t n;      // sequence
+  int64_t b;      // row of the batch
+  int64_t t0;     // first row
+  int rows;       // 0: no such chunk
+};
+
+__device__ __forceinline__ ChunkAt chunk_at(const DeltaParams& p, int64_t c) {
+  ChunkAt r;
+  if (p.seq.cu == nullptr) {
+    r.n = r.b = c / p.chunks_per_b;
+    r.t0 = (c % p.chunks_per_b) * kChunk;
+    r.rows = int(min(int64_t(kChunk), p.T - r.t0));
+    return r;
+  }
+  r.b = 0;
+  int64_t lo = 0, hi = p.seq.n;  // last sequence whose first chunk is <= c
+  while (hi - lo > 1) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (p.seq_chunk[mid] <= c) lo = mid; else hi = mid;
+  }
+  r.n = lo;
+  r.t0 = p.seq_lo[lo] + (c - p.seq_chunk[lo]) * kChunk;
+  const int64_t left = p.seq_lo[lo + 1] - r.t0;
+  r.rows = int(max(int64_t(0), min(int64_t(kChunk), left)));
+  return r;
+}
+
+// First chunk, number of chunks, first row and length of sequence n.
+struct SeqAt {
+  int64_t chunk0, lo, len, b;
+};
+__device__ __forceinline__ SeqAt seq_at(const DeltaParams& p, int64_t n) {
+  if (p.seq.cu == nullptr) return {n * p.chunks_per_b, 0, p.T, n};
+  return {p.seq_chunk[n], p.seq_lo[n], p.seq_lo[n + 1] - p.seq_lo[n], 0};
+}
+
+// ---- plan of a packed batch ------------------------------------------------------
+// Block 0: running maximum of the clamped offsets, and the chunks before each
+// sequence.  The other blocks zero the rows that no sequence owns.
+struct ZeroRows {
+  void* base[5];
+  int64_t row_bytes[5];  // multiples of 2
+};
+
+__global__ void __launch_bounds__(1024) delta_plan_kernel(const SeqTable s, int64_t* seq_lo,
+                                                          int64_t* seq_chunk, const ZeroRows z) {
+  __shared__ int64_t sh[1024];
+  __shared__ int64_t carry_lo, carry_chunk;
+  const int tid = threadIdx.x;
+  if (blockIdx.x != 0) {
+    int64_t top = 0;
+    for (int64_t i = tid; i <= s.n; i += 1024) top = max(top, s.at(i));
+    sh[tid] = top;
+    __syncthreads();
+    for (int d = 512; d; d >>= 1) {
+      if (tid < d) sh[tid] = max(sh[tid], sh[tid + d]);
+      __syncthreads();
+    }
+    top = sh[0];
+    const int64_t first = s.at(0), step = int64_t(gridDim.x - 1) * 1024;
+    const int64_t at = int64_t(blockIdx.x - 1) * 1024 + tid;
+    for (int i = 0; i < 5; ++i) {
+      if (z.base[i] == nullptr) continue;
+      uint16_t* base = static_cast<uint16_t*>(z.base[i]);
+      const int64_t per = z.row_bytes[i] / 2;
+      for (int64_t e = at; e < first * per; e += step) base[e] = 0;
+      for (int64_t e = top * per + at; e < s.T * per; e += step) base[e] = 0;
+    }
+    return;
+  }
+  if (tid == 0) carry_lo = 0, carry_chunk = 0;
+  for (int64_t i0 = 0; i0 <= s.n; i0 += 1024) {
+    const int64_t i = i0 + tid;
+    __syncthreads();
+    sh[tid] = i <= s.n ? s.at(i) : 0;
+    __syncthreads();
+    for (int d = 1; d < 1024; d <<= 1) {
+      const int64_t v = tid >= d ? sh[tid - d] : 0;
+      __syncthreads();
+      sh[tid] = max(sh[tid], v);
+      __syncthreads();
+    }
+    const int64_t lo = max(sh[tid], carry_lo);
+    const int64_t before = max(tid ? sh[tid - 1] : 0, carry_lo);
+    __syncthreads();
+    const bool ends = i >= 1 && i <= s.n;  // sequence i-1 is [before, lo)
+    sh[tid] = ends ? (lo - before + kChunk - 1) / kChunk : 0;
+    __syncthreads();
+    for (int d = 1; d < 1024; d <<= 1) {
+      const int64_t v = tid >= d ? sh[tid - d] : 0;
+      __syncthreads();
+      sh[tid] += v;
+      __syncthreads();
+    }
+    if (i <= s.n) {
+      seq_lo[i] = lo;
+      seq_chunk[i] = carry_chunk + sh[tid];
+    }
+    __syncthreads();
+    if (tid == 1023) carry_lo = lo, carry_chunk += sh[1023];
+  }
+}
+
+// ---- shared pieces -------------------------------------------------------------------
+// rows x (16 * vecs bytes) into shared memory with row stride ld elements;
+// rows behind `valid` become zeros.
+__device__ __forceinline__ void copy_rows(uint32_t dst, int ld, const uint16_t* src, int64_t stride,
+                                          int rows, int valid, int vecs, int tid, int threads) {
+  for (int i = tid; i < rows * vecs; i += threads) {
+    const int r = i / vecs, c = i % vecs;
+    cp_async16(dst + 2 * (r * ld + 8 * c), src + (r < valid ? r * stride : 0) + 8 * c, r < valid);
+  }
+}
+
+__device__ __forceinline__ float load_beta(const DeltaParams& p, bool bf16, int64_t i) {
+  if (p.beta_f32) return static_cast<const float*>(p.beta)[i];
+  return bf16 ? to_float<BF16>(p.beta, i) : to_float<F16>(p.beta, i);
+}
+
+// Running sum of g over a chunk in fp64 (differences of far sums have to keep
+// fp32's precision), by the first warp; two tokens a lane.
+__device__ __forceinline__ void chunk_decay(const DeltaParams& p, const ChunkAt& at, int hv,
+                                            double* G, int lane) {
+  double v[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int t = 2 * lane + i;
+    float g = t < at.rows ? p.g[at.b * p.g_sb + (at.t0 + t) * p.g_st + hv] : 0.f;
+    v[i] = g < -200.f ? -200.0 : double(g);
+  }
+  double sum = v[0] + v[1];
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const double o = __shfl_up_sync(0xffffffffu, sum, d);
+    if (lane >= d) sum += o;
+  }
+  G[2 * lane + 1] = sum;
+  G[2 * lane] = sum - v[1];
+}
+
+// ---- T and P of every chunk -------------------------------------------------------
+// One block a chunk and key head; 4 warps, 16 rows each.  Bound by the
+// triangular inverse: diagonal blocks of 16 by substitution, one column a
+// thread, then joined twice, inv([[P, 0], [B, R]]) = [[P', 0], [-R' B P', R']].
+constexpr int kLdF = kChunk + 1;  // row of the fp32 tiles
+
+// dst[.. n x n at (r0, c0)] = sign * a[n x n] b[n x n]; all fp32 in shared memory.
+__device__ __forceinline__ void small_product(float* dst, int ldd, const float* a, int lda,
+                                              const float* b, int ldb, int n, float sign, int i0,
+                                              int step) {
+  for (int e = i0; e < n * n; e += step) {
+    const int r = e / n, c = e % n;
+    float s = 0.f;
+    for (int m = 0; m < n; ++m) s = fmaf(a[r * lda + m], b[m * ldb + c], s);
+    dst[r * ldd + c] = sign * s;
+  }
+}
+
+// sT = (I + sA)^-1 for strictly lower triangular sA; tmp holds 32 x 33 floats.
+__device__ __forceinline__ void unit_lower_inverse(const float* sA, float* sT, float* tmp, int tid) {
+  for (int e = tid; e < kChunk * kChunk; e += 128) sT[(e / kChunk) * kLdF + e % kChunk] = 0.f;
+  __syncthreads();
+  if (tid < kChunk) {
+    const int o = (tid / 16) * 16, c = tid % 16;
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float s = i == c ? 1.f : 0.f;
+#pragma unroll
+      for (int m = 0; m < i; ++m) s = fmaf(-sA[(o + i) * kLdF + o + m], x[m], s);
+      x[i] = s;
+      sT[(o + i) * kLdF + o + c] = s;
+    }
+  }
+  __syncthreads();
+  {
+    const int h = tid / 64, o = 32 * h, i0 = tid % 64;  // blocks (0,1) and (2,3)
+    float* t = tmp + h * 16 * 17;
+    small_product(t, 17, sA + (o + 16) * kLdF + o, kLdF, sT + o * kLdF + o, kLdF, 16, 1.f, i0, 64);
+    __syncthreads();
+    small_product(sT + (o + 16) * kLdF + o, kLdF, sT + (o + 16) * kLdF + o + 16, kLdF, t, 17, 16,
+                  -1.f, i0, 64);
+  }
+  __syncthreads();
+  small_product(tmp, 33, sA + 32 * kLdF, kLdF, sT, kLdF, 32, 1.f, tid, 128);
+  __syncthreads();
+  small_product(sT + 32 * kLdF, kLdF, sT + 32 * kLdF + 32, kLdF, tmp, 33, 32, -1.f, tid, 128);
+  __syncthreads();
+}
+
+template <int DK>
+constexpr size_t prepare_smem() {
+  return size_t(2) * kChunk * (DK + 8) * 2 + size_t(2) * kChunk * kLdF * 4 + 32 * 33 * 4 +
+         kChunk * 8 + kChunk * 4;
+}
+
+template <class E, int DK>
+__global__ void __launch_bounds__(128) delta_prepare_kernel(const DeltaParams p) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  constexpr int ld = DK + 8;
+  const int64_t chunk = blockIdx.x;
+  const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const ChunkAt at = chunk_at(p, chunk);
+  if (at.rows == 0) return;
+  const uint32_t sq = smem_addr(raw), sk = sq + kChunk * ld * 2;
+  float* sA = reinterpret_cast<float*>(raw + 2 * kChunk * ld * 2);
+  float* sT = sA + kChunk * kLdF;
+  float* tmp = sT + kChunk * kLdF;
+  double* G = reinterpret_cast<double*>(tmp + 32 * 33);
+  float* sB = reinterpret_cast<float*>(G + kChunk);
+  const uint16_t* q = static_cast<const uint16_t*>(p.q) + at.b * p.q_sb + at.t0 * p.q_st + h * p.q_sh;
+  const uint16_t* k = static_cast<const uint16_t*>(p.k) + at.b * p.k_sb + at.t0 * p.k_st + h * p.k_sh;
+  copy_rows(sq, ld, q, p.q_st, kChunk, at.rows, DK / 8, tid, 128);
+  copy_rows(sk, ld, k, p.k_st, kChunk, at.rows, DK / 8, tid, 128);
+  cp_async_commit();
+  cp_async_wait<0>();
+  __syncthreads();
+  // Rows 16 warp .. + 15 of Q K^T and K K^T (both operands exact).
+  float qk[8][4] = {}, kk[8][4] = {};
+#pragma unroll
+  for (int ks = 0; ks < DK / 16; ++ks) {
+    uint32_t aq[4], ak[4];
+    ldsm4(aq, addr_a(sq, ld, 16 * warp, 16 * ks, lane));
+    ldsm4(ak, addr_a(sk, ld, 16 * warp, 16 * ks, lane));
+#pragma unroll
+    for (int np = 0; np < 4; ++np) {
+      if (np > warp) break;  // columns behind the rows are not used
+      uint32_t bk[4];
+      ldsm4(bk, addr_b(sk, ld, 16 * np, 16 * ks, lane));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        mma_elem<E>(qk[2 * np + i], aq, bk[2 * i], bk[2 * i + 1]);
+        mma_elem<E>(kk[2 * np + i], ak, bk[2 * i], bk[2 * i + 1]);
+      }
+    }
+  }
+  const int g = lane >> 2, t2 = (lane & 3) * 2;
+  for (int gi = 0; gi < p.group; ++gi) {
+    const int hv = h * p.group + gi;
+    const int64_t slot = chunk * p.HV + hv;
+    if (warp == 0) chunk_decay(p, at, hv, G, lane);
+    if (tid >= 64) {
+      const int t = tid - 64;
+      sB[t] = t < at.rows ? load_beta(p, std::is_same_v<E, BF16>,
+                                      at.b * p.b_sb + (at.t0 + t) * p.b_st + hv)
+                          : 0.f;
+    }
+    __syncthreads();
+    if (tid < kChunk) {
+      float* coef = p.coef + slot * 3 * kChunk;
+      coef[tid] = expf(float(G[tid]));
+      coef[kChunk + tid] = expf(float(G[kChunk - 1] - G[tid]));
+      coef[2 * kChunk + tid] = sB[tid];
+    }
+    __nv_bfloat16* pm = p.pm + slot * 2 * kSq;
+#pragma unroll
+    for (int nt = 0; nt < 8; ++nt) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int i = 16 * warp + g + 8 * half, j = 8 * nt + t2;
+        float pv[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float gam = i >= j + u ? __expf(float(G[i] - G[j + u])) : 0.f;
+          pv[u] = i >= j + u ? p.scale * gam * qk[nt][2 * half + u] : 0.f;
+          sA[i * kLdF + j + u] = i > j + u ? kk[nt][2 * half + u] * gam * sB[j + u] : 0.f;
+        }
+        uint32_t hi, lo;
+        split2(pv[0], pv[1], hi, lo);
+        *reinterpret_cast<uint32_t*>(pm + i * kChunk + j) = hi;
+        *reinterpret_cast<uint32_t*>(pm + kSq + i * kChunk + j) = lo;
+      }
+    }
+    __syncthreads();
+    unit_lower_inverse(sA, sT, tmp, tid);
+    __nv_bfloat16* tm = p.tm + slot * 2 * kSq;
+    for (int e = tid; e < kSq / 2; e += 128) {
+      const int i = e / (kChunk / 2), j = 2 * (e % (kChunk / 2));
+      uint32_t hi, lo;
+      split2(sT[i * kLdF + j], sT[i * kLdF + j + 1], hi, lo);
+      *reinterpret_cast<uint32_t*>(tm + i * kChunk + j) = hi;
+      *reinterpret_cast<uint32_t*>(tm + kSq + i * kChunk + j) = lo;
+    }
+    __syncthreads();
+  }
+}
+
+// ---- the walk over a sequence's chunks ---------------------------------------------
+// Stages of the two-deep ring: K, Q, V slice, T, P, coefficients.
+template <int DK, int W>
+struct ScanStage {
+  static constexpr int ld = DK + 8, ldv = 16 * W + 8;
+  static constexpr int k = 0;
+  static constexpr int q = k + kChunk * ld * 2;
+  static constexpr int v = q + kChunk * ld * 2;
+  static constexpr int t = v + kChunk * ldv * 2;
+  static constexpr int p = t + 2 * kChunk * kLdT * 2;
+  static constexpr int coef = p + 2 * kChunk * kLdT * 2;
+  static constexpr int bytes = coef + 3 * kChunk * 4;
+};
+
+// x^T [16 x 64] (accumulators) times M^T, M lower triangular [64][64] split in
+// shared memory: out^T = x^T M^T, i.e. out = M x.
+__device__ __forceinline__ void lower_product(float out[8][4], const float x[8][4], uint32_t m,
+                                              int lane) {
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) {
+    uint32_t ah[4], al[4];
+    split_frag(x[2 * ks], x[2 * ks + 1], ah, al);
+#pragma unroll
+    for (int np = ks; np < 4; ++np) {
+      uint32_t bh[4], bl[4];
+      ldsm4(bh, addr_b(m, kLdT, 16 * np, 16 * ks, lane));
+      ldsm4(bl, addr_b(m + kChunk * kLdT * 2, kLdT, 16 * np, 16 * ks, lane));
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        mma_split(out[2 * np + i], ah, al, bh[2 * i], bh[2 * i + 1], bl[2 * i], bl[2 * i + 1]);
+    }
+  }
+}
+
+// out = M^T x: out^T = x^T M.
+__device__ __forceinline__ void lower_product_t(float out[8][4], const float x[8][4], uint32_t m,
+                                                int lane) {
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) {
+    uint32_t ah[4], al[4];
+    split_frag(x[2 * ks], x[2 * ks + 1], ah, al);
+#pragma unroll
+    for (int np = 0; np <= ks; ++np) {
+      uint32_t bh[4], bl[4];
+      ldsm4_t(bh, addr_bt(m, kLdT, 16 * np, 16 * ks, lane));
+      ldsm4_t(bl, addr_bt(m + kChunk * kLdT * 2, kLdT, 16 * np, 16 * ks, lane));
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        mma_split(out[2 * np + i], ah, al, bh[2 * i], bh[2 * i + 1], bl[2 * i], bl[2 * i + 1]);
+    }
+  }
+}
+
+// out^T [16 x 64] += S^T [16 x DK] M^T, M [64][DK] in the element type.
+template <class E, int DK>
+__device__ __forceinline__ void state_product(float out[8][4], const float s[DK / 8][4], uint32_t m,
+                                              int lane) {
+#pragma unroll
+  for (int ks = 0; ks < DK / 16; ++ks) {
+    uint32_t ah[4], al[4];
+    split_frag(s[2 * ks], s[2 * ks + 1], ah, al);
+#pragma unroll
+    for (int np = 0; np < 4; ++np) {
+      uint32_t b[4];
+      ldsm4(b, addr_b(m, DK + 8, 16 * np, 16 * ks, lane));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) mma_split_elem<E>(out[2 * np + i], ah, al, b[2 * i], b[2 * i + 1]);
+    }
+  }
+}
+
+// S^T [16 x DK] += x^T M, with x^T's A fragment of 16 tokens given split.
+template <class E, int DK>
+__device__ __forceinline__ void state_update(float s[DK / 8][4], const uint32_t ah[4],
+                                             const uint32_t al[4], uint32_t m, int ks, int lane) {
+#pragma unroll
+  for (int np = 0; np < DK / 16; ++np) {
+    uint32_t b[4];
+    ldsm4_t(b, addr_bt(m, DK + 8, 16 * np, 16 * ks, lane));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) mma_split_elem<E>(s[2 * np + i], ah, al, b[2 * i], b[2 * i + 1]);
+  }
+}
+
+// Writes x^T [16 x cols] (accumulators) split into rows r0.. of [rows][ldg].
+template <int NT>
+__device__ __forceinline__ void store_split(__nv_bfloat16* dst, int64_t part, int ldg,
+                                            const float x[NT][4], int lane) {
+  const int g = lane >> 2, t2 = (lane & 3) * 2;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t hi, lo;
+      split2(x[nt][2 * half], x[nt][2 * half + 1], hi, lo);
+      __nv_bfloat16* d = dst + (g + 8 * half) * ldg + 8 * nt + t2;
+      *reinterpret_cast<uint32_t*>(d) = hi;
+      *reinterpret_cast<uint32_t*>(d + part) = lo;
+    }
+}
+
+// S^T [16 x DK] of a warp from and to a state [DK][V] at value channel c0.
+template <int DK>
+__device__ __forceinline__ void load_state(float s[DK / 8][4], const float* src, int V, int lane) {
+  const int g = lane >> 2, t2 = (lane & 3) * 2;
+#pragma unroll
+  for (int nt = 0; nt < DK / 8; ++nt)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      s[nt][e] = src == nullptr ? 0.f : src[int64_t(8 * nt + t2 + (e & 1)) * V + g + 8 * (e >> 1)];
+}
+template <int DK>
+__device__ __forceinline__ void store_state(float* dst, const float s[DK / 8][4], int V, int lane) {
+  const int g = lane >> 2, t2 = (lane & 3) * 2;
+#pragma unroll
+  for (int nt = 0; nt < DK / 8; ++nt)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) dst[int64_t(8 * nt + t2 + (e & 1)) * V + g + 8 * (e >> 1)] = s[nt][e];
+}
+
+// The 16-bit rows of a warp's 16 value channels: accumulators x^T [16 x 64]
+// to dst [token][..] through the warp's own columns of a shared tile.
+template <class E>
+__device__ __forceinline__ void store_rows(const float x[8][4], uint32_t tile, int ldv, int c0,
+                                           const unsigned char* raw_tile, uint16_t* dst,
+                                           int64_t stride, int rows, int lane) {
+  __syncwarp();
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) {
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      r[2 * i] = pack2_rn<E>(x[2 * ks + i][0], x[2 * ks + i][1]);
+      r[2 * i + 1] = pack2_rn<E>(x[2 * ks + i][2], x[2 * ks + i][3]);
+    }
+    stsm4_t(addr_at(tile, ldv, c0, 16 * ks, lane), r);
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int e = i * 32 + lane, r = e >> 1, c = (e & 1) * 8;
+    if (r < rows)
+      *reinterpret_cast<uint4*>(dst + r * stride + c) =
+          *reinterpret_cast<const uint4*>(raw_tile + 2 * (r * ldv + c0 + c));
+  }
+}
+
+// MODE 0: the forward (o and the final state).  MODE 1: the forward once more
+// for the gradients: U of each chunk and the state before it.
+template <class E, int DK, int W, int MODE>
+__global__ void __launch_bounds__(32 * W) delta_scan_kernel(const DeltaParams p) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  using St = ScanStage<DK, W>;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int hv = blockIdx.y, h = hv / p.group;
+  const int tiles = p.V / (16 * W);
+  const int64_t n = blockIdx.x / tiles;
+  const int v0 = (blockIdx.x % tiles) * 16 * W, c0 = 16 * warp;
+  const SeqAt s = seq_at(p, n);
+  const int chunks = int((s.len + kChunk - 1) / kChunk);
+  const uint16_t* q = static_cast<const uint16_t*>(p.q) + s.b * p.q_sb + s.lo * p.q_st + h * p.q_sh;
+  const uint16_t* k = static_cast<const uint16_t*>(p.k) + s.b * p.k_sb + s.lo * p.k_st + h * p.k_sh;
+  const uint16_t* v = static_cast<const uint16_t*>(p.v) + s.b * p.v_sb + s.lo * p.v_st + hv * p.v_sh + v0;
+
+  auto fetch = [&](int c) {
+    const uint32_t st = smem_addr(raw) + (c & 1) * St::bytes;
+    const int64_t t0 = int64_t(c) * kChunk, slot = (s.chunk0 + c) * p.HV + hv;
+    const int rows = int(min(int64_t(kChunk), s.len - t0));
+    copy_rows(st + St::k, St::ld, k + t0 * p.k_st, p.k_st, kChunk, rows, DK / 8, tid, 32 * W);
+    copy_rows(st + St::v, St::ldv, v + t0 * p.v_st, p.v_st, kChunk, rows, 2 * W, tid, 32 * W);
+    copy_rows(st + St::t, kLdT, reinterpret_cast<const uint16_t*>(p.tm) + slot * 2 * kSq, kChunk,
+              2 * kChunk, 2 * kChunk, kChunk / 8, tid, 32 * W);
+    if constexpr (MODE == 0) {
+      copy_rows(st + St::q, St::ld, q + t0 * p.q_st, p.q_st, kChunk, rows, DK / 8, tid, 32 * W);
+      copy_rows(st + St::p, kLdT, reinterpret_cast<const uint16_t*>(p.pm) + slot * 2 * kSq, kChunk,
+                2 * kChunk, 2 * kChunk, kChunk / 8, tid, 32 * W);
+    }
+    const float* coef = p.coef + slot * 3 * kChunk;
+    for (int i = tid; i < 3 * kChunk / 4; i += 32 * W)
+      cp_async16(st + St::coef + 16 * i, coef + 4 * i, true);
+    cp_async_commit();
+  };
+
+  const int64_t state_at = ((n * p.HV + hv) * DK) * int64_t(p.V) + v0 + c0;
+  float S[DK / 8][4];
+  load_state<DK>(S, p.init == nullptr ? nullptr : p.init + state_at, p.V, lane);
+  if (chunks > 0) fetch(0);
+  for (int c = 0; c < chunks; ++c) {
+    if (c + 1 < chunks) {
+      fetch(c + 1);
+      cp_async_wait<1>();
+    } else {
+      cp_async_wait<0>();
+    }
+    __syncthreads();
+    unsigned char* stage = raw + (c & 1) * St::bytes;
+    const uint32_t st = smem_addr(stage);
+    const float* coef = reinterpret_cast<const float*>(stage + St::coef);
+    const int t2 = (lane & 3) * 2;
+    const int64_t slot = (s.chunk0 + c) * p.HV + hv;
+    if constexpr (MODE == 1) {
+      store_split<DK / 8>(p.sm + (slot * 2 * p.V + v0 + c0) * DK, int64_t(p.V) * DK, DK, S, lane);
+    }
+    float X[8][4] = {}, O[8][4] = {};
+    state_product<E, DK>(X, S, st + St::k, lane);
+    if constexpr (MODE == 0) state_product<E, DK>(O, S, st + St::q, lane);
+    // X = V - gam (K S), transposed: columns are tokens.
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      uint32_t r[4];
+      ldsm4_t(r, addr_at(st + St::v, St::ldv, c0, 16 * ks, lane));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int nt = 2 * ks + i;
+        const float2 gam = *reinterpret_cast<const float2*>(coef + 8 * nt + t2);
+        float a, b;
+        unpack2<E>(r[2 * i], a, b);
+        X[nt][0] = a - gam.x * X[nt][0];
+        X[nt][1] = b - gam.y * X[nt][1];
+        unpack2<E>(r[2 * i + 1], a, b);
+        X[nt][2] = a - gam.x * X[nt][2];
+        X[nt][3] = b - gam.y * X[nt][3];
+        O[nt][0] *= p.scale * gam.x;
+        O[nt][1] *= p.scale * gam.y;
+        O[nt][2] *= p.scale * gam.x;
+        O[nt][3] *= p.scale * gam.y;
+      }
+    }
+    float U[8][4] = {};
+    lower_product(U, X, st + St::t, lane);
+    if constexpr (MODE == 1) {
+      store_split<8>(p.um + (slot * 2 * p.V + v0 + c0) * kChunk, int64_t(p.V) * kChunk, kChunk, U,
+                     lane);
+    }
+#pragma unroll
+    for (int nt = 0; nt < 8; ++nt) {
+      const float2 be = *reinterpret_cast<const float2*>(coef + 2 * kChunk + 8 * nt + t2);
+      U[nt][0] *= be.x;
+      U[nt][1] *= be.y;
+      U[nt][2] *= be.x;
+      U[nt][3] *= be.y;
+    }
+    if constexpr (MODE == 0) {
+      lower_product(O, U, st + St::p, lane);
+      uint16_t* o = static_cast<uint16_t*>(p.o) +
+                    ((s.b * p.T + s.lo + int64_t(c) * kChunk) * p.HV + hv) * p.V + v0 + c0;
+      store_rows<E>(O, st + St::v, St::ldv, c0, stage + St::v, o, int64_t(p.HV) * p.V,
+                    int(min(int64_t(kChunk), s.len - int64_t(c) * kChunk)), lane);
+    }
+    // S = gam_63 S + K^T (w V')
+    const float last = coef[kChunk - 1];
+#pragma unroll
+    for (int nt = 0; nt < DK / 8; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[nt][e] *= last;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+#pragma unroll
+      for (int nt = 2 * ks; nt < 2 * ks + 2; ++nt) {
+        const float2 w = *reinterpret_cast<const float2*>(coef + kChunk + 8 * nt + t2);
+        U[nt][0] *= w.x;
+        U[nt][1] *= w.y;
+        U[nt][2] *= w.x;
+        U[nt][3] *= w.y;
+      }
+      uint32_t ah[4], al[4];
+      split_frag(U[2 * ks], U[2 * ks + 1], ah, al);
+      state_update<E, DK>(S, ah, al, st + St::k, ks, lane);
+    }
+    __syncthreads();
+  }
+  if (MODE == 0 && p.final_state != nullptr) store_state<DK>(p.final_state + state_at, S, p.V, lane);
+}
+
+// ---- gradients: the walk back ---------------------------------------------------------
+//   dV' = P^T dO + diag(w) K dS      dX = T^T diag(beta) dV'  (= dV)
+//   dS <- gam_63 dS + scale Q^T diag(gam) dO - K^T diag(gam) dX
+// dS^T [16 x K] stays in a warp's accumulators as S^T does; dS behind each
+// chunk and dX go to the workspace for delta_grad_kernel.
+template <class E, int DK, int W>
+__global__ void __launch_bounds__(32 * W) delta_scan_back_kernel(const DeltaParams p) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  using St = ScanStage<DK, W>;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int hv = blockIdx.y, h = hv / p.group;
+  const int tiles = p.V / (16 * W);
+  const int64_t n = blockIdx.x / tiles;
+  const int v0 = (blockIdx.x % tiles) * 16 * W, c0 = 16 * warp;
+  const SeqAt s = seq_at(p, n);
+  const int chunks = int((s.len + kChunk - 1) / kChunk);
+  const uint16_t* q = static_cast<const uint16_t*>(p.q) + s.b * p.q_sb + s.lo * p.q_st + h * p.q_sh;
+  const uint16_t* k = static_cast<const uint16_t*>(p.k) + s.b * p.k_sb + s.lo * p.k_st + h * p.k_sh;
+  const uint16_t* d_o = static_cast<const uint16_t*>(p.d_o) + s.b * p.do_sb + s.lo * p.do_st +
+                        hv * p.do_sh + v0;
+
+  auto fetch = [&](int c) {
+    const uint32_t st = smem_addr(raw) + (c & 1) * St::bytes;
+    const int64_t t0 = int64_t(c) * kChunk, slot = (s.chunk0 + c) * p.HV + hv;
+    const int rows = int(min(int64_t(kChunk), s.len - t0));
+    copy_rows(st + St::k, St::ld, k + t0 * p.k_st, p.k_st, kChunk, rows, DK / 8, tid, 32 * W);
+    copy_rows(st + St::q, St::ld, q + t0 * p.q_st, p.q_st, kChunk, rows, DK / 8, tid, 32 * W);
+    copy_rows(st + St::v, St::ldv, d_o + t0 * p.do_st, p.do_st, kChunk, rows, 2 * W, tid, 32 * W);
+    copy_rows(st + St::t, kLdT, reinterpret_cast<const uint16_t*>(p.tm) + slot * 2 * kSq, kChunk,
+              2 * kChunk, 2 * kChunk, kChunk / 8, tid, 32 * W);
+    copy_rows(st + St::p, kLdT, reinterpret_cast<const uint16_t*>(p.pm) + slot * 2 * kSq, kChunk,
+              2 * kChunk, 2 * kChunk, kChunk / 8, tid, 32 * W);
+    const float* coef = p.coef + slot * 3 * kChunk;
+    for (int i = tid; i < 3 * kChunk / 4; i += 32 * W)
+      cp_async16(st + St::coef + 16 * i, coef + 4 * i, true);
+    cp_async_commit();
+  };
+
+  const int64_t state_at = ((n * p.HV + hv) * DK) * int64_t(p.V) + v0 + c0;
+  float D[DK / 8][4];
+  load_state<DK>(D, p.dfinal == nullptr ? nullptr : p.dfinal + state_at, p.V, lane);
+  if (chunks > 0) fetch(chunks - 1);
+  for (int c = chunks - 1; c >= 0; --c) {
+    if (c > 0) {
+      fetch(c - 1);
+      cp_async_wait<1>();
+    } else {
+      cp_async_wait<0>();
+    }
+    __syncthreads();
+    unsigned char* stage = raw + (c & 1) * St::bytes;
+    const uint32_t st = smem_addr(stage);
+    const float* coef = reinterpret_cast<const float*>(stage + St::coef);
+    const int t2 = (lane & 3) * 2;
+    const int64_t slot = (s.chunk0 + c) * p.HV + hv;
+    store_split<DK / 8>(p.dm + (slot * 2 * p.V + v0 + c0) * DK, int64_t(p.V) * DK, DK, D, lane);
+    float X[8][4] = {};
+    state_product<E, DK>(X, D, st + St::k, lane);
+#pragma unroll
+    for (int nt = 0; nt < 8; ++nt) {
+      const float2 w = *reinterpret_cast<const float2*>(coef + kChunk + 8 * nt + t2);
+      X[nt][0] *= w.x;
+      X[nt][1] *= w.y;
+      X[nt][2] *= w.x;
+      X[nt][3] *= w.y;
+    }
+    // += dO^T P, dO^T exact (fp16: split exactly)
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      uint32_t a[4], ah[4], al[4];
+      ldsm4_t(a, addr_at(st + St::v, St::ldv, c0, 16 * ks, lane));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) split_elem<E>(a[i], ah[i], al[i]);
+#pragma unroll
+      for (int np = 0; np <= ks; ++np) {
+        uint32_t bh[4], bl[4];
+        ldsm4_t(bh, addr_bt(st + St::p, kLdT, 16 * np, 16 * ks, lane));
+        ldsm4_t(bl, addr_bt(st + St::p + kChunk * kLdT * 2, kLdT, 16 * np, 16 * ks, lane));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          mma_bf16(X[2 * np + i], ah, bh[2 * i], bh[2 * i + 1]);
+          mma_bf16(X[2 * np + i], ah, bl[2 * i], bl[2 * i + 1]);
+          if constexpr (!std::is_same_v<E, BF16>) mma_bf16(X[2 * np + i], al, bh[2 * i], bh[2 * i + 1]);
+        }
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < 8; ++nt) {
+      const float2 be = *reinterpret_cast<const float2*>(coef + 2 * kChunk + 8 * nt + t2);
+      X[nt][0] *= be.x;
+      X[nt][1] *= be.y;
+      X[nt][2] *= be.x;
+      X[nt][3] *= be.y;
+    }
+    float Y[8][4] = {};
+    lower_product_t(Y, X, st + St::t, lane);
+    store_split<8>(p.xm + (slot * 2 * p.V + v0 + c0) * kChunk, int64_t(p.V) * kChunk, kChunk, Y, lane);
+    const float last = coef[kChunk - 1];
+#pragma unroll
+    for (int nt = 0; nt < DK / 8; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) D[nt][e] *= last;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      uint32_t a[4], ah[4], al[4];
+      ldsm4_t(a, addr_at(st + St::v, St::ldv, c0, 16 * ks, lane));
+      float z[2][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float2 gam = *reinterpret_cast<const float2*>(coef + 8 * (2 * ks + i) + t2);
+        unpack2<E>(a[2 * i], z[i][0], z[i][1]);
+        unpack2<E>(a[2 * i + 1], z[i][2], z[i][3]);
+        z[i][0] *= p.scale * gam.x;
+        z[i][1] *= p.scale * gam.y;
+        z[i][2] *= p.scale * gam.x;
+        z[i][3] *= p.scale * gam.y;
+      }
+      split_frag(z[0], z[1], ah, al);
+      state_update<E, DK>(D, ah, al, st + St::q, ks, lane);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float2 gam = *reinterpret_cast<const float2*>(coef + 8 * (2 * ks + i) + t2);
+        z[i][0] = -gam.x * Y[2 * ks + i][0];
+        z[i][1] = -gam.y * Y[2 * ks + i][1];
+        z[i][2] = -gam.x * Y[2 * ks + i][2];
+        z[i][3] = -gam.y * Y[2 * ks + i][3];
+      }
+      split_frag(z[0], z[1], ah, al);
+      state_update<E, DK>(D, ah, al, st + St::k, ks, lane);
+    }
+    uint16_t* dv = static_cast<uint16_t*>(p.dv) +
+                   ((s.b * p.T + s.lo + int64_t(c) * kChunk) * p.HV + hv) * p.V + v0 + c0;
+    store_rows<E>(Y, st + St::v, St::ldv, c0, stage + St::v, dv, int64_t(p.HV) * p.V,
+                  int(min(int64_t(kChunk), s.len - int64_t(c) * kChunk)), lane);
+    __syncthreads();
+  }
+  if (p.dinit != nullptr) store_state<DK>(p.dinit + state_at, D, p.V, lane);
+}
+
+// ---- gradients of a chunk ------------------------------------------------------------
+// One block a chunk and key head, all chunks at once.  With D = dO U^T and
+// M = dX U^T (lower parts):
+//   dQ = scale gam (dO S^T) + Dt K                     Dt = scale Gam beta_j D
+//   dK = -gam (dX S^T) + w beta (U dS^T) + Dt^T Q + (N + N^T) K,  N = -M beta_j Gam
+//   dbeta_j = sum_i P_ij D_ij - sum_i M_ij L_ij + w_j k_j.(U dS^T)_j
+//   dG_i = rows(E) - cols(E) + scale gam q.(dO S^T) - gam k.(dX S^T) - w beta k.(U dS^T),
+//     E = beta_j (P D - M L); the last row adds the sum of w beta k.(U dS^T) and
+//     gam_63 <dS, S>;  dg = sum of dG from the row to the chunk's end.
+// 8 warps: 4 groups of 16 rows by 2 halves of the columns.  The value channels
+// are walked in tiles of 64.
+template <int DK>
+struct GradSmem {
+  static constexpr int ld = DK + 8;
+  static constexpr int q = 0;
+  static constexpr int k = q + kChunk * ld * 2;
+  static constexpr int s = k + kChunk * ld * 2;           // [2][64][ld]
+  static constexpr int d = s + 2 * 64 * ld * 2;           // [2][64][ld]
+  static constexpr int u = d + 2 * 64 * ld * 2;           // [2][64][72], later Dt
+  static constexpr int x = u + 2 * 64 * kLdT * 2;         // [2][64][72], later N
+  static constexpr int o = x + 2 * 64 * kLdT * 2;         // [64][72]
+  static constexpr int G = o + 64 * kLdT * 2;             // double [64]
+  static constexpr int coef = G + 64 * 8;                 // [3][64]
+  static constexpr int rows = coef + 3 * 64 * 4;          // [2][4][64]: row sums of both halves
+  static constexpr int cols = rows + 2 * 4 * 64 * 4;      // [4][2][64]: column sums of the row groups
+  static constexpr int dot = cols + 4 * 2 * 64 * 4;       // [8] + dG [64]
+  static constexpr int bytes = dot + 8 * 4 + 64 * 4;
+};
+
+template <class E, int DK>
+__global__ void __launch_bounds__(256, 1) delta_grad_kernel(const DeltaParams p) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  using Sm = GradSmem<DK>;
+  constexpr int ld = Sm::ld, NT = DK / 16;  // 8-column tiles of a half of K
+  const int64_t chunk = blockIdx.x;
+  const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rg = warp & 3, ch = warp >> 2;
+  const ChunkAt at = chunk_at(p, chunk);
+  if (at.rows == 0) return;
+  const uint32_t sb = smem_addr(raw);
+  double* G = reinterpret_cast<double*>(raw + Sm::G);
+  float* coef = reinterpret_cast<float*>(raw + Sm::coef);
+  float* rows = reinterpret_cast<float*>(raw + Sm::rows);
+  float* cols = reinterpret_cast<float*>(raw + Sm::cols);
+  float* dot = reinterpret_cast<float*>(raw + Sm::dot);
+  float* dG = dot + 8;
+  const uint16_t* q = static_cast<const uint16_t*>(p.q) + at.b * p.q_sb + at.t0 * p.q_st + h * p.q_sh;
+  const uint16_t* k = static_cast<const uint16_t*>(p.k) + at.b * p.k_sb + at.t0 * p.k_st + h * p.k_sh;
+  copy_rows(sb + Sm::q, ld, q, p.q_st, kChunk, at.rows, DK / 8, tid, 256);
+  copy_rows(sb + Sm::k, ld, k, p.k_st, kChunk, at.rows, DK / 8, tid, 256);
+  const int g = lane >> 2, t2 = (lane & 3) * 2;
+  const int i0 = 16 * rg + g;        // this thread's rows: i0, i0 + 8
+  const int kc0 = ch * (DK / 2);     // its half of K's columns
+  float dq[NT][4] = {}, dk[NT][4] = {};
+
+  for (int gi = 0; gi < p.group; ++gi) {
+    const int hv = h * p.group + gi;
+    const int64_t slot = chunk * p.HV + hv;
+    const uint16_t* d_o = static_cast<const uint16_t*>(p.d_o) + at.b * p.do_sb + at.t0 * p.do_st +
+                          hv * p.do_sh;
+    float os[NT][4] = {}, xs[NT][4] = {}, us[NT][4] = {}, D[4][4] = {}, M[4][4] = {};
+    float dsum = 0.f;
+    for (int v0 = 0; v0 < p.V; v0 += 64) {
+      __syncthreads();
+      const uint16_t* sm = reinterpret_cast<const uint16_t*>(p.sm) + (slot * 2 * p.V + v0) * DK;
+      const uint16_t* dm = reinterpret_cast<const uint16_t*>(p.dm) + (slot * 2 * p.V + v0) * DK;
+      const uint16_t* um = reinterpret_cast<const uint16_t*>(p.um) + (slot * 2 * p.V + v0) * kChunk;
+      const uint16_t* xm = reinterpret_cast<const uint16_t*>(p.xm) + (slot * 2 * p.V + v0) * kChunk;
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        copy_rows(sb + Sm::s + part * 64 * ld * 2, ld, sm + int64_t(part) * p.V * DK, DK, 64, 64,
+                  DK / 8, tid, 256);
+        copy_rows(sb + Sm::d + part * 64 * ld * 2, ld, dm + int64_t(part) * p.V * DK, DK, 64, 64,
+                  DK / 8, tid, 256);
+        copy_rows(sb + Sm::u + part * 64 * kLdT * 2, kLdT, um + int64_t(part) * p.V * kChunk, kChunk,
+                  64, 64, 8, tid, 256);
+        copy_rows(sb + Sm::x + part * 64 * kLdT * 2, kLdT, xm + int64_t(part) * p.V * kChunk, kChunk,
+                  64, 64, 8, tid, 256);
+      }
+      copy_rows(sb + Sm::o, kLdT, d_o + v0, p.do_st, kChunk, at.rows, 8, tid, 256);
+      cp_async_commit();
+      if (v0 == 0) {
+        if (warp == 0) chunk_decay(p, at, hv, G, lane);
+        const float* src = p.coef + slot * 3 * kChunk;
+        if (tid >= 64) coef[tid - 64] = src[tid - 64];
+      }
+      cp_async_wait<0>();
+      __syncthreads();
+      // <dS, S>
+      for (int e = tid; e < 64 * DK / 2; e += 256) {
+        const int r = e / (DK / 2), c = 2 * (e % (DK / 2));
+        float a[2][2], b[2][2];
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          const int off = part * 64 * ld * 2 + 2 * (r * ld + c);
+          unpack2<BF16>(*reinterpret_cast<const uint32_t*>(raw + Sm::s + off), a[part][0], a[part][1]);
+          unpack2<BF16>(*reinterpret_cast<const uint32_t*>(raw + Sm::d + off), b[part][0], b[part][1]);
+        }
+        dsum = fmaf(a[0][0] + a[1][0], b[0][0] + b[1][0], dsum);
+        dsum = fmaf(a[0][1] + a[1][1], b[0][1] + b[1][1], dsum);
+      }
+#pragma unroll 1
+      for (int ks = 0; ks < 4; ++ks) {
+        uint32_t a[4], oh[4], ol[4], xh[4], xl[4], uh[4], ul[4];
+        ldsm4(a, addr_a(sb + Sm::o, kLdT, 16 * rg, 16 * ks, lane));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) split_elem<E>(a[i], oh[i], ol[i]);
+        ldsm4_t(xh, addr_at(sb + Sm::x, kLdT, 16 * rg, 16 * ks, lane));
+        ldsm4_t(xl, addr_at(sb + Sm::x + 64 * kLdT * 2, kLdT, 16 * rg, 16 * ks, lane));
+        ldsm4_t(uh, addr_at(sb + Sm::u, kLdT, 16 * rg, 16 * ks, lane));
+        ldsm4_t(ul, addr_at(sb + Sm::u + 64 * kLdT * 2, kLdT, 16 * rg, 16 * ks, lane));
+        // D and M: columns are tokens 32 ch .. + 31, from U^T [channel][token]
+#pragma unroll
+        for (int np = 0; np < 2; ++np) {
+          if (32 * ch + 16 * np > 16 * rg) continue;  // above the diagonal
+          uint32_t bh[4], bl[4];
+          ldsm4_t(bh, addr_bt(sb + Sm::u, kLdT, 32 * ch + 16 * np, 16 * ks, lane));
+          ldsm4_t(bl, addr_bt(sb + Sm::u + 64 * kLdT * 2, kLdT, 32 * ch + 16 * np, 16 * ks, lane));
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            mma_bf16(D[2 * np + i], oh, bh[2 * i], bh[2 * i + 1]);
+            mma_bf16(D[2 * np + i], oh, bl[2 * i], bl[2 * i + 1]);
+            if constexpr (!std::is_same_v<E, BF16>)
+              mma_bf16(D[2 * np + i], ol, bh[2 * i], bh[2 * i + 1]);
+            mma_split(M[2 * np + i], xh, xl, bh[2 * i], bh[2 * i + 1], bl[2 * i], bl[2 * i + 1]);
+          }
+        }
+        // dO S^T, dX S^T, U dS^T: columns kc0 .. of K, from S^T [channel][K]
+#pragma unroll
+        for (int np = 0; np < NT / 2; ++np) {
+          uint32_t bh[4], bl[4];
+          ldsm4_t(bh, addr_bt(sb + Sm::s, ld, kc0 + 16 * np, 16 * ks, lane));
+          ldsm4_t(bl, addr_bt(sb + Sm::s + 64 * ld * 2, ld, kc0 + 16 * np, 16 * ks, lane));
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            mma_bf16(os[2 * np + i], oh, bh[2 * i], bh[2 * i + 1]);
+            mma_bf16(os[2 * np + i], oh, bl[2 * i], bl[2 * i + 1]);
+            if constexpr (!std::is_same_v<E, BF16>)
+              mma_bf16(os[2 * np + i], ol, bh[2 * i], bh[2 * i + 1]);
+            mma_split(xs[2 * np + i], xh, xl, bh[2 * i], bh[2 * i + 1], bl[2 * i], bl[2 * i + 1]);
+          }
+          ldsm4_t(bh, addr_bt(sb + Sm::d, ld, kc0 + 16 * np, 16 * ks, lane));
+          ldsm4_t(bl, addr_bt(sb + Sm::d + 64 * ld * 2, ld, kc0 + 16 * np, 16 * ks, lane));
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            mma_split(us[2 * np + i], uh, ul, bh[2 * i], bh[2 * i + 1], bl[2 * i], bl[2 * i + 1]);
+        }
+      }
+    }
+    // Row sums with q and k, and the three products into dq and dk.
+    float r[2][3] = {};  // [row i0 / i0 + 8][q.dOS, k.dXS, k.UdS]
+    const float ga[2] = {coef[i0], coef[i0 + 8]};
+    const float wb[2] = {coef[64 + i0] * coef[128 + i0], coef[64 + i0 + 8] * coef[128 + i0 + 8]};
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int off = 2 * ((i0 + 8 * half) * ld + kc0 + 8 * nt + t2);
+        float qv[2], kv[2];
+        unpack2<E>(*reinterpret_cast<const uint32_t*>(raw + Sm::q + off), qv[0], qv[1]);
+        unpack2<E>(*reinterpret_cast<const uint32_t*>(raw + Sm::k + off), kv[0], kv[1]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int e = 2 * half + u;
+          r[half][0] = fmaf(qv[u], os[nt][e], r[half][0]);
+          r[half][1] = fmaf(kv[u], xs[nt][e], r[half][1]);
+          r[half][2] = fmaf(kv[u], us[nt][e], r[half][2]);
+          dq[nt][e] = fmaf(p.scale * ga[half], os[nt][e], dq[nt][e]);
+          dk[nt][e] += wb[half] * us[nt][e] - ga[half] * xs[nt][e];
+        }
+      }
+    // Q K^T and K K^T once more, for this warp's 16 x 32 part.
+    float qk[4][4] = {}, kk[4][4] = {};
+#pragma unroll 2
+    for (int ks = 0; ks < DK / 16; ++ks) {
+      uint32_t aq[4], ak[4];
+      ldsm4(aq, addr_a(sb + Sm::q, ld, 16 * rg, 16 * ks, lane));
+      ldsm4(ak, addr_a(sb + Sm::k, ld, 16 * rg, 16 * ks, lane));
+#pragma unroll
+      for (int np = 0; np < 2; ++np) {
+        uint32_t b[4];
+        ldsm4(b, addr_b(sb + Sm::k, ld, 32 * ch + 16 * np, 16 * ks, lane));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          mma_elem<E>(qk[2 * np + i], aq, b[2 * i], b[2 * i + 1]);
+          mma_elem<E>(kk[2 * np + i], ak, b[2 * i], b[2 * i + 1]);
+        }
+      }
+    }
+    float re[2] = {};  // row sums of E
+    __syncthreads();   // u and x are free: Dt and N take their place
+#pragma unroll
+    for (int nt = 0; nt < 4; ++nt) {
+      float cd[2] = {}, cm[2] = {};  // column sums of P D and M L over this thread's two rows
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int i = i0 + 8 * half, j = 32 * ch + 8 * nt + t2;
+        float dt[2], nn[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int e = 2 * half + u;
+          const float gam = i >= j + u ? __expf(float(G[i] - G[j + u])) : 0.f;
+          const float be = coef[128 + j + u];
+          const float dv = i >= j + u ? D[nt][e] : 0.f, mv = i > j + u ? M[nt][e] : 0.f;
+          const float pd = p.scale * gam * qk[nt][e] * dv, ml = gam * kk[nt][e] * mv;
+          cd[u] += pd;
+          cm[u] += ml;
+          re[half] = fmaf(be, pd - ml, re[half]);
+          dt[u] = p.scale * gam * be * dv;
+          nn[u] = -mv * be * gam;
+        }
+        uint32_t hi, lo;
+        const int off = 2 * (i * kLdT + j);
+        split2(dt[0], dt[1], hi, lo);
+        *reinterpret_cast<uint32_t*>(raw + Sm::u + off) = hi;
+        *reinterpret_cast<uint32_t*>(raw + Sm::u + 64 * kLdT * 2 + off) = lo;
+        split2(nn[0], nn[1], hi, lo);
+        *reinterpret_cast<uint32_t*>(raw + Sm::x + off) = hi;
+        *reinterpret_cast<uint32_t*>(raw + Sm::x + 64 * kLdT * 2 + off) = lo;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          cd[u] += __shfl_xor_sync(0xffffffffu, cd[u], d);
+          cm[u] += __shfl_xor_sync(0xffffffffu, cm[u], d);
+        }
+        if (g == 0) {
+          cols[(rg * 2 + 0) * 64 + 32 * ch + 8 * nt + t2 + u] = cd[u];
+          cols[(rg * 2 + 1) * 64 + 32 * ch + 8 * nt + t2 + u] = cm[u];
+        }
+      }
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int d = 1; d < 4; d <<= 1) {
+        re[half] += __shfl_xor_sync(0xffffffffu, re[half], d);
+#pragma unroll
+        for (int j = 0; j < 3; ++j) r[half][j] += __shfl_xor_sync(0xffffffffu, r[half][j], d);
+      }
+      if ((lane & 3) == 0) {
+#pragma unroll
+        for (int j = 0; j < 3; ++j) rows[(ch * 4 + j) * 64 + i0 + 8 * half] = r[half][j];
+        rows[(ch * 4 + 3) * 64 + i0 + 8 * half] = re[half];
+      }
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) dsum += __shfl_xor_sync(0xffffffffu, dsum, d);
+    if (lane == 0) dot[warp] = dsum;
+    __syncthreads();
+    // dq += Dt K; dk += Dt^T Q + (N + N^T) K
+#pragma unroll 1
+    for (int ks = 0; ks < 4; ++ks) {
+      uint32_t ah[4], al[4], nh[4], nl[4];
+      if (ks <= rg) {
+        ldsm4(ah, addr_a(sb + Sm::u, kLdT, 16 * rg, 16 * ks, lane));
+        ldsm4(al, addr_a(sb + Sm::u + 64 * kLdT * 2, kLdT, 16 * rg, 16 * ks, lane));
+        ldsm4(nh, addr_a(sb + Sm::x, kLdT, 16 * rg, 16 * ks, lane));
+        ldsm4(nl, addr_a(sb + Sm::x + 64 * kLdT * 2, kLdT, 16 * rg, 16 * ks, lane));
+#pragma unroll
+        for (int np = 0; np < NT / 2; ++np) {
+          uint32_t b[4];
+          ldsm4_t(b, addr_bt(sb + Sm::k, ld, kc0 + 16 * np, 16 * ks, lane));
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            mma_split_elem<E>(dq[2 * np + i], ah, al, b[2 * i], b[2 * i + 1]);
+            mma_split_elem<E>(dk[2 * np + i], nh, nl, b[2 * i], b[2 * i + 1]);
+          }
+        }
+      }
+      if (ks >= rg) {
+        ldsm4_t(ah, addr_at(sb + Sm::u, kLdT, 16 * rg, 16 * ks, lane));
+        ldsm4_t(al, addr_at(sb + Sm::u + 64 * kLdT * 2, kLdT, 16 * rg, 16 * ks, lane));
+        ldsm4_t(nh, addr_at(sb + Sm::x, kLdT, 16 * rg, 16 * ks, lane));
+        ldsm4_t(nl, addr_at(sb + Sm::x + 64 * kLdT * 2, kLdT, 16 * rg, 16 * ks, lane));
+#pragma unroll
+        for (int np = 0; np < NT / 2; ++np) {
+          uint32_t b[4], c[4];
+          ldsm4_t(b, addr_bt(sb + Sm::q, ld, kc0 + 16 * np, 16 * ks, lane));
+          ldsm4_t(c, addr_bt(sb + Sm::k, ld, kc0 + 16 * np, 16 * ks, lane));
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            mma_split_elem<E>(dk[2 * np + i], ah, al, b[2 * i], b[2 * i + 1]);
+            mma_split_elem<E>(dk[2 * np + i], nh, nl, c[2 * i], c[2 * i + 1]);
+          }
+        }
+      }
+    }
+    // dbeta and dg
+    if (tid < 64) {
+      const int i = tid;
+      const float ga1 = coef[i], w1 = coef[64 + i], be = coef[128 + i];
+      float s0[4], c0 = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s0[j] = rows[j * 64 + i] + rows[(4 + j) * 64 + i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) c0 += cols[(j * 2) * 64 + i] - cols[(j * 2 + 1) * 64 + i];
+      const float tail = w1 * be * s0[2];
+      if (i < at.rows) {
+        const int64_t o = (at.b * p.T + at.t0 + i) * p.HV + hv;
+        const float db = c0 + w1 * s0[2];
+        if (p.beta_f32) static_cast<float*>(p.dbeta)[o] = db;
+        else store_float<E>(p.dbeta, o, db);
+      }
+      dG[i] = s0[3] - be * c0 + p.scale * ga1 * s0[0] - ga1 * s0[1] - tail;
+      rows[i] = tail;  // (each thread's own entry has been read)
+    }
+    __syncthreads();
+    if (warp == 0) {
+      // dg_i = sum of dG from i to the end; the tails and gam_63 <dS, S> belong to the last row
+      float tails = rows[lane] + rows[lane + 32];
+#pragma unroll
+      for (int d = 16; d; d >>= 1) tails += __shfl_xor_sync(0xffffffffu, tails, d);
+      float ds = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ds += dot[i];
+      const float extra = tails + coef[63] * ds;
+      const float a = dG[2 * lane], b = dG[2 * lane + 1];
+      float sum = a + b;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const float o = __shfl_down_sync(0xffffffffu, sum, d);
+        if (lane + d < 32) sum += o;
+      }
+      const int64_t o = (at.b * p.T + at.t0 + 2 * lane) * p.HV + hv;
+      if (2 * lane < at.rows) p.dg[o] = sum + extra;
+      if (2 * lane + 1 < at.rows) p.dg[o + p.HV] = sum - a + extra;
+    }
+  }
+  // dq and dk rows
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int i = i0 + 8 * half;
+    if (i >= at.rows) continue;
+    const int64_t o = ((at.b * p.T + at.t0 + i) * p.H + h) * DK + kc0 + t2;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.dq) + o + 8 * nt) =
+          pack2_rn<E>(dq[nt][2 * half], dq[nt][2 * half + 1]);
+      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.dk) + o + 8 * nt) =
+          pack2_rn<E>(dk[nt][2 * half], dk[nt][2 * half + 1]);
+    }
+  }
+}
+
+// ---- running sequences ---------------------------------------------------------------
+// One block a request, value head and 32 value channels; a thread holds 4
+// channels of DK / 16 rows of S.  Reads and writes the state once: bound by
+// memory (8 bytes and 7 flops a value).  k.S~, q.S~ and q.k are summed over
+// the rows together, so a token costs one exchange through shared memory:
+//   o = scale (S~^T q + beta (q.k) u).
+template <class E, int DK>
+__global__ void __launch_bounds__(128) delta_step_kernel(const DeltaParams p, float* state,
+                                                         const void* idx, bool idx64,
+                                                         int64_t slots) {
+  constexpr int R = DK / 16;  // rows a thread holds
+  __shared__ float red[4][9][8];
+  const int64_t b = blockIdx.x;
+  const int hv = blockIdx.y, h = hv / p.group, tid = threadIdx.x;
+  const int lane = tid & 31, warp = tid >> 5, cl = tid & 7, rgp = tid >> 3;
+  const int vc = blockIdx.z * 32 + 4 * cl;
+  const int64_t slot = slot_of(idx, idx64, b, slots, tid, 128);
+  uint16_t* o = static_cast<uint16_t*>(p.o) + (b * p.T * p.HV + hv) * p.V + vc;
+  const int64_t ostep = int64_t(p.HV) * p.V;
+  if (slot < 0) {
+    const uint32_t f = slot == -1 ? 0u : nan16<E>() * 0x10001u;
+    if (rgp == 0)
+      for (int64_t t = 0; t < p.T; ++t) *reinterpret_cast<uint2*>(o + t * ostep) = make_uint2(f, f);
+    return;
+  }
+  float* sp = state + ((slot * p.HV + hv) * DK + rgp * R) * int64_t(p.V) + vc;
+  float4 S[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) S[r] = *reinterpret_cast<const float4*>(sp + int64_t(r) * p.V);
+  for (int64_t t = 0; t < p.T; ++t) {
+    const float gr = p.g[b * p.g_sb + t * p.g_st + hv];
+    const float decay = expf(gr < -200.f ? -200.f : gr);
+    const float beta = load_beta(p, std::is_same_v<E, BF16>, b * p.b_sb + t * p.b_st + hv);
+    const uint16_t* qp = static_cast<const uint16_t*>(p.q) + b * p.q_sb + t * p.q_st + h * p.q_sh + rgp * R;
+    const uint16_t* kp = static_cast<const uint16_t*>(p.k) + b * p.k_sb + t * p.k_st + h * p.k_sh + rgp * R;
+    float q[R], k[R], v[4];
+#pragma unroll
+    for (int r = 0; r < R; r += 4) {
+      const uint2 a = *reinterpret_cast<const uint2*>(qp + r), c = *reinterpret_cast<const uint2*>(kp + r);
+      unpack2<E>(a.x, q[r], q[r + 1]);
+      unpack2<E>(a.y, q[r + 2], q[r + 3]);
+      unpack2<E>(c.x, k[r], k[r + 1]);
+      unpack2<E>(c.y, k[r + 2], k[r + 3]);
+    }
+    const uint2 vv = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.v) + b * p.v_sb +
+                                                     t * p.v_st + hv * p.v_sh + vc);
+    unpack2<E>(vv.x, v[0], v[1]);
+    unpack2<E>(vv.y, v[2], v[3]);
+    float a[9] = {};  // k.S~ (4), q.S~ (4), q.k
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      S[r].x *= decay, S[r].y *= decay, S[r].z *= decay, S[r].w *= decay;
+      a[0] = fmaf(k[r], S[r].x, a[0]);
+      a[1] = fmaf(k[r], S[r].y, a[1]);
+      a[2] = fmaf(k[r], S[r].z, a[2]);
+      a[3] = fmaf(k[r], S[r].w, a[3]);
+      a[4] = fmaf(q[r], S[r].x, a[4]);
+      a[5] = fmaf(q[r], S[r].y, a[5]);
+      a[6] = fmaf(q[r], S[r].z, a[6]);
+      a[7] = fmaf(q[r], S[r].w, a[7]);
+      a[8] = fmaf(q[r], k[r], a[8]);
+    }
+#pragma unroll
+    for (int i = 0; i < 9; ++i) {
+      a[i] += __shfl_xor_sync(0xffffffffu, a[i], 8);
+      a[i] += __shfl_xor_sync(0xffffffffu, a[i], 16);
+    }
+    __syncthreads();
+    if (lane < 8) {
+#pragma unroll
+      for (int i = 0; i < 9; ++i) red[warp][i][lane] = a[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 9; ++i) a[i] = red[0][i][cl] + red[1][i][cl] + red[2][i][cl] + red[3][i][cl];
+    float u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = beta * (v[i] - a[i]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      S[r].x = fmaf(k[r], u[0], S[r].x);
+      S[r].y = fmaf(k[r], u[1], S[r].y);
+      S[r].z = fmaf(k[r], u[2], S[r].z);
+      S[r].w = fmaf(k[r], u[3], S[r].w);
+    }
+    if (rgp == 0) {
+      float y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = p.scale * fmaf(a[8], u[i], a[4 + i]);
+      *reinterpret_cast<uint2*>(o + t * ostep) =
+          make_uint2(pack2_rn<E>(y[0], y[1]), pack2_rn<E>(y[2], y[3]));
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) *reinterpret_cast<float4*>(sp + int64_t(r) * p.V) = S[r];
+}
+
+}  // namespace tdc

@@ -1,0 +1,229 @@
+// tdc_seq_common.cuh — what the sequence kernels share: packed-batch lookups,
+// slot indices, 16-byte vectors of 16-bit elements, warp matrix instructions
+// and the split of an fp32 operand into two bf16 ones.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "tdc_ptx.cuh"
+
+namespace tdc {
+
+// ---- packed batches -----------------------------------------------------------
+// Row offsets of a packed batch, int32 or int64, read as the header states:
+// clamped to [0, T].
+struct SeqTable {
+  const void* cu;   // null: a [B, T] batch, every sequence has T rows
+  int64_t n;        // number of sequences
+  int64_t T;
+  bool is64;
+
+  __device__ __forceinline__ int64_t at(int64_t i) const {
+    const int64_t v = is64 ? static_cast<const int64_t*>(cu)[i]
+                           : int64_t(static_cast<const int32_t*>(cu)[i]);
+    return v < 0 ? 0 : (v > T ? T : v);
+  }
+  // First sequence that ends behind row t (n if none does).
+  __device__ __forceinline__ int64_t first_ending_after(int64_t t) const {
+    int64_t lo = 0, hi = n;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (at(mid + 1) > t) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+  }
+};
+
+// ---- slots --------------------------------------------------------------------
+// Slot of request b: >= 0 a state to update, -1 padding (zeros), -2 an index
+// that no state may be read or written for (NaN).  An index that an earlier
+// request has already is refused, so no two blocks update one state; every
+// thread of the block calls this, and all get the same answer.
+__device__ __forceinline__ int64_t slot_of(const void* idx, bool is64, int64_t b, int64_t slots,
+                                           int tid, int threads) {
+  if (idx == nullptr) return b < slots ? b : -2;
+  auto get = [&](int64_t i) {
+    return is64 ? static_cast<const int64_t*>(idx)[i]
+                : int64_t(static_cast<const int32_t*>(idx)[i]);
+  };
+  const int64_t mine = get(b);
+  bool again = false;
+  for (int64_t i = tid; i < b; i += threads) again |= get(i) == mine;
+  again = __syncthreads_or(again);
+  if (mine < 0) return -1;
+  return (again || mine >= slots) ? -2 : mine;
+}
+
+// ---- vectors --------------------------------------------------------------------
+template <class E>
+__device__ __forceinline__ void unpack8(const uint4& v, float f[8]) {
+  unpack2<E>(v.x, f[0], f[1]);
+  unpack2<E>(v.y, f[2], f[3]);
+  unpack2<E>(v.z, f[4], f[5]);
+  unpack2<E>(v.w, f[6], f[7]);
+}
+
+template <class E>
+__device__ __forceinline__ uint4 pack8(const float f[8]) {
+  return make_uint4(pack2_rn<E>(f[0], f[1]), pack2_rn<E>(f[2], f[3]), pack2_rn<E>(f[4], f[5]),
+                    pack2_rn<E>(f[6], f[7]));
+}
+
+template <class E>
+__device__ __forceinline__ uint16_t nan16() {
+  return std::is_same_v<E, BF16> ? 0x7FC0 : 0x7E00;
+}
+
+template <class E>
+__device__ __forceinline__ float to_float(const void* p, int64_t i) {
+  if constexpr (std::is_same_v<E, BF16>) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  else return __half2float(static_cast<const __half*>(p)[i]);
+}
+
+template <class E>
+__device__ __forceinline__ void store_float(void* p, int64_t i, float v) {
+  if constexpr (std::is_same_v<E, BF16>) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else static_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+// 1 / (1 + exp(-z)): an overflowing exp gives 0, as the limit is.
+__device__ __forceinline__ float sigmoid_f(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+
+// ---- asynchronous copies ----------------------------------------------------------
+// 16 bytes global -> shared; with `valid` false the destination gets zeros and
+// nothing is read.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(valid ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// ---- warp matrix instructions -------------------------------------------------------
+// Fragments of mma.m16n8k16 (g = lane / 4, t = lane % 4; a register holds two
+// neighbouring columns of A, or rows of B):
+//   A: a0 (g, 2t), a1 (g+8, 2t), a2 (g, 2t+8), a3 (g+8, 2t+8)
+//   B: b0 (2t, g), b1 (2t+8, g);   C: c0,c1 (g, 2t), c2,c3 (g+8, 2t)
+// so the C fragments of two neighbouring 8-column tiles are, once packed, the
+// A fragment of a 16-deep step: products chain in registers.
+__device__ __forceinline__ void mma_bf16(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Both operands in the element type (their products are exact in fp32).
+template <class E>
+__device__ __forceinline__ void mma_elem(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same_v<E, BF16>) mma_bf16(c, a, b0, b1);
+  else mma_f16(c, a, b0, b1);
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t r[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t r[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void stsm4_t(uint32_t addr, const uint32_t r[4]) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+
+// An fp32 pair as bf16 high parts plus bf16 remainders: together 16 bits of
+// mantissa or more, so a product with an exact bf16 operand costs two matrix
+// instructions and is off by about 2^-18 of its size (against 2^-9 with the
+// high parts alone).
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = pack2_rn<BF16>(x, y);
+  lo = pack2_rn<BF16>(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
+}
+
+// A packed pair of elements as bf16 high parts and remainders: bf16 is itself;
+// fp16's 11 bits fit the two exactly.
+template <class E>
+__device__ __forceinline__ void split_elem(uint32_t v, uint32_t& hi, uint32_t& lo) {
+  if constexpr (std::is_same_v<E, BF16>) {
+    hi = v;
+    lo = 0;
+  } else {
+    float x, y;
+    unpack2<E>(v, x, y);
+    split2(x, y, hi, lo);
+  }
+}
+
+// The A fragment of step `ks` from the C fragments of tiles 2ks, 2ks+1, split.
+__device__ __forceinline__ void split_frag(const float c0[4], const float c1[4], uint32_t hi[4],
+                                           uint32_t lo[4]) {
+  split2(c0[0], c0[1], hi[0], lo[0]);
+  split2(c0[2], c0[3], hi[1], lo[1]);
+  split2(c1[0], c1[1], hi[2], lo[2]);
+  split2(c1[2], c1[3], hi[3], lo[3]);
+}
+
+// c += A B with A split and B exact in the element type.
+template <class E>
+__device__ __forceinline__ void mma_split_elem(float c[4], const uint32_t ah[4],
+                                               const uint32_t al[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same_v<E, BF16>) {
+    mma_bf16(c, ah, b0, b1);
+    mma_bf16(c, al, b0, b1);
+  } else {
+    uint32_t h0, l0, h1, l1;
+    split_elem<E>(b0, h0, l0);
+    split_elem<E>(b1, h1, l1);
+    mma_bf16(c, ah, h0, h1);
+    mma_bf16(c, al, h0, h1);
+    mma_bf16(c, ah, l0, l1);
+  }
+}
+// Both split (the product of the two remainders is below the others' rounding).
+__device__ __forceinline__ void mma_split(float c[4], const uint32_t ah[4], const uint32_t al[4],
+                                          uint32_t bh0, uint32_t bh1, uint32_t bl0, uint32_t bl1) {
+  mma_bf16(c, ah, bh0, bh1);
+  mma_bf16(c, al, bh0, bh1);
+  mma_bf16(c, ah, bl0, bl1);
+}
+
+// Addresses for ldmatrix.x4 over a row-major 16-bit tile with `ld` elements a
+// row (ld * 2 bytes an odd multiple of 16, so that 8 rows hit all banks).
+// B fragments of two 8-column tiles from a tile stored [n][k]:
+//   r0,r1 = b0,b1 of columns n0..n0+7, r2,r3 of n0+8..n0+15.
+__device__ __forceinline__ uint32_t addr_b(uint32_t base, int ld, int n0, int k0, int lane) {
+  return base + 2 * ((n0 + (lane & 7) + ((lane >> 4) << 3)) * ld + k0 + ((lane >> 3) & 1) * 8);
+}
+// The same from a tile stored [k][n] (with .trans).
+__device__ __forceinline__ uint32_t addr_bt(uint32_t base, int ld, int n0, int k0, int lane) {
+  return base + 2 * ((k0 + (lane & 7) + ((lane >> 3) & 1) * 8) * ld + n0 + ((lane >> 4) << 3));
+}
+// An A fragment from a tile stored [m][k].
+__device__ __forceinline__ uint32_t addr_a(uint32_t base, int ld, int m0, int k0, int lane) {
+  return base + 2 * ((m0 + (lane & 7) + ((lane >> 3) & 1) * 8) * ld + k0 + ((lane >> 4) << 3));
+}
+// An A fragment from a tile stored [k][m] (with .trans); as a store address
+// for stmatrix.trans: C fragments of two neighbouring tiles into [col][row].
+__device__ __forceinline__ uint32_t addr_at(uint32_t base, int ld, int m0, int k0, int lane) {
+  return base + 2 * ((k0 + (lane & 7) + ((lane >> 4) << 3)) * ld + m0 + ((lane >> 3) & 1) * 8);
+}
+
+}  // namespace tdc

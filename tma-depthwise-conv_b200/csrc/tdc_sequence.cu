@@ -1,0 +1,682 @@
+// tdc_sequence.cu — host half of the sequence operators: argument checks,
+// launch shapes and workspaces behind the C ABI of include/tdc_sequence.h.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <cstring>
+
+#include "tdc_sequence.h"
+#include "tdc_conv1d.cuh"
+#include "tdc_delta.cuh"
+#include "tdc_host.h"
+#include "tdc_qknorm.cuh"
+
+namespace {
+
+using tdc::host::cuda_fail;
+using tdc::host::prepare_device;
+
+constexpr int64_t kMaxDim = int64_t(1) << 40;
+
+bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
+bool bad_stride(int64_t s) { return s % 8 != 0; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+int launched() {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? TDC_OK : cuda_fail(int(e));
+}
+
+template <class K>
+int allow_smem(K kernel, size_t bytes) {
+  // Idempotent and cheap (no device work); kernels below 48 KB need none.
+  if (bytes <= 48 * 1024) return TDC_OK;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+  return e == cudaSuccess ? TDC_OK : cuda_fail(int(e));
+}
+
+// ---- causal depthwise convolution ---------------------------------------------
+int check_conv(int64_t B, int64_t T, int64_t C, int64_t K, int64_t dtype, int64_t act,
+               int64_t x_sb, int64_t x_st) {
+  if (dtype != TDC_F16 && dtype != TDC_BF16) return TDC_ERR_UNSUPPORTED;
+  if (act != TDC_ACT_NONE && act != TDC_ACT_SILU) return TDC_ERR_ACT;
+  if (B < 0 || T < 0 || C < 0) return TDC_ERR_BAD_SHAPE;
+  if (K < 2 || K > 8) return TDC_ERR_FILTER_SHAPE;
+  if (C % 8 != 0) return TDC_ERR_CHANNELS;
+  if (B > kMaxDim || T > kMaxDim || C > kMaxDim) return TDC_ERR_TOO_LARGE;
+  if (bad_stride(x_sb) || bad_stride(x_st)) return TDC_ERR_ALIGNMENT;
+  return TDC_OK;
+}
+
+int check_conv_args(const tdc_conv1d_args* a) {
+  if (a == nullptr) return TDC_ERR_NULL_POINTER;
+  const int rc = check_conv(a->B, a->T, a->C, a->K, a->dtype, a->act, a->x_sb, a->x_st);
+  if (rc != TDC_OK) return rc;
+  if (a->cu_seqlens != nullptr && (a->B != 1 || a->num_seqs < 1)) return TDC_ERR_BAD_SHAPE;
+  return TDC_OK;
+}
+
+tdc::Conv1dParams conv_params(const tdc_conv1d_args* a) {
+  tdc::Conv1dParams p;
+  std::memset(&p, 0, sizeof p);
+  p.x = a->x;
+  p.w = a->w;
+  p.bias = a->bias;
+  p.init = a->initial_state;
+  p.final_state = a->final_state;
+  p.y = a->y;
+  p.seq.cu = a->cu_seqlens;
+  p.seq.n = a->cu_seqlens != nullptr ? a->num_seqs : a->B;
+  p.seq.T = a->T;
+  p.seq.is64 = a->cu_is_64 != 0;
+  p.B = a->B;
+  p.T = a->T;
+  p.C = a->C;
+  p.x_sb = a->x_sb;
+  p.x_st = a->x_st;
+  return p;
+}
+
+template <class E, int K>
+int conv_fwd_k(const tdc::Conv1dParams& p, bool silu, int64_t blocks, cudaStream_t st) {
+  if (silu) tdc::conv1d_fwd_kernel<E, K, true><<<unsigned(blocks), 256, 0, st>>>(p);
+  else tdc::conv1d_fwd_kernel<E, K, false><<<unsigned(blocks), 256, 0, st>>>(p);
+  return launched();
+}
+
+// Backward launch shape: a block is LX vectors of channels by 256 / LX runs.
+struct ConvBwdPlan {
+  int vec, lx, run;
+  int64_t runs_per_b, groups, cblocks;
+};
+
+ConvBwdPlan conv_bwd_plan(const tdc_conv1d_args* a) {
+  ConvBwdPlan pl;
+  pl.vec = a->K <= 4 ? 8 : 4;  // beyond 4 taps 8 channels' windows no longer fit the registers
+  const int64_t vecs = a->C / pl.vec;
+  pl.lx = vecs >= 32 ? 32 : vecs >= 16 ? 16 : 8;
+  pl.cblocks = ceil_div(vecs, pl.lx);
+  // One wave of 2 blocks on each of 148 SMs; a run of at least 8 rows, or the
+  // K-1 rows that it recomputes behind its end would cost more than they save.
+  const int64_t lanes = 148 * 512;
+  const int64_t want = std::max<int64_t>(1, lanes / std::max<int64_t>(1, pl.cblocks * pl.lx));
+  const int64_t rows = std::max<int64_t>(1, a->B * a->T);
+  int64_t run = std::max<int64_t>(8, ceil_div(rows, want));
+  run = std::min(run, std::max<int64_t>(1, a->T));
+  pl.runs_per_b = ceil_div(std::max<int64_t>(1, a->T), run);
+  pl.run = int(std::min<int64_t>(ceil_div(std::max<int64_t>(1, a->T), pl.runs_per_b), 1 << 30));
+  pl.groups = std::max<int64_t>(1, ceil_div(a->B * pl.runs_per_b, 256 / pl.lx));
+  return pl;
+}
+
+template <class E, int K, bool SILU>
+int conv_bwd_t(const tdc::Conv1dParams& p, const ConvBwdPlan& pl, void* dw, void* dbias,
+               cudaStream_t st) {
+  constexpr int VEC = K <= 4 ? 8 : 4;
+  const dim3 block(pl.lx, 256 / pl.lx), grid(unsigned(pl.groups), unsigned(pl.cblocks));
+  const size_t smem = size_t(256) * VEC * sizeof(float);
+  tdc::conv1d_bwd_kernel<E, K, VEC, SILU><<<grid, block, smem, st>>>(p);
+  int rc = launched();
+  if (rc != TDC_OK) return rc;
+  const int64_t values = (K + 1) * p.C;
+  tdc::conv1d_wsum_kernel<E><<<unsigned(ceil_div(values, 32)), 256, 0, st>>>(p.partial, pl.groups, K,
+                                                                          p.C, dw, dbias);
+  rc = launched();
+  if (rc != TDC_OK || p.dinit == nullptr || p.seq.n == 0) return rc;
+  tdc::conv1d_dinit_kernel<E, K, SILU>
+      <<<unsigned(ceil_div(p.seq.n * (p.C / 4), 128)), 128, 0, st>>>(p);
+  return launched();
+}
+
+template <class E, int K>
+int conv_step_k(const tdc::Conv1dParams& p, bool silu, cudaStream_t st) {
+  const int threads = p.C / 8 >= 128 ? 128 : p.C / 8 > 32 ? 64 : 32;
+  const dim3 grid(unsigned(p.B), unsigned(ceil_div(p.C / 8, threads)));
+  if (silu) tdc::conv1d_step_kernel<E, K, true><<<grid, threads, 0, st>>>(p);
+  else tdc::conv1d_step_kernel<E, K, false><<<grid, threads, 0, st>>>(p);
+  return launched();
+}
+
+// f<E, K>(...) for a call's element type and number of taps.
+#define TDC_FOR_TAPS(E, K_, CALL)   \
+  switch (K_) {                     \
+    case 2: return CALL(E, 2);      \
+    case 3: return CALL(E, 3);      \
+    case 4: return CALL(E, 4);      \
+    case 5: return CALL(E, 5);      \
+    case 6: return CALL(E, 6);      \
+    case 7: return CALL(E, 7);      \
+    default: return CALL(E, 8);     \
+  }
+#define TDC_FOR_CONV(DTYPE, K_, CALL)                                        \
+  do {                                                                       \
+    if ((DTYPE) == TDC_BF16) { TDC_FOR_TAPS(tdc::BF16, K_, CALL) }           \
+    TDC_FOR_TAPS(tdc::F16, K_, CALL)                                         \
+  } while (0)
+
+int conv_fwd_any(const tdc::Conv1dParams& p, int64_t K, int64_t dtype, bool silu, int64_t blocks,
+                 cudaStream_t st) {
+#define TDC_CALL(E, K_) conv_fwd_k<E, K_>(p, silu, blocks, st)
+  TDC_FOR_CONV(dtype, K, TDC_CALL);
+#undef TDC_CALL
+}
+int conv_bwd_any(const tdc::Conv1dParams& p, const ConvBwdPlan& pl, int64_t K, int64_t dtype,
+                 bool silu, void* dw, void* db, cudaStream_t st) {
+#define TDC_CALL(E, K_) \
+  (silu ? conv_bwd_t<E, K_, true>(p, pl, dw, db, st) : conv_bwd_t<E, K_, false>(p, pl, dw, db, st))
+  TDC_FOR_CONV(dtype, K, TDC_CALL);
+#undef TDC_CALL
+}
+int conv_step_any(const tdc::Conv1dParams& p, int64_t K, int64_t dtype, bool silu, cudaStream_t st) {
+#define TDC_CALL(E, K_) conv_step_k<E, K_>(p, silu, st)
+  TDC_FOR_CONV(dtype, K, TDC_CALL);
+#undef TDC_CALL
+}
+
+// ---- norms and rotation -----------------------------------------------------------
+int check_qk(const tdc_qk_args* a) {
+  if (a == nullptr) return TDC_ERR_NULL_POINTER;
+  if (a->dtype != TDC_F16 && a->dtype != TDC_BF16) return TDC_ERR_UNSUPPORTED;
+  if (a->norm < TDC_NORM_NONE || a->norm > TDC_NORM_L2) return TDC_ERR_UNSUPPORTED;
+  if (a->B < 0 || a->T < 0 || a->Hq < 0 || a->Hk < 0) return TDC_ERR_BAD_SHAPE;
+  if (a->Hq > 65535 || a->Hk > 65535 || a->B > kMaxDim || a->T > kMaxDim) return TDC_ERR_TOO_LARGE;
+  if (a->T > 0 && a->B > ((int64_t(1) << 31) - 1) / a->T) return TDC_ERR_TOO_LARGE;
+  if (a->D < 8 || a->D > 256 || a->D % 8 != 0) return TDC_ERR_CHANNELS;
+  if (a->R < 0 || a->R > a->D || a->R % 16 != 0) return TDC_ERR_BAD_SHAPE;
+  if (a->R > 0) {
+    if (a->cos == nullptr || a->sin == nullptr) return TDC_ERR_NULL_POINTER;
+    if (a->table_rows < 0) return TDC_ERR_BAD_SHAPE;
+    if (misaligned(a->cos) || misaligned(a->sin)) return TDC_ERR_ALIGNMENT;
+  }
+  if (!(a->eps >= 0)) return TDC_ERR_BAD_SHAPE;
+  for (int64_t s : {a->q_sb, a->q_st, a->q_sh, a->k_sb, a->k_st, a->k_sh})
+    if (bad_stride(s)) return TDC_ERR_ALIGNMENT;
+  if ((a->Hq > 0 && misaligned(a->q)) || (a->Hk > 0 && misaligned(a->k)) ||
+      misaligned(a->q_weight) || misaligned(a->k_weight))
+    return TDC_ERR_ALIGNMENT;
+  return TDC_OK;
+}
+
+tdc::QkParams qk_params(const tdc_qk_args* a) {
+  tdc::QkParams p;
+  std::memset(&p, 0, sizeof p);
+  p.q = a->q, p.k = a->k, p.qw = a->q_weight, p.kw = a->k_weight;
+  p.cos = a->cos, p.sin = a->sin, p.pos = a->positions;
+  p.qo = a->q_out, p.ko = a->k_out;
+  p.T = a->T;
+  p.Hq = int(a->Hq), p.Hk = int(a->Hk), p.D = int(a->D), p.R = int(a->R);
+  p.q_sb = a->q_sb, p.q_st = a->q_st, p.q_sh = a->q_sh;
+  p.k_sb = a->k_sb, p.k_st = a->k_st, p.k_sh = a->k_sh;
+  p.p_sb = a->p_sb, p.p_st = a->p_st;
+  p.table_rows = a->table_rows;
+  p.rows = a->B * a->T;
+  p.pos64 = a->positions_are_64 != 0;
+  p.interleaved = a->interleaved != 0;
+  p.norm = int(a->norm);
+  p.eps = float(a->eps);
+  return p;
+}
+
+int qk_lanes(int64_t D) { return D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32; }
+
+int qk_threads(const tdc_qk_args* a) {
+  const int64_t want = (a->Hq + a->Hk) * qk_lanes(a->D);
+  return int(std::min<int64_t>(256, ceil_div(want, 32) * 32));
+}
+
+// Blocks of the gradient kernel: 4 on each of 148 SMs, or one for each row.
+int64_t qk_bwd_rows(const tdc_qk_args* a) {
+  return std::max<int64_t>(1, ceil_div(a->B * a->T, 148 * 4));
+}
+int64_t qk_bwd_blocks(const tdc_qk_args* a) { return ceil_div(a->B * a->T, qk_bwd_rows(a)); }
+
+template <class E>
+int qk_fwd_e(const tdc::QkParams& p, int threads, cudaStream_t st) {
+  const unsigned grid = unsigned(p.rows);
+  switch (qk_lanes(p.D)) {
+    case 4: tdc::qk_norm_rope_kernel<E, 4><<<grid, threads, 0, st>>>(p); break;
+    case 8: tdc::qk_norm_rope_kernel<E, 8><<<grid, threads, 0, st>>>(p); break;
+    case 16: tdc::qk_norm_rope_kernel<E, 16><<<grid, threads, 0, st>>>(p); break;
+    default: tdc::qk_norm_rope_kernel<E, 32><<<grid, threads, 0, st>>>(p); break;
+  }
+  return launched();
+}
+
+template <class E>
+int qk_bwd_e(const tdc::QkParams& p, int threads, int64_t blocks, void* dqw, void* dkw,
+             cudaStream_t st) {
+  const unsigned grid = unsigned(blocks);
+  switch (qk_lanes(p.D)) {
+    case 4: tdc::qk_norm_rope_bwd_kernel<E, 4><<<grid, threads, 0, st>>>(p); break;
+    case 8: tdc::qk_norm_rope_bwd_kernel<E, 8><<<grid, threads, 0, st>>>(p); break;
+    case 16: tdc::qk_norm_rope_bwd_kernel<E, 16><<<grid, threads, 0, st>>>(p); break;
+    default: tdc::qk_norm_rope_bwd_kernel<E, 32><<<grid, threads, 0, st>>>(p); break;
+  }
+  const int rc = launched();
+  if (rc != TDC_OK || p.partial == nullptr) return rc;
+  tdc::qk_wsum_kernel<E><<<unsigned(ceil_div(2 * p.D, 8)), 256, 0, st>>>(p.partial, blocks, p.D, dqw,
+                                                                         dkw);
+  return launched();
+}
+
+// ---- gated delta rule -------------------------------------------------------------
+int check_delta(const tdc_delta_args* a) {
+  if (a == nullptr) return TDC_ERR_NULL_POINTER;
+  if (a->dtype != TDC_F16 && a->dtype != TDC_BF16) return TDC_ERR_UNSUPPORTED;
+  if (a->B < 0 || a->T < 0 || a->H < 1 || a->HV < 1 || a->HV % a->H != 0) return TDC_ERR_BAD_SHAPE;
+  if (a->K != 64 && a->K != 128) return TDC_ERR_CHANNELS;
+  if (a->V != 64 && a->V != 128 && a->V != 256) return TDC_ERR_CHANNELS;
+  if (a->HV > 65535 || a->B > (int64_t(1) << 24) || a->T > (int64_t(1) << 36))
+    return TDC_ERR_TOO_LARGE;
+  if (a->cu_seqlens != nullptr && (a->B != 1 || a->num_seqs < 1)) return TDC_ERR_BAD_SHAPE;
+  if (a->num_seqs > (int64_t(1) << 24)) return TDC_ERR_TOO_LARGE;
+  for (int64_t s : {a->q_sb, a->q_st, a->q_sh, a->k_sb, a->k_st, a->k_sh, a->v_sb, a->v_st, a->v_sh})
+    if (bad_stride(s)) return TDC_ERR_ALIGNMENT;
+  if (misaligned(a->q) || misaligned(a->k) || misaligned(a->v)) return TDC_ERR_ALIGNMENT;
+  return TDC_OK;
+}
+
+int64_t delta_seqs(const tdc_delta_args* a) { return a->cu_seqlens != nullptr ? a->num_seqs : a->B; }
+int64_t delta_chunks(const tdc_delta_args* a) {
+  return a->cu_seqlens != nullptr ? a->T / tdc::kChunk + a->num_seqs
+                                  : a->B * ceil_div(a->T, tdc::kChunk);
+}
+
+// Lays the workspace out (base may be null: only the size is wanted).
+int64_t delta_layout(const tdc_delta_args* a, bool grads, unsigned char* base, tdc::DeltaParams* p) {
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    unsigned char* r = base + at;
+    at += ceil_div(bytes, 256) * 256;
+    return r;
+  };
+  const int64_t slots = delta_chunks(a) * a->HV;
+  unsigned char* plan = take(2 * (delta_seqs(a) + 1) * 8);
+  unsigned char* tm = take(slots * 2 * tdc::kSq * 2);
+  unsigned char* pm = take(slots * 2 * tdc::kSq * 2);
+  unsigned char* coef = take(slots * 3 * tdc::kChunk * 4);
+  unsigned char *um = nullptr, *xm = nullptr, *sm = nullptr, *dm = nullptr;
+  if (grads) {
+    um = take(slots * 2 * a->V * tdc::kChunk * 2);
+    xm = take(slots * 2 * a->V * tdc::kChunk * 2);
+    sm = take(slots * 2 * a->V * a->K * 2);
+    dm = take(slots * 2 * a->V * a->K * 2);
+  }
+  if (p != nullptr) {
+    p->seq_lo = reinterpret_cast<int64_t*>(plan);
+    p->seq_chunk = p->seq_lo + delta_seqs(a) + 1;
+    p->tm = reinterpret_cast<__nv_bfloat16*>(tm);
+    p->pm = reinterpret_cast<__nv_bfloat16*>(pm);
+    p->coef = reinterpret_cast<float*>(coef);
+    p->um = reinterpret_cast<__nv_bfloat16*>(um);
+    p->xm = reinterpret_cast<__nv_bfloat16*>(xm);
+    p->sm = reinterpret_cast<__nv_bfloat16*>(sm);
+    p->dm = reinterpret_cast<__nv_bfloat16*>(dm);
+  }
+  return at;
+}
+
+tdc::DeltaParams delta_params(const tdc_delta_args* a) {
+  tdc::DeltaParams p;
+  std::memset(&p, 0, sizeof p);
+  p.q = a->q, p.k = a->k, p.v = a->v, p.beta = a->beta, p.g = a->g;
+  p.init = a->initial_state, p.final_state = a->final_state, p.o = a->o;
+  p.T = a->T;
+  p.H = int(a->H), p.HV = int(a->HV), p.V = int(a->V), p.group = int(a->HV / a->H);
+  p.q_sb = a->q_sb, p.q_st = a->q_st, p.q_sh = a->q_sh;
+  p.k_sb = a->k_sb, p.k_st = a->k_st, p.k_sh = a->k_sh;
+  p.v_sb = a->v_sb, p.v_st = a->v_st, p.v_sh = a->v_sh;
+  p.g_sb = a->g_sb, p.g_st = a->g_st, p.b_sb = a->b_sb, p.b_st = a->b_st;
+  p.seq.cu = a->cu_seqlens;
+  p.seq.n = delta_seqs(a);
+  p.seq.T = a->T;
+  p.seq.is64 = a->cu_is_64 != 0;
+  p.chunks_per_b = ceil_div(a->T, tdc::kChunk);
+  p.max_chunks = delta_chunks(a);
+  p.beta_f32 = a->beta_is_f32 != 0;
+  p.scale = float(a->scale);
+  return p;
+}
+
+// Warps a block of the walk: as many as still leave a block for every SM, so
+// that K, Q, T and P are fetched for as many value channels as possible; few
+// sequences and heads take small blocks.
+int delta_warps(const tdc_delta_args* a) {
+  const int64_t walks = delta_seqs(a) * a->HV;
+  for (int w : {8, 4})
+    if (a->V % (16 * w) == 0 && walks * (a->V / (16 * w)) >= 148) return w;
+  return 2;
+}
+
+int delta_plan(const tdc::DeltaParams& p, const tdc::ZeroRows& z, cudaStream_t st) {
+  if (p.seq.cu == nullptr) return TDC_OK;
+  tdc::delta_plan_kernel<<<33, 1024, 0, st>>>(p.seq, p.seq_lo, p.seq_chunk, z);
+  return launched();
+}
+
+template <class E, int DK>
+int delta_prepare(const tdc::DeltaParams& p, cudaStream_t st) {
+  if (p.max_chunks == 0) return TDC_OK;
+  auto* k = &tdc::delta_prepare_kernel<E, DK>;
+  const size_t smem = tdc::prepare_smem<DK>();
+  const int rc = allow_smem(k, smem);
+  if (rc != TDC_OK) return rc;
+  k<<<dim3(unsigned(p.max_chunks), unsigned(p.H)), 128, smem, st>>>(p);
+  return launched();
+}
+
+template <class E, int DK, int W, int MODE>
+int delta_scan_w(const tdc::DeltaParams& p, cudaStream_t st) {
+  if (p.seq.n == 0) return TDC_OK;
+  auto* k = &tdc::delta_scan_kernel<E, DK, W, MODE>;
+  const size_t smem = 2 * tdc::ScanStage<DK, W>::bytes;
+  const int rc = allow_smem(k, smem);
+  if (rc != TDC_OK) return rc;
+  k<<<dim3(unsigned(p.seq.n * (p.V / (16 * W))), unsigned(p.HV)), 32 * W, smem, st>>>(p);
+  return launched();
+}
+template <class E, int DK, int W>
+int delta_back_w(const tdc::DeltaParams& p, cudaStream_t st) {
+  if (p.seq.n == 0) return TDC_OK;
+  auto* k = &tdc::delta_scan_back_kernel<E, DK, W>;
+  const size_t smem = 2 * tdc::ScanStage<DK, W>::bytes;
+  const int rc = allow_smem(k, smem);
+  if (rc != TDC_OK) return rc;
+  k<<<dim3(unsigned(p.seq.n * (p.V / (16 * W))), unsigned(p.HV)), 32 * W, smem, st>>>(p);
+  return launched();
+}
+
+template <class E, int DK, int MODE>
+int delta_scan(const tdc::DeltaParams& p, int w, cudaStream_t st) {
+  return w == 8   ? delta_scan_w<E, DK, 8, MODE>(p, st)
+         : w == 4 ? delta_scan_w<E, DK, 4, MODE>(p, st)
+                  : delta_scan_w<E, DK, 2, MODE>(p, st);
+}
+
+template <class E, int DK>
+int delta_fwd_t(const tdc::DeltaParams& p, int w, cudaStream_t st) {
+  int rc = delta_prepare<E, DK>(p, st);
+  if (rc == TDC_OK) rc = delta_scan<E, DK, 0>(p, w, st);
+  return rc;
+}
+
+template <class E, int DK>
+int delta_bwd_t(const tdc::DeltaParams& p, int w, cudaStream_t st) {
+  int rc = delta_prepare<E, DK>(p, st);
+  if (rc == TDC_OK) rc = delta_scan<E, DK, 1>(p, w, st);
+  if (rc == TDC_OK)
+    rc = w == 8   ? delta_back_w<E, DK, 8>(p, st)
+         : w == 4 ? delta_back_w<E, DK, 4>(p, st)
+                  : delta_back_w<E, DK, 2>(p, st);
+  if (rc != TDC_OK || p.max_chunks == 0) return rc;
+  auto* k = &tdc::delta_grad_kernel<E, DK>;
+  const size_t smem = tdc::GradSmem<DK>::bytes;
+  rc = allow_smem(k, smem);
+  if (rc != TDC_OK) return rc;
+  k<<<dim3(unsigned(p.max_chunks), unsigned(p.H)), 256, smem, st>>>(p);
+  return launched();
+}
+
+template <class E, int DK>
+int delta_step_t(const tdc::DeltaParams& p, int64_t B, float* state, int64_t slots, const void* idx,
+                 bool idx64, cudaStream_t st) {
+  tdc::delta_step_kernel<E, DK>
+      <<<dim3(unsigned(B), unsigned(p.HV), unsigned(p.V / 32)), 128, 0, st>>>(p, state, idx, idx64,
+                                                                             slots);
+  return launched();
+}
+
+}  // namespace
+
+extern "C" {
+
+TDC_API int tdc_conv1d_fwd(const tdc_conv1d_args* a, void* stream) {
+  int rc = check_conv_args(a);
+  if (rc != TDC_OK) return rc;
+  tdc::Conv1dParams p = conv_params(a);
+  const int64_t vecs = a->C / 8;
+  const bool rows = a->B > 0 && a->T > 0;
+  if (vecs == 0 || (!rows && (a->final_state == nullptr || p.seq.n == 0))) return TDC_OK;
+  if ((rows && (a->x == nullptr || a->w == nullptr || a->y == nullptr))) return TDC_ERR_NULL_POINTER;
+  if (misaligned(a->x) || misaligned(a->w) || misaligned(a->y) || misaligned(a->bias) ||
+      misaligned(a->initial_state) || misaligned(a->final_state))
+    return TDC_ERR_ALIGNMENT;
+  // A run of up to 16 rows a thread (it reads K-1 rows more than it writes);
+  // shorter runs while 148 SMs would not get 1024 threads each.
+  p.run = 16;
+  while (p.run > 1 && vecs * a->B * ceil_div(a->T, p.run) < 148 * 1024) p.run /= 2;
+  p.runs_per_b = ceil_div(a->T, p.run);
+  p.main_threads = a->B * p.runs_per_b * vecs;
+  const int64_t tail = a->final_state != nullptr ? p.seq.n * (a->K - 1) * vecs : 0;
+  const int64_t blocks = ceil_div(p.main_threads + tail, 256);
+  if (blocks > 0x7fffffff) return TDC_ERR_TOO_LARGE;
+  rc = prepare_device();
+  if (rc != TDC_OK) return rc;
+  return conv_fwd_any(p, a->K, a->dtype, a->act == TDC_ACT_SILU, blocks,
+                      static_cast<cudaStream_t>(stream));
+}
+
+TDC_API int64_t tdc_conv1d_bwd_workspace(const tdc_conv1d_args* a) {
+  const int rc = check_conv_args(a);
+  if (rc != TDC_OK) return rc;
+  return std::max<int64_t>(16, conv_bwd_plan(a).groups * (a->K + 1) * a->C * 4);
+}
+
+TDC_API int tdc_conv1d_bwd(const tdc_conv1d_args* a, const void* dy, int64_t dy_sb, int64_t dy_st,
+                           const void* dfinal, void* dx, void* dw, void* dbias, void* dinitial,
+                           void* workspace, int64_t workspace_bytes, void* stream) {
+  int rc = check_conv_args(a);
+  if (rc != TDC_OK) return rc;
+  if (a->C == 0) return TDC_OK;
+  if (a->w == nullptr || dw == nullptr || workspace == nullptr) return TDC_ERR_NULL_POINTER;
+  if (a->B * a->T > 0 && (a->x == nullptr || dy == nullptr || dx == nullptr))
+    return TDC_ERR_NULL_POINTER;
+  if (a->bias != nullptr && dbias == nullptr) return TDC_ERR_NULL_POINTER;
+  if (workspace_bytes < tdc_conv1d_bwd_workspace(a)) return TDC_ERR_WORKSPACE;
+  if (bad_stride(dy_sb) || bad_stride(dy_st)) return TDC_ERR_ALIGNMENT;
+  for (const void* q : {a->x, a->w, a->bias, a->initial_state, dy, dfinal,
+                        static_cast<const void*>(dx), static_cast<const void*>(dinitial),
+                        static_cast<const void*>(workspace)})
+    if (misaligned(q)) return TDC_ERR_ALIGNMENT;
+  const ConvBwdPlan pl = conv_bwd_plan(a);
+  if (pl.groups > 0x7fffffff || pl.cblocks > 65535) return TDC_ERR_TOO_LARGE;
+  tdc::Conv1dParams p = conv_params(a);
+  p.run = pl.run;
+  p.runs_per_b = pl.runs_per_b;
+  if (a->T == 0) p.B = 0;  // no rows: only zero weight gradients and the states'
+  p.dy = dy, p.dy_sb = dy_sb, p.dy_st = dy_st;
+  p.dfinal = dfinal, p.dx = dx, p.dinit = dinitial;
+  p.partial = static_cast<float*>(workspace);
+  p.groups = pl.groups;
+  rc = prepare_device();
+  if (rc != TDC_OK) return rc;
+  return conv_bwd_any(p, pl, a->K, a->dtype, a->act == TDC_ACT_SILU, dw,
+                      a->bias != nullptr ? dbias : nullptr, static_cast<cudaStream_t>(stream));
+}
+
+TDC_API int tdc_conv1d_step(const tdc_conv1d_step_args* a, void* stream) {
+  if (a == nullptr) return TDC_ERR_NULL_POINTER;
+  int rc = check_conv(a->B, a->T, a->C, a->K, a->dtype, a->act, a->x_sb, a->x_st);
+  if (rc != TDC_OK) return rc;
+  if (a->slots < 0) return TDC_ERR_BAD_SHAPE;
+  if (a->B == 0 || a->T == 0 || a->C == 0) return TDC_OK;
+  if (a->B > 0x7fffffff || a->C > 65535 * 256) return TDC_ERR_TOO_LARGE;
+  if (a->x == nullptr || a->w == nullptr || a->y == nullptr ||
+      (a->state == nullptr && a->slots > 0))
+    return TDC_ERR_NULL_POINTER;
+  for (const void* q : {a->x, a->w, a->bias, static_cast<const void*>(a->state),
+                        static_cast<const void*>(a->y)})
+    if (misaligned(q)) return TDC_ERR_ALIGNMENT;
+  tdc::Conv1dParams p;
+  std::memset(&p, 0, sizeof p);
+  p.x = a->x, p.w = a->w, p.bias = a->bias, p.y = a->y;
+  p.B = a->B, p.T = a->T, p.C = a->C, p.x_sb = a->x_sb, p.x_st = a->x_st;
+  p.state = a->state, p.idx = a->state_indices, p.slots = a->slots;
+  p.idx64 = a->indices_are_64 != 0;
+  rc = prepare_device();
+  if (rc != TDC_OK) return rc;
+  return conv_step_any(p, a->K, a->dtype, a->act == TDC_ACT_SILU, static_cast<cudaStream_t>(stream));
+}
+
+TDC_API int tdc_qk_norm_rope(const tdc_qk_args* a, void* stream) {
+  int rc = check_qk(a);
+  if (rc != TDC_OK) return rc;
+  if (a->B * a->T == 0 || a->Hq + a->Hk == 0) return TDC_OK;
+  if ((a->Hq > 0 && (a->q == nullptr || a->q_out == nullptr)) ||
+      (a->Hk > 0 && (a->k == nullptr || a->k_out == nullptr)))
+    return TDC_ERR_NULL_POINTER;
+  if (misaligned(a->q_out) || misaligned(a->k_out)) return TDC_ERR_ALIGNMENT;
+  rc = prepare_device();
+  if (rc != TDC_OK) return rc;
+  const tdc::QkParams p = qk_params(a);
+  auto st = static_cast<cudaStream_t>(stream);
+  return a->dtype == TDC_BF16 ? qk_fwd_e<tdc::BF16>(p, qk_threads(a), st)
+                              : qk_fwd_e<tdc::F16>(p, qk_threads(a), st);
+}
+
+TDC_API int64_t tdc_qk_norm_rope_bwd_workspace(const tdc_qk_args* a) {
+  const int rc = check_qk(a);
+  if (rc != TDC_OK) return rc;
+  return std::max<int64_t>(16, qk_bwd_blocks(a) * 2 * a->D * 4);
+}
+
+TDC_API int tdc_qk_norm_rope_bwd(const tdc_qk_args* a, const tdc_qk_grad_args* g, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
+  int rc = check_qk(a);
+  if (rc != TDC_OK) return rc;
+  if (g == nullptr) return TDC_ERR_NULL_POINTER;
+  const bool weights = a->q_weight != nullptr || a->k_weight != nullptr;
+  if ((a->q_weight != nullptr && g->dq_weight == nullptr) ||
+      (a->k_weight != nullptr && g->dk_weight == nullptr))
+    return TDC_ERR_NULL_POINTER;
+  if (weights && workspace == nullptr) return TDC_ERR_NULL_POINTER;
+  if (weights && workspace_bytes < tdc_qk_norm_rope_bwd_workspace(a)) return TDC_ERR_WORKSPACE;
+  const bool rows = a->B * a->T > 0 && a->Hq + a->Hk > 0;
+  if (!rows && !weights) return TDC_OK;
+  if (rows && ((a->Hq > 0 && (a->q == nullptr || g->dq == nullptr || g->dq_out == nullptr)) ||
+               (a->Hk > 0 && (a->k == nullptr || g->dk == nullptr || g->dk_out == nullptr))))
+    return TDC_ERR_NULL_POINTER;
+  for (int64_t s : {g->gq_sb, g->gq_st, g->gq_sh, g->gk_sb, g->gk_st, g->gk_sh})
+    if (bad_stride(s)) return TDC_ERR_ALIGNMENT;
+  for (const void* q : {g->dq_out, g->dk_out, static_cast<const void*>(g->dq),
+                        static_cast<const void*>(g->dk)})
+    if (misaligned(q)) return TDC_ERR_ALIGNMENT;
+  rc = prepare_device();
+  if (rc != TDC_OK) return rc;
+  tdc::QkParams p = qk_params(a);
+  p.gq = g->dq_out, p.gk = g->dk_out, p.dq = g->dq, p.dk = g->dk;
+  p.gq_sb = g->gq_sb, p.gq_st = g->gq_st, p.gq_sh = g->gq_sh;
+  p.gk_sb = g->gk_sb, p.gk_st = g->gk_st, p.gk_sh = g->gk_sh;
+  p.partial = weights ? static_cast<float*>(workspace) : nullptr;
+  p.rows_per_block = int(std::min<int64_t>(qk_bwd_rows(a), 0x7fffffff));
+  auto st = static_cast<cudaStream_t>(stream);
+  const int64_t blocks = std::max<int64_t>(1, qk_bwd_blocks(a));  // no rows: zero weight gradients
+  return a->dtype == TDC_BF16
+             ? qk_bwd_e<tdc::BF16>(p, qk_threads(a), blocks, g->dq_weight, g->dk_weight, st)
+             : qk_bwd_e<tdc::F16>(p, qk_threads(a), blocks, g->dq_weight, g->dk_weight, st);
+}
+
+TDC_API int64_t tdc_delta_fwd_workspace(const tdc_delta_args* a) {
+  const int rc = check_delta(a);
+  return rc != TDC_OK ? rc : delta_layout(a, false, nullptr, nullptr);
+}
+
+TDC_API int64_t tdc_delta_bwd_workspace(const tdc_delta_args* a) {
+  const int rc = check_delta(a);
+  return rc != TDC_OK ? rc : delta_layout(a, true, nullptr, nullptr);
+}
+
+TDC_API int tdc_delta_fwd(const tdc_delta_args* a, void* workspace, int64_t workspace_bytes,
+                          void* stream) {
+  int rc = check_delta(a);
+  if (rc != TDC_OK) return rc;
+  if (workspace == nullptr) return TDC_ERR_NULL_POINTER;
+  if (workspace_bytes < tdc_delta_fwd_workspace(a)) return TDC_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return TDC_ERR_ALIGNMENT;
+  if (a->B * a->T > 0 && (a->q == nullptr || a->k == nullptr || a->v == nullptr ||
+                          a->g == nullptr || a->beta == nullptr || a->o == nullptr))
+    return TDC_ERR_NULL_POINTER;
+  if (misaligned(a->o) || misaligned(a->initial_state) || misaligned(a->final_state))
+    return TDC_ERR_ALIGNMENT;
+  rc = prepare_device();
+  if (rc != TDC_OK) return rc;
+  tdc::DeltaParams p = delta_params(a);
+  delta_layout(a, false, static_cast<unsigned char*>(workspace), &p);
+  if (p.max_chunks > 0x7fffffff) return TDC_ERR_TOO_LARGE;
+  auto st = static_cast<cudaStream_t>(stream);
+  tdc::ZeroRows z = {};
+  z.base[0] = a->o, z.row_bytes[0] = a->HV * a->V * 2;
+  rc = delta_plan(p, z, st);
+  if (rc != TDC_OK) return rc;
+  const int w = delta_warps(a);
+  if (a->dtype == TDC_BF16)
+    return a->K == 128 ? delta_fwd_t<tdc::BF16, 128>(p, w, st) : delta_fwd_t<tdc::BF16, 64>(p, w, st);
+  return a->K == 128 ? delta_fwd_t<tdc::F16, 128>(p, w, st) : delta_fwd_t<tdc::F16, 64>(p, w, st);
+}
+
+TDC_API int tdc_delta_bwd(const tdc_delta_args* a, const tdc_delta_grad_args* g, void* workspace,
+                          int64_t workspace_bytes, void* stream) {
+  int rc = check_delta(a);
+  if (rc != TDC_OK) return rc;
+  if (g == nullptr || workspace == nullptr) return TDC_ERR_NULL_POINTER;
+  if (workspace_bytes < tdc_delta_bwd_workspace(a)) return TDC_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return TDC_ERR_ALIGNMENT;
+  if (a->B * a->T > 0 &&
+      (a->q == nullptr || a->k == nullptr || a->v == nullptr || a->g == nullptr ||
+       a->beta == nullptr || g->d_o == nullptr || g->dq == nullptr || g->dk == nullptr ||
+       g->dv == nullptr || g->dg == nullptr || g->dbeta == nullptr))
+    return TDC_ERR_NULL_POINTER;
+  for (int64_t s : {g->do_sb, g->do_st, g->do_sh})
+    if (bad_stride(s)) return TDC_ERR_ALIGNMENT;
+  for (const void* q : {g->d_o, static_cast<const void*>(g->dq), static_cast<const void*>(g->dk),
+                        static_cast<const void*>(g->dv)})
+    if (misaligned(q)) return TDC_ERR_ALIGNMENT;
+  rc = prepare_device();
+  if (rc != TDC_OK) return rc;
+  tdc::DeltaParams p = delta_params(a);
+  delta_layout(a, true, static_cast<unsigned char*>(workspace), &p);
+  if (p.max_chunks > 0x7fffffff) return TDC_ERR_TOO_LARGE;
+  p.d_o = g->d_o;
+  p.do_sb = g->do_sb, p.do_st = g->do_st, p.do_sh = g->do_sh;
+  p.dfinal = g->dfinal, p.dq = g->dq, p.dk = g->dk, p.dv = g->dv;
+  p.dg = g->dg, p.dbeta = g->dbeta, p.dinit = g->dinitial;
+  auto st = static_cast<cudaStream_t>(stream);
+  tdc::ZeroRows z = {};
+  z.base[0] = g->dq, z.row_bytes[0] = a->H * a->K * 2;
+  z.base[1] = g->dk, z.row_bytes[1] = a->H * a->K * 2;
+  z.base[2] = g->dv, z.row_bytes[2] = a->HV * a->V * 2;
+  z.base[3] = g->dg, z.row_bytes[3] = a->HV * 4;
+  z.base[4] = g->dbeta, z.row_bytes[4] = a->HV * (a->beta_is_f32 ? 4 : 2);
+  rc = delta_plan(p, z, st);
+  if (rc != TDC_OK) return rc;
+  const int w = delta_warps(a);
+  if (a->dtype == TDC_BF16)
+    return a->K == 128 ? delta_bwd_t<tdc::BF16, 128>(p, w, st) : delta_bwd_t<tdc::BF16, 64>(p, w, st);
+  return a->K == 128 ? delta_bwd_t<tdc::F16, 128>(p, w, st) : delta_bwd_t<tdc::F16, 64>(p, w, st);
+}
+
+TDC_API int tdc_delta_step(const tdc_delta_args* a, float* state, int64_t slots,
+                           const void* state_indices, int64_t indices_are_64, void* stream) {
+  int rc = check_delta(a);
+  if (rc != TDC_OK) return rc;
+  if (slots < 0) return TDC_ERR_BAD_SHAPE;
+  if (a->B == 0 || a->T == 0) return TDC_OK;
+  if (a->q == nullptr || a->k == nullptr || a->v == nullptr || a->g == nullptr ||
+      a->beta == nullptr || a->o == nullptr || (state == nullptr && slots > 0))
+    return TDC_ERR_NULL_POINTER;
+  if (misaligned(a->o) || misaligned(state)) return TDC_ERR_ALIGNMENT;
+  rc = prepare_device();
+  if (rc != TDC_OK) return rc;
+  tdc::DeltaParams p = delta_params(a);
+  auto st = static_cast<cudaStream_t>(stream);
+  const bool i64 = indices_are_64 != 0;
+  if (a->dtype == TDC_BF16)
+    return a->K == 128 ? delta_step_t<tdc::BF16, 128>(p, a->B, state, slots, state_indices, i64, st)
+                       : delta_step_t<tdc::BF16, 64>(p, a->B, state, slots, state_indices, i64, st);
+  return a->K == 128 ? delta_step_t<tdc::F16, 128>(p, a->B, state, slots, state_indices, i64, st)
+                     : delta_step_t<tdc::F16, 64>(p, a->B, state, slots, state_indices, i64, st);
+}
+
+}  // extern "C"

@@ -2,9 +2,10 @@
 
   libtdc_sm100.so                 nvcc, -gencode arch=compute_100a,code=sm_100a:
                                   the kernels + the C ABI of include/tdc_dwconv.h
+                                  and include/tdc_sequence.h, one object a source
                                   (static cudart, no libcuda link: the TMA encoder
                                   is fetched with cudaGetDriverEntryPoint)
-  _tma_dwconv_C<EXT_SUFFIX>       g++: the PyTorch extension (csrc/bindings.cpp),
+  _tma_dwconv_C<EXT_SUFFIX>       g++: the PyTorch extension (csrc/bindings*.cpp),
                                   linked to libtdc_sm100.so through rpath $ORIGIN
 
 Both land next to this file, so the directory is importable as-is
@@ -17,6 +18,7 @@ import os
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(HERE)
@@ -46,9 +48,19 @@ def _run(cmd: list[str]) -> str:
     return r.stdout + r.stderr
 
 
+#: The library's translation units with the headers each is built from.
+UNITS = {
+    "tdc_capi.cu": ["tdc_dgrad_s2.cuh", "tdc_host.h", "tdc_kernels.cuh", "tdc_plain.cuh",
+                    "tdc_ptx.cuh", "tdc_wgrad.cuh"],
+    "tdc_sequence.cu": ["tdc_conv1d.cuh", "tdc_delta.cuh", "tdc_host.h", "tdc_ptx.cuh",
+                        "tdc_qknorm.cuh", "tdc_seq_common.cuh"],
+}
+EXT_SOURCES = ("bindings.cpp", "bindings_sequence.cpp")
+
+
 def _deps(*names: str) -> list[str]:
-    hdrs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
-    return [os.path.join(CSRC, n) for n in names] + hdrs + [os.path.join(INCLUDE, "tdc_dwconv.h")]
+    return ([os.path.join(CSRC, n) for n in names]
+            + [os.path.join(INCLUDE, h) for h in ("tdc_dwconv.h", "tdc_sequence.h")])
 
 
 def _tmp(path: str) -> str:
@@ -58,35 +70,56 @@ def _tmp(path: str) -> str:
     return os.path.join(d, f".{f}.{os.getpid()}.tmp")
 
 
+def _build_unit(nvcc: str, name: str, force: bool) -> str:
+    """Object file of one .cu source, with its ptxas report beside it."""
+    obj = os.path.join(HERE, name.replace(".cu", ".o"))
+    if force or _stale(obj, _deps(name, *UNITS[name])):
+        tmp = _tmp(obj)
+        out = _run([nvcc, *NVCC_FLAGS, "-c", f"-I{INCLUDE}", f"-I{CSRC}",
+                    os.path.join(CSRC, name), "-o", tmp])
+        os.replace(tmp, obj)
+        with open(obj.replace(".o", ".ptxas.txt"), "w") as f:
+            f.write("\n".join(l for l in out.splitlines() if "ptxas" in l or "spill" in l) + "\n")
+    return obj
+
+
 def build_lib(force: bool = False) -> str:
-    deps = _deps("tdc_capi.cu")
+    deps = _deps(*UNITS, *{h for hs in UNITS.values() for h in hs})
     if force or _stale(LIB, deps):
         nvcc = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "bin", "nvcc")
+        with ThreadPoolExecutor(len(UNITS)) as pool:  # one nvcc process for each source
+            objs = list(pool.map(lambda n: _build_unit(nvcc, n, force), UNITS))
         tmp = _tmp(LIB)
-        out = _run([nvcc, *NVCC_FLAGS, "-shared", f"-I{INCLUDE}", f"-I{CSRC}",
-                    os.path.join(CSRC, "tdc_capi.cu"), "-o", tmp])
+        _run([nvcc, *NVCC_FLAGS[:2], "-shared", *objs, "-o", tmp])
         os.replace(tmp, LIB)
-        with open(os.path.join(HERE, "libtdc_sm100.ptxas.txt"), "w") as f:
-            f.write("\n".join(l for l in out.splitlines() if "ptxas" in l or "spill" in l) + "\n")
     return LIB
 
 
 def build_ext(force: bool = False) -> str:
-    deps = _deps("bindings.cpp") + [LIB]
+    deps = _deps(*EXT_SOURCES, "bindings_common.h") + [LIB]
     if force or _stale(EXT, deps):
         import torch
         import torch.utils.cpp_extension as ce
         incs = ce.include_paths("cuda") + [sysconfig.get_paths()["include"], INCLUDE]
         libdirs = ce.library_paths("cuda")
-        cmd = ["g++", "-shared", "-fPIC", "-O2", "-std=c++17",
-               "-DTORCH_EXTENSION_NAME=_tma_dwconv_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
-               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-               *[f"-I{i}" for i in incs], os.path.join(CSRC, "bindings.cpp"), "-o", _tmp(EXT),
-               f"-L{HERE}", "-ltdc_sm100", "-Wl,-rpath,$ORIGIN",
-               *[f"-L{d}" for d in libdirs],
-               "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10_cuda", "-ltorch_cuda",
-               "-lcudart"]
-        _run(cmd)
+        flags = ["-fPIC", "-O2", "-std=c++17", "-DTORCH_EXTENSION_NAME=_tma_dwconv_C",
+                 "-DTORCH_API_INCLUDE_EXTENSION_H",
+                 f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                 *[f"-I{i}" for i in incs]]
+
+        def unit(name: str) -> str:
+            obj = os.path.join(HERE, name.replace(".cpp", ".o"))
+            if force or _stale(obj, _deps(name, "bindings_common.h")):
+                _run(["g++", "-c", *flags, os.path.join(CSRC, name), "-o", _tmp(obj)])
+                os.replace(_tmp(obj), obj)
+            return obj
+
+        with ThreadPoolExecutor(len(EXT_SOURCES)) as pool:
+            objs = list(pool.map(unit, EXT_SOURCES))
+        _run(["g++", "-shared", *objs, "-o", _tmp(EXT), f"-L{HERE}", "-ltdc_sm100",
+              "-Wl,-rpath,$ORIGIN", *[f"-L{d}" for d in libdirs],
+              "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10_cuda", "-ltorch_cuda",
+              "-lcudart"])
         os.replace(_tmp(EXT), EXT)
     return EXT
 
