@@ -161,6 +161,18 @@ def test_equal_keys():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("K,V", [(64, 64), (128, 128)])
+def test_decay_of_a_first_token_without_state_has_no_effect(K, V):
+    # nothing stands behind it: its gradient is exactly zero, not a rounding
+    c = _case(3, 1, 2, 4, K, V, "bf16")
+    got = _run(c)
+    assert not got["dg"].any() and got["dv"].any()
+    c = _case(1, 150, 1, 2, K, V, "bf16", cu=[0, 1, 2, 70, 71, 150])
+    got = _run(c)
+    assert not got["dg"][0, [0, 1, 2, 70, 71]].any() and got["dg"][0, 3:70].any()
+
+
+@pytest.mark.gpu
 def test_scale_and_no_final_state():
     c = _case(1, 80, 1, 1, 128, 64, "fp16")
     _check(_run(c, scale=1.0, final=False), _want(c, scale=1.0, final=False))

@@ -170,6 +170,16 @@ __global__ void __launch_bounds__(1024) delta_plan_kernel(const SeqTable s, int6
 }
 
 // ---- shared pieces -------------------------------------------------------------------
+// The blocks on and below the diagonal of a split [2][64][64] tile.
+__device__ __forceinline__ void copy_lower(uint32_t dst, const __nv_bfloat16* src, int tid,
+                                           int threads) {
+  for (int e = tid; e < 2 * kChunk * 8; e += threads) {
+    const int c = e & 7, r = e >> 3;
+    if (c < 2 * ((r & 63) / 16 + 1))
+      cp_async16(dst + 2 * (r * kLdT + 8 * c), src + r * kChunk + 8 * c, true);
+  }
+}
+
 // rows x (16 * vecs bytes) into shared memory with row stride ld elements;
 // rows behind `valid` become zeros.
 __device__ __forceinline__ void copy_rows(uint32_t dst, int ld, const uint16_t* src, int64_t stride,
@@ -207,79 +217,105 @@ __device__ __forceinline__ void chunk_decay(const DeltaParams& p, const ChunkAt&
 }
 
 // ---- T and P of every chunk -------------------------------------------------------
-// One block a chunk and key head; 4 warps, 16 rows each.  Bound by the
-// triangular inverse: diagonal blocks of 16 by substitution, one column a
-// thread, then joined twice, inv([[P, 0], [B, R]]) = [[P', 0], [-R' B P', R']].
-constexpr int kLdF = kChunk + 1;  // row of the fp32 tiles
+// One block a chunk and key head; 4 warps, 16 rows each.  The triangular
+// inverse: diagonal blocks of 16 by substitution in fp32, one column a thread,
+// then joined twice with matrix instructions (split operands),
+// inv([[P, 0], [B, R]]) = [[P', 0], [-R' B P', R']].  Only the 16 x 16 blocks
+// on and below the diagonal of T and P are written, and none above is read.
+template <int DK>
+struct PrepareSmem {
+  static constexpr int ld = DK + 8;
+  static constexpr int part = kChunk * kLdT * 2;       // one [64][72] tile
+  static constexpr int q = 0;                          // [64][ld], later T hi, lo and P hi
+  static constexpr int k = kChunk * ld * 2;            // [64][ld]
+  static constexpr int t = 0;
+  static constexpr int p = 2 * part;
+  static constexpr int a = 2 * kChunk * ld * 2 > 4 * part ? 2 * kChunk * ld * 2 : 4 * part;
+  static constexpr int diag = a + 2 * part;            // float [4][16][17]
+  static constexpr int G = diag + 4 * 16 * 17 * 4;     // double [64]
+  static constexpr int beta = G + 64 * 8;
+  static constexpr int bytes = beta + 64 * 4;
+};
 
-// dst[.. n x n at (r0, c0)] = sign * a[n x n] b[n x n]; all fp32 in shared memory.
-__device__ __forceinline__ void small_product(float* dst, int ldd, const float* a, int lda,
-                                              const float* b, int ldb, int n, float sign, int i0,
-                                              int step) {
-  for (int e = i0; e < n * n; e += step) {
-    const int r = e / n, c = e % n;
-    float s = 0.f;
-    for (int m = 0; m < n; ++m) s = fmaf(a[r * lda + m], b[m * ldb + c], s);
-    dst[r * ldd + c] = sign * s;
-  }
-}
-
-// sT = (I + sA)^-1 for strictly lower triangular sA; tmp holds 32 x 33 floats.
-__device__ __forceinline__ void unit_lower_inverse(const float* sA, float* sT, float* tmp, int tid) {
-  for (int e = tid; e < kChunk * kChunk; e += 128) sT[(e / kChunk) * kLdF + e % kChunk] = 0.f;
-  __syncthreads();
-  if (tid < kChunk) {
-    const int o = (tid / 16) * 16, c = tid % 16;
-    float x[16];
+// Joins the inverses of two diagonal blocks of n columns at o and o + n: one
+// warp makes 16 columns, from c0, of X = -R' B P'.  All operands are split tiles.
+template <int n>
+__device__ __forceinline__ void join_inverse(uint32_t a, uint32_t t, int o, int c0, int lane) {
+  constexpr int part = kChunk * kLdT * 2, NT = n / 8, KS = n / 16;
+  float w[NT][4] = {};  // (B P')^T: 16 columns of P' by the rows of B
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float s = i == c ? 1.f : 0.f;
+  for (int ks = 0; ks < KS; ++ks) {
+    if (16 * ks < c0) continue;  // P' is lower triangular: nothing is stored above
+    uint32_t ph[4], pl[4];
+    ldsm4_t(ph, addr_at(t, kLdT, o + c0, o + 16 * ks, lane));
+    ldsm4_t(pl, addr_at(t + part, kLdT, o + c0, o + 16 * ks, lane));
 #pragma unroll
-      for (int m = 0; m < i; ++m) s = fmaf(-sA[(o + i) * kLdF + o + m], x[m], s);
-      x[i] = s;
-      sT[(o + i) * kLdF + o + c] = s;
+    for (int np = 0; np < NT / 2; ++np) {
+      uint32_t bh[4], bl[4];
+      ldsm4(bh, addr_b(a, kLdT, o + n + 16 * np, o + 16 * ks, lane));
+      ldsm4(bl, addr_b(a + part, kLdT, o + n + 16 * np, o + 16 * ks, lane));
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        mma_split(w[2 * np + i], ph, pl, bh[2 * i], bh[2 * i + 1], bl[2 * i], bl[2 * i + 1]);
     }
   }
-  __syncthreads();
-  {
-    const int h = tid / 64, o = 32 * h, i0 = tid % 64;  // blocks (0,1) and (2,3)
-    float* t = tmp + h * 16 * 17;
-    small_product(t, 17, sA + (o + 16) * kLdF + o, kLdF, sT + o * kLdF + o, kLdF, 16, 1.f, i0, 64);
-    __syncthreads();
-    small_product(sT + (o + 16) * kLdF + o, kLdF, sT + (o + 16) * kLdF + o + 16, kLdF, t, 17, 16,
-                  -1.f, i0, 64);
+  float x[NT][4] = {};
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    uint32_t wh[4], wl[4];
+    split_frag(w[2 * ks], w[2 * ks + 1], wh, wl);
+#pragma unroll
+    for (int np = ks; np < NT / 2; ++np) {
+      uint32_t rh[4], rl[4];
+      ldsm4(rh, addr_b(t, kLdT, o + n + 16 * np, o + n + 16 * ks, lane));
+      ldsm4(rl, addr_b(t + part, kLdT, o + n + 16 * np, o + n + 16 * ks, lane));
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        mma_split(x[2 * np + i], wh, wl, rh[2 * i], rh[2 * i + 1], rl[2 * i], rl[2 * i + 1]);
+    }
   }
-  __syncthreads();
-  small_product(tmp, 33, sA + 32 * kLdF, kLdF, sT, kLdF, 32, 1.f, tid, 128);
-  __syncthreads();
-  small_product(sT + 32 * kLdF, kLdF, sT + 32 * kLdF + 32, kLdF, tmp, 33, 32, -1.f, tid, 128);
-  __syncthreads();
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {  // X^T's tiles into rows o + n .. of T
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float* v = x[2 * ks + i];
+      split2(-v[0], -v[1], hi[2 * i], lo[2 * i]);
+      split2(-v[2], -v[3], hi[2 * i + 1], lo[2 * i + 1]);
+    }
+    stsm4_t(addr_at(t, kLdT, o + c0, o + n + 16 * ks, lane), hi);
+    stsm4_t(addr_at(t + part, kLdT, o + c0, o + n + 16 * ks, lane), lo);
+  }
 }
 
-template <int DK>
-constexpr size_t prepare_smem() {
-  return size_t(2) * kChunk * (DK + 8) * 2 + size_t(2) * kChunk * kLdF * 4 + 32 * 33 * 4 +
-         kChunk * 8 + kChunk * 4;
+// Blocks on and below the diagonal of a split [64][64] tile, to [2][64][64].
+__device__ __forceinline__ void store_lower(__nv_bfloat16* dst, const unsigned char* tile, int tid,
+                                            int threads) {
+  for (int e = tid; e < 2 * kChunk * 8; e += threads) {
+    const int c = e & 7, r = (e >> 3) & 63, part = e >> 9;
+    if (c < 2 * (r / 16 + 1))
+      *reinterpret_cast<uint4*>(dst + part * kSq + r * kChunk + 8 * c) =
+          *reinterpret_cast<const uint4*>(tile + part * kChunk * kLdT * 2 + 2 * (r * kLdT + 8 * c));
+  }
 }
 
 template <class E, int DK>
 __global__ void __launch_bounds__(128) delta_prepare_kernel(const DeltaParams p) {
   extern __shared__ __align__(16) unsigned char raw[];
-  constexpr int ld = DK + 8;
+  using Sm = PrepareSmem<DK>;
+  constexpr int ld = Sm::ld, part = Sm::part;
   const int64_t chunk = blockIdx.x;
   const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const ChunkAt at = chunk_at(p, chunk);
   if (at.rows == 0) return;
-  const uint32_t sq = smem_addr(raw), sk = sq + kChunk * ld * 2;
-  float* sA = reinterpret_cast<float*>(raw + 2 * kChunk * ld * 2);
-  float* sT = sA + kChunk * kLdF;
-  float* tmp = sT + kChunk * kLdF;
-  double* G = reinterpret_cast<double*>(tmp + 32 * 33);
-  float* sB = reinterpret_cast<float*>(G + kChunk);
+  const uint32_t sb = smem_addr(raw);
+  float* diag = reinterpret_cast<float*>(raw + Sm::diag);
+  double* G = reinterpret_cast<double*>(raw + Sm::G);
+  float* sB = reinterpret_cast<float*>(raw + Sm::beta);
   const uint16_t* q = static_cast<const uint16_t*>(p.q) + at.b * p.q_sb + at.t0 * p.q_st + h * p.q_sh;
   const uint16_t* k = static_cast<const uint16_t*>(p.k) + at.b * p.k_sb + at.t0 * p.k_st + h * p.k_sh;
-  copy_rows(sq, ld, q, p.q_st, kChunk, at.rows, DK / 8, tid, 128);
-  copy_rows(sk, ld, k, p.k_st, kChunk, at.rows, DK / 8, tid, 128);
+  copy_rows(sb + Sm::q, ld, q, p.q_st, kChunk, at.rows, DK / 8, tid, 128);
+  copy_rows(sb + Sm::k, ld, k, p.k_st, kChunk, at.rows, DK / 8, tid, 128);
   cp_async_commit();
   cp_async_wait<0>();
   __syncthreads();
@@ -288,13 +324,13 @@ __global__ void __launch_bounds__(128) delta_prepare_kernel(const DeltaParams p)
 #pragma unroll
   for (int ks = 0; ks < DK / 16; ++ks) {
     uint32_t aq[4], ak[4];
-    ldsm4(aq, addr_a(sq, ld, 16 * warp, 16 * ks, lane));
-    ldsm4(ak, addr_a(sk, ld, 16 * warp, 16 * ks, lane));
+    ldsm4(aq, addr_a(sb + Sm::q, ld, 16 * warp, 16 * ks, lane));
+    ldsm4(ak, addr_a(sb + Sm::k, ld, 16 * warp, 16 * ks, lane));
 #pragma unroll
     for (int np = 0; np < 4; ++np) {
       if (np > warp) break;  // columns behind the rows are not used
       uint32_t bk[4];
-      ldsm4(bk, addr_b(sk, ld, 16 * np, 16 * ks, lane));
+      ldsm4(bk, addr_b(sb + Sm::k, ld, 16 * np, 16 * ks, lane));
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         mma_elem<E>(qk[2 * np + i], aq, bk[2 * i], bk[2 * i + 1]);
@@ -306,6 +342,7 @@ __global__ void __launch_bounds__(128) delta_prepare_kernel(const DeltaParams p)
   for (int gi = 0; gi < p.group; ++gi) {
     const int hv = h * p.group + gi;
     const int64_t slot = chunk * p.HV + hv;
+    __syncthreads();  // q and k, or the last head's tiles, are free
     if (warp == 0) chunk_decay(p, at, hv, G, lane);
     if (tid >= 64) {
       const int t = tid - 64;
@@ -320,36 +357,54 @@ __global__ void __launch_bounds__(128) delta_prepare_kernel(const DeltaParams p)
       coef[kChunk + tid] = expf(float(G[kChunk - 1] - G[tid]));
       coef[2 * kChunk + tid] = sB[tid];
     }
-    __nv_bfloat16* pm = p.pm + slot * 2 * kSq;
 #pragma unroll
     for (int nt = 0; nt < 8; ++nt) {
+      if (nt > 2 * warp + 1) break;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int i = 16 * warp + g + 8 * half, j = 8 * nt + t2;
-        float pv[2];
+        float pv[2], av[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const float gam = i >= j + u ? __expf(float(G[i] - G[j + u])) : 0.f;
           pv[u] = i >= j + u ? p.scale * gam * qk[nt][2 * half + u] : 0.f;
-          sA[i * kLdF + j + u] = i > j + u ? kk[nt][2 * half + u] * gam * sB[j + u] : 0.f;
+          av[u] = i > j + u ? kk[nt][2 * half + u] * gam * sB[j + u] : 0.f;
+          if (nt >= 2 * warp) diag[(warp * 16 + g + 8 * half) * 17 + j + u - 16 * warp] = av[u];
         }
         uint32_t hi, lo;
+        const int off = 2 * (i * kLdT + j);
         split2(pv[0], pv[1], hi, lo);
-        *reinterpret_cast<uint32_t*>(pm + i * kChunk + j) = hi;
-        *reinterpret_cast<uint32_t*>(pm + kSq + i * kChunk + j) = lo;
+        *reinterpret_cast<uint32_t*>(raw + Sm::p + off) = hi;
+        *reinterpret_cast<uint32_t*>(raw + Sm::p + part + off) = lo;
+        split2(av[0], av[1], hi, lo);
+        *reinterpret_cast<uint32_t*>(raw + Sm::a + off) = hi;
+        *reinterpret_cast<uint32_t*>(raw + Sm::a + part + off) = lo;
+      }
+    }
+    __syncwarp();
+    if (lane < 16) {  // the warp's diagonal block, one column a lane
+      const float* d = diag + warp * 16 * 17;
+      float x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float v = i == lane ? 1.f : 0.f;
+#pragma unroll
+        for (int m = 0; m < i; ++m) v = fmaf(-d[i * 17 + m], x[m], v);
+        x[i] = v;
+        const __nv_bfloat16 hi = __float2bfloat16_rn(v);
+        __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(raw + Sm::t) +
+                             (16 * warp + i) * kLdT + 16 * warp + lane;
+        dst[0] = hi;
+        dst[part / 2] = __float2bfloat16_rn(v - __bfloat162float(hi));
       }
     }
     __syncthreads();
-    unit_lower_inverse(sA, sT, tmp, tid);
-    __nv_bfloat16* tm = p.tm + slot * 2 * kSq;
-    for (int e = tid; e < kSq / 2; e += 128) {
-      const int i = e / (kChunk / 2), j = 2 * (e % (kChunk / 2));
-      uint32_t hi, lo;
-      split2(sT[i * kLdF + j], sT[i * kLdF + j + 1], hi, lo);
-      *reinterpret_cast<uint32_t*>(tm + i * kChunk + j) = hi;
-      *reinterpret_cast<uint32_t*>(tm + kSq + i * kChunk + j) = lo;
-    }
+    if (warp < 2) join_inverse<16>(sb + Sm::a, sb + Sm::t, 32 * warp, 0, lane);
+    else store_lower(p.pm + slot * 2 * kSq, raw + Sm::p, tid - 64, 64);
     __syncthreads();
+    if (warp < 2) join_inverse<32>(sb + Sm::a, sb + Sm::t, 0, 16 * warp, lane);
+    __syncthreads();
+    store_lower(p.tm + slot * 2 * kSq, raw + Sm::t, tid, 128);
   }
 }
 
@@ -523,12 +578,10 @@ __global__ void __launch_bounds__(32 * W) delta_scan_kernel(const DeltaParams p)
     const int rows = int(min(int64_t(kChunk), s.len - t0));
     copy_rows(st + St::k, St::ld, k + t0 * p.k_st, p.k_st, kChunk, rows, DK / 8, tid, 32 * W);
     copy_rows(st + St::v, St::ldv, v + t0 * p.v_st, p.v_st, kChunk, rows, 2 * W, tid, 32 * W);
-    copy_rows(st + St::t, kLdT, reinterpret_cast<const uint16_t*>(p.tm) + slot * 2 * kSq, kChunk,
-              2 * kChunk, 2 * kChunk, kChunk / 8, tid, 32 * W);
+    copy_lower(st + St::t, p.tm + slot * 2 * kSq, tid, 32 * W);
     if constexpr (MODE == 0) {
       copy_rows(st + St::q, St::ld, q + t0 * p.q_st, p.q_st, kChunk, rows, DK / 8, tid, 32 * W);
-      copy_rows(st + St::p, kLdT, reinterpret_cast<const uint16_t*>(p.pm) + slot * 2 * kSq, kChunk,
-                2 * kChunk, 2 * kChunk, kChunk / 8, tid, 32 * W);
+      copy_lower(st + St::p, p.pm + slot * 2 * kSq, tid, 32 * W);
     }
     const float* coef = p.coef + slot * 3 * kChunk;
     for (int i = tid; i < 3 * kChunk / 4; i += 32 * W)
@@ -655,10 +708,8 @@ __global__ void __launch_bounds__(32 * W) delta_scan_back_kernel(const DeltaPara
     copy_rows(st + St::k, St::ld, k + t0 * p.k_st, p.k_st, kChunk, rows, DK / 8, tid, 32 * W);
     copy_rows(st + St::q, St::ld, q + t0 * p.q_st, p.q_st, kChunk, rows, DK / 8, tid, 32 * W);
     copy_rows(st + St::v, St::ldv, d_o + t0 * p.do_st, p.do_st, kChunk, rows, 2 * W, tid, 32 * W);
-    copy_rows(st + St::t, kLdT, reinterpret_cast<const uint16_t*>(p.tm) + slot * 2 * kSq, kChunk,
-              2 * kChunk, 2 * kChunk, kChunk / 8, tid, 32 * W);
-    copy_rows(st + St::p, kLdT, reinterpret_cast<const uint16_t*>(p.pm) + slot * 2 * kSq, kChunk,
-              2 * kChunk, 2 * kChunk, kChunk / 8, tid, 32 * W);
+    copy_lower(st + St::t, p.tm + slot * 2 * kSq, tid, 32 * W);
+    copy_lower(st + St::p, p.pm + slot * 2 * kSq, tid, 32 * W);
     const float* coef = p.coef + slot * 3 * kChunk;
     for (int i = tid; i < 3 * kChunk / 4; i += 32 * W)
       cp_async16(st + St::coef + 16 * i, coef + 4 * i, true);
@@ -771,10 +822,13 @@ __global__ void __launch_bounds__(32 * W) delta_scan_back_kernel(const DeltaPara
 // M = dX U^T (lower parts):
 //   dQ = scale gam (dO S^T) + Dt K                     Dt = scale Gam beta_j D
 //   dK = -gam (dX S^T) + w beta (U dS^T) + Dt^T Q + (N + N^T) K,  N = -M beta_j Gam
-//   dbeta_j = sum_i P_ij D_ij - sum_i M_ij L_ij + w_j k_j.(U dS^T)_j
-//   dG_i = rows(E) - cols(E) + scale gam q.(dO S^T) - gam k.(dX S^T) - w beta k.(U dS^T),
-//     E = beta_j (P D - M L); the last row adds the sum of w beta k.(U dS^T) and
-//     gam_63 <dS, S>;  dg = sum of dG from the row to the chunk's end.
+//   dbeta_j = sum_i (P_ij D_ij - M_ij L_ij) + w_j k_j.(U dS^T)_j
+// The decay of row t stands in front of everything that reaches from before t to
+// t or behind it, so with E_ij = beta_j (P_ij D_ij - M_ij L_ij), i > j,
+//   dg_t = sum_{i >= t} (scale gam q.(dO S^T) - gam k.(dX S^T))_i
+//        + sum_{j < t} (w beta k.(U dS^T))_j + sum_{i >= t > j} E_ij + gam_63 <dS, S>:
+// no terms that cancel (a first token without a state gets exactly 0); the
+// double sum grows by the column sum of E and falls by its row sum from row to row.
 // 8 warps: 4 groups of 16 rows by 2 halves of the columns.  The value channels
 // are walked in tiles of 64.
 template <int DK>
@@ -790,9 +844,11 @@ struct GradSmem {
   static constexpr int G = o + 64 * kLdT * 2;             // double [64]
   static constexpr int coef = G + 64 * 8;                 // [3][64]
   static constexpr int rows = coef + 3 * 64 * 4;          // [2][4][64]: row sums of both halves
-  static constexpr int cols = rows + 2 * 4 * 64 * 4;      // [4][2][64]: column sums of the row groups
-  static constexpr int dot = cols + 4 * 2 * 64 * 4;       // [8] + dG [64]
-  static constexpr int bytes = dot + 8 * 4 + 64 * 4;
+  static constexpr int cols = rows + 2 * 4 * 64 * 4;      // [4][64]: column sums of the row groups
+  static constexpr int diag = cols + 4 * 64 * 4;          // [64]
+  static constexpr int dot = diag + 64 * 4;               // [8]
+  static constexpr int dg = dot + 8 * 4;                  // [2][64]
+  static constexpr int bytes = dg + 2 * 64 * 4;
 };
 
 template <class E, int DK>
@@ -811,7 +867,8 @@ __global__ void __launch_bounds__(256, 1) delta_grad_kernel(const DeltaParams p)
   float* rows = reinterpret_cast<float*>(raw + Sm::rows);
   float* cols = reinterpret_cast<float*>(raw + Sm::cols);
   float* dot = reinterpret_cast<float*>(raw + Sm::dot);
-  float* dG = dot + 8;
+  float* diag = reinterpret_cast<float*>(raw + Sm::diag);
+  float* dgs = reinterpret_cast<float*>(raw + Sm::dg);
   const uint16_t* q = static_cast<const uint16_t*>(p.q) + at.b * p.q_sb + at.t0 * p.q_st + h * p.q_sh;
   const uint16_t* k = static_cast<const uint16_t*>(p.k) + at.b * p.k_sb + at.t0 * p.k_st + h * p.k_sh;
   copy_rows(sb + Sm::q, ld, q, p.q_st, kChunk, at.rows, DK / 8, tid, 256);
@@ -955,11 +1012,11 @@ __global__ void __launch_bounds__(256, 1) delta_grad_kernel(const DeltaParams p)
         }
       }
     }
-    float re[2] = {};  // row sums of E
+    float re[2] = {};  // row sums of E below the diagonal
     __syncthreads();   // u and x are free: Dt and N take their place
 #pragma unroll
     for (int nt = 0; nt < 4; ++nt) {
-      float cd[2] = {}, cm[2] = {};  // column sums of P D and M L over this thread's two rows
+      float cs[2] = {};  // column sums of P D - M L below the diagonal, this thread's two rows
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int i = i0 + 8 * half, j = 32 * ch + 8 * nt + t2;
@@ -971,9 +1028,12 @@ __global__ void __launch_bounds__(256, 1) delta_grad_kernel(const DeltaParams p)
           const float be = coef[128 + j + u];
           const float dv = i >= j + u ? D[nt][e] : 0.f, mv = i > j + u ? M[nt][e] : 0.f;
           const float pd = p.scale * gam * qk[nt][e] * dv, ml = gam * kk[nt][e] * mv;
-          cd[u] += pd;
-          cm[u] += ml;
-          re[half] = fmaf(be, pd - ml, re[half]);
+          if (i > j + u) {
+            cs[u] += pd - ml;
+            re[half] = fmaf(be, pd - ml, re[half]);
+          } else if (i == j + u) {
+            diag[i] = pd;
+          }
           dt[u] = p.scale * gam * be * dv;
           nn[u] = -mv * be * gam;
         }
@@ -990,13 +1050,9 @@ __global__ void __launch_bounds__(256, 1) delta_grad_kernel(const DeltaParams p)
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) {
-          cd[u] += __shfl_xor_sync(0xffffffffu, cd[u], d);
-          cm[u] += __shfl_xor_sync(0xffffffffu, cm[u], d);
+          cs[u] += __shfl_xor_sync(0xffffffffu, cs[u], d);
         }
-        if (g == 0) {
-          cols[(rg * 2 + 0) * 64 + 32 * ch + 8 * nt + t2 + u] = cd[u];
-          cols[(rg * 2 + 1) * 64 + 32 * ch + 8 * nt + t2 + u] = cm[u];
-        }
+        if (g == 0) cols[rg * 64 + 32 * ch + 8 * nt + t2 + u] = cs[u];
       }
     }
 #pragma unroll
@@ -1063,37 +1119,40 @@ __global__ void __launch_bounds__(256, 1) delta_grad_kernel(const DeltaParams p)
 #pragma unroll
       for (int j = 0; j < 4; ++j) s0[j] = rows[j * 64 + i] + rows[(4 + j) * 64 + i];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) c0 += cols[(j * 2) * 64 + i] - cols[(j * 2 + 1) * 64 + i];
-      const float tail = w1 * be * s0[2];
+      for (int j = 0; j < 4; ++j) c0 += cols[j * 64 + i];
       if (i < at.rows) {
         const int64_t o = (at.b * p.T + at.t0 + i) * p.HV + hv;
-        const float db = c0 + w1 * s0[2];
+        const float db = c0 + diag[i] + w1 * s0[2];
         if (p.beta_f32) static_cast<float*>(p.dbeta)[o] = db;
         else store_float<E>(p.dbeta, o, db);
       }
-      dG[i] = s0[3] - be * c0 + p.scale * ga1 * s0[0] - ga1 * s0[1] - tail;
-      rows[i] = tail;  // (each thread's own entry has been read)
+      dgs[i] = p.scale * ga1 * s0[0] - ga1 * s0[1];
+      dgs[64 + i] = be * c0 - s0[3] + w1 * be * s0[2];
     }
     __syncthreads();
     if (warp == 0) {
-      // dg_i = sum of dG from i to the end; the tails and gam_63 <dS, S> belong to the last row
-      float tails = rows[lane] + rows[lane + 32];
-#pragma unroll
-      for (int d = 16; d; d >>= 1) tails += __shfl_xor_sync(0xffffffffu, tails, d);
       float ds = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) ds += dot[i];
-      const float extra = tails + coef[63] * ds;
-      const float a = dG[2 * lane], b = dG[2 * lane + 1];
-      float sum = a + b;
+      ds *= coef[63];
+      // sums from the row to the end, and over the rows before it
+      const float a0 = dgs[2 * lane], a1 = dgs[2 * lane + 1];
+      const float f0 = dgs[64 + 2 * lane], f1 = dgs[64 + 2 * lane + 1];
+      float up = a0 + a1, down = f0 + f1;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
-        const float o = __shfl_down_sync(0xffffffffu, sum, d);
-        if (lane + d < 32) sum += o;
+        const float x = __shfl_down_sync(0xffffffffu, up, d);
+        const float y = __shfl_up_sync(0xffffffffu, down, d);
+        if (lane + d < 32) up += x;
+        if (lane >= d) down += y;
       }
+      const float above = __shfl_down_sync(0xffffffffu, up, 1);
+      float before = __shfl_up_sync(0xffffffffu, down, 1);
+      if (lane == 0) before = 0.f;
       const int64_t o = (at.b * p.T + at.t0 + 2 * lane) * p.HV + hv;
-      if (2 * lane < at.rows) p.dg[o] = sum + extra;
-      if (2 * lane + 1 < at.rows) p.dg[o + p.HV] = sum - a + extra;
+      if (2 * lane < at.rows) p.dg[o] = up + before + ds;
+      if (2 * lane + 1 < at.rows)
+        p.dg[o + p.HV] = a1 + (lane < 31 ? above : 0.f) + before + f0 + ds;
     }
   }
   // dq and dk rows

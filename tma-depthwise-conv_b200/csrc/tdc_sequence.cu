@@ -360,7 +360,7 @@ template <class E, int DK>
 int delta_prepare(const tdc::DeltaParams& p, cudaStream_t st) {
   if (p.max_chunks == 0) return TDC_OK;
   auto* k = &tdc::delta_prepare_kernel<E, DK>;
-  const size_t smem = tdc::prepare_smem<DK>();
+  const size_t smem = tdc::PrepareSmem<DK>::bytes;
   const int rc = allow_smem(k, smem);
   if (rc != TDC_OK) return rc;
   k<<<dim3(unsigned(p.max_chunks), unsigned(p.H)), 128, smem, st>>>(p);
