@@ -1699,6 +1699,24 @@ int prepare_device() {
   return current_device(&info, nullptr);
 }
 
+int wait_record(WaitRecord* r) {
+  int dev = -1;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return ::cuda_fail(e);
+  if (dev < 0 || dev >= kMaxDevices) return TDC_ERR_NO_DEVICE;
+  static std::atomic<void*> words[kMaxDevices];
+  void* w = words[dev].load(std::memory_order_acquire);
+  if (w == nullptr) {
+    e = cudaGetSymbolAddress(&w, tdc::g_tdc_status);
+    if (e != cudaSuccess) return ::cuda_fail(e);
+    words[dev].store(w, std::memory_order_release);
+  }
+  r->timeout_ns = uint64_t(g_timeout_ns.load());
+  r->words = static_cast<int*>(w);
+  r->host = status_slot(dev, true);
+  return TDC_OK;
+}
+
 }  // namespace host
 }  // namespace tdc
 

@@ -7,13 +7,8 @@
 //   T = (I + A)^-1                                P = scale * lower(Q K^T) * Gam
 //   X = V - diag(gam) K S,  U = T X,  V' = diag(beta) U
 //   O = scale diag(gam) Q S + P V'                S <- gam_63 S + K^T diag(w) V'
-// delta_prepare makes T and P of all chunks at once; delta_scan walks the
-// chunks of a sequence.  The columns of S (the value channels) do not mix, so
-// a warp keeps 16 of them, as S^T [16 x K], in the accumulators of its matrix
-// instructions for the whole sequence, and every product of the chain
-// (transposed) takes its A operand straight from the accumulators of the one
-// before it: the warps of a block share tiles but never wait for one another's
-// results.
+// delta_prepare makes T and P of all chunks at once; delta_walk (its own file)
+// walks the chunks of a sequence on the tensor cores.
 //
 // Precision: states, decays, sums and all accumulators are fp32.  An fp32
 // operand of a matrix instruction is split into two bf16 parts (16 bits of
@@ -49,9 +44,12 @@ struct DeltaParams {
   bool beta_f32;
   float scale;
   // workspace of all chunks, [chunk][HV] each
-  __nv_bfloat16* tm;      // [2][64][64]: T, high parts and remainders
-  __nv_bfloat16* pm;      // [2][64][64]: P
+  // (tiles in the order of WalkTiles; 8 x 8 blocks, see tdc_tc.cuh)
+  __nv_bfloat16* tp;      // T and P, high parts and remainders: [4][64 x 64]
   float* coef;            // [3][64]: gam, w, beta
+  unsigned char* kq;      // [chunk][H]: K and Q, [2][parts][64 x K]
+  uint64_t timeout_ns;    // of the bounded waits
+  int *status_words, *status_host;
   // gradients
   __nv_bfloat16* um;      // [2][V][64]: U^T
   __nv_bfloat16* xm;      // [2][V][64]: dX^T
@@ -170,16 +168,6 @@ __global__ void __launch_bounds__(1024) delta_plan_kernel(const SeqTable s, int6
 }
 
 // ---- shared pieces -------------------------------------------------------------------
-// The blocks on and below the diagonal of a split [2][64][64] tile.
-__device__ __forceinline__ void copy_lower(uint32_t dst, const __nv_bfloat16* src, int tid,
-                                           int threads) {
-  for (int e = tid; e < 2 * kChunk * 8; e += threads) {
-    const int c = e & 7, r = e >> 3;
-    if (c < 2 * ((r & 63) / 16 + 1))
-      cp_async16(dst + 2 * (r * kLdT + 8 * c), src + r * kChunk + 8 * c, true);
-  }
-}
-
 // rows x (16 * vecs bytes) into shared memory with row stride ld elements;
 // rows behind `valid` become zeros.
 __device__ __forceinline__ void copy_rows(uint32_t dst, int ld, const uint16_t* src, int64_t stride,
@@ -222,6 +210,13 @@ __device__ __forceinline__ void chunk_decay(const DeltaParams& p, const ChunkAt&
 // then joined twice with matrix instructions (split operands),
 // inv([[P, 0], [B, R]]) = [[P', 0], [-R' B P', R']].  Only the 16 x 16 blocks
 // on and below the diagonal of T and P are written, and none above is read.
+//
+// The fp32 rows (16 floats) of the diagonal blocks of A lie in the unused
+// blocks above T's diagonal: row i of block w in row i or 16 + i of one part.
+__device__ __forceinline__ int diag_offset(int w, int i) {
+  return (w & 1) * kChunk * kLdT * 2 + ((w >> 1) * 16 + i) * kLdT * 2 + (w >> 1 ? 64 : 32);
+}
+
 template <int DK>
 struct PrepareSmem {
   static constexpr int ld = DK + 8;
@@ -231,8 +226,7 @@ struct PrepareSmem {
   static constexpr int t = 0;
   static constexpr int p = 2 * part;
   static constexpr int a = 2 * kChunk * ld * 2 > 4 * part ? 2 * kChunk * ld * 2 : 4 * part;
-  static constexpr int diag = a + 2 * part;            // float [4][16][17]
-  static constexpr int G = diag + 4 * 16 * 17 * 4;     // double [64]
+  static constexpr int G = a + 2 * part;               // double [64]
   static constexpr int beta = G + 64 * 8;
   static constexpr int bytes = beta + 64 * 4;
 };
@@ -288,14 +282,42 @@ __device__ __forceinline__ void join_inverse(uint32_t a, uint32_t t, int o, int 
   }
 }
 
-// Blocks on and below the diagonal of a split [64][64] tile, to [2][64][64].
+// Element offset of 16 bytes at row r, columns 8 c .. + 7 of a 64-row tile in
+// 8 x 8 blocks.
+__device__ __forceinline__ int block_offset(int r, int c) {
+  return c * (kChunk * 8) + r * 8;
+}
+
+// Blocks on and below the diagonal of a split [64][64] tile, to [2][64 x 64].
 __device__ __forceinline__ void store_lower(__nv_bfloat16* dst, const unsigned char* tile, int tid,
                                             int threads) {
   for (int e = tid; e < 2 * kChunk * 8; e += threads) {
-    const int c = e & 7, r = (e >> 3) & 63, part = e >> 9;
+    const int r = e & 63, c = (e >> 6) & 7, part = e >> 9;
     if (c < 2 * (r / 16 + 1))
-      *reinterpret_cast<uint4*>(dst + part * kSq + r * kChunk + 8 * c) =
+      *reinterpret_cast<uint4*>(dst + part * kSq + block_offset(r, c)) =
           *reinterpret_cast<const uint4*>(tile + part * kChunk * kLdT * 2 + 2 * (r * kLdT + 8 * c));
+  }
+}
+
+// A [64][DK] tile of the element type to its parts in 8 x 8 blocks.
+template <class E, int DK>
+__device__ __forceinline__ void store_keys(unsigned char* dst, const unsigned char* tile, int tid,
+                                           int threads) {
+  for (int e = tid; e < kChunk * (DK / 8); e += threads) {
+    const int r = e & 63, c = e >> 6;
+    const uint4 v = *reinterpret_cast<const uint4*>(tile + 2 * (r * (DK + 8) + 8 * c));
+    uint4* d = reinterpret_cast<uint4*>(dst + 2 * block_offset(r, c));
+    if constexpr (std::is_same_v<E, BF16>) {
+      *d = v;
+    } else {
+      uint4 hi, lo;
+      split_elem<E>(v.x, hi.x, lo.x);
+      split_elem<E>(v.y, hi.y, lo.y);
+      split_elem<E>(v.z, hi.z, lo.z);
+      split_elem<E>(v.w, hi.w, lo.w);
+      *d = hi;
+      d[kChunk * DK / 8] = lo;
+    }
   }
 }
 
@@ -309,7 +331,6 @@ __global__ void __launch_bounds__(128) delta_prepare_kernel(const DeltaParams p)
   const ChunkAt at = chunk_at(p, chunk);
   if (at.rows == 0) return;
   const uint32_t sb = smem_addr(raw);
-  float* diag = reinterpret_cast<float*>(raw + Sm::diag);
   double* G = reinterpret_cast<double*>(raw + Sm::G);
   float* sB = reinterpret_cast<float*>(raw + Sm::beta);
   const uint16_t* q = static_cast<const uint16_t*>(p.q) + at.b * p.q_sb + at.t0 * p.q_st + h * p.q_sh;
@@ -337,6 +358,12 @@ __global__ void __launch_bounds__(128) delta_prepare_kernel(const DeltaParams p)
         mma_elem<E>(kk[2 * np + i], ak, bk[2 * i], bk[2 * i + 1]);
       }
     }
+  }
+  {
+    constexpr int64_t bytes = int64_t(std::is_same_v<E, BF16> ? 1 : 2) * kChunk * DK * 2;
+    unsigned char* kq = p.kq + (chunk * p.H + h) * 2 * bytes;
+    store_keys<E, DK>(kq, raw + Sm::k, tid, 128);
+    store_keys<E, DK>(kq + bytes, raw + Sm::q, tid, 128);
   }
   const int g = lane >> 2, t2 = (lane & 3) * 2;
   for (int gi = 0; gi < p.group; ++gi) {
@@ -369,8 +396,10 @@ __global__ void __launch_bounds__(128) delta_prepare_kernel(const DeltaParams p)
           const float gam = i >= j + u ? __expf(float(G[i] - G[j + u])) : 0.f;
           pv[u] = i >= j + u ? p.scale * gam * qk[nt][2 * half + u] : 0.f;
           av[u] = i > j + u ? kk[nt][2 * half + u] * gam * sB[j + u] : 0.f;
-          if (nt >= 2 * warp) diag[(warp * 16 + g + 8 * half) * 17 + j + u - 16 * warp] = av[u];
         }
+        if (nt >= 2 * warp)
+          *reinterpret_cast<float2*>(raw + Sm::t + diag_offset(warp, g + 8 * half) +
+                                     4 * (j - 16 * warp)) = make_float2(av[0], av[1]);
         uint32_t hi, lo;
         const int off = 2 * (i * kLdT + j);
         split2(pv[0], pv[1], hi, lo);
@@ -383,13 +412,13 @@ __global__ void __launch_bounds__(128) delta_prepare_kernel(const DeltaParams p)
     }
     __syncwarp();
     if (lane < 16) {  // the warp's diagonal block, one column a lane
-      const float* d = diag + warp * 16 * 17;
       float x[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
+        const float* d = reinterpret_cast<const float*>(raw + Sm::t + diag_offset(warp, i));
         float v = i == lane ? 1.f : 0.f;
 #pragma unroll
-        for (int m = 0; m < i; ++m) v = fmaf(-d[i * 17 + m], x[m], v);
+        for (int m = 0; m < i; ++m) v = fmaf(-d[m], x[m], v);
         x[i] = v;
         const __nv_bfloat16 hi = __float2bfloat16_rn(v);
         __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(raw + Sm::t) +
@@ -400,421 +429,12 @@ __global__ void __launch_bounds__(128) delta_prepare_kernel(const DeltaParams p)
     }
     __syncthreads();
     if (warp < 2) join_inverse<16>(sb + Sm::a, sb + Sm::t, 32 * warp, 0, lane);
-    else store_lower(p.pm + slot * 2 * kSq, raw + Sm::p, tid - 64, 64);
+    else store_lower(p.tp + slot * 4 * kSq + 2 * kSq, raw + Sm::p, tid - 64, 64);
     __syncthreads();
     if (warp < 2) join_inverse<32>(sb + Sm::a, sb + Sm::t, 0, 16 * warp, lane);
     __syncthreads();
-    store_lower(p.tm + slot * 2 * kSq, raw + Sm::t, tid, 128);
+    store_lower(p.tp + slot * 4 * kSq, raw + Sm::t, tid, 128);
   }
-}
-
-// ---- the walk over a sequence's chunks ---------------------------------------------
-// Stages of the two-deep ring: K, Q, V slice, T, P, coefficients.
-template <int DK, int W>
-struct ScanStage {
-  static constexpr int ld = DK + 8, ldv = 16 * W + 8;
-  static constexpr int k = 0;
-  static constexpr int q = k + kChunk * ld * 2;
-  static constexpr int v = q + kChunk * ld * 2;
-  static constexpr int t = v + kChunk * ldv * 2;
-  static constexpr int p = t + 2 * kChunk * kLdT * 2;
-  static constexpr int coef = p + 2 * kChunk * kLdT * 2;
-  static constexpr int bytes = coef + 3 * kChunk * 4;
-};
-
-// x^T [16 x 64] (accumulators) times M^T, M lower triangular [64][64] split in
-// shared memory: out^T = x^T M^T, i.e. out = M x.
-__device__ __forceinline__ void lower_product(float out[8][4], const float x[8][4], uint32_t m,
-                                              int lane) {
-#pragma unroll
-  for (int ks = 0; ks < 4; ++ks) {
-    uint32_t ah[4], al[4];
-    split_frag(x[2 * ks], x[2 * ks + 1], ah, al);
-#pragma unroll
-    for (int np = ks; np < 4; ++np) {
-      uint32_t bh[4], bl[4];
-      ldsm4(bh, addr_b(m, kLdT, 16 * np, 16 * ks, lane));
-      ldsm4(bl, addr_b(m + kChunk * kLdT * 2, kLdT, 16 * np, 16 * ks, lane));
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        mma_split(out[2 * np + i], ah, al, bh[2 * i], bh[2 * i + 1], bl[2 * i], bl[2 * i + 1]);
-    }
-  }
-}
-
-// out = M^T x: out^T = x^T M.
-__device__ __forceinline__ void lower_product_t(float out[8][4], const float x[8][4], uint32_t m,
-                                                int lane) {
-#pragma unroll
-  for (int ks = 0; ks < 4; ++ks) {
-    uint32_t ah[4], al[4];
-    split_frag(x[2 * ks], x[2 * ks + 1], ah, al);
-#pragma unroll
-    for (int np = 0; np <= ks; ++np) {
-      uint32_t bh[4], bl[4];
-      ldsm4_t(bh, addr_bt(m, kLdT, 16 * np, 16 * ks, lane));
-      ldsm4_t(bl, addr_bt(m + kChunk * kLdT * 2, kLdT, 16 * np, 16 * ks, lane));
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        mma_split(out[2 * np + i], ah, al, bh[2 * i], bh[2 * i + 1], bl[2 * i], bl[2 * i + 1]);
-    }
-  }
-}
-
-// out^T [16 x 64] += S^T [16 x DK] M^T, M [64][DK] in the element type.
-template <class E, int DK>
-__device__ __forceinline__ void state_product(float out[8][4], const float s[DK / 8][4], uint32_t m,
-                                              int lane) {
-#pragma unroll
-  for (int ks = 0; ks < DK / 16; ++ks) {
-    uint32_t ah[4], al[4];
-    split_frag(s[2 * ks], s[2 * ks + 1], ah, al);
-#pragma unroll
-    for (int np = 0; np < 4; ++np) {
-      uint32_t b[4];
-      ldsm4(b, addr_b(m, DK + 8, 16 * np, 16 * ks, lane));
-#pragma unroll
-      for (int i = 0; i < 2; ++i) mma_split_elem<E>(out[2 * np + i], ah, al, b[2 * i], b[2 * i + 1]);
-    }
-  }
-}
-
-// S^T [16 x DK] += x^T M, with x^T's A fragment of 16 tokens given split.
-template <class E, int DK>
-__device__ __forceinline__ void state_update(float s[DK / 8][4], const uint32_t ah[4],
-                                             const uint32_t al[4], uint32_t m, int ks, int lane) {
-#pragma unroll
-  for (int np = 0; np < DK / 16; ++np) {
-    uint32_t b[4];
-    ldsm4_t(b, addr_bt(m, DK + 8, 16 * np, 16 * ks, lane));
-#pragma unroll
-    for (int i = 0; i < 2; ++i) mma_split_elem<E>(s[2 * np + i], ah, al, b[2 * i], b[2 * i + 1]);
-  }
-}
-
-// Writes x^T [16 x cols] (accumulators) split into rows r0.. of [rows][ldg].
-template <int NT>
-__device__ __forceinline__ void store_split(__nv_bfloat16* dst, int64_t part, int ldg,
-                                            const float x[NT][4], int lane) {
-  const int g = lane >> 2, t2 = (lane & 3) * 2;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      uint32_t hi, lo;
-      split2(x[nt][2 * half], x[nt][2 * half + 1], hi, lo);
-      __nv_bfloat16* d = dst + (g + 8 * half) * ldg + 8 * nt + t2;
-      *reinterpret_cast<uint32_t*>(d) = hi;
-      *reinterpret_cast<uint32_t*>(d + part) = lo;
-    }
-}
-
-// S^T [16 x DK] of a warp from and to a state [DK][V] at value channel c0.
-template <int DK>
-__device__ __forceinline__ void load_state(float s[DK / 8][4], const float* src, int V, int lane) {
-  const int g = lane >> 2, t2 = (lane & 3) * 2;
-#pragma unroll
-  for (int nt = 0; nt < DK / 8; ++nt)
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      s[nt][e] = src == nullptr ? 0.f : src[int64_t(8 * nt + t2 + (e & 1)) * V + g + 8 * (e >> 1)];
-}
-template <int DK>
-__device__ __forceinline__ void store_state(float* dst, const float s[DK / 8][4], int V, int lane) {
-  const int g = lane >> 2, t2 = (lane & 3) * 2;
-#pragma unroll
-  for (int nt = 0; nt < DK / 8; ++nt)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) dst[int64_t(8 * nt + t2 + (e & 1)) * V + g + 8 * (e >> 1)] = s[nt][e];
-}
-
-// The 16-bit rows of a warp's 16 value channels: accumulators x^T [16 x 64]
-// to dst [token][..] through the warp's own columns of a shared tile.
-template <class E>
-__device__ __forceinline__ void store_rows(const float x[8][4], uint32_t tile, int ldv, int c0,
-                                           const unsigned char* raw_tile, uint16_t* dst,
-                                           int64_t stride, int rows, int lane) {
-  __syncwarp();
-#pragma unroll
-  for (int ks = 0; ks < 4; ++ks) {
-    uint32_t r[4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      r[2 * i] = pack2_rn<E>(x[2 * ks + i][0], x[2 * ks + i][1]);
-      r[2 * i + 1] = pack2_rn<E>(x[2 * ks + i][2], x[2 * ks + i][3]);
-    }
-    stsm4_t(addr_at(tile, ldv, c0, 16 * ks, lane), r);
-  }
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int e = i * 32 + lane, r = e >> 1, c = (e & 1) * 8;
-    if (r < rows)
-      *reinterpret_cast<uint4*>(dst + r * stride + c) =
-          *reinterpret_cast<const uint4*>(raw_tile + 2 * (r * ldv + c0 + c));
-  }
-}
-
-// MODE 0: the forward (o and the final state).  MODE 1: the forward once more
-// for the gradients: U of each chunk and the state before it.
-template <class E, int DK, int W, int MODE>
-__global__ void __launch_bounds__(32 * W) delta_scan_kernel(const DeltaParams p) {
-  extern __shared__ __align__(16) unsigned char raw[];
-  using St = ScanStage<DK, W>;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int hv = blockIdx.y, h = hv / p.group;
-  const int tiles = p.V / (16 * W);
-  const int64_t n = blockIdx.x / tiles;
-  const int v0 = (blockIdx.x % tiles) * 16 * W, c0 = 16 * warp;
-  const SeqAt s = seq_at(p, n);
-  const int chunks = int((s.len + kChunk - 1) / kChunk);
-  const uint16_t* q = static_cast<const uint16_t*>(p.q) + s.b * p.q_sb + s.lo * p.q_st + h * p.q_sh;
-  const uint16_t* k = static_cast<const uint16_t*>(p.k) + s.b * p.k_sb + s.lo * p.k_st + h * p.k_sh;
-  const uint16_t* v = static_cast<const uint16_t*>(p.v) + s.b * p.v_sb + s.lo * p.v_st + hv * p.v_sh + v0;
-
-  auto fetch = [&](int c) {
-    const uint32_t st = smem_addr(raw) + (c & 1) * St::bytes;
-    const int64_t t0 = int64_t(c) * kChunk, slot = (s.chunk0 + c) * p.HV + hv;
-    const int rows = int(min(int64_t(kChunk), s.len - t0));
-    copy_rows(st + St::k, St::ld, k + t0 * p.k_st, p.k_st, kChunk, rows, DK / 8, tid, 32 * W);
-    copy_rows(st + St::v, St::ldv, v + t0 * p.v_st, p.v_st, kChunk, rows, 2 * W, tid, 32 * W);
-    copy_lower(st + St::t, p.tm + slot * 2 * kSq, tid, 32 * W);
-    if constexpr (MODE == 0) {
-      copy_rows(st + St::q, St::ld, q + t0 * p.q_st, p.q_st, kChunk, rows, DK / 8, tid, 32 * W);
-      copy_lower(st + St::p, p.pm + slot * 2 * kSq, tid, 32 * W);
-    }
-    const float* coef = p.coef + slot * 3 * kChunk;
-    for (int i = tid; i < 3 * kChunk / 4; i += 32 * W)
-      cp_async16(st + St::coef + 16 * i, coef + 4 * i, true);
-    cp_async_commit();
-  };
-
-  const int64_t state_at = ((n * p.HV + hv) * DK) * int64_t(p.V) + v0 + c0;
-  float S[DK / 8][4];
-  load_state<DK>(S, p.init == nullptr ? nullptr : p.init + state_at, p.V, lane);
-  if (chunks > 0) fetch(0);
-  for (int c = 0; c < chunks; ++c) {
-    if (c + 1 < chunks) {
-      fetch(c + 1);
-      cp_async_wait<1>();
-    } else {
-      cp_async_wait<0>();
-    }
-    __syncthreads();
-    unsigned char* stage = raw + (c & 1) * St::bytes;
-    const uint32_t st = smem_addr(stage);
-    const float* coef = reinterpret_cast<const float*>(stage + St::coef);
-    const int t2 = (lane & 3) * 2;
-    const int64_t slot = (s.chunk0 + c) * p.HV + hv;
-    if constexpr (MODE == 1) {
-      store_split<DK / 8>(p.sm + (slot * 2 * p.V + v0 + c0) * DK, int64_t(p.V) * DK, DK, S, lane);
-    }
-    float X[8][4] = {}, O[8][4] = {};
-    state_product<E, DK>(X, S, st + St::k, lane);
-    if constexpr (MODE == 0) state_product<E, DK>(O, S, st + St::q, lane);
-    // X = V - gam (K S), transposed: columns are tokens.
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      uint32_t r[4];
-      ldsm4_t(r, addr_at(st + St::v, St::ldv, c0, 16 * ks, lane));
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int nt = 2 * ks + i;
-        const float2 gam = *reinterpret_cast<const float2*>(coef + 8 * nt + t2);
-        float a, b;
-        unpack2<E>(r[2 * i], a, b);
-        X[nt][0] = a - gam.x * X[nt][0];
-        X[nt][1] = b - gam.y * X[nt][1];
-        unpack2<E>(r[2 * i + 1], a, b);
-        X[nt][2] = a - gam.x * X[nt][2];
-        X[nt][3] = b - gam.y * X[nt][3];
-        O[nt][0] *= p.scale * gam.x;
-        O[nt][1] *= p.scale * gam.y;
-        O[nt][2] *= p.scale * gam.x;
-        O[nt][3] *= p.scale * gam.y;
-      }
-    }
-    float U[8][4] = {};
-    lower_product(U, X, st + St::t, lane);
-    if constexpr (MODE == 1) {
-      store_split<8>(p.um + (slot * 2 * p.V + v0 + c0) * kChunk, int64_t(p.V) * kChunk, kChunk, U,
-                     lane);
-    }
-#pragma unroll
-    for (int nt = 0; nt < 8; ++nt) {
-      const float2 be = *reinterpret_cast<const float2*>(coef + 2 * kChunk + 8 * nt + t2);
-      U[nt][0] *= be.x;
-      U[nt][1] *= be.y;
-      U[nt][2] *= be.x;
-      U[nt][3] *= be.y;
-    }
-    if constexpr (MODE == 0) {
-      lower_product(O, U, st + St::p, lane);
-      uint16_t* o = static_cast<uint16_t*>(p.o) +
-                    ((s.b * p.T + s.lo + int64_t(c) * kChunk) * p.HV + hv) * p.V + v0 + c0;
-      store_rows<E>(O, st + St::v, St::ldv, c0, stage + St::v, o, int64_t(p.HV) * p.V,
-                    int(min(int64_t(kChunk), s.len - int64_t(c) * kChunk)), lane);
-    }
-    // S = gam_63 S + K^T (w V')
-    const float last = coef[kChunk - 1];
-#pragma unroll
-    for (int nt = 0; nt < DK / 8; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) S[nt][e] *= last;
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-#pragma unroll
-      for (int nt = 2 * ks; nt < 2 * ks + 2; ++nt) {
-        const float2 w = *reinterpret_cast<const float2*>(coef + kChunk + 8 * nt + t2);
-        U[nt][0] *= w.x;
-        U[nt][1] *= w.y;
-        U[nt][2] *= w.x;
-        U[nt][3] *= w.y;
-      }
-      uint32_t ah[4], al[4];
-      split_frag(U[2 * ks], U[2 * ks + 1], ah, al);
-      state_update<E, DK>(S, ah, al, st + St::k, ks, lane);
-    }
-    __syncthreads();
-  }
-  if (MODE == 0 && p.final_state != nullptr) store_state<DK>(p.final_state + state_at, S, p.V, lane);
-}
-
-// ---- gradients: the walk back ---------------------------------------------------------
-//   dV' = P^T dO + diag(w) K dS      dX = T^T diag(beta) dV'  (= dV)
-//   dS <- gam_63 dS + scale Q^T diag(gam) dO - K^T diag(gam) dX
-// dS^T [16 x K] stays in a warp's accumulators as S^T does; dS behind each
-// chunk and dX go to the workspace for delta_grad_kernel.
-template <class E, int DK, int W>
-__global__ void __launch_bounds__(32 * W) delta_scan_back_kernel(const DeltaParams p) {
-  extern __shared__ __align__(16) unsigned char raw[];
-  using St = ScanStage<DK, W>;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int hv = blockIdx.y, h = hv / p.group;
-  const int tiles = p.V / (16 * W);
-  const int64_t n = blockIdx.x / tiles;
-  const int v0 = (blockIdx.x % tiles) * 16 * W, c0 = 16 * warp;
-  const SeqAt s = seq_at(p, n);
-  const int chunks = int((s.len + kChunk - 1) / kChunk);
-  const uint16_t* q = static_cast<const uint16_t*>(p.q) + s.b * p.q_sb + s.lo * p.q_st + h * p.q_sh;
-  const uint16_t* k = static_cast<const uint16_t*>(p.k) + s.b * p.k_sb + s.lo * p.k_st + h * p.k_sh;
-  const uint16_t* d_o = static_cast<const uint16_t*>(p.d_o) + s.b * p.do_sb + s.lo * p.do_st +
-                        hv * p.do_sh + v0;
-
-  auto fetch = [&](int c) {
-    const uint32_t st = smem_addr(raw) + (c & 1) * St::bytes;
-    const int64_t t0 = int64_t(c) * kChunk, slot = (s.chunk0 + c) * p.HV + hv;
-    const int rows = int(min(int64_t(kChunk), s.len - t0));
-    copy_rows(st + St::k, St::ld, k + t0 * p.k_st, p.k_st, kChunk, rows, DK / 8, tid, 32 * W);
-    copy_rows(st + St::q, St::ld, q + t0 * p.q_st, p.q_st, kChunk, rows, DK / 8, tid, 32 * W);
-    copy_rows(st + St::v, St::ldv, d_o + t0 * p.do_st, p.do_st, kChunk, rows, 2 * W, tid, 32 * W);
-    copy_lower(st + St::t, p.tm + slot * 2 * kSq, tid, 32 * W);
-    copy_lower(st + St::p, p.pm + slot * 2 * kSq, tid, 32 * W);
-    const float* coef = p.coef + slot * 3 * kChunk;
-    for (int i = tid; i < 3 * kChunk / 4; i += 32 * W)
-      cp_async16(st + St::coef + 16 * i, coef + 4 * i, true);
-    cp_async_commit();
-  };
-
-  const int64_t state_at = ((n * p.HV + hv) * DK) * int64_t(p.V) + v0 + c0;
-  float D[DK / 8][4];
-  load_state<DK>(D, p.dfinal == nullptr ? nullptr : p.dfinal + state_at, p.V, lane);
-  if (chunks > 0) fetch(chunks - 1);
-  for (int c = chunks - 1; c >= 0; --c) {
-    if (c > 0) {
-      fetch(c - 1);
-      cp_async_wait<1>();
-    } else {
-      cp_async_wait<0>();
-    }
-    __syncthreads();
-    unsigned char* stage = raw + (c & 1) * St::bytes;
-    const uint32_t st = smem_addr(stage);
-    const float* coef = reinterpret_cast<const float*>(stage + St::coef);
-    const int t2 = (lane & 3) * 2;
-    const int64_t slot = (s.chunk0 + c) * p.HV + hv;
-    store_split<DK / 8>(p.dm + (slot * 2 * p.V + v0 + c0) * DK, int64_t(p.V) * DK, DK, D, lane);
-    float X[8][4] = {};
-    state_product<E, DK>(X, D, st + St::k, lane);
-#pragma unroll
-    for (int nt = 0; nt < 8; ++nt) {
-      const float2 w = *reinterpret_cast<const float2*>(coef + kChunk + 8 * nt + t2);
-      X[nt][0] *= w.x;
-      X[nt][1] *= w.y;
-      X[nt][2] *= w.x;
-      X[nt][3] *= w.y;
-    }
-    // += dO^T P, dO^T exact (fp16: split exactly)
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      uint32_t a[4], ah[4], al[4];
-      ldsm4_t(a, addr_at(st + St::v, St::ldv, c0, 16 * ks, lane));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) split_elem<E>(a[i], ah[i], al[i]);
-#pragma unroll
-      for (int np = 0; np <= ks; ++np) {
-        uint32_t bh[4], bl[4];
-        ldsm4_t(bh, addr_bt(st + St::p, kLdT, 16 * np, 16 * ks, lane));
-        ldsm4_t(bl, addr_bt(st + St::p + kChunk * kLdT * 2, kLdT, 16 * np, 16 * ks, lane));
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          mma_bf16(X[2 * np + i], ah, bh[2 * i], bh[2 * i + 1]);
-          mma_bf16(X[2 * np + i], ah, bl[2 * i], bl[2 * i + 1]);
-          if constexpr (!std::is_same_v<E, BF16>) mma_bf16(X[2 * np + i], al, bh[2 * i], bh[2 * i + 1]);
-        }
-      }
-    }
-#pragma unroll
-    for (int nt = 0; nt < 8; ++nt) {
-      const float2 be = *reinterpret_cast<const float2*>(coef + 2 * kChunk + 8 * nt + t2);
-      X[nt][0] *= be.x;
-      X[nt][1] *= be.y;
-      X[nt][2] *= be.x;
-      X[nt][3] *= be.y;
-    }
-    float Y[8][4] = {};
-    lower_product_t(Y, X, st + St::t, lane);
-    store_split<8>(p.xm + (slot * 2 * p.V + v0 + c0) * kChunk, int64_t(p.V) * kChunk, kChunk, Y, lane);
-    const float last = coef[kChunk - 1];
-#pragma unroll
-    for (int nt = 0; nt < DK / 8; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) D[nt][e] *= last;
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      uint32_t a[4], ah[4], al[4];
-      ldsm4_t(a, addr_at(st + St::v, St::ldv, c0, 16 * ks, lane));
-      float z[2][4];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float2 gam = *reinterpret_cast<const float2*>(coef + 8 * (2 * ks + i) + t2);
-        unpack2<E>(a[2 * i], z[i][0], z[i][1]);
-        unpack2<E>(a[2 * i + 1], z[i][2], z[i][3]);
-        z[i][0] *= p.scale * gam.x;
-        z[i][1] *= p.scale * gam.y;
-        z[i][2] *= p.scale * gam.x;
-        z[i][3] *= p.scale * gam.y;
-      }
-      split_frag(z[0], z[1], ah, al);
-      state_update<E, DK>(D, ah, al, st + St::q, ks, lane);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float2 gam = *reinterpret_cast<const float2*>(coef + 8 * (2 * ks + i) + t2);
-        z[i][0] = -gam.x * Y[2 * ks + i][0];
-        z[i][1] = -gam.y * Y[2 * ks + i][1];
-        z[i][2] = -gam.x * Y[2 * ks + i][2];
-        z[i][3] = -gam.y * Y[2 * ks + i][3];
-      }
-      split_frag(z[0], z[1], ah, al);
-      state_update<E, DK>(D, ah, al, st + St::k, ks, lane);
-    }
-    uint16_t* dv = static_cast<uint16_t*>(p.dv) +
-                   ((s.b * p.T + s.lo + int64_t(c) * kChunk) * p.HV + hv) * p.V + v0 + c0;
-    store_rows<E>(Y, st + St::v, St::ldv, c0, stage + St::v, dv, int64_t(p.HV) * p.V,
-                  int(min(int64_t(kChunk), s.len - int64_t(c) * kChunk)), lane);
-    __syncthreads();
-  }
-  if (p.dinit != nullptr) store_state<DK>(p.dinit + state_at, D, p.V, lane);
 }
 
 // ---- gradients of a chunk ------------------------------------------------------------

@@ -1,0 +1,635 @@
+// tdc_delta_walk.cuh — the walk over a sequence's chunks, forward and back, on
+// the 5th-generation tensor cores.
+//
+// The columns of S (the value channels) do not mix, so one block takes 128
+// value channels of one head of one sequence and keeps S^T: one lane of TMEM
+// a channel.  Every product of a chunk then has the state's side as its A
+// operand (M = 128 channels, in TMEM) and a tile that all channels share as B
+// (K, Q, T, P, in shared memory):
+//   Y^T = S^T K^T                  X^T = V^T - gam Y^T
+//   U^T = X^T T^T                  V'^T = beta U^T
+//   O^T = scale gam (S^T Q^T) + V'^T P^T
+//   S^T <- gam_63 S^T + (w V'^T) K
+// A thread owns one channel and half of the columns, so scaling, splitting and
+// the running state are thread-local; what a chunk costs is the chain of three
+// dependent products (the walk is bound by its latency, with few sequences and
+// heads, and by nothing else before the number of blocks passes the SMs).  Q's
+// and P's products and the output run beside the chain.
+//
+// Warps 0-7 compute (warp % 4 picks the lanes, warp / 4 the half of the
+// columns), warp 8 issues the products, warp 9 the bulk copies of the next
+// chunk's tiles (two stages; delta_prepare has laid them out as the tensor
+// cores read them, rows behind the sequence's end zeroed).  Every wait is
+// bounded; a wait that gives up records the failure and ends the block.
+#pragma once
+
+#include "tdc_delta.cuh"
+#include "tdc_tc.cuh"
+
+namespace tdc {
+
+// Tiles of a chunk in the workspace and in shared memory, in order.  KP: parts
+// of an exact element (1 bf16, 2 fp16).
+template <class E, int DK>
+struct WalkTiles {
+  static constexpr int KP = std::is_same_v<E, BF16> ? 1 : 2;
+  static constexpr int keys = kChunk * DK * 2;        // one part of K or Q
+  static constexpr int k = 0;
+  static constexpr int q = k + KP * keys;
+  static constexpr int t = q + KP * keys;
+  static constexpr int p = t + 2 * kSq * 2;
+  static constexpr int coef = p + 2 * kSq * 2;
+  static constexpr int stage = coef + 3 * kChunk * 4;
+};
+
+// Shared memory behind the two stages.
+struct WalkSync {
+  uint64_t full[2], free[2];
+  uint64_t y, u, q, s, o;                 // products done
+  uint64_t sr, xr, vr, qr, gr;            // operands ready (or results read)
+  uint64_t drain;
+  uint32_t tmem;
+  int abort;
+};
+
+constexpr int kWalkThreads = 320;
+constexpr uint32_t kTmemColumns = 512;
+
+struct Waiter {
+  volatile int* abort;
+  uint64_t timeout_ns;
+  int* words;
+  int* host;
+  int block;
+
+  // False once the block has to end.
+  __device__ __forceinline__ bool operator()(uint64_t& bar, uint32_t parity, int code, int64_t at) const {
+    if (mbar_wait_bounded(smem_addr(&bar), parity & 1u, abort, true, timeout_ns)) return true;
+    if (!*abort) {
+      record_wait_failure(words, host, code, block, int(parity & 1u), at);
+      *abort = 1;
+    }
+    return false;
+  }
+};
+
+// v as bf16 high parts and remainders, 16 packed columns each, to TMEM columns
+// at and at + step; both are left in hi and lo.
+__device__ __forceinline__ void split_to_tmem(const float (&v)[32], uint32_t at, uint32_t step,
+                                              uint32_t (&hi)[16], uint32_t (&lo)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) split2(v[2 * i], v[2 * i + 1], hi[i], lo[i]);
+  tmem_st(at, hi);
+  tmem_st(at + step, lo);
+}
+
+// For whole warps: all lanes go on, or none does.
+__device__ __forceinline__ bool warp_wait(const Waiter& wait, uint64_t& bar, int phase) {
+  const bool ok = wait(bar, uint32_t(phase), TDC_DEVICE_FULL_TIMEOUT, phase);
+  return __all_sync(0xffffffffu, ok);
+}
+
+// Operands are stored: make them visible to the tensor core and tell warp 8.
+__device__ __forceinline__ void operand_ready(uint64_t& bar, int lane) {
+  tmem_wait_st();
+  tc_fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(smem_addr(&bar));
+}
+
+// The 8 computing warps, between one's TMEM loads and another's stores.
+__device__ __forceinline__ void compute_sync() {
+  tc_fence_before();
+  asm volatile("bar.sync 1, 256;" ::: "memory");
+  tc_fence_after();
+}
+
+// d (+)= A B over DEPTH contraction elements; A split in two parts at a, a +
+// astep (columns), B in BP parts bstep bytes apart.  kstep: bytes from 16
+// contraction elements of B to the next.  The remainders' product is left out.
+template <int DEPTH, int BP>
+__device__ __forceinline__ void issue_product(uint32_t d, uint32_t a, uint32_t astep, uint32_t b,
+                                              uint32_t bstep, uint32_t kstep, uint32_t leading,
+                                              uint32_t stride, uint32_t desc, bool accumulate) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < BP; ++j) {
+      if (i + j > 1) continue;
+#pragma unroll
+      for (int ks = 0; ks < DEPTH / 16; ++ks) {
+        tc_mma(d, a + i * astep + 8 * ks, smem_desc(b + j * bstep + ks * kstep, leading, stride), desc,
+               accumulate || i + j + ks > 0);
+      }
+    }
+}
+
+// d = A M^T (back: A M) for a lower triangular split [64][64] tile M: only the
+// blocks on and below the diagonal are read.  AP: parts of A.
+template <bool BACK, int AP>
+__device__ __forceinline__ void issue_lower(uint32_t d, uint32_t a, uint32_t astep, uint32_t m,
+                                            bool accumulate) {
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const int ks = BACK ? 3 - x : x;  // the step that fills all columns first
+    const uint32_t n = BACK ? 16 * (ks + 1) : 64 - 16 * ks;
+#pragma unroll
+    for (int i = 0; i < AP; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (i + j > 1) continue;
+        const uint32_t b = m + j * kSq * 2;
+        if constexpr (BACK)
+          tc_mma(d, a + i * astep + 8 * ks, smem_desc(b + ks * 2 * kRowBlock, kRowBlock, kColBlock),
+                 mma_desc(n, true), accumulate || x + i + j > 0);
+        else
+          tc_mma(d + 16 * ks, a + i * astep + 8 * ks,
+                 smem_desc(b + ks * (2 * kRowBlock + 2 * kColBlock), kColBlock, kRowBlock),
+                 mma_desc(n, false), accumulate || x + i + j > 0);
+      }
+  }
+}
+
+__device__ __forceinline__ void walk_setup(WalkSync* sy, int tid, int warp) {
+  if (warp == 8) tmem_alloc(smem_addr(&sy->tmem), kTmemColumns);
+  if (tid == 0) {
+    for (uint64_t* b : {&sy->full[0], &sy->full[1], &sy->free[0], &sy->free[1], &sy->y, &sy->u,
+                        &sy->q, &sy->s, &sy->o, &sy->drain})
+      mbar_init(smem_addr(b), 1);
+    for (uint64_t* b : {&sy->sr, &sy->xr, &sy->vr, &sy->qr, &sy->gr}) mbar_init(smem_addr(b), 8);
+    sy->abort = 0;
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+}
+
+// Warp 9, one thread: the tiles of each chunk in turn.
+template <class E, int DK, bool KEYS_ONLY>
+__device__ __forceinline__ void walk_fetch(const DeltaParams& p, unsigned char* raw, WalkSync* sy,
+                                           const Waiter& wait, const SeqAt& s, int chunks, int h,
+                                           int hv, bool back) {
+  using W = WalkTiles<E, DK>;
+  int issued = 0;
+  for (int c = 0; c < chunks; ++c) {
+    const int st = c & 1;
+    if (c >= 2 && !wait(sy->free[st], uint32_t((c >> 1) - 1), TDC_DEVICE_EMPTY_TIMEOUT, c)) break;
+    const int64_t chunk = s.chunk0 + (back ? chunks - 1 - c : c), slot = chunk * p.HV + hv;
+    const uint32_t dst = smem_addr(raw) + st * W::stage, bar = smem_addr(&sy->full[st]);
+    const unsigned char* keys = p.kq + (chunk * p.H + h) * (2 * W::KP * W::keys);
+    constexpr uint32_t kbytes = KEYS_ONLY ? W::KP * W::keys : 2 * W::KP * W::keys;
+    constexpr uint32_t tbytes = KEYS_ONLY ? 2 * kSq * 2 : 4 * kSq * 2;
+    mbar_arrive_expect_tx(bar, kbytes + tbytes + 3 * kChunk * 4);
+    bulk_load(dst + W::k, keys, kbytes, bar);
+    bulk_load(dst + W::t, p.tp + slot * (4 * kSq), tbytes, bar);
+    bulk_load(dst + W::coef, p.coef + slot * 3 * kChunk, 3 * kChunk * 4, bar);
+    issued = c + 1;
+  }
+  // No copy is in flight when the block ends.
+  for (int c = issued > 2 ? issued - 2 : 0; c < issued; ++c)
+    mbar_wait_bounded(smem_addr(&sy->full[c & 1]), uint32_t(c >> 1) & 1u, wait.abort, false,
+                      wait.timeout_ns);
+}
+
+// S^T of this thread: its channel, DK / 2 keys from k0.
+template <int DK>
+__device__ __forceinline__ void walk_load(float (&S)[DK / 2], const float* src, int V, bool live) {
+#pragma unroll
+  for (int i = 0; i < DK / 2; ++i) S[i] = src != nullptr && live ? src[int64_t(i) * V] : 0.f;
+}
+template <int DK>
+__device__ __forceinline__ void walk_store(float* dst, const float (&S)[DK / 2], int V, bool live) {
+  if (!live) return;
+#pragma unroll
+  for (int i = 0; i < DK / 2; ++i) dst[int64_t(i) * V] = S[i];
+}
+
+// 32 tokens of this thread's channel, raw 16-bit, zeros behind `rows`.
+__device__ __forceinline__ void walk_column(uint32_t (&v)[32], const uint16_t* src, int64_t stride,
+                                            int t0, int rows, bool live) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = live && t0 + i < rows ? src[(t0 + i) * stride] : 0u;
+}
+
+template <class E>
+__device__ __forceinline__ float widen(uint32_t raw) {
+  if constexpr (std::is_same_v<E, BF16>) return __uint_as_float(raw << 16);
+  else return __half2float(__ushort_as_half(static_cast<unsigned short>(raw)));
+}
+
+// 16 packed pairs (32 tokens or keys) to a row of the workspace.
+__device__ __forceinline__ void store_pairs(__nv_bfloat16* dst, const uint32_t (&r)[16], bool live) {
+  if (!live) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    reinterpret_cast<uint4*>(dst)[i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+}
+
+// MODE 0: the forward (o and the final state).  MODE 1: the forward once more
+// for the gradients: U of each chunk and the state before it.
+template <class E, int DK, int MODE>
+__global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const DeltaParams p) {
+  extern __shared__ __align__(1024) unsigned char raw[];
+  using W = WalkTiles<E, DK>;
+  constexpr int KP = W::KP;
+  WalkSync* sy = reinterpret_cast<WalkSync*>(raw + 2 * W::stage);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int hv = blockIdx.y, h = hv / p.group;
+  const int tiles = (p.V + 127) / 128;
+  const int64_t n = blockIdx.x / tiles;
+  const int v0 = int(blockIdx.x % tiles) * 128;
+  const SeqAt s = seq_at(p, n);
+  const int chunks = int((s.len + kChunk - 1) / kChunk);
+  walk_setup(sy, tid, warp);
+  const Waiter wait{&sy->abort, p.timeout_ns, p.status_words, p.status_host, int(blockIdx.x)};
+  const uint32_t tm = sy->tmem;
+  // TMEM columns: Y, then U; O; S^T parts, then the state's update; X, then w V'; V'
+  constexpr uint32_t cY = 0, cO = 64, cS = 128, cX = 320, cV = 416;
+  constexpr uint32_t sStep = DK / 2, xStep = 32;
+
+  if (warp == 9) {
+    if (lane == 0) walk_fetch<E, DK, MODE == 1>(p, raw, sy, wait, s, chunks, h, hv, false);
+  } else if (warp == 8) {
+    if (lane == 0) {
+      for (int c = 0; c < chunks; ++c) {
+        const uint32_t st = smem_addr(raw) + (c & 1) * W::stage;
+        if (!wait(sy->full[c & 1], uint32_t(c >> 1), TDC_DEVICE_FULL_TIMEOUT, c)) break;
+        if (!wait(sy->sr, uint32_t(c), TDC_DEVICE_FULL_TIMEOUT, c)) break;
+        tc_fence_after();
+        issue_product<DK, KP>(tm + cY, tm + cS, sStep, st + W::k, W::keys, 2 * kColBlock, kColBlock,
+                              kRowBlock, mma_desc(64, false), false);
+        tc_commit(smem_addr(&sy->y));
+        if (!wait(sy->xr, uint32_t(c), TDC_DEVICE_FULL_TIMEOUT, c)) break;
+        tc_fence_after();
+        issue_lower<false, 2>(tm + cY, tm + cX, xStep, st + W::t, false);
+        tc_commit(smem_addr(&sy->u));
+        if constexpr (MODE == 0) {
+          issue_product<DK, KP>(tm + cO, tm + cS, sStep, st + W::q, W::keys, 2 * kColBlock, kColBlock,
+                                kRowBlock, mma_desc(64, false), false);
+          tc_commit(smem_addr(&sy->q));
+        }
+        if (!wait(sy->vr, uint32_t(c), TDC_DEVICE_FULL_TIMEOUT, c)) break;
+        tc_fence_after();
+        issue_product<kChunk, KP>(tm + cS, tm + cX, xStep, st + W::k, W::keys, 2 * kRowBlock,
+                                  kRowBlock, kColBlock, mma_desc(DK, true), false);
+        tc_commit(smem_addr(&sy->s));
+        if constexpr (MODE == 0) {
+          if (!wait(sy->qr, uint32_t(c), TDC_DEVICE_FULL_TIMEOUT, c)) break;
+          tc_fence_after();
+          issue_lower<false, 2>(tm + cO, tm + cV, xStep, st + W::p, false);
+          tc_commit(smem_addr(&sy->o));
+        }
+        tc_commit(smem_addr(&sy->free[c & 1]));
+      }
+      tc_commit(smem_addr(&sy->drain));
+      mbar_wait_bounded(smem_addr(&sy->drain), 0, wait.abort, false, wait.timeout_ns);
+    }
+  } else {
+    const uint32_t lanes = tm + (uint32_t(warp & 3) << 21);  // 32 lanes a quadrant
+    const int half = warp >> 2, ch = v0 + 32 * (warp & 3) + lane, t0 = 32 * half;
+    const bool live = ch < p.V;
+    const int64_t state_at = ((n * p.HV + hv) * DK + half * (DK / 2)) * int64_t(p.V) + ch;
+    const uint16_t* v = static_cast<const uint16_t*>(p.v) + s.b * p.v_sb + s.lo * p.v_st + hv * p.v_sh + ch;
+    uint16_t* o = static_cast<uint16_t*>(p.o) + ((s.b * p.T + s.lo) * p.HV + hv) * p.V + ch;
+    float S[DK / 2];
+    walk_load<DK>(S, p.init == nullptr ? nullptr : p.init + state_at, p.V, live);
+    uint32_t vr[32], hi[16], lo[16];
+    walk_column(vr, v, p.v_st, t0, int(min(int64_t(kChunk), s.len)), live);
+    float qs[32];     // scale gam S^T Q^T of the chunk
+    float last = 1.f; // gam_63 of the chunk before
+    bool ok = true;
+    // Output of a chunk: qs plus P's product.
+    auto put_out = [&](int c) {
+      ok = warp_wait(wait, sy->o, c);
+      if (!ok) return;
+      tc_fence_after();
+      uint32_t r[32];
+      tmem_ld(lanes + cO + t0, r);
+      const int64_t at = int64_t(c) * kChunk + t0;
+      const int rows = int(min(int64_t(32), s.len - at));
+      if (!live) return;
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i < rows)
+          o[(at + i) * p.HV * p.V] = uint16_t(pack2_rn<E>(qs[i] + __uint_as_float(r[i]), 0.f));
+    };
+    // The state after the chunk before: gam_63 S + its update.
+    auto advance = [&](int c) {
+      ok = warp_wait(wait, sy->s, c);
+      if (!ok) return;
+      tc_fence_after();
+      uint32_t r[DK / 2];
+      tmem_ld(lanes + cS + half * (DK / 2), r);
+#pragma unroll
+      for (int i = 0; i < DK / 2; ++i) S[i] = fmaf(last, S[i], __uint_as_float(r[i]));
+    };
+    for (int c = 0; c < chunks; ++c) {
+      const float* coef =
+          reinterpret_cast<const float*>(raw + (c & 1) * W::stage + W::coef);
+      const int64_t slot = (s.chunk0 + c) * p.HV + hv;
+      if (c > 0) {
+        advance(c - 1);
+        if (!ok) break;
+        compute_sync();  // the update lies where S^T's parts go: everyone has read it first
+      }
+#pragma unroll
+      for (int x = 0; x < DK / 64; ++x) {
+        float w[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) w[i] = S[32 * x + i];
+        split_to_tmem(w, lanes + cS + half * (DK / 4) + 16 * x, sStep, hi, lo);
+        if constexpr (MODE == 1) {
+          __nv_bfloat16* dst = p.sm + (slot * 2 * p.V + ch) * DK + half * (DK / 2) + 32 * x;
+          store_pairs(dst, hi, live);
+          store_pairs(dst + int64_t(p.V) * DK, lo, live);
+        }
+      }
+      operand_ready(sy->sr, lane);
+      if (MODE == 0 && c > 0) {
+        put_out(c - 1);
+        if (!ok) break;
+      }
+      // X = V - gam Y
+      ok = warp_wait(wait, sy->full[c & 1], c >> 1);  // (the coefficients)
+      if (!ok) break;
+      ok = warp_wait(wait, sy->y, c);
+      if (!ok) break;
+      tc_fence_after();
+      {
+        uint32_t r[32];
+        tmem_ld(lanes + cY + t0, r);
+        float x[32];
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 gam = *reinterpret_cast<const float4*>(coef + t0 + i);
+          x[i] = widen<E>(vr[i]) - gam.x * __uint_as_float(r[i]);
+          x[i + 1] = widen<E>(vr[i + 1]) - gam.y * __uint_as_float(r[i + 1]);
+          x[i + 2] = widen<E>(vr[i + 2]) - gam.z * __uint_as_float(r[i + 2]);
+          x[i + 3] = widen<E>(vr[i + 3]) - gam.w * __uint_as_float(r[i + 3]);
+        }
+        split_to_tmem(x, lanes + cX + t0 / 2, xStep, hi, lo);
+      }
+      operand_ready(sy->xr, lane);
+      if (c + 1 < chunks)
+        walk_column(vr, v + int64_t(c + 1) * kChunk * p.v_st, p.v_st, t0,
+                    int(min(int64_t(kChunk), s.len - int64_t(c + 1) * kChunk)), live);
+      // V' = beta U and w V'
+      ok = warp_wait(wait, sy->u, c);
+      if (!ok) break;
+      tc_fence_after();
+      last = coef[kChunk - 1];
+      {
+        uint32_t r[32];
+        tmem_ld(lanes + cY + t0, r);
+        float u[32], x[32];
+        if constexpr (MODE == 1) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            split2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), hi[i], lo[i]);
+          __nv_bfloat16* dst = p.um + (slot * 2 * p.V + ch) * kChunk + t0;
+          store_pairs(dst, hi, live);
+          store_pairs(dst + int64_t(p.V) * kChunk, lo, live);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 w = *reinterpret_cast<const float4*>(coef + kChunk + t0 + i);
+          const float4 be = *reinterpret_cast<const float4*>(coef + 2 * kChunk + t0 + i);
+          u[i] = be.x * __uint_as_float(r[i]);
+          u[i + 1] = be.y * __uint_as_float(r[i + 1]);
+          u[i + 2] = be.z * __uint_as_float(r[i + 2]);
+          u[i + 3] = be.w * __uint_as_float(r[i + 3]);
+          x[i] = w.x * u[i];
+          x[i + 1] = w.y * u[i + 1];
+          x[i + 2] = w.z * u[i + 2];
+          x[i + 3] = w.w * u[i + 3];
+        }
+        split_to_tmem(x, lanes + cX + t0 / 2, xStep, hi, lo);
+        operand_ready(sy->vr, lane);
+        if constexpr (MODE == 0) {
+          // beside the chain: V' for the output, and Q's product
+          split_to_tmem(u, lanes + cV + t0 / 2, xStep, hi, lo);
+          ok = warp_wait(wait, sy->q, c);
+          if (!ok) break;
+          tc_fence_after();
+          tmem_ld(lanes + cO + t0, r);
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 gam = *reinterpret_cast<const float4*>(coef + t0 + i);
+            qs[i] = p.scale * gam.x * __uint_as_float(r[i]);
+            qs[i + 1] = p.scale * gam.y * __uint_as_float(r[i + 1]);
+            qs[i + 2] = p.scale * gam.z * __uint_as_float(r[i + 2]);
+            qs[i + 3] = p.scale * gam.w * __uint_as_float(r[i + 3]);
+          }
+          operand_ready(sy->qr, lane);
+        }
+      }
+    }
+    if (ok && chunks > 0) {
+      advance(chunks - 1);
+      if (MODE == 0 && ok) put_out(chunks - 1);
+    }
+    if (MODE == 0 && ok && p.final_state != nullptr)
+      walk_store<DK>(p.final_state + state_at, S, p.V, live);
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) tmem_free(tm, kTmemColumns);
+}
+
+// The walk back:
+//   dV' = P^T dO + w (K dS)        dX = T^T (beta dV')  (= dV)
+//   dS <- gam_63 dS + scale Q^T (gam dO) - K^T (gam dX)
+// with dS^T in the lanes.  dS behind each chunk and dX go to the workspace.
+template <class E, int DK>
+__global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const DeltaParams p) {
+  extern __shared__ __align__(1024) unsigned char raw[];
+  using W = WalkTiles<E, DK>;
+  constexpr int KP = W::KP;
+  WalkSync* sy = reinterpret_cast<WalkSync*>(raw + 2 * W::stage);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int hv = blockIdx.y, h = hv / p.group;
+  const int tiles = (p.V + 127) / 128;
+  const int64_t n = blockIdx.x / tiles;
+  const int v0 = int(blockIdx.x % tiles) * 128;
+  const SeqAt s = seq_at(p, n);
+  const int chunks = int((s.len + kChunk - 1) / kChunk);
+  walk_setup(sy, tid, warp);
+  const Waiter wait{&sy->abort, p.timeout_ns, p.status_words, p.status_host, int(blockIdx.x)};
+  const uint32_t tm = sy->tmem;
+  // TMEM columns: K dS, then dX; dS^T parts, then the state's update; P^T dO; dO (exact);
+  // gam dO; beta dV', then -gam dX
+  constexpr uint32_t cY = 0, cS = 64, cP = 192, cO = 256, cG = 320, cX = 384;
+  constexpr uint32_t sStep = DK / 2, xStep = 32;
+
+  if (warp == 9) {
+    if (lane == 0) walk_fetch<E, DK, false>(p, raw, sy, wait, s, chunks, h, hv, true);
+  } else if (warp == 8) {
+    if (lane == 0) {
+      for (int c = 0; c < chunks; ++c) {
+        const uint32_t st = smem_addr(raw) + (c & 1) * W::stage;
+        if (!wait(sy->full[c & 1], uint32_t(c >> 1), TDC_DEVICE_FULL_TIMEOUT, c)) break;
+        if (!wait(sy->gr, uint32_t(c), TDC_DEVICE_FULL_TIMEOUT, c)) break;
+        tc_fence_after();
+        issue_lower<true, KP>(tm + cP, tm + cO, xStep, st + W::p, false);
+        if (!wait(sy->sr, uint32_t(c), TDC_DEVICE_FULL_TIMEOUT, c)) break;
+        tc_fence_after();
+        issue_product<DK, KP>(tm + cY, tm + cS, sStep, st + W::k, W::keys, 2 * kColBlock, kColBlock,
+                              kRowBlock, mma_desc(64, false), false);
+        tc_commit(smem_addr(&sy->y));
+        if (!wait(sy->xr, uint32_t(c), TDC_DEVICE_FULL_TIMEOUT, c)) break;
+        tc_fence_after();
+        issue_lower<true, 2>(tm + cY, tm + cX, xStep, st + W::t, false);
+        tc_commit(smem_addr(&sy->u));
+        // (K dS has read dS^T's parts: the update may take their place)
+        if (!wait(sy->qr, uint32_t(c), TDC_DEVICE_FULL_TIMEOUT, c)) break;
+        tc_fence_after();
+        issue_product<kChunk, KP>(tm + cS, tm + cG, xStep, st + W::q, W::keys, 2 * kRowBlock,
+                                  kRowBlock, kColBlock, mma_desc(DK, true), false);
+        if (!wait(sy->vr, uint32_t(c), TDC_DEVICE_FULL_TIMEOUT, c)) break;
+        tc_fence_after();
+        issue_product<kChunk, KP>(tm + cS, tm + cX, xStep, st + W::k, W::keys, 2 * kRowBlock,
+                                  kRowBlock, kColBlock, mma_desc(DK, true), true);
+        tc_commit(smem_addr(&sy->s));
+        tc_commit(smem_addr(&sy->free[c & 1]));
+      }
+      tc_commit(smem_addr(&sy->drain));
+      mbar_wait_bounded(smem_addr(&sy->drain), 0, wait.abort, false, wait.timeout_ns);
+    }
+  } else {
+    const uint32_t lanes = tm + (uint32_t(warp & 3) << 21);
+    const int half = warp >> 2, ch = v0 + 32 * (warp & 3) + lane, t0 = 32 * half;
+    const bool live = ch < p.V;
+    const int64_t state_at = ((n * p.HV + hv) * DK + half * (DK / 2)) * int64_t(p.V) + ch;
+    const uint16_t* d_o = static_cast<const uint16_t*>(p.d_o) + s.b * p.do_sb + s.lo * p.do_st +
+                          hv * p.do_sh + ch;
+    uint16_t* dv = static_cast<uint16_t*>(p.dv) + ((s.b * p.T + s.lo) * p.HV + hv) * p.V + ch;
+    float D[DK / 2];
+    walk_load<DK>(D, p.dfinal == nullptr ? nullptr : p.dfinal + state_at, p.V, live);
+    uint32_t vr[32], hi[16], lo[16];
+    auto fetch_do = [&](int c) {  // c counts from the end
+      const int64_t at = int64_t(chunks - 1 - c) * kChunk;
+      walk_column(vr, d_o + at * p.do_st, p.do_st, t0, int(min(int64_t(kChunk), s.len - at)), live);
+    };
+    if (chunks > 0) fetch_do(0);
+    float last = 1.f;
+    bool ok = true;
+    auto advance = [&](int c) {
+      ok = warp_wait(wait, sy->s, c);
+      if (!ok) return;
+      tc_fence_after();
+      uint32_t r[DK / 2];
+      tmem_ld(lanes + cS + half * (DK / 2), r);
+#pragma unroll
+      for (int i = 0; i < DK / 2; ++i) D[i] = fmaf(last, D[i], __uint_as_float(r[i]));
+    };
+    for (int c = 0; c < chunks; ++c) {
+      const int cc = chunks - 1 - c;
+      const float* coef =
+          reinterpret_cast<const float*>(raw + (c & 1) * W::stage + W::coef);
+      const int64_t slot = (s.chunk0 + cc) * p.HV + hv;
+      // dO as it is (the last chunk's product with it was done before its update)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) split_elem<E>(vr[2 * i] | vr[2 * i + 1] << 16, hi[i], lo[i]);
+      tmem_st(lanes + cO + t0 / 2, hi);
+      if constexpr (KP == 2) tmem_st(lanes + cO + xStep + t0 / 2, lo);
+      operand_ready(sy->gr, lane);
+      if (c > 0) {
+        advance(c - 1);
+        if (!ok) break;
+        compute_sync();
+      }
+#pragma unroll
+      for (int x = 0; x < DK / 64; ++x) {
+        float w[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) w[i] = D[32 * x + i];
+        split_to_tmem(w, lanes + cS + half * (DK / 4) + 16 * x, sStep, hi, lo);
+        __nv_bfloat16* dst = p.dm + (slot * 2 * p.V + ch) * DK + half * (DK / 2) + 32 * x;
+        store_pairs(dst, hi, live);
+        store_pairs(dst + int64_t(p.V) * DK, lo, live);
+      }
+      operand_ready(sy->sr, lane);
+      // gam dO beside the chain (its region's last reader was the last chunk's update)
+      ok = warp_wait(wait, sy->full[c & 1], c >> 1);
+      if (!ok) break;
+      {
+        float x[32];
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 gam = *reinterpret_cast<const float4*>(coef + t0 + i);
+          x[i] = p.scale * gam.x * widen<E>(vr[i]);
+          x[i + 1] = p.scale * gam.y * widen<E>(vr[i + 1]);
+          x[i + 2] = p.scale * gam.z * widen<E>(vr[i + 2]);
+          x[i + 3] = p.scale * gam.w * widen<E>(vr[i + 3]);
+        }
+        split_to_tmem(x, lanes + cG + t0 / 2, xStep, hi, lo);
+        operand_ready(sy->qr, lane);
+      }
+      if (c + 1 < chunks) fetch_do(c + 1);
+      // beta dV'
+      ok = warp_wait(wait, sy->y, c);
+      if (!ok) break;
+      tc_fence_after();
+      {
+        uint32_t r[32], r2[32];
+        tmem_ld(lanes + cY + t0, r);
+        tmem_ld(lanes + cP + t0, r2);
+        float x[32];
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 w = *reinterpret_cast<const float4*>(coef + kChunk + t0 + i);
+          const float4 be = *reinterpret_cast<const float4*>(coef + 2 * kChunk + t0 + i);
+          x[i] = be.x * fmaf(w.x, __uint_as_float(r[i]), __uint_as_float(r2[i]));
+          x[i + 1] = be.y * fmaf(w.y, __uint_as_float(r[i + 1]), __uint_as_float(r2[i + 1]));
+          x[i + 2] = be.z * fmaf(w.z, __uint_as_float(r[i + 2]), __uint_as_float(r2[i + 2]));
+          x[i + 3] = be.w * fmaf(w.w, __uint_as_float(r[i + 3]), __uint_as_float(r2[i + 3]));
+        }
+        split_to_tmem(x, lanes + cX + t0 / 2, xStep, hi, lo);
+      }
+      operand_ready(sy->xr, lane);
+      // dX
+      ok = warp_wait(wait, sy->u, c);
+      if (!ok) break;
+      tc_fence_after();
+      last = coef[kChunk - 1];
+      {
+        uint32_t r[32];
+        tmem_ld(lanes + cY + t0, r);
+        float x[32];
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 gam = *reinterpret_cast<const float4*>(coef + t0 + i);
+          x[i] = -gam.x * __uint_as_float(r[i]);
+          x[i + 1] = -gam.y * __uint_as_float(r[i + 1]);
+          x[i + 2] = -gam.z * __uint_as_float(r[i + 2]);
+          x[i + 3] = -gam.w * __uint_as_float(r[i + 3]);
+        }
+        split_to_tmem(x, lanes + cX + t0 / 2, xStep, hi, lo);
+        operand_ready(sy->vr, lane);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          split2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), hi[i], lo[i]);
+        __nv_bfloat16* dst = p.xm + (slot * 2 * p.V + ch) * kChunk + t0;
+        store_pairs(dst, hi, live);
+        store_pairs(dst + int64_t(p.V) * kChunk, lo, live);
+        const int64_t at = int64_t(cc) * kChunk + t0;
+        const int rows = int(min(int64_t(32), s.len - at));
+        if (live) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (i < rows) dv[(at + i) * p.HV * p.V] = uint16_t(pack2_rn<E>(__uint_as_float(r[i]), 0.f));
+        }
+      }
+    }
+    if (ok && chunks > 0) advance(chunks - 1);
+    if (ok && p.dinit != nullptr) walk_store<DK>(p.dinit + state_at, D, p.V, live);
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) tmem_free(tm, kTmemColumns);
+}
+
+}  // namespace tdc

@@ -9,6 +9,25 @@
 
 namespace tdc {
 
+// ---- failed waits -----------------------------------------------------------
+// Records that a pipeline wait gave up, as the depthwise kernels do: the first
+// failure on the device in its status words {code, block, stage, load}, and in
+// the device's slot of the mapped host page, code last.
+__device__ __forceinline__ void record_wait_failure(int* words, int* host, int code, int block,
+                                                    int stage, int64_t load) {
+  if (atomicCAS(&words[0], 0, code) != 0) return;
+  words[1] = block;
+  words[2] = stage;
+  words[3] = int(load);
+  if (host == nullptr) return;
+  volatile int* h = host;
+  h[1] = block;
+  h[2] = stage;
+  h[3] = int(load);
+  __threadfence_system();
+  h[0] = code;
+}
+
 // ---- packed batches -----------------------------------------------------------
 // Row offsets of a packed batch, int32 or int64, read as the header states:
 // clamped to [0, T].

@@ -8,7 +8,7 @@
 
 #include "tdc_sequence.h"
 #include "tdc_conv1d.cuh"
-#include "tdc_delta.cuh"
+#include "tdc_delta_walk.cuh"
 #include "tdc_host.h"
 #include "tdc_qknorm.cuh"
 
@@ -278,6 +278,16 @@ int check_delta(const tdc_delta_args* a) {
   return TDC_OK;
 }
 
+int delta_wait_record(tdc::DeltaParams* p) {
+  tdc::host::WaitRecord r;
+  const int rc = tdc::host::wait_record(&r);
+  if (rc != TDC_OK) return rc;
+  p->timeout_ns = r.timeout_ns;
+  p->status_words = r.words;
+  p->status_host = r.host;
+  return TDC_OK;
+}
+
 int64_t delta_seqs(const tdc_delta_args* a) { return a->cu_seqlens != nullptr ? a->num_seqs : a->B; }
 int64_t delta_chunks(const tdc_delta_args* a) {
   return a->cu_seqlens != nullptr ? a->T / tdc::kChunk + a->num_seqs
@@ -294,8 +304,9 @@ int64_t delta_layout(const tdc_delta_args* a, bool grads, unsigned char* base, t
   };
   const int64_t slots = delta_chunks(a) * a->HV;
   unsigned char* plan = take(2 * (delta_seqs(a) + 1) * 8);
-  unsigned char* tm = take(slots * 2 * tdc::kSq * 2);
-  unsigned char* pm = take(slots * 2 * tdc::kSq * 2);
+  unsigned char* tp = take(slots * 4 * tdc::kSq * 2);
+  const int64_t parts = a->dtype == TDC_BF16 ? 1 : 2;
+  unsigned char* kq = take(delta_chunks(a) * a->H * 2 * parts * tdc::kChunk * a->K * 2);
   unsigned char* coef = take(slots * 3 * tdc::kChunk * 4);
   unsigned char *um = nullptr, *xm = nullptr, *sm = nullptr, *dm = nullptr;
   if (grads) {
@@ -307,8 +318,8 @@ int64_t delta_layout(const tdc_delta_args* a, bool grads, unsigned char* base, t
   if (p != nullptr) {
     p->seq_lo = reinterpret_cast<int64_t*>(plan);
     p->seq_chunk = p->seq_lo + delta_seqs(a) + 1;
-    p->tm = reinterpret_cast<__nv_bfloat16*>(tm);
-    p->pm = reinterpret_cast<__nv_bfloat16*>(pm);
+    p->tp = reinterpret_cast<__nv_bfloat16*>(tp);
+    p->kq = kq;
     p->coef = reinterpret_cast<float*>(coef);
     p->um = reinterpret_cast<__nv_bfloat16*>(um);
     p->xm = reinterpret_cast<__nv_bfloat16*>(xm);
@@ -340,16 +351,6 @@ tdc::DeltaParams delta_params(const tdc_delta_args* a) {
   return p;
 }
 
-// Warps a block of the walk: as many as still leave a block for every SM, so
-// that K, Q, T and P are fetched for as many value channels as possible; few
-// sequences and heads take small blocks.
-int delta_warps(const tdc_delta_args* a) {
-  const int64_t walks = delta_seqs(a) * a->HV;
-  for (int w : {8, 4})
-    if (a->V % (16 * w) == 0 && walks * (a->V / (16 * w)) >= 148) return w;
-  return 2;
-}
-
 int delta_plan(const tdc::DeltaParams& p, const tdc::ZeroRows& z, cudaStream_t st) {
   if (p.seq.cu == nullptr) return TDC_OK;
   tdc::delta_plan_kernel<<<33, 1024, 0, st>>>(p.seq, p.seq_lo, p.seq_chunk, z);
@@ -367,49 +368,28 @@ int delta_prepare(const tdc::DeltaParams& p, cudaStream_t st) {
   return launched();
 }
 
-template <class E, int DK, int W, int MODE>
-int delta_scan_w(const tdc::DeltaParams& p, cudaStream_t st) {
+// One block for 128 value channels of a head of a sequence.
+template <class E, int DK, class Kernel>
+int delta_walk(Kernel* k, const tdc::DeltaParams& p, cudaStream_t st) {
   if (p.seq.n == 0) return TDC_OK;
-  auto* k = &tdc::delta_scan_kernel<E, DK, W, MODE>;
-  const size_t smem = 2 * tdc::ScanStage<DK, W>::bytes;
+  const size_t smem = 2 * tdc::WalkTiles<E, DK>::stage + sizeof(tdc::WalkSync);
   const int rc = allow_smem(k, smem);
   if (rc != TDC_OK) return rc;
-  k<<<dim3(unsigned(p.seq.n * (p.V / (16 * W))), unsigned(p.HV)), 32 * W, smem, st>>>(p);
-  return launched();
-}
-template <class E, int DK, int W>
-int delta_back_w(const tdc::DeltaParams& p, cudaStream_t st) {
-  if (p.seq.n == 0) return TDC_OK;
-  auto* k = &tdc::delta_scan_back_kernel<E, DK, W>;
-  const size_t smem = 2 * tdc::ScanStage<DK, W>::bytes;
-  const int rc = allow_smem(k, smem);
-  if (rc != TDC_OK) return rc;
-  k<<<dim3(unsigned(p.seq.n * (p.V / (16 * W))), unsigned(p.HV)), 32 * W, smem, st>>>(p);
+  k<<<dim3(unsigned(p.seq.n * ceil_div(p.V, 128)), unsigned(p.HV)), tdc::kWalkThreads, smem, st>>>(p);
   return launched();
 }
 
-template <class E, int DK, int MODE>
-int delta_scan(const tdc::DeltaParams& p, int w, cudaStream_t st) {
-  return w == 8   ? delta_scan_w<E, DK, 8, MODE>(p, st)
-         : w == 4 ? delta_scan_w<E, DK, 4, MODE>(p, st)
-                  : delta_scan_w<E, DK, 2, MODE>(p, st);
+template <class E, int DK>
+int delta_fwd_t(const tdc::DeltaParams& p, cudaStream_t st) {
+  const int rc = delta_prepare<E, DK>(p, st);
+  return rc != TDC_OK ? rc : delta_walk<E, DK>(&tdc::delta_walk_kernel<E, DK, 0>, p, st);
 }
 
 template <class E, int DK>
-int delta_fwd_t(const tdc::DeltaParams& p, int w, cudaStream_t st) {
+int delta_bwd_t(const tdc::DeltaParams& p, cudaStream_t st) {
   int rc = delta_prepare<E, DK>(p, st);
-  if (rc == TDC_OK) rc = delta_scan<E, DK, 0>(p, w, st);
-  return rc;
-}
-
-template <class E, int DK>
-int delta_bwd_t(const tdc::DeltaParams& p, int w, cudaStream_t st) {
-  int rc = delta_prepare<E, DK>(p, st);
-  if (rc == TDC_OK) rc = delta_scan<E, DK, 1>(p, w, st);
-  if (rc == TDC_OK)
-    rc = w == 8   ? delta_back_w<E, DK, 8>(p, st)
-         : w == 4 ? delta_back_w<E, DK, 4>(p, st)
-                  : delta_back_w<E, DK, 2>(p, st);
+  if (rc == TDC_OK) rc = delta_walk<E, DK>(&tdc::delta_walk_kernel<E, DK, 1>, p, st);
+  if (rc == TDC_OK) rc = delta_walk<E, DK>(&tdc::delta_walk_back_kernel<E, DK>, p, st);
   if (rc != TDC_OK || p.max_chunks == 0) return rc;
   auto* k = &tdc::delta_grad_kernel<E, DK>;
   const size_t smem = tdc::GradSmem<DK>::bytes;
@@ -608,12 +588,12 @@ TDC_API int tdc_delta_fwd(const tdc_delta_args* a, void* workspace, int64_t work
   auto st = static_cast<cudaStream_t>(stream);
   tdc::ZeroRows z = {};
   z.base[0] = a->o, z.row_bytes[0] = a->HV * a->V * 2;
-  rc = delta_plan(p, z, st);
+  rc = delta_wait_record(&p);
+  if (rc == TDC_OK) rc = delta_plan(p, z, st);
   if (rc != TDC_OK) return rc;
-  const int w = delta_warps(a);
   if (a->dtype == TDC_BF16)
-    return a->K == 128 ? delta_fwd_t<tdc::BF16, 128>(p, w, st) : delta_fwd_t<tdc::BF16, 64>(p, w, st);
-  return a->K == 128 ? delta_fwd_t<tdc::F16, 128>(p, w, st) : delta_fwd_t<tdc::F16, 64>(p, w, st);
+    return a->K == 128 ? delta_fwd_t<tdc::BF16, 128>(p, st) : delta_fwd_t<tdc::BF16, 64>(p, st);
+  return a->K == 128 ? delta_fwd_t<tdc::F16, 128>(p, st) : delta_fwd_t<tdc::F16, 64>(p, st);
 }
 
 TDC_API int tdc_delta_bwd(const tdc_delta_args* a, const tdc_delta_grad_args* g, void* workspace,
@@ -649,12 +629,12 @@ TDC_API int tdc_delta_bwd(const tdc_delta_args* a, const tdc_delta_grad_args* g,
   z.base[2] = g->dv, z.row_bytes[2] = a->HV * a->V * 2;
   z.base[3] = g->dg, z.row_bytes[3] = a->HV * 4;
   z.base[4] = g->dbeta, z.row_bytes[4] = a->HV * (a->beta_is_f32 ? 4 : 2);
-  rc = delta_plan(p, z, st);
+  rc = delta_wait_record(&p);
+  if (rc == TDC_OK) rc = delta_plan(p, z, st);
   if (rc != TDC_OK) return rc;
-  const int w = delta_warps(a);
   if (a->dtype == TDC_BF16)
-    return a->K == 128 ? delta_bwd_t<tdc::BF16, 128>(p, w, st) : delta_bwd_t<tdc::BF16, 64>(p, w, st);
-  return a->K == 128 ? delta_bwd_t<tdc::F16, 128>(p, w, st) : delta_bwd_t<tdc::F16, 64>(p, w, st);
+    return a->K == 128 ? delta_bwd_t<tdc::BF16, 128>(p, st) : delta_bwd_t<tdc::BF16, 64>(p, st);
+  return a->K == 128 ? delta_bwd_t<tdc::F16, 128>(p, st) : delta_bwd_t<tdc::F16, 64>(p, st);
 }
 
 TDC_API int tdc_delta_step(const tdc_delta_args* a, float* state, int64_t slots,

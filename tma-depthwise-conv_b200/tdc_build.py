@@ -52,8 +52,8 @@ def _run(cmd: list[str]) -> str:
 UNITS = {
     "tdc_capi.cu": ["tdc_dgrad_s2.cuh", "tdc_host.h", "tdc_kernels.cuh", "tdc_plain.cuh",
                     "tdc_ptx.cuh", "tdc_wgrad.cuh"],
-    "tdc_sequence.cu": ["tdc_conv1d.cuh", "tdc_delta.cuh", "tdc_host.h", "tdc_ptx.cuh",
-                        "tdc_qknorm.cuh", "tdc_seq_common.cuh"],
+    "tdc_sequence.cu": ["tdc_conv1d.cuh", "tdc_delta.cuh", "tdc_delta_walk.cuh", "tdc_host.h",
+                        "tdc_ptx.cuh", "tdc_qknorm.cuh", "tdc_seq_common.cuh", "tdc_tc.cuh"],
 }
 EXT_SOURCES = ("bindings.cpp", "bindings_sequence.cpp")
 
