@@ -51,6 +51,7 @@ struct DeltaParams {
   uint64_t timeout_ns;    // of the bounded waits
   int *status_words, *status_host;
   // gradients
+  // (in blocks of R = min(V, 128) channels: [V / R][columns / 8][R][8] a part)
   __nv_bfloat16* um;      // [2][V][64]: U^T
   __nv_bfloat16* xm;      // [2][V][64]: dX^T
   __nv_bfloat16* sm;      // [2][V][K]: S^T before the chunk
@@ -175,6 +176,15 @@ __device__ __forceinline__ void copy_rows(uint32_t dst, int ld, const uint16_t* 
   for (int i = tid; i < rows * vecs; i += threads) {
     const int r = i / vecs, c = i % vecs;
     cp_async16(dst + 2 * (r * ld + 8 * c), src + (r < valid ? r * stride : 0) + 8 * c, r < valid);
+  }
+}
+
+// 64 rows of [vecs][R][8] into [64][ld] in shared memory.
+__device__ __forceinline__ void copy_columns(uint32_t dst, int ld, const __nv_bfloat16* src, int R,
+                                             int vecs, int tid, int threads) {
+  for (int i = tid; i < 64 * vecs; i += threads) {
+    const int r = i & 63, c = i >> 6;
+    cp_async16(dst + 2 * (r * ld + 8 * c), src + (int64_t(c) * R + r) * 8, true);
   }
 }
 
@@ -507,20 +517,17 @@ __global__ void __launch_bounds__(256, 1) delta_grad_kernel(const DeltaParams p)
     float dsum = 0.f;
     for (int v0 = 0; v0 < p.V; v0 += 64) {
       __syncthreads();
-      const uint16_t* sm = reinterpret_cast<const uint16_t*>(p.sm) + (slot * 2 * p.V + v0) * DK;
-      const uint16_t* dm = reinterpret_cast<const uint16_t*>(p.dm) + (slot * 2 * p.V + v0) * DK;
-      const uint16_t* um = reinterpret_cast<const uint16_t*>(p.um) + (slot * 2 * p.V + v0) * kChunk;
-      const uint16_t* xm = reinterpret_cast<const uint16_t*>(p.xm) + (slot * 2 * p.V + v0) * kChunk;
+      // 64 channels of a block of R, from v0
+      const int R = min(p.V, 128);
+      const int64_t block = v0 / R * R, row = v0 % R;
 #pragma unroll
       for (int part = 0; part < 2; ++part) {
-        copy_rows(sb + Sm::s + part * 64 * ld * 2, ld, sm + int64_t(part) * p.V * DK, DK, 64, 64,
-                  DK / 8, tid, 256);
-        copy_rows(sb + Sm::d + part * 64 * ld * 2, ld, dm + int64_t(part) * p.V * DK, DK, 64, 64,
-                  DK / 8, tid, 256);
-        copy_rows(sb + Sm::u + part * 64 * kLdT * 2, kLdT, um + int64_t(part) * p.V * kChunk, kChunk,
-                  64, 64, 8, tid, 256);
-        copy_rows(sb + Sm::x + part * 64 * kLdT * 2, kLdT, xm + int64_t(part) * p.V * kChunk, kChunk,
-                  64, 64, 8, tid, 256);
+        const int64_t st = ((slot * 2 + part) * p.V + block) * DK + row * 8;
+        const int64_t ut = ((slot * 2 + part) * p.V + block) * kChunk + row * 8;
+        copy_columns(sb + Sm::s + part * 64 * ld * 2, ld, p.sm + st, R, DK / 8, tid, 256);
+        copy_columns(sb + Sm::d + part * 64 * ld * 2, ld, p.dm + st, R, DK / 8, tid, 256);
+        copy_columns(sb + Sm::u + part * 64 * kLdT * 2, kLdT, p.um + ut, R, 8, tid, 256);
+        copy_columns(sb + Sm::x + part * 64 * kLdT * 2, kLdT, p.xm + ut, R, 8, tid, 256);
       }
       copy_rows(sb + Sm::o, kLdT, d_o + v0, p.do_st, kChunk, at.rows, 8, tid, 256);
       cp_async_commit();

@@ -52,7 +52,9 @@ struct WalkSync {
   int abort;
 };
 
-constexpr int kWalkThreads = 320;
+// Three warpgroups; the third (products, copies) hands registers to the two that
+// compute: 2 x 128 x 216 + 128 x 72 = 384 x 168, what the block starts with.
+constexpr int kWalkThreads = 384, kWalkRegs = 216, kIssueRegs = 72;
 constexpr uint32_t kTmemColumns = 512;
 
 struct Waiter {
@@ -205,11 +207,42 @@ __device__ __forceinline__ void walk_store(float* dst, const float (&S)[DK / 2],
   for (int i = 0; i < DK / 2; ++i) dst[int64_t(i) * V] = S[i];
 }
 
-// 32 tokens of this thread's channel, raw 16-bit, zeros behind `rows`.
-__device__ __forceinline__ void walk_column(uint32_t (&v)[32], const uint16_t* src, int64_t stride,
-                                            int t0, int rows, bool live) {
+// 32 tokens of this thread's channel, raw 16-bit, zeros behind `rows` (of the
+// 32); stride in bytes.
+__device__ __forceinline__ void walk_column(uint32_t (&v)[32], const void* src, uint32_t stride,
+                                            int rows, bool live) {
+  const char* at = static_cast<const char*>(src);
+  if (live && rows >= 32) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = live && t0 + i < rows ? src[(t0 + i) * stride] : 0u;
+    for (int i = 0; i < 32; ++i)
+      v[i] = *reinterpret_cast<const uint16_t*>(at + uint64_t(uint32_t(i)) * stride);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      v[i] = live && i < rows
+                 ? *reinterpret_cast<const uint16_t*>(at + uint64_t(uint32_t(i)) * stride)
+                 : 0u;
+  }
+}
+// The same tokens' results, rounded to the element type.
+template <class E>
+__device__ __forceinline__ void walk_put(void* dst, uint32_t stride, const float (&x)[32], int rows,
+                                         bool live) {
+  char* at = static_cast<char*>(dst);
+  if (live && rows >= 32) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      const uint32_t two = pack2_rn<E>(x[i], x[i + 1]);
+      *reinterpret_cast<uint16_t*>(at + uint64_t(uint32_t(i)) * stride) = uint16_t(two);
+      *reinterpret_cast<uint16_t*>(at + uint64_t(uint32_t(i + 1)) * stride) = uint16_t(two >> 16);
+    }
+  } else if (live) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < rows)
+        *reinterpret_cast<uint16_t*>(at + uint64_t(uint32_t(i)) * stride) =
+            uint16_t(pack2_rn<E>(x[i], 0.f));
+  }
 }
 
 template <class E>
@@ -218,12 +251,16 @@ __device__ __forceinline__ float widen(uint32_t raw) {
   else return __half2float(__ushort_as_half(static_cast<unsigned short>(raw)));
 }
 
-// 16 packed pairs (32 tokens or keys) to a row of the workspace.
-__device__ __forceinline__ void store_pairs(__nv_bfloat16* dst, const uint32_t (&r)[16], bool live) {
+// 16 packed pairs (32 tokens or keys) of a channel to the workspace, where 8
+// columns of all channels of the block lie together (16 bytes a channel): the
+// warp's stores are whole lines.
+__device__ __forceinline__ void store_pairs(__nv_bfloat16* dst, int channels, const uint32_t (&r)[16],
+                                            bool live) {
   if (!live) return;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    reinterpret_cast<uint4*>(dst)[i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+    *reinterpret_cast<uint4*>(dst + i * channels * 8) =
+        make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
 }
 
 // MODE 0: the forward (o and the final state).  MODE 1: the forward once more
@@ -248,20 +285,23 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
   constexpr uint32_t cY = 0, cO = 64, cS = 128, cX = 320, cV = 416;
   constexpr uint32_t sStep = DK / 2, xStep = 32;
 
-  if (warp == 9) {
-    if (lane == 0) walk_fetch<E, DK, MODE == 1>(p, raw, sy, wait, s, chunks, h, hv, false);
-  } else if (warp == 8) {
-    if (lane == 0) {
-      for (int c = 0; c < chunks; ++c) {
-        const uint32_t st = smem_addr(raw) + (c & 1) * W::stage;
-        if (!wait(sy->full[c & 1], uint32_t(c >> 1), TDC_DEVICE_FULL_TIMEOUT, c)) break;
-        if (!wait(sy->sr, uint32_t(c), TDC_DEVICE_FULL_TIMEOUT, c)) break;
-        tc_fence_after();
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+    if (warp == 9 && lane == 0) walk_fetch<E, DK, MODE == 1>(p, raw, sy, wait, s, chunks, h, hv, false);
+    if (warp == 8) {
+    for (int c = 0; c < chunks; ++c) {
+      const uint32_t st = smem_addr(raw) + (c & 1) * W::stage;
+      if (!warp_wait(wait, sy->full[c & 1], c >> 1) || !warp_wait(wait, sy->sr, c)) break;
+      tc_fence_after();
+      if (elect_one()) {
         issue_product<DK, KP>(tm + cY, tm + cS, sStep, st + W::k, W::keys, 2 * kColBlock, kColBlock,
                               kRowBlock, mma_desc(64, false), false);
         tc_commit(smem_addr(&sy->y));
-        if (!wait(sy->xr, uint32_t(c), TDC_DEVICE_FULL_TIMEOUT, c)) break;
-        tc_fence_after();
+      }
+      __syncwarp();
+      if (!warp_wait(wait, sy->xr, c)) break;
+      tc_fence_after();
+      if (elect_one()) {
         issue_lower<false, 2>(tm + cY, tm + cX, xStep, st + W::t, false);
         tc_commit(smem_addr(&sy->u));
         if constexpr (MODE == 0) {
@@ -269,23 +309,34 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
                                 kRowBlock, mma_desc(64, false), false);
           tc_commit(smem_addr(&sy->q));
         }
-        if (!wait(sy->vr, uint32_t(c), TDC_DEVICE_FULL_TIMEOUT, c)) break;
-        tc_fence_after();
+      }
+      __syncwarp();
+      if (!warp_wait(wait, sy->vr, c)) break;
+      tc_fence_after();
+      if (elect_one()) {
         issue_product<kChunk, KP>(tm + cS, tm + cX, xStep, st + W::k, W::keys, 2 * kRowBlock,
                                   kRowBlock, kColBlock, mma_desc(DK, true), false);
         tc_commit(smem_addr(&sy->s));
-        if constexpr (MODE == 0) {
-          if (!wait(sy->qr, uint32_t(c), TDC_DEVICE_FULL_TIMEOUT, c)) break;
-          tc_fence_after();
+        if constexpr (MODE == 1) tc_commit(smem_addr(&sy->free[c & 1]));
+      }
+      __syncwarp();
+      if constexpr (MODE == 0) {
+        if (!warp_wait(wait, sy->qr, c)) break;
+        tc_fence_after();
+        if (elect_one()) {
           issue_lower<false, 2>(tm + cO, tm + cV, xStep, st + W::p, false);
           tc_commit(smem_addr(&sy->o));
+          tc_commit(smem_addr(&sy->free[c & 1]));
         }
-        tc_commit(smem_addr(&sy->free[c & 1]));
+        __syncwarp();
       }
-      tc_commit(smem_addr(&sy->drain));
-      mbar_wait_bounded(smem_addr(&sy->drain), 0, wait.abort, false, wait.timeout_ns);
+    }
+    if (elect_one()) tc_commit(smem_addr(&sy->drain));
+    __syncwarp();
+    mbar_wait_bounded(smem_addr(&sy->drain), 0, wait.abort, false, wait.timeout_ns);
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWalkRegs));
     const uint32_t lanes = tm + (uint32_t(warp & 3) << 21);  // 32 lanes a quadrant
     const int half = warp >> 2, ch = v0 + 32 * (warp & 3) + lane, t0 = 32 * half;
     const bool live = ch < p.V;
@@ -295,7 +346,12 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
     float S[DK / 2];
     walk_load<DK>(S, p.init == nullptr ? nullptr : p.init + state_at, p.V, live);
     uint32_t vr[32], hi[16], lo[16];
-    walk_column(vr, v, p.v_st, t0, int(min(int64_t(kChunk), s.len)), live);
+    const uint32_t vstep = uint32_t(p.v_st * 2), ostep = uint32_t(p.HV * p.V * 2);
+    const int channels = min(p.V, 128), cl = ch - v0;  // of this block, and this thread's
+    auto rows_of = [&](int c) {  // of this thread's 32 tokens
+      return int(min(int64_t(32), s.len - int64_t(c) * kChunk - t0));
+    };
+    walk_column(vr, v + t0 * p.v_st, vstep, rows_of(0), live);
     float qs[32];     // scale gam S^T Q^T of the chunk
     float last = 1.f; // gam_63 of the chunk before
     bool ok = true;
@@ -306,13 +362,9 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
       tc_fence_after();
       uint32_t r[32];
       tmem_ld(lanes + cO + t0, r);
-      const int64_t at = int64_t(c) * kChunk + t0;
-      const int rows = int(min(int64_t(32), s.len - at));
-      if (!live) return;
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (i < rows)
-          o[(at + i) * p.HV * p.V] = uint16_t(pack2_rn<E>(qs[i] + __uint_as_float(r[i]), 0.f));
+      for (int i = 0; i < 32; ++i) qs[i] += __uint_as_float(r[i]);
+      walk_put<E>(o + (int64_t(c) * kChunk + t0) * p.HV * p.V, ostep, qs, rows_of(c), live);
     };
     // The state after the chunk before: gam_63 S + its update.
     auto advance = [&](int c) {
@@ -340,9 +392,10 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         for (int i = 0; i < 32; ++i) w[i] = S[32 * x + i];
         split_to_tmem(w, lanes + cS + half * (DK / 4) + 16 * x, sStep, hi, lo);
         if constexpr (MODE == 1) {
-          __nv_bfloat16* dst = p.sm + (slot * 2 * p.V + ch) * DK + half * (DK / 2) + 32 * x;
-          store_pairs(dst, hi, live);
-          store_pairs(dst + int64_t(p.V) * DK, lo, live);
+          __nv_bfloat16* dst = p.sm + (slot * 2 * p.V + v0) * DK +
+                               (half * (DK / 16) + 4 * x) * channels * 8 + cl * 8;
+          store_pairs(dst, channels, hi, live);
+          store_pairs(dst + int64_t(p.V) * DK, channels, lo, live);
         }
       }
       operand_ready(sy->sr, lane);
@@ -372,8 +425,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
       }
       operand_ready(sy->xr, lane);
       if (c + 1 < chunks)
-        walk_column(vr, v + int64_t(c + 1) * kChunk * p.v_st, p.v_st, t0,
-                    int(min(int64_t(kChunk), s.len - int64_t(c + 1) * kChunk)), live);
+        walk_column(vr, v + (int64_t(c + 1) * kChunk + t0) * p.v_st, vstep, rows_of(c + 1), live);
       // V' = beta U and w V'
       ok = warp_wait(wait, sy->u, c);
       if (!ok) break;
@@ -387,9 +439,10 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             split2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), hi[i], lo[i]);
-          __nv_bfloat16* dst = p.um + (slot * 2 * p.V + ch) * kChunk + t0;
-          store_pairs(dst, hi, live);
-          store_pairs(dst + int64_t(p.V) * kChunk, lo, live);
+          __nv_bfloat16* dst =
+              p.um + (slot * 2 * p.V + v0) * kChunk + t0 * channels + cl * 8;
+          store_pairs(dst, channels, hi, live);
+          store_pairs(dst + int64_t(p.V) * kChunk, channels, lo, live);
         }
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
@@ -463,41 +516,54 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
   constexpr uint32_t cY = 0, cS = 64, cP = 192, cO = 256, cG = 320, cX = 384;
   constexpr uint32_t sStep = DK / 2, xStep = 32;
 
-  if (warp == 9) {
-    if (lane == 0) walk_fetch<E, DK, false>(p, raw, sy, wait, s, chunks, h, hv, true);
-  } else if (warp == 8) {
-    if (lane == 0) {
-      for (int c = 0; c < chunks; ++c) {
-        const uint32_t st = smem_addr(raw) + (c & 1) * W::stage;
-        if (!wait(sy->full[c & 1], uint32_t(c >> 1), TDC_DEVICE_FULL_TIMEOUT, c)) break;
-        if (!wait(sy->gr, uint32_t(c), TDC_DEVICE_FULL_TIMEOUT, c)) break;
-        tc_fence_after();
-        issue_lower<true, KP>(tm + cP, tm + cO, xStep, st + W::p, false);
-        if (!wait(sy->sr, uint32_t(c), TDC_DEVICE_FULL_TIMEOUT, c)) break;
-        tc_fence_after();
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+    if (warp == 9 && lane == 0) walk_fetch<E, DK, false>(p, raw, sy, wait, s, chunks, h, hv, true);
+    if (warp == 8) {
+    for (int c = 0; c < chunks; ++c) {
+      const uint32_t st = smem_addr(raw) + (c & 1) * W::stage;
+      if (!warp_wait(wait, sy->full[c & 1], c >> 1) || !warp_wait(wait, sy->gr, c)) break;
+      tc_fence_after();
+      if (elect_one()) issue_lower<true, KP>(tm + cP, tm + cO, xStep, st + W::p, false);
+      __syncwarp();
+      if (!warp_wait(wait, sy->sr, c)) break;
+      tc_fence_after();
+      if (elect_one()) {
         issue_product<DK, KP>(tm + cY, tm + cS, sStep, st + W::k, W::keys, 2 * kColBlock, kColBlock,
                               kRowBlock, mma_desc(64, false), false);
         tc_commit(smem_addr(&sy->y));
-        if (!wait(sy->xr, uint32_t(c), TDC_DEVICE_FULL_TIMEOUT, c)) break;
-        tc_fence_after();
-        issue_lower<true, 2>(tm + cY, tm + cX, xStep, st + W::t, false);
-        tc_commit(smem_addr(&sy->u));
-        // (K dS has read dS^T's parts: the update may take their place)
-        if (!wait(sy->qr, uint32_t(c), TDC_DEVICE_FULL_TIMEOUT, c)) break;
-        tc_fence_after();
+      }
+      __syncwarp();
+      // (K dS comes first and has read dS^T's parts: the update may take their place)
+      if (!warp_wait(wait, sy->qr, c)) break;
+      tc_fence_after();
+      if (elect_one())
         issue_product<kChunk, KP>(tm + cS, tm + cG, xStep, st + W::q, W::keys, 2 * kRowBlock,
                                   kRowBlock, kColBlock, mma_desc(DK, true), false);
-        if (!wait(sy->vr, uint32_t(c), TDC_DEVICE_FULL_TIMEOUT, c)) break;
-        tc_fence_after();
+      __syncwarp();
+      if (!warp_wait(wait, sy->xr, c)) break;
+      tc_fence_after();
+      if (elect_one()) {
+        issue_lower<true, 2>(tm + cY, tm + cX, xStep, st + W::t, false);
+        tc_commit(smem_addr(&sy->u));
+      }
+      __syncwarp();
+      if (!warp_wait(wait, sy->vr, c)) break;
+      tc_fence_after();
+      if (elect_one()) {
         issue_product<kChunk, KP>(tm + cS, tm + cX, xStep, st + W::k, W::keys, 2 * kRowBlock,
                                   kRowBlock, kColBlock, mma_desc(DK, true), true);
         tc_commit(smem_addr(&sy->s));
         tc_commit(smem_addr(&sy->free[c & 1]));
       }
-      tc_commit(smem_addr(&sy->drain));
-      mbar_wait_bounded(smem_addr(&sy->drain), 0, wait.abort, false, wait.timeout_ns);
+      __syncwarp();
+    }
+    if (elect_one()) tc_commit(smem_addr(&sy->drain));
+    __syncwarp();
+    mbar_wait_bounded(smem_addr(&sy->drain), 0, wait.abort, false, wait.timeout_ns);
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWalkRegs));
     const uint32_t lanes = tm + (uint32_t(warp & 3) << 21);
     const int half = warp >> 2, ch = v0 + 32 * (warp & 3) + lane, t0 = 32 * half;
     const bool live = ch < p.V;
@@ -508,9 +574,12 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
     float D[DK / 2];
     walk_load<DK>(D, p.dfinal == nullptr ? nullptr : p.dfinal + state_at, p.V, live);
     uint32_t vr[32], hi[16], lo[16];
+    const uint32_t dostep = uint32_t(p.do_st * 2), dvstep = uint32_t(p.HV * p.V * 2);
+    const int channels = min(p.V, 128), cl = ch - v0;
+    auto rows_of = [&](int cc) { return int(min(int64_t(32), s.len - int64_t(cc) * kChunk - t0)); };
     auto fetch_do = [&](int c) {  // c counts from the end
-      const int64_t at = int64_t(chunks - 1 - c) * kChunk;
-      walk_column(vr, d_o + at * p.do_st, p.do_st, t0, int(min(int64_t(kChunk), s.len - at)), live);
+      const int cc = chunks - 1 - c;
+      walk_column(vr, d_o + (int64_t(cc) * kChunk + t0) * p.do_st, dostep, rows_of(cc), live);
     };
     if (chunks > 0) fetch_do(0);
     float last = 1.f;
@@ -546,9 +615,10 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
 #pragma unroll
         for (int i = 0; i < 32; ++i) w[i] = D[32 * x + i];
         split_to_tmem(w, lanes + cS + half * (DK / 4) + 16 * x, sStep, hi, lo);
-        __nv_bfloat16* dst = p.dm + (slot * 2 * p.V + ch) * DK + half * (DK / 2) + 32 * x;
-        store_pairs(dst, hi, live);
-        store_pairs(dst + int64_t(p.V) * DK, lo, live);
+        __nv_bfloat16* dst = p.dm + (slot * 2 * p.V + v0) * DK +
+                             (half * (DK / 16) + 4 * x) * channels * 8 + cl * 8;
+        store_pairs(dst, channels, hi, live);
+        store_pairs(dst + int64_t(p.V) * DK, channels, lo, live);
       }
       operand_ready(sy->sr, lane);
       // gam dO beside the chain (its region's last reader was the last chunk's update)
@@ -611,16 +681,12 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           split2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), hi[i], lo[i]);
-        __nv_bfloat16* dst = p.xm + (slot * 2 * p.V + ch) * kChunk + t0;
-        store_pairs(dst, hi, live);
-        store_pairs(dst + int64_t(p.V) * kChunk, lo, live);
-        const int64_t at = int64_t(cc) * kChunk + t0;
-        const int rows = int(min(int64_t(32), s.len - at));
-        if (live) {
+        __nv_bfloat16* dst = p.xm + (slot * 2 * p.V + v0) * kChunk + t0 * channels + cl * 8;
+        store_pairs(dst, channels, hi, live);
+        store_pairs(dst + int64_t(p.V) * kChunk, channels, lo, live);
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (i < rows) dv[(at + i) * p.HV * p.V] = uint16_t(pack2_rn<E>(__uint_as_float(r[i]), 0.f));
-        }
+        for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
+        walk_put<E>(dv + (int64_t(cc) * kChunk + t0) * p.HV * p.V, dvstep, x, rows_of(cc), live);
       }
     }
     if (ok && chunks > 0) advance(chunks - 1);

@@ -18,6 +18,7 @@ using tdc::host::cuda_fail;
 using tdc::host::prepare_device;
 
 constexpr int64_t kMaxDim = int64_t(1) << 40;
+constexpr int64_t kMaxRow = int64_t(1) << 31;  // elements of 2 bytes
 
 bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
 bool bad_stride(int64_t s) { return s % 8 != 0; }
@@ -274,6 +275,8 @@ int check_delta(const tdc_delta_args* a) {
   if (a->num_seqs > (int64_t(1) << 24)) return TDC_ERR_TOO_LARGE;
   for (int64_t s : {a->q_sb, a->q_st, a->q_sh, a->k_sb, a->k_st, a->k_sh, a->v_sb, a->v_st, a->v_sh})
     if (bad_stride(s)) return TDC_ERR_ALIGNMENT;
+  // rows of v and o are addressed by 32-bit byte strides in a chunk
+  if (a->v_st < 0 || a->v_st >= kMaxRow || a->HV * a->V >= kMaxRow) return TDC_ERR_TOO_LARGE;
   if (misaligned(a->q) || misaligned(a->k) || misaligned(a->v)) return TDC_ERR_ALIGNMENT;
   return TDC_OK;
 }
@@ -610,6 +613,7 @@ TDC_API int tdc_delta_bwd(const tdc_delta_args* a, const tdc_delta_grad_args* g,
     return TDC_ERR_NULL_POINTER;
   for (int64_t s : {g->do_sb, g->do_st, g->do_sh})
     if (bad_stride(s)) return TDC_ERR_ALIGNMENT;
+  if (g->do_st < 0 || g->do_st >= kMaxRow) return TDC_ERR_TOO_LARGE;
   for (const void* q : {g->d_o, static_cast<const void*>(g->dq), static_cast<const void*>(g->dk),
                         static_cast<const void*>(g->dv)})
     if (misaligned(q)) return TDC_ERR_ALIGNMENT;

@@ -109,6 +109,21 @@ __device__ __forceinline__ void tc_mma(uint32_t d, uint32_t a, uint64_t b, uint3
       "r"(a), "l"(b), "r"(desc), "r"(uint32_t(accumulate))
       : "memory");
 }
+// One lane of a converged warp, the same one every time.  The products are
+// issued under it in code that the whole warp runs: then their operands stay in
+// uniform registers (32 cycles a product of N = 64; issued by `lane == 0` alone
+// each took 64 to 120).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n"
+      " .reg .pred p;\n"
+      " elect.sync _|p, 0xffffffff;\n"
+      " selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(one));
+  return one != 0;
+}
 // Arrives on `bar` once the products issued so far by this thread are done.
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
   asm volatile(
