@@ -106,23 +106,23 @@ __device__ __forceinline__ void compute_sync() {
   tc_fence_after();
 }
 
-// d (+)= A B over DEPTH contraction elements; A split in two parts at a, a +
-// astep (columns), B in BP parts bstep bytes apart.  kstep: bytes from 16
-// contraction elements of B to the next.  The remainders' product is left out.
-template <int DEPTH, int BP>
+// d[128 x N] (+)= A B; A split in two parts at a, a + astep (columns), B a tile
+// at b in BP parts bstep bytes apart, its rows (n_major false) or its columns as
+// N, DEPTH elements of the contraction.  The remainders' product is left out.
+template <int DEPTH, int N, bool N_MAJOR, int BP>
 __device__ __forceinline__ void issue_product(uint32_t d, uint32_t a, uint32_t astep, uint32_t b,
-                                              uint32_t bstep, uint32_t kstep, uint32_t leading,
-                                              uint32_t stride, uint32_t desc, bool accumulate) {
+                                              uint32_t bstep, bool accumulate) {
+  const uint32_t low = tile_desc(b, N_MAJOR);
+  constexpr uint32_t kstep = (N_MAJOR ? 2 * kRowBlock : 2 * kColBlock) / 16;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < BP; ++j) {
       if (i + j > 1) continue;
 #pragma unroll
-      for (int ks = 0; ks < DEPTH / 16; ++ks) {
-        tc_mma(d, a + i * astep + 8 * ks, smem_desc(b + j * bstep + ks * kstep, leading, stride), desc,
-               accumulate || i + j + ks > 0);
-      }
+      for (int ks = 0; ks < DEPTH / 16; ++ks)
+        tc_mma(d, a + i * astep + 8 * ks, low + j * (bstep / 16) + ks * kstep, tile_desc_high(N_MAJOR),
+               mma_desc(N, N_MAJOR), accumulate || i + j + ks > 0);
     }
 }
 
@@ -131,23 +131,19 @@ __device__ __forceinline__ void issue_product(uint32_t d, uint32_t a, uint32_t a
 template <bool BACK, int AP>
 __device__ __forceinline__ void issue_lower(uint32_t d, uint32_t a, uint32_t astep, uint32_t m,
                                             bool accumulate) {
+  const uint32_t low = tile_desc(m, BACK);
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
     const int ks = BACK ? 3 - x : x;  // the step that fills all columns first
     const uint32_t n = BACK ? 16 * (ks + 1) : 64 - 16 * ks;
+    const uint32_t from = BACK ? ks * 2 * kRowBlock : ks * (2 * kRowBlock + 2 * kColBlock);
 #pragma unroll
     for (int i = 0; i < AP; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         if (i + j > 1) continue;
-        const uint32_t b = m + j * kSq * 2;
-        if constexpr (BACK)
-          tc_mma(d, a + i * astep + 8 * ks, smem_desc(b + ks * 2 * kRowBlock, kRowBlock, kColBlock),
-                 mma_desc(n, true), accumulate || x + i + j > 0);
-        else
-          tc_mma(d + 16 * ks, a + i * astep + 8 * ks,
-                 smem_desc(b + ks * (2 * kRowBlock + 2 * kColBlock), kColBlock, kRowBlock),
-                 mma_desc(n, false), accumulate || x + i + j > 0);
+        tc_mma(BACK ? d : d + 16 * ks, a + i * astep + 8 * ks, low + (from + j * kSq * 2) / 16,
+               tile_desc_high(BACK), mma_desc(n, BACK), accumulate || x + i + j > 0);
       }
   }
 }
@@ -224,24 +220,26 @@ __device__ __forceinline__ void walk_column(uint32_t (&v)[32], const void* src, 
                  : 0u;
   }
 }
-// The same tokens' results, rounded to the element type.
-template <class E>
-__device__ __forceinline__ void walk_put(void* dst, uint32_t stride, const float (&x)[32], int rows,
+// Tokens' results, rounded to the element type.
+template <class E, int N>
+__device__ __forceinline__ void walk_put(void* dst, uint32_t stride, const float (&x)[N], int rows,
                                          bool live) {
   char* at = static_cast<char*>(dst);
-  if (live && rows >= 32) {
+  if (live && rows >= N) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) {
+    for (int i = 0; i < N; i += 2) {
       const uint32_t two = pack2_rn<E>(x[i], x[i + 1]);
       *reinterpret_cast<uint16_t*>(at + uint64_t(uint32_t(i)) * stride) = uint16_t(two);
       *reinterpret_cast<uint16_t*>(at + uint64_t(uint32_t(i + 1)) * stride) = uint16_t(two >> 16);
     }
   } else if (live) {
+#pragma unroll 1
+    for (int i = 0; i < rows; ++i) {
+      float v = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < rows)
-        *reinterpret_cast<uint16_t*>(at + uint64_t(uint32_t(i)) * stride) =
-            uint16_t(pack2_rn<E>(x[i], 0.f));
+      for (int j = 0; j < N; ++j) v = j == i ? x[j] : v;
+      *reinterpret_cast<uint16_t*>(at + uint64_t(uint32_t(i)) * stride) = uint16_t(pack2_rn<E>(v, 0.f));
+    }
   }
 }
 
@@ -294,8 +292,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
       if (!warp_wait(wait, sy->full[c & 1], c >> 1) || !warp_wait(wait, sy->sr, c)) break;
       tc_fence_after();
       if (elect_one()) {
-        issue_product<DK, KP>(tm + cY, tm + cS, sStep, st + W::k, W::keys, 2 * kColBlock, kColBlock,
-                              kRowBlock, mma_desc(64, false), false);
+        issue_product<DK, 64, false, KP>(tm + cY, tm + cS, sStep, st + W::k, W::keys, false);
         tc_commit(smem_addr(&sy->y));
       }
       __syncwarp();
@@ -305,8 +302,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         issue_lower<false, 2>(tm + cY, tm + cX, xStep, st + W::t, false);
         tc_commit(smem_addr(&sy->u));
         if constexpr (MODE == 0) {
-          issue_product<DK, KP>(tm + cO, tm + cS, sStep, st + W::q, W::keys, 2 * kColBlock, kColBlock,
-                                kRowBlock, mma_desc(64, false), false);
+          issue_product<DK, 64, false, KP>(tm + cO, tm + cS, sStep, st + W::q, W::keys, false);
           tc_commit(smem_addr(&sy->q));
         }
       }
@@ -314,8 +310,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
       if (!warp_wait(wait, sy->vr, c)) break;
       tc_fence_after();
       if (elect_one()) {
-        issue_product<kChunk, KP>(tm + cS, tm + cX, xStep, st + W::k, W::keys, 2 * kRowBlock,
-                                  kRowBlock, kColBlock, mma_desc(DK, true), false);
+        issue_product<kChunk, DK, true, KP>(tm + cS, tm + cX, xStep, st + W::k, W::keys, false);
         tc_commit(smem_addr(&sy->s));
         if constexpr (MODE == 1) tc_commit(smem_addr(&sy->free[c & 1]));
       }
@@ -529,17 +524,15 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
       if (!warp_wait(wait, sy->sr, c)) break;
       tc_fence_after();
       if (elect_one()) {
-        issue_product<DK, KP>(tm + cY, tm + cS, sStep, st + W::k, W::keys, 2 * kColBlock, kColBlock,
-                              kRowBlock, mma_desc(64, false), false);
+        issue_product<DK, 64, false, KP>(tm + cY, tm + cS, sStep, st + W::k, W::keys, false);
         tc_commit(smem_addr(&sy->y));
       }
       __syncwarp();
       // (K dS comes first and has read dS^T's parts: the update may take their place)
-      if (!warp_wait(wait, sy->qr, c)) break;
+      if (!warp_wait(wait, sy->y, c) || !warp_wait(wait, sy->qr, c)) break;
       tc_fence_after();
       if (elect_one())
-        issue_product<kChunk, KP>(tm + cS, tm + cG, xStep, st + W::q, W::keys, 2 * kRowBlock,
-                                  kRowBlock, kColBlock, mma_desc(DK, true), false);
+        issue_product<kChunk, DK, true, KP>(tm + cS, tm + cG, xStep, st + W::q, W::keys, false);
       __syncwarp();
       if (!warp_wait(wait, sy->xr, c)) break;
       tc_fence_after();
@@ -551,8 +544,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
       if (!warp_wait(wait, sy->vr, c)) break;
       tc_fence_after();
       if (elect_one()) {
-        issue_product<kChunk, KP>(tm + cS, tm + cX, xStep, st + W::k, W::keys, 2 * kRowBlock,
-                                  kRowBlock, kColBlock, mma_desc(DK, true), true);
+        issue_product<kChunk, DK, true, KP>(tm + cS, tm + cX, xStep, st + W::k, W::keys, true);
         tc_commit(smem_addr(&sy->s));
         tc_commit(smem_addr(&sy->free[c & 1]));
       }

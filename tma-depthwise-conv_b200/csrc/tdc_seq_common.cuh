@@ -174,7 +174,8 @@ __device__ __forceinline__ void stsm4_t(uint32_t addr, const uint32_t r[4]) {
 // high parts alone).
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
   hi = pack2_rn<BF16>(x, y);
-  lo = pack2_rn<BF16>(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
+  fma2<BF16>(hi, 0xBF80BF80u, x, y);  // x - high part, exact (times -1, no unpacking)
+  lo = pack2_rn<BF16>(x, y);
 }
 
 // A packed pair of elements as bf16 high parts and remainders: bf16 is itself;

@@ -85,12 +85,16 @@ __device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&r)[64]) {
 // (columns are the contraction) and with the columns as N (rows are).
 constexpr uint32_t kRowBlock = 128, kColBlock = 1024;
 
-// Bits 0-13 start address / 16, 16-29 leading and 32-45 stride byte offset / 16
-// (K-major: contraction blocks and N blocks apart; N-major: contraction blocks
-// and N blocks as well, whose places in the tile swap), bit 46 set.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t leading, uint32_t stride) {
-  return uint64_t((addr >> 4) & 0x3fff) | (uint64_t(leading >> 4) << 16) |
-         (uint64_t(stride >> 4) << 32) | (uint64_t(1) << 46);
+// Descriptor of such a tile in two words.  Low: bits 0-13 start address / 16,
+// 16-29 the leading byte offset / 16 (K-major: from 8 contraction columns to the
+// next; N-major: from 8 contraction rows to the next).  High: bits 0-13 the
+// stride byte offset / 16 (from 8 of N to the next), bit 14 set.  Adding bytes /
+// 16 to the low word moves the start.
+__device__ __forceinline__ uint32_t tile_desc(uint32_t addr, bool n_major) {
+  return (addr >> 4) | ((n_major ? kRowBlock : kColBlock) >> 4) << 16;
+}
+__host__ __device__ constexpr uint32_t tile_desc_high(bool n_major) {
+  return ((n_major ? kColBlock : kRowBlock) >> 4) | 1u << 14;
 }
 // bf16 operands, fp32 accumulators, M = 128.
 __device__ __forceinline__ uint32_t mma_desc(uint32_t n, bool n_major) {
@@ -98,15 +102,17 @@ __device__ __forceinline__ uint32_t mma_desc(uint32_t n, bool n_major) {
          ((128u >> 4) << 24);
 }
 // d[128 x N] (+)= a[128 x 16] b[16 x N]; one thread issues it.
-__device__ __forceinline__ void tc_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t desc,
-                                       bool accumulate) {
+__device__ __forceinline__ void tc_mma(uint32_t d, uint32_t a, uint32_t b_low, uint32_t b_high,
+                                       uint32_t desc, bool accumulate) {
   asm volatile(
       "{\n"
       " .reg .pred p;\n"
-      " setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      " .reg .b64 b;\n"
+      " setp.ne.b32 p, %5, 0;\n"
+      " mov.b64 b, {%2, %3};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n"
       "}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(desc), "r"(uint32_t(accumulate))
+      "r"(a), "r"(b_low), "r"(b_high), "r"(desc), "r"(uint32_t(accumulate))
       : "memory");
 }
 // One lane of a converged warp, the same one every time.  The products are
