@@ -98,8 +98,9 @@ __device__ __forceinline__ void conv_dot(float z[8], const uint4 win[K], const u
   }
 }
 
-template <class E, int K, bool SILU>
-__global__ void __launch_bounds__(256) conv1d_fwd_kernel(const Conv1dParams p) {
+// PACKED: sequences may end inside a run (cu_seqlens).
+template <class E, int K, bool SILU, bool PACKED>
+__global__ void __launch_bounds__(256, 2) conv1d_fwd_kernel(const Conv1dParams p) {
   const int64_t id = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
   const int64_t vecs = p.C / 8;
   if (id >= p.main_threads) {
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(256) conv1d_fwd_kernel(const Conv1dParams p) {
     const int64_t c = (r % vecs) * 8, j = (r / vecs) % (K - 1), n = r / (vecs * (K - 1));
     SeqSpan s{n, 0, p.T, true};
     int64_t xbase = n * p.x_sb;
-    if (p.seq.cu != nullptr) {
+    if (PACKED) {
       s.lo = p.seq.at(n);
       s.hi = max(s.lo, p.seq.at(n + 1));
       xbase = 0;
@@ -120,49 +121,58 @@ __global__ void __launch_bounds__(256) conv1d_fwd_kernel(const Conv1dParams p) {
   }
   const int64_t c = (id % vecs) * 8, run = id / vecs;
   const int64_t b = run / p.runs_per_b, t0 = (run % p.runs_per_b) * p.run;
-  const int64_t t1 = min(t0 + p.run, p.T);
-  const int64_t xbase = b * p.x_sb, ybase = b * p.T * p.C + c;
-  SeqSpan s = span_at(p.seq, b, t0);
+  const int rows = int(min(int64_t(p.run), p.T - t0));
+  const int64_t xbase = b * p.x_sb;
+  const uint16_t* x = static_cast<const uint16_t*>(p.x) + xbase + t0 * p.x_st + c;
+  uint16_t* y = static_cast<uint16_t*>(p.y) + (b * p.T + t0) * p.C + c;
+  SeqSpan s{b, 0, p.T, true};
+  if (PACKED) s = span_at(p.seq, b, t0);
 
-  uint4 w[K];
+  // win: the K-1 inputs before the first of 4 rows, then those rows.
+  uint4 win[K + 3], next[4], w[K];
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (u < rows) next[u] = ld16(x, u * p.x_st);
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j)
+    win[j] = s.covered ? conv_input(p, K, s, xbase, t0 - (K - 1) + j, c) : make_uint4(0, 0, 0, 0);
 #pragma unroll
   for (int j = 0; j < K; ++j) w[j] = ld16(p.w, j * p.C + c);
   float bias[8] = {};
   if (p.bias != nullptr) unpack8<E>(ld16(p.bias, c), bias);
 
-  uint4 win[K];  // win[0..K-2]: the inputs before the current row
+  for (int t = 0; t < rows; t += 4) {
 #pragma unroll
-  for (int j = 0; j < K - 1; ++j)
-    win[j] = s.covered ? conv_input(p, K, s, xbase, t0 - (K - 1) + j, c) : make_uint4(0, 0, 0, 0);
-
-  for (int64_t t = t0; t < t1; t += 4) {
-    uint4 next[4];
+    for (int u = 0; u < 4; ++u) win[K - 1 + u] = next[u];
+    x += 4 * p.x_st;
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (t + u < t1) next[u] = ld16(p.x, xbase + (t + u) * p.x_st + c);
+      if (t + 4 + u < rows) next[u] = ld16(x, u * p.x_st);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      if (t + u >= t1) break;
-      if (t + u >= s.hi) {  // only in packed batches: the next sequence (or gap) starts here
-        s = span_from(p.seq, s.n, t + u);
-        if (s.covered) {
+      if (t + u < rows) {
+        if (PACKED && t0 + t + u >= s.hi) {  // the next sequence (or gap) starts here
+          s = span_from(p.seq, s.n, t0 + t + u);
+          if (s.covered) {
 #pragma unroll
-          for (int j = 0; j < K - 1; ++j) win[j] = conv_input(p, K, s, xbase, s.lo - (K - 1) + j, c);
+            for (int j = 0; j < K - 1; ++j)
+              win[u + j] = conv_input(p, K, s, xbase, s.lo - (K - 1) + j, c);
+          }
         }
+        float z[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = bias[i];
+        conv_dot<E, K>(z, win + u, w);
+        if constexpr (SILU) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) z[i] *= sigmoid_f(z[i]);
+        }
+        st16(y, 0, !PACKED || s.covered ? pack8<E>(z) : make_uint4(0, 0, 0, 0));
+        y += p.C;
       }
-      win[K - 1] = next[u];
-      float z[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) z[i] = bias[i];
-      conv_dot<E, K>(z, win, w);
-      if constexpr (SILU) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) z[i] *= sigmoid_f(z[i]);
-      }
-      st16(p.y, ybase + (t + u) * p.C, s.covered ? pack8<E>(z) : make_uint4(0, 0, 0, 0));
-#pragma unroll
-      for (int j = 0; j < K - 1; ++j) win[j] = win[j + 1];
     }
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) win[j] = win[j + 4];
   }
 }
 
@@ -170,145 +180,159 @@ __global__ void __launch_bounds__(256) conv1d_fwd_kernel(const Conv1dParams p) {
 // With dz = dy * act'(z): dx[t] = sum_j w[j] dz[t + K-1-j] within the sequence
 // (plus dfinal where the row is among the sequence's last K-1 inputs), dw[j] =
 // sum_t dz[t] x[t-(K-1)+j], dbias = sum dz.  z is recomputed from x, so the
-// pass reads x and dy and writes dx: bound by memory.  A thread owns VEC
-// channels and a run of rows, recomputes the K-1 values of dz behind the run,
-// and keeps its share of dw and dbias in registers; the runs of a block are
+// pass reads x and dy and writes dx: bound by memory.  A thread owns 4 channels
+// (8 would not leave registers for the taps' sums) and a run of rows.  The last
+// K inputs and the K unfinished rows of dx sit in rings of registers whose
+// places are fixed by unrolling K rows; dz[t] is added to the rows it reaches.
+// The K-1 values of dz behind the run are recomputed.  The runs of a block are
 // added in shared memory and one partial sum per block goes to the workspace,
 // which conv1d_wsum_kernel adds in a fixed order.
-template <class E, int VEC>
-__device__ __forceinline__ void ldv(const void* base, int64_t elem, float f[VEC]) {
-  if constexpr (VEC == 8) {
-    unpack8<E>(ld16(base, elem), f);
-  } else {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + elem));
-    unpack2<E>(v.x, f[0], f[1]);
-    unpack2<E>(v.y, f[2], f[3]);
-  }
+constexpr int kGradVec = 4;
+
+template <class E>
+__device__ __forceinline__ void unpack4(const uint2& v, float f[4]) {
+  unpack2<E>(v.x, f[0], f[1]);
+  unpack2<E>(v.y, f[2], f[3]);
 }
-template <class E, int VEC>
-__device__ __forceinline__ void stv(void* base, int64_t elem, const float f[VEC]) {
-  if constexpr (VEC == 8) {
-    st16(base, elem, pack8<E>(f));
-  } else {
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + elem) =
-        make_uint2(pack2_rn<E>(f[0], f[1]), pack2_rn<E>(f[2], f[3]));
-  }
+__device__ __forceinline__ uint2 ld8(const void* base, int64_t elem) {
+  return __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + elem));
+}
+template <class E>
+__device__ __forceinline__ void st8(void* base, int64_t elem, const float f[4]) {
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + elem) =
+      make_uint2(pack2_rn<E>(f[0], f[1]), pack2_rn<E>(f[2], f[3]));
 }
 
-template <class E, int VEC>
-__device__ __forceinline__ void conv_input_v(const Conv1dParams& p, int taps, const SeqSpan& s,
-                                             int64_t xbase, int64_t t, int64_t c, float f[VEC]) {
-  if (t >= s.lo) return ldv<E, VEC>(p.x, xbase + t * p.x_st + c, f);
+__device__ __forceinline__ uint2 conv_input4(const Conv1dParams& p, int taps, const SeqSpan& s,
+                                             int64_t xbase, int64_t t, int64_t c) {
+  if (t >= s.lo) return ld8(p.x, xbase + t * p.x_st + c);
   const int64_t row = t - s.lo + taps - 1;
-  if (p.init == nullptr || row < 0) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = 0.f;
-    return;
-  }
-  ldv<E, VEC>(p.init, (s.n * (taps - 1) + row) * p.C + c, f);
+  if (p.init == nullptr || row < 0) return make_uint2(0, 0);
+  return ld8(p.init, (s.n * (taps - 1) + row) * p.C + c);
 }
 
-// dz of one row from its window of inputs (win[K-1] is the row itself).
-template <class E, int K, int VEC, bool SILU>
-__device__ __forceinline__ void conv_dz(float dz[VEC], const float win[K][VEC],
-                                        const float w[K][VEC], const float bias[VEC],
-                                        const float dy[VEC]) {
+// dz = dy act'(z), z from the inputs at(0) .. at(K-1) (the last is the row's own).
+template <class E, int K, bool SILU, class At>
+__device__ __forceinline__ void conv_dz(float dz[4], At at, const uint2 w[K], const float bias[4],
+                                        const uint2& dy) {
+  unpack4<E>(dy, dz);
+  if constexpr (SILU) {
+    float z[4] = {bias[0], bias[1], bias[2], bias[3]};
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    if constexpr (SILU) {
-      float z = bias[i];
+    for (int j = 0; j < K; ++j) {
+      const uint2 v = at(j);
+      fma2<E>(v.x, w[j].x, z[0], z[1]);
+      fma2<E>(v.y, w[j].y, z[2], z[3]);
+    }
 #pragma unroll
-      for (int j = 0; j < K; ++j) z = fmaf(win[j][i], w[j][i], z);
-      const float sg = sigmoid_f(z);
-      dz[i] = dy[i] * sg * fmaf(z, 1.f - sg, 1.f);
-    } else {
-      dz[i] = dy[i];
+    for (int i = 0; i < 4; ++i) {
+      const float sg = sigmoid_f(z[i]);
+      dz[i] *= sg * fmaf(z[i], 1.f - sg, 1.f);
     }
   }
 }
 
-template <class E, int K, int VEC, bool SILU>
-__global__ void __launch_bounds__(256, 2) conv1d_bwd_kernel(const Conv1dParams p) {
-  extern __shared__ float red[];  // [blockDim.y][blockDim.x * VEC]
-  const int64_t c = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * VEC;
+template <class E, int K, bool SILU, bool PACKED>
+__global__ void __launch_bounds__(256, K <= 4 ? 2 : 1) conv1d_bwd_kernel(const Conv1dParams p) {
+  __shared__ float red[256 * kGradVec];  // [blockDim.y][blockDim.x * 4]
+  const int64_t c = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * kGradVec;
   const int64_t run = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
   const int64_t b = run / p.runs_per_b;
   const bool live = c < p.C && b < p.B;
-  float dw[K][VEC] = {}, db[VEC] = {};
+  float dw[K][4] = {}, db[4] = {};
   if (live) {
     const int64_t t0 = (run % p.runs_per_b) * p.run, t1 = min(t0 + p.run, p.T);
-    const int64_t xbase = b * p.x_sb, dybase = b * p.dy_sb, dxbase = b * p.T * p.C + c;
-    float w[K][VEC], bias[VEC] = {};
+    const int64_t xbase = b * p.x_sb;
+    uint2 w[K];
+    float bias[4] = {};
 #pragma unroll
-    for (int j = 0; j < K; ++j) ldv<E, VEC>(p.w, j * p.C + c, w[j]);
-    if (p.bias != nullptr) ldv<E, VEC>(p.bias, c, bias);
-    SeqSpan s = span_at(p.seq, b, t0);
+    for (int j = 0; j < K; ++j) w[j] = ld8(p.w, j * p.C + c);
+    if (p.bias != nullptr) unpack4<E>(ld8(p.bias, c), bias);
+    SeqSpan s{b, 0, p.T, true};
+    if (PACKED) s = span_at(p.seq, b, t0);
     int64_t a = t0;
     while (a < t1) {  // the part [a, e) of the run that lies in one sequence (or gap)
       const int64_t e = min(t1, s.hi);
-      if (!s.covered) {
-        const float zero[VEC] = {};
-        for (int64_t t = a; t < e; ++t) stv<E, VEC>(p.dx, dxbase + t * p.C, zero);
+      const uint16_t* x = static_cast<const uint16_t*>(p.x) + xbase + a * p.x_st + c;
+      const uint16_t* dy = static_cast<const uint16_t*>(p.dy) + b * p.dy_sb + a * p.dy_st + c;
+      uint16_t* dx = static_cast<uint16_t*>(p.dx) + (b * p.T + a) * p.C + c;
+      if (PACKED && !s.covered) {
+        const float zero[4] = {};
+        for (int64_t t = a; t < e; ++t, dx += p.C) st8<E>(dx, 0, zero);
       } else {
-        float win[K][VEC], q[K][VEC];  // inputs; q[K-1-i] = dz[t - i]
+        const int own = int(e - a);                                       // rows of dx
+        const int known = int(min(int64_t(own + K - 1), s.hi - a));       // rows of dz
+        const int64_t to_final = K - 1 - (s.hi - a);  // row i is row i + to_final of final_state
+        uint2 xr[K], xn[K], dn[K];
+        float acc[K][4] = {};
+        // row a - (K-1) + j has place (j + 1) % K
 #pragma unroll
-        for (int j = 0; j < K - 1; ++j) {
-          conv_input_v<E, VEC>(p, K, s, xbase, a - (K - 1) + j, c, win[j]);
+        for (int j = 0; j < K - 1; ++j) xr[j + 1] = conv_input4(p, K, s, xbase, a - (K - 1) + j, c);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) q[j][i] = 0.f;
-        }
-        const int64_t last = min(e + K - 1, s.hi);  // dz is wanted for rows [a, last)
-        for (int64_t t = a; t < e + K - 1; ++t) {
-          if (t < last) {
-            float dyv[VEC];
-            ldv<E, VEC>(p.x, xbase + t * p.x_st + c, win[K - 1]);
-            ldv<E, VEC>(p.dy, dybase + t * p.dy_st + c, dyv);
-            conv_dz<E, K, VEC, SILU>(q[K - 1], win, w, bias, dyv);
-            if (t < e) {
+        for (int u = 0; u < K; ++u)
+          if (u < known) {
+            xn[u] = ld8(x, u * p.x_st);
+            dn[u] = ld8(dy, u * p.dy_st);
+          }
+        for (int i0 = 0; i0 < own + K - 1; i0 += K) {
+          x += K * p.x_st;
+          dy += K * p.dy_st;
 #pragma unroll
-              for (int i = 0; i < VEC; ++i) {
-                db[i] += q[K - 1][i];
+          for (int u = 0; u < K; ++u) {
+            const int i = i0 + u;
+            // row i takes place u of both rings
 #pragma unroll
-                for (int j = 0; j < K; ++j) dw[j][i] = fmaf(q[K - 1][i], win[j][i], dw[j][i]);
+            for (int q = 0; q < 4; ++q) acc[u][q] = 0.f;
+            if (p.dfinal != nullptr && i < own && i + to_final >= 0)
+              unpack4<E>(ld8(p.dfinal, (s.n * (K - 1) + i + to_final) * p.C + c), acc[u]);
+            if (i < known) {
+              xr[u] = xn[u];
+              const uint2 dyv = dn[u];
+              if (i + K < known) {  // the row that takes this place next
+                xn[u] = ld8(x, u * p.x_st);
+                dn[u] = ld8(dy, u * p.dy_st);
+              }
+              float dz[4];
+              conv_dz<E, K, SILU>(dz, [&](int j) { return xr[(u + 1 + j) % K]; }, w, bias, dyv);
+              if (i < own) {
+#pragma unroll
+                for (int j = 0; j < K; ++j) {
+                  float f[4];
+                  unpack4<E>(xr[(u + 1 + j) % K], f);
+#pragma unroll
+                  for (int q = 0; q < 4; ++q) dw[j][q] = fmaf(dz[q], f[q], dw[j][q]);
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) db[q] += dz[q];
+              }
+#pragma unroll
+              for (int j = 0; j < K; ++j) {  // to row i - (K-1) + j
+                float f[4];
+                unpack4<E>(w[j], f);
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  acc[(u + 1 + j) % K][q] = fmaf(f[q], dz[q], acc[(u + 1 + j) % K][q]);
               }
             }
-          } else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) q[K - 1][i] = 0.f;
-          }
-          const int64_t to = t - (K - 1);  // the row whose dz window is complete
-          if (to >= a) {
-            float d[VEC] = {};
-            const int64_t f = to + K - 1 - s.hi;  // the row of final_state that it is
-            if (p.dfinal != nullptr && f >= 0)
-              ldv<E, VEC>(p.dfinal, (s.n * (K - 1) + f) * p.C + c, d);
-#pragma unroll
-            for (int j = 0; j < K; ++j)
-#pragma unroll
-              for (int i = 0; i < VEC; ++i) d[i] = fmaf(w[j][i], q[K - 1 - j][i], d[i]);
-            stv<E, VEC>(p.dx, dxbase + to * p.C, d);
-          }
-#pragma unroll
-          for (int j = 0; j < K - 1; ++j)
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-              win[j][i] = win[j + 1][i];
-              q[j][i] = q[j + 1][i];
+            if (i >= K - 1 && i < own + K - 1) {
+              st8<E>(dx, 0, acc[(u + 1) % K]);
+              dx += p.C;
             }
+          }
         }
       }
       a = e;
-      if (a < t1) s = span_from(p.seq, s.n, a);
+      if (PACKED && a < t1) s = span_from(p.seq, s.n, a);
     }
   }
   // Add the block's runs, tap by tap (K is the bias).
-  const int width = blockDim.x * VEC;
+  const int width = blockDim.x * kGradVec;
 #pragma unroll
   for (int j = 0; j <= K; ++j) {
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < VEC; ++i)
-      red[threadIdx.y * width + threadIdx.x * VEC + i] = j < K ? dw[j < K ? j : 0][i] : db[i];
+    for (int i = 0; i < kGradVec; ++i)
+      red[threadIdx.y * width + threadIdx.x * kGradVec + i] = j < K ? dw[j < K ? j : 0][i] : db[i];
     __syncthreads();
     for (int i = threadIdx.y * blockDim.x + threadIdx.x; i < width; i += blockDim.x * blockDim.y) {
       const int64_t cc = int64_t(blockIdx.y) * width + i;
@@ -356,38 +380,38 @@ __global__ void __launch_bounds__(128) conv1d_dinit_kernel(const Conv1dParams p)
     b = 0;
   }
   const int64_t len = s.hi - s.lo;
-  float w[K][4], bias[4] = {}, win[K][4], d[K - 1][4] = {};
+  uint2 w[K], win[2 * K - 2];
+  float bias[4] = {}, d[K - 1][4] = {};
 #pragma unroll
-  for (int j = 0; j < K; ++j) ldv<E, 4>(p.w, j * p.C + c, w[j]);
-  if (p.bias != nullptr) ldv<E, 4>(p.bias, c, bias);
+  for (int j = 0; j < K; ++j) w[j] = ld8(p.w, j * p.C + c);
+  if (p.bias != nullptr) unpack4<E>(ld8(p.bias, c), bias);
   if (p.dfinal != nullptr) {  // input r + len of the K-1 + len ones is row r of final_state
 #pragma unroll
     for (int r = 0; r < K - 1; ++r)
-      if (r >= len) ldv<E, 4>(p.dfinal, (n * (K - 1) + r - len) * p.C + c, d[r]);
+      if (r >= len) unpack4<E>(ld8(p.dfinal, (n * (K - 1) + r - len) * p.C + c), d[r]);
   }
 #pragma unroll
   for (int j = 0; j < K - 1; ++j)
-    conv_input_v<E, 4>(p, K, s, b * p.x_sb, s.lo - (K - 1) + j, c, win[j]);
+    win[j] = conv_input4(p, K, s, b * p.x_sb, s.lo - (K - 1) + j, c);
 #pragma unroll
   for (int t = 0; t < K - 1; ++t) {
     if (t < len) {
-      float dyv[4], dz[4];
-      ldv<E, 4>(p.x, b * p.x_sb + (s.lo + t) * p.x_st + c, win[K - 1]);
-      ldv<E, 4>(p.dy, b * p.dy_sb + (s.lo + t) * p.dy_st + c, dyv);
-      conv_dz<E, K, 4, SILU>(dz, win, w, bias, dyv);
+      win[K - 1 + t] = ld8(p.x, b * p.x_sb + (s.lo + t) * p.x_st + c);
+      float dz[4];
+      conv_dz<E, K, SILU>(dz, [&](int j) { return win[t + j]; }, w, bias,
+                          ld8(p.dy, b * p.dy_sb + (s.lo + t) * p.dy_st + c));
       // dz[t] reaches inputs t .. t+K-1 through w[0 .. K-1]
 #pragma unroll
-      for (int r = t; r < K - 1; ++r)
+      for (int r = t; r < K - 1; ++r) {
+        float f[4];
+        unpack4<E>(w[r - t], f);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[r][i] = fmaf(w[r - t][i], dz[i], d[r][i]);
-#pragma unroll
-      for (int j = 0; j < K - 1; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) win[j][i] = win[j + 1][i];
+        for (int i = 0; i < 4; ++i) d[r][i] = fmaf(f[i], dz[i], d[r][i]);
+      }
     }
   }
 #pragma unroll
-  for (int r = 0; r < K - 1; ++r) stv<E, 4>(p.dinit, (n * (K - 1) + r) * p.C + c, d[r]);
+  for (int r = 0; r < K - 1; ++r) st8<E>(p.dinit, (n * (K - 1) + r) * p.C + c, d[r]);
 }
 
 // ---- running sequences ---------------------------------------------------------

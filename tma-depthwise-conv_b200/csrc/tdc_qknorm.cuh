@@ -117,45 +117,71 @@ __device__ __forceinline__ float inv_norm(const QkParams& p, const float f[8]) {
   return rsqrtf(p.norm == 1 ? s / float(p.D) + p.eps : s + p.eps);
 }
 
-// A block takes one row of [B, T]; its groups of LANES lanes go over the
-// heads, queries first.
-template <class E, int LANES>
+// Where head h (queries first) of row (b, t) starts.
+struct HeadAt {
+  const void* in;
+  int64_t at;
+  bool is_q, has;
+  int hh;
+};
+__device__ __forceinline__ HeadAt head_at(const QkParams& p, int64_t b, int64_t t, int h) {
+  HeadAt r;
+  r.has = h < p.Hq + p.Hk;
+  r.is_q = h < p.Hq;
+  r.hh = r.is_q ? h : h - p.Hq;
+  r.in = r.is_q ? p.q : p.k;
+  r.at = r.is_q ? b * p.q_sb + t * p.q_st + r.hh * p.q_sh : b * p.k_sb + t * p.k_st + r.hh * p.k_sh;
+  return r;
+}
+
+// A block takes one row of [B, T]; its groups of LANES lanes go over the heads,
+// queries first, HEADS of a group's at a time: their loads are all under way
+// before the first sum is needed (one at a time left the pass waiting for
+// memory at a third of its bandwidth).
+template <class E, int LANES, int HEADS>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkParams p) {
   const int64_t row = blockIdx.x;
   const int64_t b = row / p.T, t = row % p.T;
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const int groups = blockDim.x / LANES;
   const bool live = 8 * lane < p.D;
-  Turn turn;
-  if (p.R > 0 && 8 * lane < p.R) load_turn(p, b, t, lane, turn);
   const int heads = p.Hq + p.Hk;
   // whole warps stay together in the shuffles, so a warp goes on while any of
   // its groups has a head left
-  const int per_warp = 32 / LANES;
-  for (int h0 = (group / per_warp) * per_warp; h0 < heads; h0 += groups) {
-    const int h = h0 + group % per_warp;
-    const bool has = h < heads, isq = h < p.Hq;
-    const int hh = isq ? h : h - p.Hq;
-    float f[8] = {};
-    if (has && live) {
-      const int64_t at = isq ? b * p.q_sb + t * p.q_st + hh * p.q_sh
-                             : b * p.k_sb + t * p.k_st + hh * p.k_sh;
-      unpack8<E>(ldg16(isq ? p.q : p.k, at + 8 * lane), f);
-    }
-    const float inv = inv_norm<LANES>(p, f);
-    const void* w = isq ? p.qw : p.kw;
-    float wv[8];
-    if (w != nullptr && live) unpack8<E>(ldg16(w, 8 * lane), wv);
+  const int per_warp = 32 / LANES, first = (group / per_warp) * per_warp;
+  for (int h0 = first; h0 < heads; h0 += HEADS * groups) {
+    uint4 v[HEADS];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      f[i] *= inv;
-      if (w != nullptr) f[i] *= wv[i];
+    for (int i = 0; i < HEADS; ++i) {
+      const HeadAt at = head_at(p, b, t, h0 + i * groups + group % per_warp);
+      v[i] = at.has && live ? ldg16(at.in, at.at + 8 * lane) : make_uint4(0, 0, 0, 0);
     }
-    if (p.R > 0) rotate<LANES>(p, turn, lane, 1.f, f);
-    if (has && live) {
-      uint16_t* out = static_cast<uint16_t*>(isq ? p.qo : p.ko) +
-                      (row * (isq ? p.Hq : p.Hk) + hh) * p.D + 8 * lane;
-      *reinterpret_cast<uint4*>(out) = pack8<E>(f);
+    Turn turn;
+    if (p.R > 0 && 8 * lane < p.R) load_turn(p, b, t, lane, turn);
+    uint4 wq = make_uint4(0, 0, 0, 0), wk = wq;  // (lanes behind D hold zeros)
+    if (p.qw != nullptr && live) wq = ldg16(p.qw, 8 * lane);
+    if (p.kw != nullptr && live) wk = ldg16(p.kw, 8 * lane);
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) {
+      if (h0 + i * groups >= heads) break;
+      const HeadAt at = head_at(p, b, t, h0 + i * groups + group % per_warp);
+      float f[8];
+      unpack8<E>(v[i], f);
+      const float inv = inv_norm<LANES>(p, f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] *= inv;
+      if ((at.is_q ? p.qw : p.kw) != nullptr) {
+        float w[8];
+        unpack8<E>(at.is_q ? wq : wk, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] *= w[j];
+      }
+      if (p.R > 0) rotate<LANES>(p, turn, lane, 1.f, f);
+      if (at.has && live) {
+        uint16_t* out = static_cast<uint16_t*>(at.is_q ? p.qo : p.ko) +
+                        (row * (at.is_q ? p.Hq : p.Hk) + at.hh) * p.D + 8 * lane;
+        *reinterpret_cast<uint4*>(out) = pack8<E>(f);
+      }
     }
   }
 }
@@ -165,56 +191,67 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkParams p) {
 // rows_per_block rows; each group of lanes keeps its share of the two
 // weights' gradients in registers, the block adds its groups in shared memory
 // and writes one partial sum, which qk_wsum_kernel adds in block order.
-template <class E, int LANES>
+template <class E, int LANES, int HEADS>
 __global__ void __launch_bounds__(256) qk_norm_rope_bwd_kernel(const QkParams p) {
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const int groups = blockDim.x / LANES, per_warp = 32 / LANES;
+  const int first = (group / per_warp) * per_warp;
   const bool live = 8 * lane < p.D;
   const int heads = p.Hq + p.Hk;
   float dqw[8] = {}, dkw[8] = {};
-  float qw[8], kw[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) qw[i] = kw[i] = 1.f;
-  if (p.qw != nullptr && live) unpack8<E>(ldg16(p.qw, 8 * lane), qw);
-  if (p.kw != nullptr && live) unpack8<E>(ldg16(p.kw, 8 * lane), kw);
+  uint4 wq = make_uint4(0, 0, 0, 0), wk = wq;  // (lanes behind D hold zeros)
+  if (p.qw != nullptr && live) wq = ldg16(p.qw, 8 * lane);
+  if (p.kw != nullptr && live) wk = ldg16(p.kw, 8 * lane);
   const int64_t r0 = int64_t(blockIdx.x) * p.rows_per_block;
   const int64_t r1 = min(r0 + p.rows_per_block, p.rows);
   for (int64_t row = r0; row < r1; ++row) {
     const int64_t b = row / p.T, t = row % p.T;
-    Turn turn;
-    if (p.R > 0 && 8 * lane < p.R) load_turn(p, b, t, lane, turn);
-    for (int h0 = (group / per_warp) * per_warp; h0 < heads; h0 += groups) {
-      const int h = h0 + group % per_warp;
-      const bool has = h < heads, isq = h < p.Hq;
-      const int hh = isq ? h : h - p.Hq;
-      float f[8] = {}, d[8] = {};
-      if (has && live) {
-        const int64_t at = isq ? b * p.q_sb + t * p.q_st + hh * p.q_sh
-                               : b * p.k_sb + t * p.k_st + hh * p.k_sh;
-        const int64_t ga = isq ? b * p.gq_sb + t * p.gq_st + hh * p.gq_sh
-                               : b * p.gk_sb + t * p.gk_st + hh * p.gk_sh;
-        unpack8<E>(ldg16(isq ? p.q : p.k, at + 8 * lane), f);
-        unpack8<E>(ldg16(isq ? p.gq : p.gk, ga + 8 * lane), d);
-      }
-      const float inv = inv_norm<LANES>(p, f);
-      if (p.R > 0) rotate<LANES>(p, turn, lane, -1.f, d);
-      float m = 0.f;
+    for (int h0 = first; h0 < heads; h0 += HEADS * groups) {
+      uint4 v[HEADS], g[HEADS];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        f[i] *= inv;
-        const float g = d[i] * f[i];
-        if (isq) dqw[i] += g; else dkw[i] += g;
-        d[i] *= isq ? qw[i] : kw[i];
-        m = fmaf(d[i], f[i], m);
+      for (int i = 0; i < HEADS; ++i) {
+        const HeadAt at = head_at(p, b, t, h0 + i * groups + group % per_warp);
+        const int64_t ga = at.is_q ? b * p.gq_sb + t * p.gq_st + at.hh * p.gq_sh
+                                   : b * p.gk_sb + t * p.gk_st + at.hh * p.gk_sh;
+        const bool go = at.has && live;
+        v[i] = go ? ldg16(at.in, at.at + 8 * lane) : make_uint4(0, 0, 0, 0);
+        g[i] = go ? ldg16(at.is_q ? p.gq : p.gk, ga + 8 * lane) : make_uint4(0, 0, 0, 0);
       }
-      m = lane_sum<LANES>(m);
-      m = p.norm == 0 ? 0.f : p.norm == 1 ? m / float(p.D) : m;
+      Turn turn;
+      if (p.R > 0 && 8 * lane < p.R) load_turn(p, b, t, lane, turn);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) d[i] = inv * (d[i] - f[i] * m);
-      if (has && live) {
-        uint16_t* out = static_cast<uint16_t*>(isq ? p.dq : p.dk) +
-                        (row * (isq ? p.Hq : p.Hk) + hh) * p.D + 8 * lane;
-        *reinterpret_cast<uint4*>(out) = pack8<E>(d);
+      for (int i = 0; i < HEADS; ++i) {
+        if (h0 + i * groups >= heads) break;
+        const HeadAt at = head_at(p, b, t, h0 + i * groups + group % per_warp);
+        float f[8], d[8];
+        unpack8<E>(v[i], f);
+        unpack8<E>(g[i], d);
+        const float inv = inv_norm<LANES>(p, f);
+        if (p.R > 0) rotate<LANES>(p, turn, lane, -1.f, d);
+        float m = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] *= inv;
+        if ((at.is_q ? p.qw : p.kw) != nullptr) {
+          float w[8];
+          unpack8<E>(at.is_q ? wq : wk, w);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float dw = d[j] * f[j];
+            if (at.is_q) dqw[j] += dw; else dkw[j] += dw;
+            d[j] *= w[j];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = fmaf(d[j], f[j], m);
+        m = lane_sum<LANES>(m);
+        m = p.norm == 0 ? 0.f : p.norm == 1 ? m / float(p.D) : m;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j] = inv * (d[j] - f[j] * m);
+        if (at.has && live) {
+          uint16_t* out = static_cast<uint16_t*>(at.is_q ? p.dq : p.dk) +
+                          (row * (at.is_q ? p.Hq : p.Hk) + at.hh) * p.D + 8 * lane;
+          *reinterpret_cast<uint4*>(out) = pack8<E>(d);
+        }
       }
     }
   }

@@ -105,8 +105,13 @@ __device__ __forceinline__ void store_float(void* p, int64_t i, float v) {
   else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
-// 1 / (1 + exp(-z)): an overflowing exp gives 0, as the limit is.
-__device__ __forceinline__ float sigmoid_f(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+// 1 / (1 + exp(-z)), both steps in hardware's approximate forms (2^-21 or
+// better); an overflowing exp gives 0, as the limit is.
+__device__ __forceinline__ float sigmoid_f(float z) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + __expf(-z)));
+  return r;
+}
 
 // ---- asynchronous copies ----------------------------------------------------------
 // 16 bytes global -> shared; with `valid` false the destination gets zeros and

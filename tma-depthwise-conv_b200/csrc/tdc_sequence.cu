@@ -82,29 +82,32 @@ tdc::Conv1dParams conv_params(const tdc_conv1d_args* a) {
 
 template <class E, int K>
 int conv_fwd_k(const tdc::Conv1dParams& p, bool silu, int64_t blocks, cudaStream_t st) {
-  if (silu) tdc::conv1d_fwd_kernel<E, K, true><<<unsigned(blocks), 256, 0, st>>>(p);
-  else tdc::conv1d_fwd_kernel<E, K, false><<<unsigned(blocks), 256, 0, st>>>(p);
+  const bool packed = p.seq.cu != nullptr;
+  auto* k = silu ? (packed ? &tdc::conv1d_fwd_kernel<E, K, true, true>
+                           : &tdc::conv1d_fwd_kernel<E, K, true, false>)
+                 : (packed ? &tdc::conv1d_fwd_kernel<E, K, false, true>
+                           : &tdc::conv1d_fwd_kernel<E, K, false, false>);
+  k<<<unsigned(blocks), 256, 0, st>>>(p);
   return launched();
 }
 
-// Backward launch shape: a block is LX vectors of channels by 256 / LX runs.
+// Backward launch shape: a block is LX vectors of 4 channels by 256 / LX runs.
 struct ConvBwdPlan {
-  int vec, lx, run;
+  int lx, run;
   int64_t runs_per_b, groups, cblocks;
 };
 
 ConvBwdPlan conv_bwd_plan(const tdc_conv1d_args* a) {
   ConvBwdPlan pl;
-  pl.vec = a->K <= 4 ? 8 : 4;  // beyond 4 taps 8 channels' windows no longer fit the registers
-  const int64_t vecs = a->C / pl.vec;
+  const int64_t vecs = a->C / tdc::kGradVec;
   pl.lx = vecs >= 32 ? 32 : vecs >= 16 ? 16 : 8;
   pl.cblocks = ceil_div(vecs, pl.lx);
-  // One wave of 2 blocks on each of 148 SMs; a run of at least 8 rows, or the
-  // K-1 rows that it recomputes behind its end would cost more than they save.
-  const int64_t lanes = 148 * 512;
-  const int64_t want = std::max<int64_t>(1, lanes / std::max<int64_t>(1, pl.cblocks * pl.lx));
+  // One wave on 148 SMs (2 blocks each, 1 beyond 4 taps); a run of at least 8 rows, or
+  // the K-1 rows that it recomputes behind its end would cost more than they save.
+  const int64_t blocks = 148 * (a->K <= 4 ? 2 : 1);
   const int64_t rows = std::max<int64_t>(1, a->B * a->T);
-  int64_t run = std::max<int64_t>(8, ceil_div(rows, want));
+  const int64_t groups = std::max<int64_t>(1, blocks / pl.cblocks);
+  int64_t run = std::max<int64_t>(8, ceil_div(rows, groups * (256 / pl.lx)));
   run = std::min(run, std::max<int64_t>(1, a->T));
   pl.runs_per_b = ceil_div(std::max<int64_t>(1, a->T), run);
   pl.run = int(std::min<int64_t>(ceil_div(std::max<int64_t>(1, a->T), pl.runs_per_b), 1 << 30));
@@ -115,10 +118,10 @@ ConvBwdPlan conv_bwd_plan(const tdc_conv1d_args* a) {
 template <class E, int K, bool SILU>
 int conv_bwd_t(const tdc::Conv1dParams& p, const ConvBwdPlan& pl, void* dw, void* dbias,
                cudaStream_t st) {
-  constexpr int VEC = K <= 4 ? 8 : 4;
   const dim3 block(pl.lx, 256 / pl.lx), grid(unsigned(pl.groups), unsigned(pl.cblocks));
-  const size_t smem = size_t(256) * VEC * sizeof(float);
-  tdc::conv1d_bwd_kernel<E, K, VEC, SILU><<<grid, block, smem, st>>>(p);
+  auto* k = p.seq.cu != nullptr ? &tdc::conv1d_bwd_kernel<E, K, SILU, true>
+                                : &tdc::conv1d_bwd_kernel<E, K, SILU, false>;
+  k<<<grid, block, 0, st>>>(p);
   int rc = launched();
   if (rc != TDC_OK) return rc;
   const int64_t values = (K + 1) * p.C;
@@ -237,10 +240,10 @@ template <class E>
 int qk_fwd_e(const tdc::QkParams& p, int threads, cudaStream_t st) {
   const unsigned grid = unsigned(p.rows);
   switch (qk_lanes(p.D)) {
-    case 4: tdc::qk_norm_rope_kernel<E, 4><<<grid, threads, 0, st>>>(p); break;
-    case 8: tdc::qk_norm_rope_kernel<E, 8><<<grid, threads, 0, st>>>(p); break;
-    case 16: tdc::qk_norm_rope_kernel<E, 16><<<grid, threads, 0, st>>>(p); break;
-    default: tdc::qk_norm_rope_kernel<E, 32><<<grid, threads, 0, st>>>(p); break;
+    case 4: tdc::qk_norm_rope_kernel<E, 4, 4><<<grid, threads, 0, st>>>(p); break;
+    case 8: tdc::qk_norm_rope_kernel<E, 8, 4><<<grid, threads, 0, st>>>(p); break;
+    case 16: tdc::qk_norm_rope_kernel<E, 16, 4><<<grid, threads, 0, st>>>(p); break;
+    default: tdc::qk_norm_rope_kernel<E, 32, 4><<<grid, threads, 0, st>>>(p); break;
   }
   return launched();
 }
@@ -250,10 +253,10 @@ int qk_bwd_e(const tdc::QkParams& p, int threads, int64_t blocks, void* dqw, voi
              cudaStream_t st) {
   const unsigned grid = unsigned(blocks);
   switch (qk_lanes(p.D)) {
-    case 4: tdc::qk_norm_rope_bwd_kernel<E, 4><<<grid, threads, 0, st>>>(p); break;
-    case 8: tdc::qk_norm_rope_bwd_kernel<E, 8><<<grid, threads, 0, st>>>(p); break;
-    case 16: tdc::qk_norm_rope_bwd_kernel<E, 16><<<grid, threads, 0, st>>>(p); break;
-    default: tdc::qk_norm_rope_bwd_kernel<E, 32><<<grid, threads, 0, st>>>(p); break;
+    case 4: tdc::qk_norm_rope_bwd_kernel<E, 4, 3><<<grid, threads, 0, st>>>(p); break;
+    case 8: tdc::qk_norm_rope_bwd_kernel<E, 8, 3><<<grid, threads, 0, st>>>(p); break;
+    case 16: tdc::qk_norm_rope_bwd_kernel<E, 16, 3><<<grid, threads, 0, st>>>(p); break;
+    default: tdc::qk_norm_rope_bwd_kernel<E, 32, 3><<<grid, threads, 0, st>>>(p); break;
   }
   const int rc = launched();
   if (rc != TDC_OK || p.partial == nullptr) return rc;
@@ -426,9 +429,9 @@ TDC_API int tdc_conv1d_fwd(const tdc_conv1d_args* a, void* stream) {
   if (misaligned(a->x) || misaligned(a->w) || misaligned(a->y) || misaligned(a->bias) ||
       misaligned(a->initial_state) || misaligned(a->final_state))
     return TDC_ERR_ALIGNMENT;
-  // A run of up to 16 rows a thread (it reads K-1 rows more than it writes);
+  // A run of up to 32 rows a thread (it reads K-1 rows more than it writes);
   // shorter runs while 148 SMs would not get 1024 threads each.
-  p.run = 16;
+  p.run = 32;
   while (p.run > 1 && vecs * a->B * ceil_div(a->T, p.run) < 148 * 1024) p.run /= 2;
   p.runs_per_b = ceil_div(a->T, p.run);
   p.main_threads = a->B * p.runs_per_b * vecs;
