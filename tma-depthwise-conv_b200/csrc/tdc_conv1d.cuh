@@ -184,23 +184,34 @@ __global__ void __launch_bounds__(256, 2) conv1d_fwd_kernel(const Conv1dParams p
 // (8 would not leave registers for the taps' sums) and a run of rows.  The last
 // K inputs and the K unfinished rows of dx sit in rings of registers whose
 // places are fixed by unrolling K rows; dz[t] is added to the rows it reaches.
+// Rows in the inside of a sequence and a run go through the loop without a test.
 // The K-1 values of dz behind the run are recomputed.  The runs of a block are
 // added in shared memory and one partial sum per block goes to the workspace,
 // which conv1d_wsum_kernel adds in a fixed order.
 constexpr int kGradVec = 4;
 
+struct Quad {  // 4 channels
+  float2 a, b;
+};
 template <class E>
-__device__ __forceinline__ void unpack4(const uint2& v, float f[4]) {
-  unpack2<E>(v.x, f[0], f[1]);
-  unpack2<E>(v.y, f[2], f[3]);
+__device__ __forceinline__ Quad unpack4(const uint2& v) {
+  Quad q;
+  unpack2<E>(v.x, q.a.x, q.a.y);
+  unpack2<E>(v.y, q.b.x, q.b.y);
+  return q;
 }
+__device__ __forceinline__ void fma4(Quad& d, const Quad& x, const Quad& y) {
+  fma_pair(d.a, x.a, y.a);
+  fma_pair(d.b, x.b, y.b);
+}
+__device__ __forceinline__ Quad zero4() { return {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}; }
 __device__ __forceinline__ uint2 ld8(const void* base, int64_t elem) {
   return __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + elem));
 }
 template <class E>
-__device__ __forceinline__ void st8(void* base, int64_t elem, const float f[4]) {
+__device__ __forceinline__ void st8(void* base, int64_t elem, const Quad& f) {
   *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + elem) =
-      make_uint2(pack2_rn<E>(f[0], f[1]), pack2_rn<E>(f[2], f[3]));
+      make_uint2(pack2_rn<E>(f.a.x, f.a.y), pack2_rn<E>(f.b.x, f.b.y));
 }
 
 __device__ __forceinline__ uint2 conv_input4(const Conv1dParams& p, int taps, const SeqSpan& s,
@@ -212,42 +223,40 @@ __device__ __forceinline__ uint2 conv_input4(const Conv1dParams& p, int taps, co
 }
 
 // dz = dy act'(z), z from the inputs at(0) .. at(K-1) (the last is the row's own).
-template <class E, int K, bool SILU, class At>
-__device__ __forceinline__ void conv_dz(float dz[4], At at, const uint2 w[K], const float bias[4],
-                                        const uint2& dy) {
-  unpack4<E>(dy, dz);
-  if constexpr (SILU) {
-    float z[4] = {bias[0], bias[1], bias[2], bias[3]};
+__device__ __forceinline__ float dsilu(float dy, float z) {
+  const float sg = sigmoid_f(z);
+  return dy * (sg * fmaf(z, 1.f - sg, 1.f));
+}
+template <int K, bool SILU, class At>
+__device__ __forceinline__ Quad conv_dz(At at, const Quad w[K], const Quad& bias, const Quad& dy) {
+  if constexpr (!SILU) {
+    return dy;
+  } else {
+    Quad z = bias;
 #pragma unroll
-    for (int j = 0; j < K; ++j) {
-      const uint2 v = at(j);
-      fma2<E>(v.x, w[j].x, z[0], z[1]);
-      fma2<E>(v.y, w[j].y, z[2], z[3]);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float sg = sigmoid_f(z[i]);
-      dz[i] *= sg * fmaf(z[i], 1.f - sg, 1.f);
-    }
+    for (int j = 0; j < K; ++j) fma4(z, at(j), w[j]);
+    return {make_float2(dsilu(dy.a.x, z.a.x), dsilu(dy.a.y, z.a.y)),
+            make_float2(dsilu(dy.b.x, z.b.x), dsilu(dy.b.y, z.b.y))};
   }
 }
 
 template <class E, int K, bool SILU, bool PACKED>
 __global__ void __launch_bounds__(256, K <= 4 ? 2 : 1) conv1d_bwd_kernel(const Conv1dParams p) {
-  __shared__ float red[256 * kGradVec];  // [blockDim.y][blockDim.x * 4]
+  __shared__ __align__(16) float red[256 * kGradVec];  // [blockDim.y][blockDim.x * 4]
   const int64_t c = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * kGradVec;
   const int64_t run = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
   const int64_t b = run / p.runs_per_b;
   const bool live = c < p.C && b < p.B;
-  float dw[K][4] = {}, db[4] = {};
+  Quad dw[K], db = zero4();
+#pragma unroll
+  for (int j = 0; j < K; ++j) dw[j] = zero4();
   if (live) {
     const int64_t t0 = (run % p.runs_per_b) * p.run, t1 = min(t0 + p.run, p.T);
     const int64_t xbase = b * p.x_sb;
-    uint2 w[K];
-    float bias[4] = {};
+    Quad w[K], bias = zero4();
 #pragma unroll
-    for (int j = 0; j < K; ++j) w[j] = ld8(p.w, j * p.C + c);
-    if (p.bias != nullptr) unpack4<E>(ld8(p.bias, c), bias);
+    for (int j = 0; j < K; ++j) w[j] = unpack4<E>(ld8(p.w, j * p.C + c));
+    if (p.bias != nullptr) bias = unpack4<E>(ld8(p.bias, c));
     SeqSpan s{b, 0, p.T, true};
     if (PACKED) s = span_at(p.seq, b, t0);
     int64_t a = t0;
@@ -257,67 +266,67 @@ __global__ void __launch_bounds__(256, K <= 4 ? 2 : 1) conv1d_bwd_kernel(const C
       const uint16_t* dy = static_cast<const uint16_t*>(p.dy) + b * p.dy_sb + a * p.dy_st + c;
       uint16_t* dx = static_cast<uint16_t*>(p.dx) + (b * p.T + a) * p.C + c;
       if (PACKED && !s.covered) {
-        const float zero[4] = {};
-        for (int64_t t = a; t < e; ++t, dx += p.C) st8<E>(dx, 0, zero);
+        for (int64_t t = a; t < e; ++t, dx += p.C) st8<E>(dx, 0, zero4());
       } else {
         const int own = int(e - a);                                       // rows of dx
         const int known = int(min(int64_t(own + K - 1), s.hi - a));       // rows of dz
         const int64_t to_final = K - 1 - (s.hi - a);  // row i is row i + to_final of final_state
-        uint2 xr[K], xn[K], dn[K];
-        float acc[K][4] = {};
+        // Rows before `inside` need no test: dz is known K rows ahead, and no row is one of
+        // the final state's.
+        const int inside = min(own, known - K);
+        uint2 xn[K], dn[K];
+        Quad xr[K], acc[K];
         // row a - (K-1) + j has place (j + 1) % K
+        xr[0] = zero4();
 #pragma unroll
-        for (int j = 0; j < K - 1; ++j) xr[j + 1] = conv_input4(p, K, s, xbase, a - (K - 1) + j, c);
+        for (int j = 0; j < K - 1; ++j)
+          xr[j + 1] = unpack4<E>(conv_input4(p, K, s, xbase, a - (K - 1) + j, c));
 #pragma unroll
-        for (int u = 0; u < K; ++u)
+        for (int u = 0; u < K; ++u) {
+          acc[u] = zero4();
           if (u < known) {
             xn[u] = ld8(x, u * p.x_st);
             dn[u] = ld8(dy, u * p.dy_st);
           }
-        for (int i0 = 0; i0 < own + K - 1; i0 += K) {
+        }
+        // Row i takes place u of both rings; K rows on its place is loaded again.
+        auto row = [&](int i, int u, auto tested) {
+          constexpr bool TEST = decltype(tested)::value;
+          acc[u] = zero4();
+          if (TEST && p.dfinal != nullptr && i < own && i + to_final >= 0)
+            acc[u] = unpack4<E>(ld8(p.dfinal, (s.n * (K - 1) + i + to_final) * p.C + c));
+          if (!TEST || i < known) {
+            xr[u] = unpack4<E>(xn[u]);
+            const Quad dyv = unpack4<E>(dn[u]);
+            if (!TEST || i + K < known) {
+              xn[u] = ld8(x, u * p.x_st);
+              dn[u] = ld8(dy, u * p.dy_st);
+            }
+            const Quad dz =
+                conv_dz<K, SILU>([&](int j) -> const Quad& { return xr[(u + 1 + j) % K]; }, w, bias, dyv);
+            if (!TEST || i < own) {
+#pragma unroll
+              for (int j = 0; j < K; ++j) fma4(dw[j], dz, xr[(u + 1 + j) % K]);
+              db.a.x += dz.a.x, db.a.y += dz.a.y, db.b.x += dz.b.x, db.b.y += dz.b.y;
+            }
+#pragma unroll
+            for (int j = 0; j < K; ++j) fma4(acc[(u + 1 + j) % K], w[j], dz);  // row i - (K-1) + j
+          }
+          if (!TEST || (i >= K - 1 && i < own + K - 1)) {
+            st8<E>(dx, 0, acc[(u + 1) % K]);
+            dx += p.C;
+          }
+        };
+        int i0 = 0;
+        for (; i0 < own + K - 1; i0 += K) {
           x += K * p.x_st;
           dy += K * p.dy_st;
+          if (i0 > 0 && i0 + K <= inside) {
 #pragma unroll
-          for (int u = 0; u < K; ++u) {
-            const int i = i0 + u;
-            // row i takes place u of both rings
+            for (int u = 0; u < K; ++u) row(i0 + u, u, std::false_type{});
+          } else {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) acc[u][q] = 0.f;
-            if (p.dfinal != nullptr && i < own && i + to_final >= 0)
-              unpack4<E>(ld8(p.dfinal, (s.n * (K - 1) + i + to_final) * p.C + c), acc[u]);
-            if (i < known) {
-              xr[u] = xn[u];
-              const uint2 dyv = dn[u];
-              if (i + K < known) {  // the row that takes this place next
-                xn[u] = ld8(x, u * p.x_st);
-                dn[u] = ld8(dy, u * p.dy_st);
-              }
-              float dz[4];
-              conv_dz<E, K, SILU>(dz, [&](int j) { return xr[(u + 1 + j) % K]; }, w, bias, dyv);
-              if (i < own) {
-#pragma unroll
-                for (int j = 0; j < K; ++j) {
-                  float f[4];
-                  unpack4<E>(xr[(u + 1 + j) % K], f);
-#pragma unroll
-                  for (int q = 0; q < 4; ++q) dw[j][q] = fmaf(dz[q], f[q], dw[j][q]);
-                }
-#pragma unroll
-                for (int q = 0; q < 4; ++q) db[q] += dz[q];
-              }
-#pragma unroll
-              for (int j = 0; j < K; ++j) {  // to row i - (K-1) + j
-                float f[4];
-                unpack4<E>(w[j], f);
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                  acc[(u + 1 + j) % K][q] = fmaf(f[q], dz[q], acc[(u + 1 + j) % K][q]);
-              }
-            }
-            if (i >= K - 1 && i < own + K - 1) {
-              st8<E>(dx, 0, acc[(u + 1) % K]);
-              dx += p.C;
-            }
+            for (int u = 0; u < K; ++u) row(i0 + u, u, std::true_type{});
           }
         }
       }
@@ -330,9 +339,9 @@ __global__ void __launch_bounds__(256, K <= 4 ? 2 : 1) conv1d_bwd_kernel(const C
 #pragma unroll
   for (int j = 0; j <= K; ++j) {
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kGradVec; ++i)
-      red[threadIdx.y * width + threadIdx.x * kGradVec + i] = j < K ? dw[j < K ? j : 0][i] : db[i];
+    const Quad part = j < K ? dw[j < K ? j : 0] : db;
+    *reinterpret_cast<float4*>(red + threadIdx.y * width + threadIdx.x * kGradVec) =
+        make_float4(part.a.x, part.a.y, part.b.x, part.b.y);
     __syncthreads();
     for (int i = threadIdx.y * blockDim.x + threadIdx.x; i < width; i += blockDim.x * blockDim.y) {
       const int64_t cc = int64_t(blockIdx.y) * width + i;
@@ -380,34 +389,29 @@ __global__ void __launch_bounds__(128) conv1d_dinit_kernel(const Conv1dParams p)
     b = 0;
   }
   const int64_t len = s.hi - s.lo;
-  uint2 w[K], win[2 * K - 2];
-  float bias[4] = {}, d[K - 1][4] = {};
+  Quad w[K], win[2 * K - 2], d[K - 1], bias = zero4();
 #pragma unroll
-  for (int j = 0; j < K; ++j) w[j] = ld8(p.w, j * p.C + c);
-  if (p.bias != nullptr) unpack4<E>(ld8(p.bias, c), bias);
-  if (p.dfinal != nullptr) {  // input r + len of the K-1 + len ones is row r of final_state
+  for (int j = 0; j < K; ++j) w[j] = unpack4<E>(ld8(p.w, j * p.C + c));
+  if (p.bias != nullptr) bias = unpack4<E>(ld8(p.bias, c));
+  // input r + len of the K-1 + len ones is row r of final_state
 #pragma unroll
-    for (int r = 0; r < K - 1; ++r)
-      if (r >= len) unpack4<E>(ld8(p.dfinal, (n * (K - 1) + r - len) * p.C + c), d[r]);
-  }
+  for (int r = 0; r < K - 1; ++r)
+    d[r] = p.dfinal != nullptr && r >= len
+               ? unpack4<E>(ld8(p.dfinal, (n * (K - 1) + r - len) * p.C + c))
+               : zero4();
 #pragma unroll
   for (int j = 0; j < K - 1; ++j)
-    win[j] = conv_input4(p, K, s, b * p.x_sb, s.lo - (K - 1) + j, c);
+    win[j] = unpack4<E>(conv_input4(p, K, s, b * p.x_sb, s.lo - (K - 1) + j, c));
 #pragma unroll
   for (int t = 0; t < K - 1; ++t) {
     if (t < len) {
-      win[K - 1 + t] = ld8(p.x, b * p.x_sb + (s.lo + t) * p.x_st + c);
-      float dz[4];
-      conv_dz<E, K, SILU>(dz, [&](int j) { return win[t + j]; }, w, bias,
-                          ld8(p.dy, b * p.dy_sb + (s.lo + t) * p.dy_st + c));
+      win[K - 1 + t] = unpack4<E>(ld8(p.x, b * p.x_sb + (s.lo + t) * p.x_st + c));
+      const Quad dz = conv_dz<K, SILU>(
+          [&](int j) -> const Quad& { return win[t + j]; }, w, bias,
+          unpack4<E>(ld8(p.dy, b * p.dy_sb + (s.lo + t) * p.dy_st + c)));
       // dz[t] reaches inputs t .. t+K-1 through w[0 .. K-1]
 #pragma unroll
-      for (int r = t; r < K - 1; ++r) {
-        float f[4];
-        unpack4<E>(w[r - t], f);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d[r][i] = fmaf(f[i], dz[i], d[r][i]);
-      }
+      for (int r = t; r < K - 1; ++r) fma4(d[r], w[r - t], dz);
     }
   }
 #pragma unroll

@@ -23,7 +23,8 @@ struct QkParams {
   int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, p_sb, p_st;
   int64_t table_rows, rows;  // rows: B * T
   bool pos64, interleaved;
-  int norm;                  // 0 none, 1 rms, 2 l2
+  bool norm;
+  float mul;                 // 1 / D (mean) or 1 (sum)
   float eps;
   // gradients
   const void *gq, *gk;
@@ -40,14 +41,22 @@ __device__ __forceinline__ float lane_sum(float v) {
   return v;
 }
 
-// cos and sin of the pairs that this lane's 8 values belong to: in the half
-// layout pair (8 * lane + i) mod R/2, in the interleaved one 4 * lane + i / 2.
+// How the pairs lie: no rotation, (i, i + R/2), (2i, 2i + 1).
+enum { kNoTurn = 0, kHalves = 1, kPairs = 2 };
+
+// cos and sin of the pairs that this lane's values belong to, for the angle
+// (sign 1) or its opposite (-1): halves, 8 of each for pair (8 lane + i) mod R/2,
+// the sine with the sign that this lane's half takes; pairs, 4 for 4 lane + i.
+template <int TURN>
 struct Turn {
-  float c[8], s[8];
+  static constexpr int N = TURN == kPairs ? 4 : 8;
+  float c[N], s[N];
 };
 
+template <int TURN>
 __device__ __forceinline__ void load_turn(const QkParams& p, int64_t b, int64_t t, int lane,
-                                          Turn& r) {
+                                          float sign, Turn<TURN>& r) {
+  constexpr int N = Turn<TURN>::N;
   const int64_t pi = b * p.p_sb + t * p.p_st;
   const int64_t at = p.pos == nullptr ? t
                      : p.pos64        ? static_cast<const int64_t*>(p.pos)[pi]
@@ -55,50 +64,44 @@ __device__ __forceinline__ void load_turn(const QkParams& p, int64_t b, int64_t 
   const int half = p.R / 2;
   if (at < 0 || at >= p.table_rows) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.c[i] = r.s[i] = __int_as_float(0x7fc00000);
+    for (int i = 0; i < N; ++i) r.c[i] = r.s[i] = __int_as_float(0x7fc00000);
     return;
   }
-  if (p.interleaved) {
-    const int64_t o = at * half + 4 * lane;
-    const float4 c = __ldg(reinterpret_cast<const float4*>(p.cos + o));
-    const float4 s = __ldg(reinterpret_cast<const float4*>(p.sin + o));
-    r.c[0] = r.c[1] = c.x, r.c[2] = r.c[3] = c.y, r.c[4] = r.c[5] = c.z, r.c[6] = r.c[7] = c.w;
-    r.s[0] = r.s[1] = s.x, r.s[2] = r.s[3] = s.y, r.s[4] = r.s[5] = s.z, r.s[6] = r.s[7] = s.w;
-  } else {
-    const int64_t o = at * half + (8 * lane) % half;
+  int from = N * lane;
+  if (TURN == kHalves) {
+    if (from >= half) from -= half; else sign = -sign;
+  }
+  const int64_t o = at * half + from;
 #pragma unroll
-    for (int i = 0; i < 8; i += 4) {
-      const float4 c = __ldg(reinterpret_cast<const float4*>(p.cos + o + i));
-      const float4 s = __ldg(reinterpret_cast<const float4*>(p.sin + o + i));
-      r.c[i] = c.x, r.c[i + 1] = c.y, r.c[i + 2] = c.z, r.c[i + 3] = c.w;
-      r.s[i] = s.x, r.s[i + 1] = s.y, r.s[i + 2] = s.z, r.s[i + 3] = s.w;
-    }
+  for (int i = 0; i < N; i += 4) {
+    const float4 c = __ldg(reinterpret_cast<const float4*>(p.cos + o + i));
+    const float4 s = __ldg(reinterpret_cast<const float4*>(p.sin + o + i));
+    r.c[i] = c.x, r.c[i + 1] = c.y, r.c[i + 2] = c.z, r.c[i + 3] = c.w;
+    r.s[i] = sign * s.x, r.s[i + 1] = sign * s.y, r.s[i + 2] = sign * s.z, r.s[i + 3] = sign * s.w;
   }
 }
 
-// Rotates the row that LANES lanes hold, by the angle (sign 1) or back (-1).
-// Lanes behind R keep their values; every lane takes part in the shuffles.
-template <int LANES>
-__device__ __forceinline__ void rotate(const QkParams& p, const Turn& r, int lane, float sign,
-                                       float f[8]) {
+// Rotates the row that LANES lanes hold.  Lanes behind R keep their values;
+// every lane takes part in the shuffles.
+template <int LANES, int TURN>
+__device__ __forceinline__ void rotate(const QkParams& p, const Turn<TURN>& r, int lane, float f[8]) {
   const bool in = 8 * lane < p.R;
-  if (p.interleaved) {
+  if constexpr (TURN == kPairs) {
     if (!in) return;
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
       const float a = f[i], b = f[i + 1];
-      f[i] = a * r.c[i] - sign * b * r.s[i];
-      f[i + 1] = b * r.c[i] + sign * a * r.s[i];
+      f[i] = a * r.c[i / 2] - b * r.s[i / 2];
+      f[i + 1] = b * r.c[i / 2] + a * r.s[i / 2];
     }
-    return;
-  }
-  const int step = p.R / 16;           // lanes from a value to its partner
-  const bool low = lane < step;        // the first of the pair
-  const int partner = low ? lane + step : lane - step;
+  } else {
+    const int step = p.R / 16;  // lanes from a value to its partner
+    const int partner = !in ? lane : lane < step ? lane + step : lane - step;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float o = __shfl_sync(0xffffffffu, f[i], in ? partner : lane, LANES);
-    if (in) f[i] = f[i] * r.c[i] + (low ? -sign : sign) * o * r.s[i];
+    for (int i = 0; i < 8; ++i) {
+      const float o = __shfl_sync(0xffffffffu, f[i], partner, LANES);
+      if (in) f[i] = fmaf(f[i], r.c[i], o * r.s[i]);
+    }
   }
 }
 
@@ -109,79 +112,88 @@ __device__ __forceinline__ uint4 ldg16(const void* base, int64_t elem) {
 // 1 / sqrt(mean or sum of squares + eps) of the row.
 template <int LANES>
 __device__ __forceinline__ float inv_norm(const QkParams& p, const float f[8]) {
-  float s = 0.f;
+  float2 q = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) s = fmaf(f[i], f[i], s);
-  s = lane_sum<LANES>(s);
-  if (p.norm == 0) return 1.f;
-  return rsqrtf(p.norm == 1 ? s / float(p.D) + p.eps : s + p.eps);
+  for (int i = 0; i < 8; i += 2) {
+    const float2 v = make_float2(f[i], f[i + 1]);
+    fma_pair(q, v, v);
+  }
+  const float s = lane_sum<LANES>(q.x + q.y);
+  return p.norm ? rsqrtf(fmaf(s, p.mul, p.eps)) : 1.f;
 }
 
-// Where head h (queries first) of row (b, t) starts.
-struct HeadAt {
-  const void* in;
-  int64_t at;
-  bool is_q, has;
-  int hh;
+// Row (b, t) of the tensors, and the heads of a group of lanes in it: queries
+// first, then keys, in elements.
+struct RowAt {
+  const uint16_t *q, *k;
+  int64_t qh, kh;  // from head to head
+  __device__ __forceinline__ const uint16_t* head(int h, int Hq) const {
+    return h < Hq ? q + h * qh : k + (h - Hq) * kh;
+  }
 };
-__device__ __forceinline__ HeadAt head_at(const QkParams& p, int64_t b, int64_t t, int h) {
-  HeadAt r;
-  r.has = h < p.Hq + p.Hk;
-  r.is_q = h < p.Hq;
-  r.hh = r.is_q ? h : h - p.Hq;
-  r.in = r.is_q ? p.q : p.k;
-  r.at = r.is_q ? b * p.q_sb + t * p.q_st + r.hh * p.q_sh : b * p.k_sb + t * p.k_st + r.hh * p.k_sh;
-  return r;
+__device__ __forceinline__ RowAt row_of(const void* q, const void* k, int64_t b, int64_t t, int64_t qb,
+                                        int64_t qt, int64_t qh, int64_t kb, int64_t kt, int64_t kh,
+                                        int lane) {
+  return {static_cast<const uint16_t*>(q) + b * qb + t * qt + 8 * lane,
+          static_cast<const uint16_t*>(k) + b * kb + t * kt + 8 * lane, qh, kh};
+}
+__device__ __forceinline__ uint4 ldg16(const uint16_t* at) {
+  return __ldg(reinterpret_cast<const uint4*>(at));
 }
 
 // A block takes one row of [B, T]; its groups of LANES lanes go over the heads,
 // queries first, HEADS of a group's at a time: their loads are all under way
-// before the first sum is needed (one at a time left the pass waiting for
-// memory at a third of its bandwidth).
-template <class E, int LANES, int HEADS>
+// before the first sum is needed.
+template <class E, int LANES, int HEADS, int TURN>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkParams p) {
-  const int64_t row = blockIdx.x;
-  const int64_t b = row / p.T, t = row % p.T;
+  const uint32_t row = blockIdx.x;
+  const uint32_t b = row / uint32_t(p.T), t = row - b * uint32_t(p.T);
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const int groups = blockDim.x / LANES;
   const bool live = 8 * lane < p.D;
   const int heads = p.Hq + p.Hk;
+  const RowAt in = row_of(p.q, p.k, b, t, p.q_sb, p.q_st, p.q_sh, p.k_sb, p.k_st, p.k_sh, lane);
+  uint16_t* qo = static_cast<uint16_t*>(p.qo) + int64_t(row) * p.Hq * p.D + 8 * lane;
+  uint16_t* ko = static_cast<uint16_t*>(p.ko) + int64_t(row) * p.Hk * p.D + 8 * lane;
+  const int per_warp = 32 / LANES;
   // whole warps stay together in the shuffles, so a warp goes on while any of
   // its groups has a head left
-  const int per_warp = 32 / LANES, first = (group / per_warp) * per_warp;
-  for (int h0 = first; h0 < heads; h0 += HEADS * groups) {
-    uint4 v[HEADS];
+  const int first = (group / per_warp) * per_warp, mine = group % per_warp;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  uint4 v[HEADS];
 #pragma unroll
-    for (int i = 0; i < HEADS; ++i) {
-      const HeadAt at = head_at(p, b, t, h0 + i * groups + group % per_warp);
-      v[i] = at.has && live ? ldg16(at.in, at.at + 8 * lane) : make_uint4(0, 0, 0, 0);
-    }
-    Turn turn;
-    if (p.R > 0 && 8 * lane < p.R) load_turn(p, b, t, lane, turn);
-    uint4 wq = make_uint4(0, 0, 0, 0), wk = wq;  // (lanes behind D hold zeros)
-    if (p.qw != nullptr && live) wq = ldg16(p.qw, 8 * lane);
-    if (p.kw != nullptr && live) wk = ldg16(p.kw, 8 * lane);
+  for (int i = 0; i < HEADS; ++i) {
+    const int h = first + mine + i * groups;
+    v[i] = h < heads && live ? ldg16(in.head(h, p.Hq)) : zero;
+  }
+  Turn<TURN> turn;
+  if (TURN != kNoTurn && 8 * lane < p.R) load_turn<TURN>(p, b, t, lane, 1.f, turn);
+  // (lanes behind D hold zeros)
+  const uint4 wq = p.qw != nullptr && live ? ldg16(p.qw, 8 * lane) : zero;
+  const uint4 wk = p.kw != nullptr && live ? ldg16(p.kw, 8 * lane) : zero;
+  for (int h0 = first; h0 < heads; h0 += HEADS * groups) {
 #pragma unroll
     for (int i = 0; i < HEADS; ++i) {
       if (h0 + i * groups >= heads) break;
-      const HeadAt at = head_at(p, b, t, h0 + i * groups + group % per_warp);
+      const int h = h0 + mine + i * groups;
+      const bool is_q = h < p.Hq;
       float f[8];
       unpack8<E>(v[i], f);
+      const int next = h + HEADS * groups;
+      v[i] = next < heads && live ? ldg16(in.head(next, p.Hq)) : zero;
       const float inv = inv_norm<LANES>(p, f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] *= inv;
-      if ((at.is_q ? p.qw : p.kw) != nullptr) {
+      if ((is_q ? p.qw : p.kw) != nullptr) {
         float w[8];
-        unpack8<E>(at.is_q ? wq : wk, w);
+        unpack8<E>(is_q ? wq : wk, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] *= w[j];
+        for (int j = 0; j < 8; ++j) f[j] *= inv * w[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] *= inv;
       }
-      if (p.R > 0) rotate<LANES>(p, turn, lane, 1.f, f);
-      if (at.has && live) {
-        uint16_t* out = static_cast<uint16_t*>(at.is_q ? p.qo : p.ko) +
-                        (row * (at.is_q ? p.Hq : p.Hk) + at.hh) * p.D + 8 * lane;
-        *reinterpret_cast<uint4*>(out) = pack8<E>(f);
-      }
+      if constexpr (TURN != kNoTurn) rotate<LANES, TURN>(p, turn, lane, f);
+      if (h < heads && live)
+        *reinterpret_cast<uint4*>(is_q ? qo + h * p.D : ko + (h - p.Hq) * p.D) = pack8<E>(f);
     }
   }
 }
@@ -191,67 +203,68 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkParams p) {
 // rows_per_block rows; each group of lanes keeps its share of the two
 // weights' gradients in registers, the block adds its groups in shared memory
 // and writes one partial sum, which qk_wsum_kernel adds in block order.
-template <class E, int LANES, int HEADS>
+template <class E, int LANES, int HEADS, int TURN>
 __global__ void __launch_bounds__(256) qk_norm_rope_bwd_kernel(const QkParams p) {
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const int groups = blockDim.x / LANES, per_warp = 32 / LANES;
-  const int first = (group / per_warp) * per_warp;
+  const int first = (group / per_warp) * per_warp, mine = group % per_warp;
   const bool live = 8 * lane < p.D;
   const int heads = p.Hq + p.Hk;
   float dqw[8] = {}, dkw[8] = {};
-  uint4 wq = make_uint4(0, 0, 0, 0), wk = wq;  // (lanes behind D hold zeros)
-  if (p.qw != nullptr && live) wq = ldg16(p.qw, 8 * lane);
-  if (p.kw != nullptr && live) wk = ldg16(p.kw, 8 * lane);
-  const int64_t r0 = int64_t(blockIdx.x) * p.rows_per_block;
-  const int64_t r1 = min(r0 + p.rows_per_block, p.rows);
-  for (int64_t row = r0; row < r1; ++row) {
-    const int64_t b = row / p.T, t = row % p.T;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  const uint4 wq = p.qw != nullptr && live ? ldg16(p.qw, 8 * lane) : zero;
+  const uint4 wk = p.kw != nullptr && live ? ldg16(p.kw, 8 * lane) : zero;
+  const uint32_t r0 = blockIdx.x * uint32_t(p.rows_per_block);
+  const uint32_t r1 = min(r0 + uint32_t(p.rows_per_block), uint32_t(p.rows));
+  for (uint32_t row = r0; row < r1; ++row) {
+    const uint32_t b = row / uint32_t(p.T), t = row - b * uint32_t(p.T);
+    const RowAt in = row_of(p.q, p.k, b, t, p.q_sb, p.q_st, p.q_sh, p.k_sb, p.k_st, p.k_sh, lane);
+    const RowAt gr = row_of(p.gq, p.gk, b, t, p.gq_sb, p.gq_st, p.gq_sh, p.gk_sb, p.gk_st, p.gk_sh, lane);
+    uint16_t* dq = static_cast<uint16_t*>(p.dq) + int64_t(row) * p.Hq * p.D + 8 * lane;
+    uint16_t* dk = static_cast<uint16_t*>(p.dk) + int64_t(row) * p.Hk * p.D + 8 * lane;
+    Turn<TURN> turn;
     for (int h0 = first; h0 < heads; h0 += HEADS * groups) {
       uint4 v[HEADS], g[HEADS];
 #pragma unroll
       for (int i = 0; i < HEADS; ++i) {
-        const HeadAt at = head_at(p, b, t, h0 + i * groups + group % per_warp);
-        const int64_t ga = at.is_q ? b * p.gq_sb + t * p.gq_st + at.hh * p.gq_sh
-                                   : b * p.gk_sb + t * p.gk_st + at.hh * p.gk_sh;
-        const bool go = at.has && live;
-        v[i] = go ? ldg16(at.in, at.at + 8 * lane) : make_uint4(0, 0, 0, 0);
-        g[i] = go ? ldg16(at.is_q ? p.gq : p.gk, ga + 8 * lane) : make_uint4(0, 0, 0, 0);
+        const int h = h0 + mine + i * groups;
+        const bool go = h < heads && live;
+        v[i] = go ? ldg16(in.head(h, p.Hq)) : zero;
+        g[i] = go ? ldg16(gr.head(h, p.Hq)) : zero;
       }
-      Turn turn;
-      if (p.R > 0 && 8 * lane < p.R) load_turn(p, b, t, lane, turn);
+      if (TURN != kNoTurn && h0 == first && 8 * lane < p.R) load_turn<TURN>(p, b, t, lane, -1.f, turn);
 #pragma unroll
       for (int i = 0; i < HEADS; ++i) {
         if (h0 + i * groups >= heads) break;
-        const HeadAt at = head_at(p, b, t, h0 + i * groups + group % per_warp);
+        const int h = h0 + mine + i * groups;
+        const bool is_q = h < p.Hq;
         float f[8], d[8];
         unpack8<E>(v[i], f);
         unpack8<E>(g[i], d);
         const float inv = inv_norm<LANES>(p, f);
-        if (p.R > 0) rotate<LANES>(p, turn, lane, -1.f, d);
-        float m = 0.f;
+        if constexpr (TURN != kNoTurn) rotate<LANES, TURN>(p, turn, lane, d);
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] *= inv;
-        if ((at.is_q ? p.qw : p.kw) != nullptr) {
+        if ((is_q ? p.qw : p.kw) != nullptr) {
           float w[8];
-          unpack8<E>(at.is_q ? wq : wk, w);
+          unpack8<E>(is_q ? wq : wk, w);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const float dw = d[j] * f[j];
-            if (at.is_q) dqw[j] += dw; else dkw[j] += dw;
+            dqw[j] += is_q ? dw : 0.f;
+            dkw[j] += is_q ? 0.f : dw;
             d[j] *= w[j];
           }
         }
+        float2 q = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = fmaf(d[j], f[j], m);
-        m = lane_sum<LANES>(m);
-        m = p.norm == 0 ? 0.f : p.norm == 1 ? m / float(p.D) : m;
+        for (int j = 0; j < 8; j += 2)
+          fma_pair(q, make_float2(d[j], d[j + 1]), make_float2(f[j], f[j + 1]));
+        const float m = p.norm ? lane_sum<LANES>(q.x + q.y) * p.mul : 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] = inv * (d[j] - f[j] * m);
-        if (at.has && live) {
-          uint16_t* out = static_cast<uint16_t*>(at.is_q ? p.dq : p.dk) +
-                          (row * (at.is_q ? p.Hq : p.Hk) + at.hh) * p.D + 8 * lane;
-          *reinterpret_cast<uint4*>(out) = pack8<E>(d);
-        }
+        for (int j = 0; j < 8; ++j) d[j] = inv * fmaf(-f[j], m, d[j]);
+        if (h < heads && live)
+          *reinterpret_cast<uint4*>(is_q ? dq + h * p.D : dk + (h - p.Hq) * p.D) = pack8<E>(d);
       }
     }
   }

@@ -88,6 +88,20 @@ __device__ __forceinline__ uint4 pack8(const float f[8]) {
                     pack2_rn<E>(f[6], f[7]));
 }
 
+// d += a b for two fp32 values in one instruction.
+__device__ __forceinline__ void fma_pair(float2& d, const float2& a, const float2& b) {
+  asm("{\n"
+      " .reg .b64 x, y, z;\n"
+      " mov.b64 x, {%2, %3};\n"
+      " mov.b64 y, {%4, %5};\n"
+      " mov.b64 z, {%0, %1};\n"
+      " fma.rn.f32x2 z, x, y, z;\n"
+      " mov.b64 {%0, %1}, z;\n"
+      "}\n"
+      : "+f"(d.x), "+f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+}
+
 template <class E>
 __device__ __forceinline__ uint16_t nan16() {
   return std::is_same_v<E, BF16> ? 0x7FC0 : 0x7E00;

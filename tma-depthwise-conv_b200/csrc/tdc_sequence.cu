@@ -218,7 +218,8 @@ tdc::QkParams qk_params(const tdc_qk_args* a) {
   p.rows = a->B * a->T;
   p.pos64 = a->positions_are_64 != 0;
   p.interleaved = a->interleaved != 0;
-  p.norm = int(a->norm);
+  p.norm = a->norm != TDC_NORM_NONE;
+  p.mul = a->norm == TDC_NORM_RMS ? 1.f / float(a->D) : 1.f;
   p.eps = float(a->eps);
   return p;
 }
@@ -236,29 +237,44 @@ int64_t qk_bwd_rows(const tdc_qk_args* a) {
 }
 int64_t qk_bwd_blocks(const tdc_qk_args* a) { return ceil_div(a->B * a->T, qk_bwd_rows(a)); }
 
+template <class E, int LANES>
+int qk_fwd_l(const tdc::QkParams& p, int threads, cudaStream_t st) {
+  auto* k = p.R == 0        ? &tdc::qk_norm_rope_kernel<E, LANES, 4, tdc::kNoTurn>
+            : p.interleaved ? &tdc::qk_norm_rope_kernel<E, LANES, 4, tdc::kPairs>
+                            : &tdc::qk_norm_rope_kernel<E, LANES, 4, tdc::kHalves>;
+  k<<<unsigned(p.rows), threads, 0, st>>>(p);
+  return launched();
+}
+
+template <class E, int LANES>
+int qk_bwd_l(const tdc::QkParams& p, int threads, int64_t blocks, cudaStream_t st) {
+  auto* k = p.R == 0        ? &tdc::qk_norm_rope_bwd_kernel<E, LANES, 3, tdc::kNoTurn>
+            : p.interleaved ? &tdc::qk_norm_rope_bwd_kernel<E, LANES, 3, tdc::kPairs>
+                            : &tdc::qk_norm_rope_bwd_kernel<E, LANES, 3, tdc::kHalves>;
+  k<<<unsigned(blocks), threads, 0, st>>>(p);
+  return launched();
+}
+
 template <class E>
 int qk_fwd_e(const tdc::QkParams& p, int threads, cudaStream_t st) {
-  const unsigned grid = unsigned(p.rows);
   switch (qk_lanes(p.D)) {
-    case 4: tdc::qk_norm_rope_kernel<E, 4, 4><<<grid, threads, 0, st>>>(p); break;
-    case 8: tdc::qk_norm_rope_kernel<E, 8, 4><<<grid, threads, 0, st>>>(p); break;
-    case 16: tdc::qk_norm_rope_kernel<E, 16, 4><<<grid, threads, 0, st>>>(p); break;
-    default: tdc::qk_norm_rope_kernel<E, 32, 4><<<grid, threads, 0, st>>>(p); break;
+    case 4: return qk_fwd_l<E, 4>(p, threads, st);
+    case 8: return qk_fwd_l<E, 8>(p, threads, st);
+    case 16: return qk_fwd_l<E, 16>(p, threads, st);
+    default: return qk_fwd_l<E, 32>(p, threads, st);
   }
-  return launched();
 }
 
 template <class E>
 int qk_bwd_e(const tdc::QkParams& p, int threads, int64_t blocks, void* dqw, void* dkw,
              cudaStream_t st) {
-  const unsigned grid = unsigned(blocks);
+  int rc;
   switch (qk_lanes(p.D)) {
-    case 4: tdc::qk_norm_rope_bwd_kernel<E, 4, 3><<<grid, threads, 0, st>>>(p); break;
-    case 8: tdc::qk_norm_rope_bwd_kernel<E, 8, 3><<<grid, threads, 0, st>>>(p); break;
-    case 16: tdc::qk_norm_rope_bwd_kernel<E, 16, 3><<<grid, threads, 0, st>>>(p); break;
-    default: tdc::qk_norm_rope_bwd_kernel<E, 32, 3><<<grid, threads, 0, st>>>(p); break;
+    case 4: rc = qk_bwd_l<E, 4>(p, threads, blocks, st); break;
+    case 8: rc = qk_bwd_l<E, 8>(p, threads, blocks, st); break;
+    case 16: rc = qk_bwd_l<E, 16>(p, threads, blocks, st); break;
+    default: rc = qk_bwd_l<E, 32>(p, threads, blocks, st); break;
   }
-  const int rc = launched();
   if (rc != TDC_OK || p.partial == nullptr) return rc;
   tdc::qk_wsum_kernel<E><<<unsigned(ceil_div(2 * p.D, 8)), 256, 0, st>>>(p.partial, blocks, p.D, dqw,
                                                                          dkw);
