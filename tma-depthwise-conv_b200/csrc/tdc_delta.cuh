@@ -193,25 +193,39 @@ __device__ __forceinline__ float load_beta(const DeltaParams& p, bool bf16, int6
   return bf16 ? to_float<BF16>(p.beta, i) : to_float<F16>(p.beta, i);
 }
 
-// Running sum of g over a chunk in fp64 (differences of far sums have to keep
-// fp32's precision), by the first warp; two tokens a lane.
-__device__ __forceinline__ void chunk_decay(const DeltaParams& p, const ChunkAt& at, int hv,
-                                            double* G, int lane) {
-  double v[2];
+// Running sum of g over a chunk, by the first warp, two tokens a lane: in fp64,
+// kept as a pair of fp32 values (differences of far sums have to keep fp32's
+// precision).
+struct Far {
+  float hi, lo;
+};
+__device__ __forceinline__ Far to_far(double v) {
+  const float hi = float(v);
+  return {hi, float(v - double(hi))};
+}
+__device__ __forceinline__ float minus(const Far& a, const Far& b) {
+  return (a.hi - b.hi) + (a.lo - b.lo);
+}
+__device__ __forceinline__ float2 load_decay(const DeltaParams& p, const ChunkAt& at, int hv,
+                                             int lane) {
+  float g[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int t = 2 * lane + i;
-    float g = t < at.rows ? p.g[at.b * p.g_sb + (at.t0 + t) * p.g_st + hv] : 0.f;
-    v[i] = g < -200.f ? -200.0 : double(g);
+    g[i] = t < at.rows ? p.g[at.b * p.g_sb + (at.t0 + t) * p.g_st + hv] : 0.f;
+    g[i] = g[i] < -200.f ? -200.f : g[i];
   }
-  double sum = v[0] + v[1];
+  return make_float2(g[0], g[1]);
+}
+__device__ __forceinline__ void chunk_decay(const float2& g, Far* G, int lane) {
+  double sum = double(g.x) + double(g.y);
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const double o = __shfl_up_sync(0xffffffffu, sum, d);
     if (lane >= d) sum += o;
   }
-  G[2 * lane + 1] = sum;
-  G[2 * lane] = sum - v[1];
+  G[2 * lane + 1] = to_far(sum);
+  G[2 * lane] = to_far(sum - double(g.y));
 }
 
 // ---- T and P of every chunk -------------------------------------------------------
@@ -236,7 +250,7 @@ struct PrepareSmem {
   static constexpr int t = 0;
   static constexpr int p = 2 * part;
   static constexpr int a = 2 * kChunk * ld * 2 > 4 * part ? 2 * kChunk * ld * 2 : 4 * part;
-  static constexpr int G = a + 2 * part;               // double [64]
+  static constexpr int G = a + 2 * part;               // Far [64]
   static constexpr int beta = G + 64 * 8;
   static constexpr int bytes = beta + 64 * 4;
 };
@@ -341,13 +355,25 @@ __global__ void __launch_bounds__(128) delta_prepare_kernel(const DeltaParams p)
   const ChunkAt at = chunk_at(p, chunk);
   if (at.rows == 0) return;
   const uint32_t sb = smem_addr(raw);
-  double* G = reinterpret_cast<double*>(raw + Sm::G);
+  Far* G = reinterpret_cast<Far*>(raw + Sm::G);
   float* sB = reinterpret_cast<float*>(raw + Sm::beta);
   const uint16_t* q = static_cast<const uint16_t*>(p.q) + at.b * p.q_sb + at.t0 * p.q_st + h * p.q_sh;
   const uint16_t* k = static_cast<const uint16_t*>(p.k) + at.b * p.k_sb + at.t0 * p.k_st + h * p.k_sh;
   copy_rows(sb + Sm::q, ld, q, p.q_st, kChunk, at.rows, DK / 8, tid, 128);
   copy_rows(sb + Sm::k, ld, k, p.k_st, kChunk, at.rows, DK / 8, tid, 128);
   cp_async_commit();
+  // A head's decays (first warp) and betas (last two), loaded one head ahead.
+  float2 decay = make_float2(0.f, 0.f);
+  float beta = 0.f;
+  auto fetch_gates = [&](int hv) {
+    if (warp == 0) decay = load_decay(p, at, hv, lane);
+    const int t = tid - 64;
+    if (t >= 0)
+      beta = t < at.rows ? load_beta(p, std::is_same_v<E, BF16>,
+                                     at.b * p.b_sb + (at.t0 + t) * p.b_st + hv)
+                         : 0.f;
+  };
+  fetch_gates(h * p.group);
   cp_async_wait<0>();
   __syncthreads();
   // Rows 16 warp .. + 15 of Q K^T and K K^T (both operands exact).
@@ -380,32 +406,33 @@ __global__ void __launch_bounds__(128) delta_prepare_kernel(const DeltaParams p)
     const int hv = h * p.group + gi;
     const int64_t slot = chunk * p.HV + hv;
     __syncthreads();  // q and k, or the last head's tiles, are free
-    if (warp == 0) chunk_decay(p, at, hv, G, lane);
-    if (tid >= 64) {
-      const int t = tid - 64;
-      sB[t] = t < at.rows ? load_beta(p, std::is_same_v<E, BF16>,
-                                      at.b * p.b_sb + (at.t0 + t) * p.b_st + hv)
-                          : 0.f;
-    }
+    if (warp == 0) chunk_decay(decay, G, lane);
+    if (tid >= 64) sB[tid - 64] = beta;
+    if (gi + 1 < p.group) fetch_gates(hv + 1);
     __syncthreads();
     if (tid < kChunk) {
       float* coef = p.coef + slot * 3 * kChunk;
-      coef[tid] = expf(float(G[tid]));
-      coef[kChunk + tid] = expf(float(G[kChunk - 1] - G[tid]));
+      coef[tid] = expf(G[tid].hi + G[tid].lo);
+      coef[kChunk + tid] = expf(minus(G[kChunk - 1], G[tid]));
       coef[2 * kChunk + tid] = sB[tid];
     }
+    const Far Gi[2] = {G[16 * warp + g], G[16 * warp + g + 8]};
 #pragma unroll
     for (int nt = 0; nt < 8; ++nt) {
       if (nt > 2 * warp + 1) break;
+      const int j = 8 * nt + t2;
+      const float4 far2 = *reinterpret_cast<const float4*>(G + j);
+      const Far Gj[2] = {{far2.x, far2.y}, {far2.z, far2.w}};
+      const float2 be = *reinterpret_cast<const float2*>(sB + j);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int i = 16 * warp + g + 8 * half, j = 8 * nt + t2;
+        const int i = 16 * warp + g + 8 * half;
         float pv[2], av[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const float gam = i >= j + u ? __expf(float(G[i] - G[j + u])) : 0.f;
+          const float gam = __expf(minus(Gi[half], Gj[u]));
           pv[u] = i >= j + u ? p.scale * gam * qk[nt][2 * half + u] : 0.f;
-          av[u] = i > j + u ? kk[nt][2 * half + u] * gam * sB[j + u] : 0.f;
+          av[u] = i > j + u ? kk[nt][2 * half + u] * gam * (u ? be.y : be.x) : 0.f;
         }
         if (nt >= 2 * warp)
           *reinterpret_cast<float2*>(raw + Sm::t + diag_offset(warp, g + 8 * half) +
@@ -471,7 +498,7 @@ struct GradSmem {
   static constexpr int u = d + 2 * 64 * ld * 2;           // [2][64][72], later Dt
   static constexpr int x = u + 2 * 64 * kLdT * 2;         // [2][64][72], later N
   static constexpr int o = x + 2 * 64 * kLdT * 2;         // [64][72]
-  static constexpr int G = o + 64 * kLdT * 2;             // double [64]
+  static constexpr int G = o + 64 * kLdT * 2;             // Far [64]
   static constexpr int coef = G + 64 * 8;                 // [3][64]
   static constexpr int rows = coef + 3 * 64 * 4;          // [2][4][64]: row sums of both halves
   static constexpr int cols = rows + 2 * 4 * 64 * 4;      // [4][64]: column sums of the row groups
@@ -492,7 +519,7 @@ __global__ void __launch_bounds__(256, 1) delta_grad_kernel(const DeltaParams p)
   const ChunkAt at = chunk_at(p, chunk);
   if (at.rows == 0) return;
   const uint32_t sb = smem_addr(raw);
-  double* G = reinterpret_cast<double*>(raw + Sm::G);
+  Far* G = reinterpret_cast<Far*>(raw + Sm::G);
   float* coef = reinterpret_cast<float*>(raw + Sm::coef);
   float* rows = reinterpret_cast<float*>(raw + Sm::rows);
   float* cols = reinterpret_cast<float*>(raw + Sm::cols);
@@ -532,7 +559,7 @@ __global__ void __launch_bounds__(256, 1) delta_grad_kernel(const DeltaParams p)
       copy_rows(sb + Sm::o, kLdT, d_o + v0, p.do_st, kChunk, at.rows, 8, tid, 256);
       cp_async_commit();
       if (v0 == 0) {
-        if (warp == 0) chunk_decay(p, at, hv, G, lane);
+        if (warp == 0) chunk_decay(load_decay(p, at, hv, lane), G, lane);
         const float* src = p.coef + slot * 3 * kChunk;
         if (tid >= 64) coef[tid - 64] = src[tid - 64];
       }
@@ -651,7 +678,7 @@ __global__ void __launch_bounds__(256, 1) delta_grad_kernel(const DeltaParams p)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int e = 2 * half + u;
-          const float gam = i >= j + u ? __expf(float(G[i] - G[j + u])) : 0.f;
+          const float gam = i >= j + u ? __expf(minus(G[i], G[j + u])) : 0.f;
           const float be = coef[128 + j + u];
           const float dv = i >= j + u ? D[nt][e] : 0.f, mv = i > j + u ? M[nt][e] : 0.f;
           const float pd = p.scale * gam * qk[nt][e] * dv, ml = gam * kk[nt][e] * mv;

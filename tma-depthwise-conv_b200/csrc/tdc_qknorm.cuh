@@ -145,7 +145,7 @@ __device__ __forceinline__ uint4 ldg16(const uint16_t* at) {
 // queries first, HEADS of a group's at a time: their loads are all under way
 // before the first sum is needed.
 template <class E, int LANES, int HEADS, int TURN>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkParams p) {
+__global__ void __launch_bounds__(256, 4) qk_norm_rope_kernel(const QkParams p) {
   const uint32_t row = blockIdx.x;
   const uint32_t b = row / uint32_t(p.T), t = row - b * uint32_t(p.T);
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
@@ -160,18 +160,15 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkParams p) {
   // its groups has a head left
   const int first = (group / per_warp) * per_warp, mine = group % per_warp;
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  uint4 v[HEADS];
-#pragma unroll
-  for (int i = 0; i < HEADS; ++i) {
-    const int h = first + mine + i * groups;
-    v[i] = h < heads && live ? ldg16(in.head(h, p.Hq)) : zero;
-  }
   Turn<TURN> turn;
-  if (TURN != kNoTurn && 8 * lane < p.R) load_turn<TURN>(p, b, t, lane, 1.f, turn);
-  // (lanes behind D hold zeros)
-  const uint4 wq = p.qw != nullptr && live ? ldg16(p.qw, 8 * lane) : zero;
-  const uint4 wk = p.kw != nullptr && live ? ldg16(p.kw, 8 * lane) : zero;
   for (int h0 = first; h0 < heads; h0 += HEADS * groups) {
+    uint4 v[HEADS];
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) {
+      const int h = h0 + mine + i * groups;
+      v[i] = h < heads && live ? ldg16(in.head(h, p.Hq)) : zero;  // (lanes behind D hold zeros)
+    }
+    if (TURN != kNoTurn && h0 == first && 8 * lane < p.R) load_turn<TURN>(p, b, t, lane, 1.f, turn);
 #pragma unroll
     for (int i = 0; i < HEADS; ++i) {
       if (h0 + i * groups >= heads) break;
@@ -179,12 +176,11 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkParams p) {
       const bool is_q = h < p.Hq;
       float f[8];
       unpack8<E>(v[i], f);
-      const int next = h + HEADS * groups;
-      v[i] = next < heads && live ? ldg16(in.head(next, p.Hq)) : zero;
       const float inv = inv_norm<LANES>(p, f);
-      if ((is_q ? p.qw : p.kw) != nullptr) {
+      const void* weight = is_q ? p.qw : p.kw;
+      if (weight != nullptr) {
         float w[8];
-        unpack8<E>(is_q ? wq : wk, w);
+        unpack8<E>(live ? ldg16(weight, 8 * lane) : zero, w);  // (from the cache)
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] *= inv * w[j];
       } else {

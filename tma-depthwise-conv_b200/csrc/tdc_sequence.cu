@@ -226,8 +226,10 @@ tdc::QkParams qk_params(const tdc_qk_args* a) {
 
 int qk_lanes(int64_t D) { return D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32; }
 
-int qk_threads(const tdc_qk_args* a) {
-  const int64_t want = (a->Hq + a->Hk) * qk_lanes(a->D);
+// Threads of a block: its groups take `heads` heads each, so that what a block
+// does once (places, the angle) is spread over several.
+int qk_threads(const tdc_qk_args* a, int64_t heads) {
+  const int64_t want = ceil_div(a->Hq + a->Hk, heads) * qk_lanes(a->D);
   return int(std::min<int64_t>(256, ceil_div(want, 32) * 32));
 }
 
@@ -534,8 +536,8 @@ TDC_API int tdc_qk_norm_rope(const tdc_qk_args* a, void* stream) {
   if (rc != TDC_OK) return rc;
   const tdc::QkParams p = qk_params(a);
   auto st = static_cast<cudaStream_t>(stream);
-  return a->dtype == TDC_BF16 ? qk_fwd_e<tdc::BF16>(p, qk_threads(a), st)
-                              : qk_fwd_e<tdc::F16>(p, qk_threads(a), st);
+  return a->dtype == TDC_BF16 ? qk_fwd_e<tdc::BF16>(p, qk_threads(a, 4), st)
+                              : qk_fwd_e<tdc::F16>(p, qk_threads(a, 4), st);
 }
 
 TDC_API int64_t tdc_qk_norm_rope_bwd_workspace(const tdc_qk_args* a) {
@@ -576,8 +578,8 @@ TDC_API int tdc_qk_norm_rope_bwd(const tdc_qk_args* a, const tdc_qk_grad_args* g
   auto st = static_cast<cudaStream_t>(stream);
   const int64_t blocks = std::max<int64_t>(1, qk_bwd_blocks(a));  // no rows: zero weight gradients
   return a->dtype == TDC_BF16
-             ? qk_bwd_e<tdc::BF16>(p, qk_threads(a), blocks, g->dq_weight, g->dk_weight, st)
-             : qk_bwd_e<tdc::F16>(p, qk_threads(a), blocks, g->dq_weight, g->dk_weight, st);
+             ? qk_bwd_e<tdc::BF16>(p, qk_threads(a, 1), blocks, g->dq_weight, g->dk_weight, st)
+             : qk_bwd_e<tdc::F16>(p, qk_threads(a, 1), blocks, g->dq_weight, g->dk_weight, st);
 }
 
 TDC_API int64_t tdc_delta_fwd_workspace(const tdc_delta_args* a) {
