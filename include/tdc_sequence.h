@@ -178,6 +178,17 @@ TDC_API int64_t tdc_delta_fwd_workspace(const tdc_delta_args* a);
 TDC_API int tdc_delta_fwd(const tdc_delta_args* a, void* workspace, int64_t workspace_bytes,
                           void* stream);
 
+/* The chunked kernels wait for their copies and products on barriers with the
+ * limit of tdc_set_wait_timeout_ns; a wait that gives up ends its block, leaves
+ * the output incomplete and is reported as for the depthwise kernels (see
+ * "pipeline-wait failure detection" in tdc_dwconv.h).  This is the forward in
+ * which no copy of chunk `withhold_chunk` (of each sequence) and later ones ever
+ * comes, so that the wait for it runs out after timeout_ns: it exists to test
+ * that path. */
+TDC_API int tdc_delta_fwd_withhold(const tdc_delta_args* a, void* workspace,
+                                   int64_t workspace_bytes, int64_t withhold_chunk,
+                                   int64_t timeout_ns, void* stream);
+
 /* All gradients of the forward from d_o (strides do_sb, do_st, do_sh) and
  * dfinal [N, HV, K, V] (fp32, or NULL).  Of `a`, o and final_state are not
  * used.  dq, dk, dv are contiguous in the element type (the key heads' sums

@@ -391,7 +391,8 @@ std::tuple<torch::Tensor, OptTensor> gated_delta_rule(torch::Tensor q, torch::Te
                                                       torch::Tensor v, torch::Tensor g,
                                                       torch::Tensor beta, double scale,
                                                       OptTensor init, OptTensor cu,
-                                                      bool want_final) {
+                                                      bool want_final, int64_t withhold_chunk,
+                                                      int64_t timeout_ns) {
   auto c = delta_call(q, k, v, g, beta, scale, init, cu);
   const c10::cuda::CUDAGuard guard(cuda_device(q));
   auto o = torch::empty(v.sizes(), v.options());
@@ -404,7 +405,11 @@ std::tuple<torch::Tensor, OptTensor> gated_delta_rule(torch::Tensor q, torch::Te
   const int64_t need = tdc_delta_fwd_workspace(&c.a);
   if (need < 0) check_status(int(need), "gated_delta_rule");
   auto ws = bytes_on(q, need);
-  check_status(tdc_delta_fwd(&c.a, ws.data_ptr(), need, stream_of(q)), "gated_delta_rule");
+  check_status(withhold_chunk < 0
+                   ? tdc_delta_fwd(&c.a, ws.data_ptr(), need, stream_of(q))
+                   : tdc_delta_fwd_withhold(&c.a, ws.data_ptr(), need, withhold_chunk, timeout_ns,
+                                            stream_of(q)),
+               "gated_delta_rule");
   return {o, fin};
 }
 
@@ -490,9 +495,11 @@ void bind_sequence(pybind11::module_& m) {
         py::arg("positions"), py::arg("norm"), py::arg("eps"), py::arg("interleaved"),
         py::arg("dq_out"), py::arg("dk_out"));
   m.def("gated_delta_rule", &gated_delta_rule,
-        "Gated delta rule over whole sequences: (o, final state or None).", py::arg("q"),
-        py::arg("k"), py::arg("v"), py::arg("g"), py::arg("beta"), py::arg("scale"),
-        py::arg("initial_state"), py::arg("cu_seqlens"), py::arg("want_final"));
+        "Gated delta rule over whole sequences: (o, final state or None).  withhold_chunk >= 0 "
+        "makes the copies of that chunk never come (tests the failure path; see device_status).",
+        py::arg("q"), py::arg("k"), py::arg("v"), py::arg("g"), py::arg("beta"), py::arg("scale"),
+        py::arg("initial_state"), py::arg("cu_seqlens"), py::arg("want_final"),
+        py::arg("withhold_chunk") = -1, py::arg("timeout_ns") = 0);
   m.def("gated_delta_rule_bwd", &gated_delta_rule_bwd,
         "Its gradients: (dq, dk, dv, dg, dbeta, dinitial or None).", py::arg("q"), py::arg("k"),
         py::arg("v"), py::arg("g"), py::arg("beta"), py::arg("scale"), py::arg("initial_state"),

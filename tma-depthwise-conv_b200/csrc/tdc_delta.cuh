@@ -49,6 +49,7 @@ struct DeltaParams {
   float* coef;            // [3][64]: gam, w, beta
   unsigned char* kq;      // [chunk][H]: K and Q, [2][parts][64 x K]
   uint64_t timeout_ns;    // of the bounded waits
+  int64_t withhold;       // first chunk of a sequence whose copies never come (-1: none)
   int *status_words, *status_host;
   // gradients
   // (in blocks of R = min(V, 128) channels: [V / R][columns / 8][R][8] a part)

@@ -170,7 +170,7 @@ __device__ __forceinline__ void walk_fetch(const DeltaParams& p, unsigned char* 
                                            int hv, bool back) {
   using W = WalkTiles<E, DK>;
   int issued = 0;
-  for (int c = 0; c < chunks; ++c) {
+  for (int c = 0; c < chunks && c != p.withhold; ++c) {
     const int st = c & 1;
     if (c >= 2 && !wait(sy->free[st], uint32_t((c >> 1) - 1), TDC_DEVICE_EMPTY_TIMEOUT, c)) break;
     const int64_t chunk = s.chunk0 + (back ? chunks - 1 - c : c), slot = chunk * p.HV + hv;

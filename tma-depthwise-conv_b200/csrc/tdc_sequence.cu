@@ -372,6 +372,7 @@ tdc::DeltaParams delta_params(const tdc_delta_args* a) {
   p.max_chunks = delta_chunks(a);
   p.beta_f32 = a->beta_is_f32 != 0;
   p.scale = float(a->scale);
+  p.withhold = -1;
   return p;
 }
 
@@ -430,6 +431,36 @@ int delta_step_t(const tdc::DeltaParams& p, int64_t B, float* state, int64_t slo
       <<<dim3(unsigned(B), unsigned(p.HV), unsigned(p.V / 32)), 128, 0, st>>>(p, state, idx, idx64,
                                                                              slots);
   return launched();
+}
+
+int delta_fwd(const tdc_delta_args* a, void* workspace, int64_t workspace_bytes, int64_t withhold,
+              int64_t timeout_ns, void* stream) {
+  int rc = check_delta(a);
+  if (rc != TDC_OK) return rc;
+  if (workspace == nullptr) return TDC_ERR_NULL_POINTER;
+  if (workspace_bytes < tdc_delta_fwd_workspace(a)) return TDC_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return TDC_ERR_ALIGNMENT;
+  if (a->B * a->T > 0 && (a->q == nullptr || a->k == nullptr || a->v == nullptr ||
+                          a->g == nullptr || a->beta == nullptr || a->o == nullptr))
+    return TDC_ERR_NULL_POINTER;
+  if (misaligned(a->o) || misaligned(a->initial_state) || misaligned(a->final_state))
+    return TDC_ERR_ALIGNMENT;
+  rc = prepare_device();
+  if (rc != TDC_OK) return rc;
+  tdc::DeltaParams p = delta_params(a);
+  delta_layout(a, false, static_cast<unsigned char*>(workspace), &p);
+  if (p.max_chunks > 0x7fffffff) return TDC_ERR_TOO_LARGE;
+  auto st = static_cast<cudaStream_t>(stream);
+  tdc::ZeroRows z = {};
+  z.base[0] = a->o, z.row_bytes[0] = a->HV * a->V * 2;
+  rc = delta_wait_record(&p);
+  p.withhold = withhold;
+  if (timeout_ns > 0) p.timeout_ns = uint64_t(timeout_ns);
+  if (rc == TDC_OK) rc = delta_plan(p, z, st);
+  if (rc != TDC_OK) return rc;
+  if (a->dtype == TDC_BF16)
+    return a->K == 128 ? delta_fwd_t<tdc::BF16, 128>(p, st) : delta_fwd_t<tdc::BF16, 64>(p, st);
+  return a->K == 128 ? delta_fwd_t<tdc::F16, 128>(p, st) : delta_fwd_t<tdc::F16, 64>(p, st);
 }
 
 }  // namespace
@@ -594,30 +625,14 @@ TDC_API int64_t tdc_delta_bwd_workspace(const tdc_delta_args* a) {
 
 TDC_API int tdc_delta_fwd(const tdc_delta_args* a, void* workspace, int64_t workspace_bytes,
                           void* stream) {
-  int rc = check_delta(a);
-  if (rc != TDC_OK) return rc;
-  if (workspace == nullptr) return TDC_ERR_NULL_POINTER;
-  if (workspace_bytes < tdc_delta_fwd_workspace(a)) return TDC_ERR_WORKSPACE;
-  if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return TDC_ERR_ALIGNMENT;
-  if (a->B * a->T > 0 && (a->q == nullptr || a->k == nullptr || a->v == nullptr ||
-                          a->g == nullptr || a->beta == nullptr || a->o == nullptr))
-    return TDC_ERR_NULL_POINTER;
-  if (misaligned(a->o) || misaligned(a->initial_state) || misaligned(a->final_state))
-    return TDC_ERR_ALIGNMENT;
-  rc = prepare_device();
-  if (rc != TDC_OK) return rc;
-  tdc::DeltaParams p = delta_params(a);
-  delta_layout(a, false, static_cast<unsigned char*>(workspace), &p);
-  if (p.max_chunks > 0x7fffffff) return TDC_ERR_TOO_LARGE;
-  auto st = static_cast<cudaStream_t>(stream);
-  tdc::ZeroRows z = {};
-  z.base[0] = a->o, z.row_bytes[0] = a->HV * a->V * 2;
-  rc = delta_wait_record(&p);
-  if (rc == TDC_OK) rc = delta_plan(p, z, st);
-  if (rc != TDC_OK) return rc;
-  if (a->dtype == TDC_BF16)
-    return a->K == 128 ? delta_fwd_t<tdc::BF16, 128>(p, st) : delta_fwd_t<tdc::BF16, 64>(p, st);
-  return a->K == 128 ? delta_fwd_t<tdc::F16, 128>(p, st) : delta_fwd_t<tdc::F16, 64>(p, st);
+  return delta_fwd(a, workspace, workspace_bytes, -1, 0, stream);
+}
+
+TDC_API int tdc_delta_fwd_withhold(const tdc_delta_args* a, void* workspace,
+                                   int64_t workspace_bytes, int64_t withhold_chunk,
+                                   int64_t timeout_ns, void* stream) {
+  if (withhold_chunk < 0 || timeout_ns <= 0) return TDC_ERR_BAD_SHAPE;
+  return delta_fwd(a, workspace, workspace_bytes, withhold_chunk, timeout_ns, stream);
 }
 
 TDC_API int tdc_delta_bwd(const tdc_delta_args* a, const tdc_delta_grad_args* g, void* workspace,

@@ -30,15 +30,17 @@ same kernels.
 from __future__ import annotations
 
 import math
+from dataclasses import dataclass
 from typing import Optional
 
 import torch
-from torch import Tensor
+from torch import Tensor, nn
 
 import _tma_dwconv_C as _C  # type: ignore
 
 __all__ = ["causal_conv1d", "causal_conv1d_step", "qk_norm_rope", "rotary_table",
-           "gated_delta_rule", "gated_delta_step", "CONV_ACTIVATIONS", "NORMS"]
+           "gated_delta_rule", "gated_delta_step", "GatedDeltaMixer", "MixerState",
+           "CONV_ACTIVATIONS", "NORMS"]
 
 #: Activations of the causal convolution.
 CONV_ACTIVATIONS = {"none": 0, "silu": 3}
@@ -129,6 +131,7 @@ def _conv_setup(ctx, inputs, output):
 
 def _conv_backward(ctx, dy, dfinal):
     x, w, bias, initial_state, cu = ctx.saved_tensors
+    dy = torch.zeros_like(x) if dy is None else dy
     dx, dw, db, ds = causal_conv1d_bwd_op(x, w, bias, initial_state, cu, ctx.act, dy,
                                           dfinal if ctx.want_final else None)
     return (dx, dw, None if bias is None else db, None if initial_state is None else ds, None,
@@ -294,6 +297,8 @@ def _qk_setup(ctx, inputs, output):
 
 def _qk_backward(ctx, dqo, dko):
     saved = ctx.saved_tensors
+    dqo = torch.zeros_like(saved[0]) if dqo is None else dqo
+    dko = torch.zeros_like(saved[1]) if dko is None else dko
     dq, dk, dqw, dkw = qk_norm_rope_bwd_op(*saved, *ctx.conf, dqo, dko)
     return (dq, dk, None if saved[2] is None else dqw, None if saved[3] is None else dkw,
             None, None, None, None, None, None)
@@ -399,6 +404,7 @@ def _delta_setup(ctx, inputs, output):
 
 def _delta_backward(ctx, d_o, dfinal):
     q, k, v, g, beta, initial_state, cu = ctx.saved_tensors
+    d_o = torch.zeros_like(v) if d_o is None else d_o
     *grads, ds = gated_delta_rule_bwd_op(q, k, v, g, beta, ctx.scale, initial_state, cu, d_o,
                                          dfinal if ctx.want_final else None)
     return (*grads, None, None if initial_state is None else ds, None, None)
@@ -453,3 +459,143 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, s
                            "call it under torch.no_grad()")
     scale = float(q.shape[-1]) ** -0.5 if scale is None else float(scale)
     return _C.gated_delta_step(q, k, v, g, beta, scale, state, state_indices)
+
+
+# --------------------------- the layer --------------------------------------------
+
+@dataclass
+class MixerState:
+    """What a ``GatedDeltaMixer`` carries of its running sequences, one slot each:
+    the convolution's last inputs [slots, taps-1, channels] and the delta rule's
+    states [slots, value heads, K, V] (fp32)."""
+    conv: Tensor
+    delta: Tensor
+
+
+class GatedDeltaMixer(nn.Module):
+    """A sequence mixer for fp16 or bf16 inputs [B, T, hidden]: one projection to
+    queries, keys, values, an output gate and the two gates of the delta rule; a
+    causal depthwise convolution with SiLU over queries, keys and values; unit
+    queries and keys (rotated if ``rotary_dim`` is given); the gated delta rule;
+    the heads' RMS norm times the output gate; the output projection.
+
+    ``forward`` is for training and prefill (also of packed batches), ``step``
+    for the next tokens of running sequences; ``new_state`` makes their slots.
+    """
+
+    def __init__(self, hidden: int, key_heads: int, value_heads: Optional[int] = None,
+                 key_dim: int = 128, value_dim: int = 128, taps: int = 4, rotary_dim: int = 0,
+                 rotary_base: float = 10000.0, max_positions: int = 0, eps: float = 1e-6,
+                 device=None, dtype=torch.bfloat16):
+        super().__init__()
+        value_heads = key_heads if value_heads is None else value_heads
+        if key_dim not in (64, 128) or value_dim not in (64, 128, 256):
+            raise ValueError(f"key_dim must be 64 or 128 and value_dim 64, 128 or 256, got "
+                             f"{key_dim}, {value_dim}")
+        if key_heads < 1 or value_heads < 1 or value_heads % key_heads:
+            raise ValueError(f"value_heads must be a multiple of key_heads, got {value_heads}, "
+                             f"{key_heads}")
+        if not 2 <= taps <= 8:
+            raise ValueError(f"taps must be 2 to 8, got {taps}")
+        if rotary_dim % 16 or not 0 <= rotary_dim <= key_dim:
+            raise ValueError(f"rotary_dim must be a multiple of 16 up to key_dim, got {rotary_dim}")
+        if rotary_dim and max_positions < 1:
+            raise ValueError("rotary_dim needs max_positions")
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"dtype must be float16 or bfloat16, got {dtype}")
+        self.key_heads, self.value_heads = key_heads, value_heads
+        self.key_dim, self.value_dim, self.taps, self.eps = key_dim, value_dim, taps, eps
+        self.sizes = (key_heads * key_dim, key_heads * key_dim, value_heads * value_dim)
+        self.channels = sum(self.sizes)
+        inner = value_heads * value_dim
+        # the gates' columns are padded to 8, so that every part of a row stays aligned
+        self.gates = -(-2 * value_heads // 8) * 8
+        make = dict(device=device, dtype=dtype)
+        self.in_proj = nn.Linear(hidden, self.channels + inner + self.gates, bias=False, **make)
+        self.conv_weight = nn.Parameter(torch.empty(taps, self.channels, **make))
+        nn.init.uniform_(self.conv_weight, -taps ** -0.5, taps ** -0.5)
+        # decay e^(-exp(log_rate) softplus(a + step_bias)): rates of 1 to 16, steps of 1e-3 to 0.1
+        rate = torch.empty(value_heads, device=device, dtype=torch.float32).uniform_(1, 16)
+        step = torch.exp(torch.empty(value_heads, device=device, dtype=torch.float32).uniform_(
+            math.log(1e-3), math.log(0.1)))
+        self.log_rate = nn.Parameter(rate.log())
+        self.step_bias = nn.Parameter(step + torch.log(-torch.expm1(-step)))
+        self.norm_weight = nn.Parameter(torch.ones(value_dim, **make))
+        self.out_proj = nn.Linear(inner, hidden, bias=False, **make)
+        self.rotary_dim = rotary_dim
+        if rotary_dim:
+            cos, sin = rotary_table(rotary_dim, max_positions, rotary_base, device=device)
+            self.register_buffer("cos", cos, persistent=False)
+            self.register_buffer("sin", sin, persistent=False)
+
+    def _apply(self, fn, *args, **kwargs):
+        # .to(dtype) casts floating buffers as well: the tables are fp32 in any case
+        tables = {n: getattr(self, n) for n in ("cos", "sin") if self.rotary_dim}
+        super()._apply(fn, *args, **kwargs)
+        for n, t in tables.items():
+            setattr(self, n, t.to(getattr(self, n).device))
+        return self
+
+    def new_state(self, slots: int) -> MixerState:
+        w = self.conv_weight
+        return MixerState(
+            torch.zeros(slots, self.taps - 1, self.channels, device=w.device, dtype=w.dtype),
+            torch.zeros(slots, self.value_heads, self.key_dim, self.value_dim, device=w.device,
+                        dtype=torch.float32))
+
+    def _project(self, x: Tensor):
+        p = self.in_proj(x)
+        mixed, gate, ab = p.split((self.channels, self.value_heads * self.value_dim, self.gates), -1)
+        a, b = ab[..., :self.value_heads], ab[..., self.value_heads:2 * self.value_heads]
+        g = -self.log_rate.float().exp() * nn.functional.softplus(a.float() + self.step_bias.float())
+        return mixed, gate, g, torch.sigmoid(b)
+
+    def _heads(self, mixed: Tensor, positions: Optional[Tensor]):
+        q, k, v = mixed.split(self.sizes, -1)
+        q = q.unflatten(-1, (self.key_heads, self.key_dim))
+        k = k.unflatten(-1, (self.key_heads, self.key_dim))
+        v = v.unflatten(-1, (self.value_heads, self.value_dim))
+        cos, sin = (self.cos, self.sin) if self.rotary_dim else (None, None)
+        q, k = qk_norm_rope(q, k, norm="l2", eps=self.eps, cos=cos, sin=sin,
+                            positions=positions if self.rotary_dim else None)
+        return q, k, v
+
+    def _finish(self, o: Tensor, gate: Tensor) -> Tensor:
+        o, _ = qk_norm_rope(o, o[:, :, :0], self.norm_weight, norm="rms", eps=self.eps)
+        return self.out_proj(o.flatten(-2) * nn.functional.silu(gate))
+
+    def forward(self, x: Tensor, state: Optional[MixerState] = None,
+                cu_seqlens: Optional[Tensor] = None, positions: Optional[Tensor] = None,
+                output_state: bool = False):
+        """y [B, T, hidden]; with ``output_state`` also the ``MixerState`` behind
+        the last tokens, one slot a sequence.  ``state`` continues earlier tokens.
+        ``positions`` ([T] or [B, T], for the rotation) default to 0 .. T-1."""
+        mixed, gate, g, beta = self._project(x)
+        conv_state, delta_state = (None, None) if state is None else (state.conv, state.delta)
+        out = causal_conv1d(mixed, self.conv_weight, activation="silu", initial_state=conv_state,
+                            cu_seqlens=cu_seqlens, output_final_state=output_state)
+        mixed, conv_final = out if output_state else (out, None)
+        q, k, v = self._heads(mixed, positions)
+        out = gated_delta_rule(q, k, v, g, beta, initial_state=delta_state, cu_seqlens=cu_seqlens,
+                               output_final_state=output_state)
+        o, delta_final = out if output_state else (out, None)
+        y = self._finish(o, gate)
+        return (y, MixerState(conv_final, delta_final)) if output_state else y
+
+    @torch.no_grad()
+    def step(self, x: Tensor, state: MixerState, state_indices: Optional[Tensor] = None,
+             positions: Optional[Tensor] = None) -> Tensor:
+        """The next tokens x [B, T, hidden] (T usually 1) of B running sequences,
+        whose slots are updated in place (``causal_conv1d_step`` says how slots
+        are picked)."""
+        mixed, gate, g, beta = self._project(x)
+        mixed = causal_conv1d_step(mixed, self.conv_weight, None, state.conv, activation="silu",
+                                   state_indices=state_indices)
+        q, k, v = self._heads(mixed, positions)
+        o = gated_delta_step(q, k, v, g, beta, state.delta, state_indices=state_indices)
+        return self._finish(o, gate)
+
+    def extra_repr(self) -> str:
+        return (f"key_heads={self.key_heads}, value_heads={self.value_heads}, "
+                f"key_dim={self.key_dim}, value_dim={self.value_dim}, taps={self.taps}, "
+                f"rotary_dim={self.rotary_dim}")
