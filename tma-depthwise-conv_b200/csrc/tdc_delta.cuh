@@ -18,7 +18,9 @@
 // fp32: with the split it is off by 4e-6.
 #pragma once
 
+#include "tdc_dwconv.h"
 #include "tdc_seq_common.cuh"
+#include "tdc_tc.cuh"
 
 namespace tdc {
 
@@ -52,11 +54,11 @@ struct DeltaParams {
   int64_t withhold;       // first chunk of a sequence whose copies never come (-1: none)
   int *status_words, *status_host;
   // gradients
-  // (in blocks of R = min(V, 128) channels: [V / R][columns / 8][R][8] a part)
-  __nv_bfloat16* um;      // [2][V][64]: U^T
-  __nv_bfloat16* xm;      // [2][V][64]: dX^T
-  __nv_bfloat16* sm;      // [2][V][K]: S^T before the chunk
-  __nv_bfloat16* dm;      // [2][V][K]: dS^T behind the chunk
+  // (32 channels together: [V / 32][2 parts][columns / 8][32][8])
+  __nv_bfloat16* um;      // U^T, 64 columns
+  __nv_bfloat16* xm;      // dX^T
+  __nv_bfloat16* sm;      // S^T before the chunk, K columns
+  __nv_bfloat16* dm;      // dS^T behind the chunk
   const void* d_o;
   int64_t do_sb, do_st, do_sh;
   const float* dfinal;
@@ -177,15 +179,6 @@ __device__ __forceinline__ void copy_rows(uint32_t dst, int ld, const uint16_t* 
   for (int i = tid; i < rows * vecs; i += threads) {
     const int r = i / vecs, c = i % vecs;
     cp_async16(dst + 2 * (r * ld + 8 * c), src + (r < valid ? r * stride : 0) + 8 * c, r < valid);
-  }
-}
-
-// 64 rows of [vecs][R][8] into [64][ld] in shared memory.
-__device__ __forceinline__ void copy_columns(uint32_t dst, int ld, const __nv_bfloat16* src, int R,
-                                             int vecs, int tid, int threads) {
-  for (int i = tid; i < 64 * vecs; i += threads) {
-    const int r = i & 63, c = i >> 6;
-    cp_async16(dst + 2 * (r * ld + 8 * c), src + (int64_t(c) * R + r) * 8, true);
   }
 }
 
@@ -488,26 +481,48 @@ __global__ void __launch_bounds__(128) delta_prepare_kernel(const DeltaParams p)
 // no terms that cancel (a first token without a state gets exactly 0); the
 // double sum grows by the column sum of E and falls by its row sum from row to row.
 // 8 warps: 4 groups of 16 rows by 2 halves of the columns.  The value channels
-// are walked in tiles of 64.
+// are walked in tiles of 32, of which the next is on its way while one is used,
+// also from one head to the next, as bulk copies (through the load unit,
+// cp.async, their issue took half of the kernel's time).
+constexpr int kTile = 32;
 template <int DK>
 struct GradSmem {
   static constexpr int ld = DK + 8;
+  static constexpr int ldo = kTile + 8;
   static constexpr int q = 0;
   static constexpr int k = q + kChunk * ld * 2;
-  static constexpr int s = k + kChunk * ld * 2;           // [2][64][ld]
-  static constexpr int d = s + 2 * 64 * ld * 2;           // [2][64][ld]
-  static constexpr int u = d + 2 * 64 * ld * 2;           // [2][64][72], later Dt
-  static constexpr int x = u + 2 * 64 * kLdT * 2;         // [2][64][72], later N
-  static constexpr int o = x + 2 * 64 * kLdT * 2;         // [64][72]
-  static constexpr int G = o + 64 * kLdT * 2;             // Far [64]
+  // a stage: S^T, dS^T, U^T, dX^T in two parts each, [columns / 8][32][8] as in the
+  // workspace, and dO
+  static constexpr int stages = k + kChunk * ld * 2;
+  static constexpr int part = kTile * DK * 2, upart = kTile * kChunk * 2;
+  static constexpr int s = 0;
+  static constexpr int d = s + 2 * part;
+  static constexpr int u = d + 2 * part;
+  static constexpr int x = u + 2 * upart;
+  static constexpr int o = x + 2 * upart;                 // [64][ldo]
+  static constexpr int stage = o + kChunk * ldo * 2;
+  static constexpr int dt = stages + 2 * stage;           // [2][64][72]
+  static constexpr int nn = dt + 2 * kChunk * kLdT * 2;   // [2][64][72]
+  static constexpr int G = nn + 2 * kChunk * kLdT * 2;    // Far [64]
   static constexpr int coef = G + 64 * 8;                 // [3][64]
   static constexpr int rows = coef + 3 * 64 * 4;          // [2][4][64]: row sums of both halves
   static constexpr int cols = rows + 2 * 4 * 64 * 4;      // [4][64]: column sums of the row groups
   static constexpr int diag = cols + 4 * 64 * 4;          // [64]
   static constexpr int dot = diag + 64 * 4;               // [8]
   static constexpr int dg = dot + 8 * 4;                  // [2][64]
-  static constexpr int bytes = dg + 2 * 64 * 4;
+  static constexpr int full = dg + 2 * 64 * 4;            // uint64 [2]
+  static constexpr int bytes = full + 2 * 8;
 };
+
+// Addresses in a [columns / 8][32][8] tile: a B fragment pair with the channels as
+// contraction, and an A fragment (both with .trans); 8 x 8 blocks of 128
+// contiguous bytes, so no bank is hit twice.
+__device__ __forceinline__ uint32_t addr_bt_blocks(uint32_t base, int n0, int k0, int lane) {
+  return base + (n0 / 8 + (lane >> 4)) * (kTile * 16) + (k0 + (lane & 7) + ((lane >> 3) & 1) * 8) * 16;
+}
+__device__ __forceinline__ uint32_t addr_at_blocks(uint32_t base, int m0, int k0, int lane) {
+  return base + (m0 / 8 + ((lane >> 3) & 1)) * (kTile * 16) + (k0 + (lane & 7) + (lane >> 4) * 8) * 16;
+}
 
 template <class E, int DK>
 __global__ void __launch_bounds__(256, 1) delta_grad_kernel(const DeltaParams p) {
@@ -536,94 +551,120 @@ __global__ void __launch_bounds__(256, 1) delta_grad_kernel(const DeltaParams p)
   const int kc0 = ch * (DK / 2);     // its half of K's columns
   float dq[NT][4] = {}, dk[NT][4] = {};
 
+  const int per_head = p.V / kTile, tiles = p.group * per_head;
+  uint64_t* full = reinterpret_cast<uint64_t*>(raw + Sm::full);
+  if (tid == 0) {
+    mbar_init(smem_addr(&full[0]), 1);
+    mbar_init(smem_addr(&full[1]), 1);
+    fence_mbar_init();
+  }
+  // Tiles come as four bulk copies, dO's rows through the load unit (one piece a
+  // thread; rows behind the sequence's end become zeros).
+  auto fetch = [&](int tile) {
+    const int head = tile / per_head, v0 = (tile - head * per_head) * kTile;
+    const int hv = h * p.group + head;
+    const uint32_t st = sb + Sm::stages + (tile & 1) * Sm::stage, bar = smem_addr(&full[tile & 1]);
+    if (tid == 0) {
+      const int64_t at32 = ((chunk * p.HV + hv) * p.V + v0) / kTile;
+      mbar_arrive_expect_tx(bar, 4 * Sm::part + 4 * Sm::upart);
+      bulk_load(st + Sm::s, p.sm + at32 * Sm::part, 2 * Sm::part, bar);
+      bulk_load(st + Sm::d, p.dm + at32 * Sm::part, 2 * Sm::part, bar);
+      bulk_load(st + Sm::u, p.um + at32 * Sm::upart, 2 * Sm::upart, bar);
+      bulk_load(st + Sm::x, p.xm + at32 * Sm::upart, 2 * Sm::upart, bar);
+    }
+    const uint16_t* d_o = static_cast<const uint16_t*>(p.d_o) + at.b * p.do_sb + at.t0 * p.do_st +
+                          hv * p.do_sh + v0;
+    copy_rows(st + Sm::o, Sm::ldo, d_o, p.do_st, kChunk, at.rows, kTile / 8, tid, 256);
+    cp_async_commit();
+  };
+  __syncthreads();
+  fetch(0);  // (Q and K go with its group)
+
   for (int gi = 0; gi < p.group; ++gi) {
     const int hv = h * p.group + gi;
     const int64_t slot = chunk * p.HV + hv;
-    const uint16_t* d_o = static_cast<const uint16_t*>(p.d_o) + at.b * p.do_sb + at.t0 * p.do_st +
-                          hv * p.do_sh;
     float os[NT][4] = {}, xs[NT][4] = {}, us[NT][4] = {}, D[4][4] = {}, M[4][4] = {};
     float dsum = 0.f;
-    for (int v0 = 0; v0 < p.V; v0 += 64) {
-      __syncthreads();
-      // 64 channels of a block of R, from v0
-      const int R = min(p.V, 128);
-      const int64_t block = v0 / R * R, row = v0 % R;
-#pragma unroll
-      for (int part = 0; part < 2; ++part) {
-        const int64_t st = ((slot * 2 + part) * p.V + block) * DK + row * 8;
-        const int64_t ut = ((slot * 2 + part) * p.V + block) * kChunk + row * 8;
-        copy_columns(sb + Sm::s + part * 64 * ld * 2, ld, p.sm + st, R, DK / 8, tid, 256);
-        copy_columns(sb + Sm::d + part * 64 * ld * 2, ld, p.dm + st, R, DK / 8, tid, 256);
-        copy_columns(sb + Sm::u + part * 64 * kLdT * 2, kLdT, p.um + ut, R, 8, tid, 256);
-        copy_columns(sb + Sm::x + part * 64 * kLdT * 2, kLdT, p.xm + ut, R, 8, tid, 256);
-      }
-      copy_rows(sb + Sm::o, kLdT, d_o + v0, p.do_st, kChunk, at.rows, 8, tid, 256);
-      cp_async_commit();
-      if (v0 == 0) {
+    for (int vt = 0; vt < per_head; ++vt) {
+      const int tile = gi * per_head + vt;
+      __syncthreads();  // the other stage (and with a new head what is kept for one) is free
+      if (tile + 1 < tiles) fetch(tile + 1);
+      if (vt == 0) {
         if (warp == 0) chunk_decay(load_decay(p, at, hv, lane), G, lane);
         const float* src = p.coef + slot * 3 * kChunk;
         if (tid >= 64) coef[tid - 64] = src[tid - 64];
       }
-      cp_async_wait<0>();
-      __syncthreads();
+      if (tile + 1 < tiles) cp_async_wait<1>(); else cp_async_wait<0>();
+      // A copy that does not come ends the block (all its threads together).
+      const bool ok = mbar_wait_bounded(smem_addr(&full[tile & 1]), uint32_t(tile >> 1) & 1u, nullptr,
+                                        false, p.timeout_ns);
+      if (!ok && tid == 0)
+        record_wait_failure(p.status_words, p.status_host, TDC_DEVICE_FULL_TIMEOUT, int(blockIdx.x),
+                            tile & 1, tile);
+      if (!__syncthreads_and(ok)) {
+        // the next tile's copies, if any are on their way, come to rest first
+        if (tile + 1 < tiles)
+          mbar_wait_bounded(smem_addr(&full[(tile + 1) & 1]), uint32_t((tile + 1) >> 1) & 1u, nullptr,
+                            false, p.timeout_ns);
+        return;
+      }
+      const unsigned char* stage = raw + Sm::stages + (tile & 1) * Sm::stage;
+      const uint32_t st = smem_addr(stage);
       // <dS, S>
-      for (int e = tid; e < 64 * DK / 2; e += 256) {
-        const int r = e / (DK / 2), c = 2 * (e % (DK / 2));
-        float a[2][2], b[2][2];
+      for (int e = tid; e < kTile * DK / 8; e += 256) {  // 8 values at the same place of all four
+        float a[2][8], b[2][8];
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
-          const int off = part * 64 * ld * 2 + 2 * (r * ld + c);
-          unpack2<BF16>(*reinterpret_cast<const uint32_t*>(raw + Sm::s + off), a[part][0], a[part][1]);
-          unpack2<BF16>(*reinterpret_cast<const uint32_t*>(raw + Sm::d + off), b[part][0], b[part][1]);
+          const int off = part * Sm::part + 16 * e;
+          unpack8<BF16>(*reinterpret_cast<const uint4*>(stage + Sm::s + off), a[part]);
+          unpack8<BF16>(*reinterpret_cast<const uint4*>(stage + Sm::d + off), b[part]);
         }
-        dsum = fmaf(a[0][0] + a[1][0], b[0][0] + b[1][0], dsum);
-        dsum = fmaf(a[0][1] + a[1][1], b[0][1] + b[1][1], dsum);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dsum = fmaf(a[0][i] + a[1][i], b[0][i] + b[1][i], dsum);
       }
 #pragma unroll 1
-      for (int ks = 0; ks < 4; ++ks) {
+      for (int ks = 0; ks < kTile / 16; ++ks) {
         uint32_t a[4], oh[4], ol[4], xh[4], xl[4], uh[4], ul[4];
-        ldsm4(a, addr_a(sb + Sm::o, kLdT, 16 * rg, 16 * ks, lane));
+        ldsm4(a, addr_a(st + Sm::o, Sm::ldo, 16 * rg, 16 * ks, lane));
 #pragma unroll
         for (int i = 0; i < 4; ++i) split_elem<E>(a[i], oh[i], ol[i]);
-        ldsm4_t(xh, addr_at(sb + Sm::x, kLdT, 16 * rg, 16 * ks, lane));
-        ldsm4_t(xl, addr_at(sb + Sm::x + 64 * kLdT * 2, kLdT, 16 * rg, 16 * ks, lane));
-        ldsm4_t(uh, addr_at(sb + Sm::u, kLdT, 16 * rg, 16 * ks, lane));
-        ldsm4_t(ul, addr_at(sb + Sm::u + 64 * kLdT * 2, kLdT, 16 * rg, 16 * ks, lane));
+        ldsm4_t(xh, addr_at_blocks(st + Sm::x, 16 * rg, 16 * ks, lane));
+        ldsm4_t(xl, addr_at_blocks(st + Sm::x + Sm::upart, 16 * rg, 16 * ks, lane));
+        ldsm4_t(uh, addr_at_blocks(st + Sm::u, 16 * rg, 16 * ks, lane));
+        ldsm4_t(ul, addr_at_blocks(st + Sm::u + Sm::upart, 16 * rg, 16 * ks, lane));
         // D and M: columns are tokens 32 ch .. + 31, from U^T [channel][token]
+        {
+          uint32_t bh[8], bl[8];
 #pragma unroll
-        for (int np = 0; np < 2; ++np) {
-          if (32 * ch + 16 * np > 16 * rg) continue;  // above the diagonal
-          uint32_t bh[4], bl[4];
-          ldsm4_t(bh, addr_bt(sb + Sm::u, kLdT, 32 * ch + 16 * np, 16 * ks, lane));
-          ldsm4_t(bl, addr_bt(sb + Sm::u + 64 * kLdT * 2, kLdT, 32 * ch + 16 * np, 16 * ks, lane));
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            mma_bf16(D[2 * np + i], oh, bh[2 * i], bh[2 * i + 1]);
-            mma_bf16(D[2 * np + i], oh, bl[2 * i], bl[2 * i + 1]);
-            if constexpr (!std::is_same_v<E, BF16>)
-              mma_bf16(D[2 * np + i], ol, bh[2 * i], bh[2 * i + 1]);
-            mma_split(M[2 * np + i], xh, xl, bh[2 * i], bh[2 * i + 1], bl[2 * i], bl[2 * i + 1]);
+          for (int np = 0; np < 2; ++np) {
+            ldsm4_t(bh + 4 * np, addr_bt_blocks(st + Sm::u, 32 * ch + 16 * np, 16 * ks, lane));
+            ldsm4_t(bl + 4 * np, addr_bt_blocks(st + Sm::u + Sm::upart, 32 * ch + 16 * np, 16 * ks, lane));
+          }
+          if (32 * ch + 16 <= 16 * rg) {  // all four tiles reach below the diagonal
+            mma_elem_split_n<E, 4>(D, oh, ol, bh, bl);
+            mma_split_n<4>(M, xh, xl, bh, bl);
+          } else if (32 * ch <= 16 * rg) {
+            mma_elem_split_n<E, 2>(D, oh, ol, bh, bl);
+            mma_split_n<2>(M, xh, xl, bh, bl);
           }
         }
-        // dO S^T, dX S^T, U dS^T: columns kc0 .. of K, from S^T [channel][K]
+        // dO S^T, dX S^T, U dS^T: columns kc0 .. of K, from S^T [channel][K], 32 at a time
 #pragma unroll
-        for (int np = 0; np < NT / 2; ++np) {
-          uint32_t bh[4], bl[4];
-          ldsm4_t(bh, addr_bt(sb + Sm::s, ld, kc0 + 16 * np, 16 * ks, lane));
-          ldsm4_t(bl, addr_bt(sb + Sm::s + 64 * ld * 2, ld, kc0 + 16 * np, 16 * ks, lane));
+        for (int nq = 0; nq < NT / 4; ++nq) {
+          uint32_t bh[8], bl[8];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            mma_bf16(os[2 * np + i], oh, bh[2 * i], bh[2 * i + 1]);
-            mma_bf16(os[2 * np + i], oh, bl[2 * i], bl[2 * i + 1]);
-            if constexpr (!std::is_same_v<E, BF16>)
-              mma_bf16(os[2 * np + i], ol, bh[2 * i], bh[2 * i + 1]);
-            mma_split(xs[2 * np + i], xh, xl, bh[2 * i], bh[2 * i + 1], bl[2 * i], bl[2 * i + 1]);
+          for (int np = 0; np < 2; ++np) {
+            ldsm4_t(bh + 4 * np, addr_bt_blocks(st + Sm::s, kc0 + 32 * nq + 16 * np, 16 * ks, lane));
+            ldsm4_t(bl + 4 * np, addr_bt_blocks(st + Sm::s + Sm::part, kc0 + 32 * nq + 16 * np, 16 * ks, lane));
           }
-          ldsm4_t(bh, addr_bt(sb + Sm::d, ld, kc0 + 16 * np, 16 * ks, lane));
-          ldsm4_t(bl, addr_bt(sb + Sm::d + 64 * ld * 2, ld, kc0 + 16 * np, 16 * ks, lane));
+          mma_elem_split_n<E, 4>(os + 4 * nq, oh, ol, bh, bl);
+          mma_split_n<4>(xs + 4 * nq, xh, xl, bh, bl);
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            mma_split(us[2 * np + i], uh, ul, bh[2 * i], bh[2 * i + 1], bl[2 * i], bl[2 * i + 1]);
+          for (int np = 0; np < 2; ++np) {
+            ldsm4_t(bh + 4 * np, addr_bt_blocks(st + Sm::d, kc0 + 32 * nq + 16 * np, 16 * ks, lane));
+            ldsm4_t(bl + 4 * np, addr_bt_blocks(st + Sm::d + Sm::part, kc0 + 32 * nq + 16 * np, 16 * ks, lane));
+          }
+          mma_split_n<4>(us + 4 * nq, uh, ul, bh, bl);
         }
       }
     }
@@ -668,7 +709,6 @@ __global__ void __launch_bounds__(256, 1) delta_grad_kernel(const DeltaParams p)
       }
     }
     float re[2] = {};  // row sums of E below the diagonal
-    __syncthreads();   // u and x are free: Dt and N take their place
 #pragma unroll
     for (int nt = 0; nt < 4; ++nt) {
       float cs[2] = {};  // column sums of P D - M L below the diagonal, this thread's two rows
@@ -695,11 +735,11 @@ __global__ void __launch_bounds__(256, 1) delta_grad_kernel(const DeltaParams p)
         uint32_t hi, lo;
         const int off = 2 * (i * kLdT + j);
         split2(dt[0], dt[1], hi, lo);
-        *reinterpret_cast<uint32_t*>(raw + Sm::u + off) = hi;
-        *reinterpret_cast<uint32_t*>(raw + Sm::u + 64 * kLdT * 2 + off) = lo;
+        *reinterpret_cast<uint32_t*>(raw + Sm::dt + off) = hi;
+        *reinterpret_cast<uint32_t*>(raw + Sm::dt + 64 * kLdT * 2 + off) = lo;
         split2(nn[0], nn[1], hi, lo);
-        *reinterpret_cast<uint32_t*>(raw + Sm::x + off) = hi;
-        *reinterpret_cast<uint32_t*>(raw + Sm::x + 64 * kLdT * 2 + off) = lo;
+        *reinterpret_cast<uint32_t*>(raw + Sm::nn + off) = hi;
+        *reinterpret_cast<uint32_t*>(raw + Sm::nn + 64 * kLdT * 2 + off) = lo;
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -732,37 +772,37 @@ __global__ void __launch_bounds__(256, 1) delta_grad_kernel(const DeltaParams p)
 #pragma unroll 1
     for (int ks = 0; ks < 4; ++ks) {
       uint32_t ah[4], al[4], nh[4], nl[4];
+      constexpr int part = kChunk * kLdT * 2;
       if (ks <= rg) {
-        ldsm4(ah, addr_a(sb + Sm::u, kLdT, 16 * rg, 16 * ks, lane));
-        ldsm4(al, addr_a(sb + Sm::u + 64 * kLdT * 2, kLdT, 16 * rg, 16 * ks, lane));
-        ldsm4(nh, addr_a(sb + Sm::x, kLdT, 16 * rg, 16 * ks, lane));
-        ldsm4(nl, addr_a(sb + Sm::x + 64 * kLdT * 2, kLdT, 16 * rg, 16 * ks, lane));
+        ldsm4(ah, addr_a(sb + Sm::dt, kLdT, 16 * rg, 16 * ks, lane));
+        ldsm4(al, addr_a(sb + Sm::dt + part, kLdT, 16 * rg, 16 * ks, lane));
+        ldsm4(nh, addr_a(sb + Sm::nn, kLdT, 16 * rg, 16 * ks, lane));
+        ldsm4(nl, addr_a(sb + Sm::nn + part, kLdT, 16 * rg, 16 * ks, lane));
 #pragma unroll
-        for (int np = 0; np < NT / 2; ++np) {
-          uint32_t b[4];
-          ldsm4_t(b, addr_bt(sb + Sm::k, ld, kc0 + 16 * np, 16 * ks, lane));
+        for (int nq = 0; nq < NT / 4; ++nq) {
+          uint32_t b[8];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            mma_split_elem<E>(dq[2 * np + i], ah, al, b[2 * i], b[2 * i + 1]);
-            mma_split_elem<E>(dk[2 * np + i], nh, nl, b[2 * i], b[2 * i + 1]);
-          }
+          for (int np = 0; np < 2; ++np)
+            ldsm4_t(b + 4 * np, addr_bt(sb + Sm::k, ld, kc0 + 32 * nq + 16 * np, 16 * ks, lane));
+          mma_split_elem_n<E, 4>(dq + 4 * nq, ah, al, b);
+          mma_split_elem_n<E, 4>(dk + 4 * nq, nh, nl, b);
         }
       }
       if (ks >= rg) {
-        ldsm4_t(ah, addr_at(sb + Sm::u, kLdT, 16 * rg, 16 * ks, lane));
-        ldsm4_t(al, addr_at(sb + Sm::u + 64 * kLdT * 2, kLdT, 16 * rg, 16 * ks, lane));
-        ldsm4_t(nh, addr_at(sb + Sm::x, kLdT, 16 * rg, 16 * ks, lane));
-        ldsm4_t(nl, addr_at(sb + Sm::x + 64 * kLdT * 2, kLdT, 16 * rg, 16 * ks, lane));
+        ldsm4_t(ah, addr_at(sb + Sm::dt, kLdT, 16 * rg, 16 * ks, lane));
+        ldsm4_t(al, addr_at(sb + Sm::dt + part, kLdT, 16 * rg, 16 * ks, lane));
+        ldsm4_t(nh, addr_at(sb + Sm::nn, kLdT, 16 * rg, 16 * ks, lane));
+        ldsm4_t(nl, addr_at(sb + Sm::nn + part, kLdT, 16 * rg, 16 * ks, lane));
 #pragma unroll
-        for (int np = 0; np < NT / 2; ++np) {
-          uint32_t b[4], c[4];
-          ldsm4_t(b, addr_bt(sb + Sm::q, ld, kc0 + 16 * np, 16 * ks, lane));
-          ldsm4_t(c, addr_bt(sb + Sm::k, ld, kc0 + 16 * np, 16 * ks, lane));
+        for (int nq = 0; nq < NT / 4; ++nq) {
+          uint32_t b[8], c[8];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            mma_split_elem<E>(dk[2 * np + i], ah, al, b[2 * i], b[2 * i + 1]);
-            mma_split_elem<E>(dk[2 * np + i], nh, nl, c[2 * i], c[2 * i + 1]);
+          for (int np = 0; np < 2; ++np) {
+            ldsm4_t(b + 4 * np, addr_bt(sb + Sm::q, ld, kc0 + 32 * nq + 16 * np, 16 * ks, lane));
+            ldsm4_t(c + 4 * np, addr_bt(sb + Sm::k, ld, kc0 + 32 * nq + 16 * np, 16 * ks, lane));
           }
+          mma_split_elem_n<E, 4>(dk + 4 * nq, ah, al, b);
+          mma_split_elem_n<E, 4>(dk + 4 * nq, nh, nl, c);
         }
       }
     }

@@ -250,14 +250,13 @@ __device__ __forceinline__ float widen(uint32_t raw) {
 }
 
 // 16 packed pairs (32 tokens or keys) of a channel to the workspace, where 8
-// columns of all channels of the block lie together (16 bytes a channel): the
-// warp's stores are whole lines.
-__device__ __forceinline__ void store_pairs(__nv_bfloat16* dst, int channels, const uint32_t (&r)[16],
-                                            bool live) {
+// columns of the warp's 32 channels lie together (16 bytes a channel): its
+// stores are whole lines.
+__device__ __forceinline__ void store_pairs(__nv_bfloat16* dst, const uint32_t (&r)[16], bool live) {
   if (!live) return;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    *reinterpret_cast<uint4*>(dst + i * channels * 8) =
+    *reinterpret_cast<uint4*>(dst + i * 32 * 8) =
         make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
 }
 
@@ -342,7 +341,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
     walk_load<DK>(S, p.init == nullptr ? nullptr : p.init + state_at, p.V, live);
     uint32_t vr[32], hi[16], lo[16];
     const uint32_t vstep = uint32_t(p.v_st * 2), ostep = uint32_t(p.HV * p.V * 2);
-    const int channels = min(p.V, 128), cl = ch - v0;  // of this block, and this thread's
+    const int group0 = v0 + 32 * (warp & 3);  // first of the warp's channels
     auto rows_of = [&](int c) {  // of this thread's 32 tokens
       return int(min(int64_t(32), s.len - int64_t(c) * kChunk - t0));
     };
@@ -387,10 +386,10 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         for (int i = 0; i < 32; ++i) w[i] = S[32 * x + i];
         split_to_tmem(w, lanes + cS + half * (DK / 4) + 16 * x, sStep, hi, lo);
         if constexpr (MODE == 1) {
-          __nv_bfloat16* dst = p.sm + (slot * 2 * p.V + v0) * DK +
-                               (half * (DK / 16) + 4 * x) * channels * 8 + cl * 8;
-          store_pairs(dst, channels, hi, live);
-          store_pairs(dst + int64_t(p.V) * DK, channels, lo, live);
+          __nv_bfloat16* dst = p.sm + (slot * p.V + group0) * 2 * DK +
+                               (half * (DK / 16) + 4 * x) * 32 * 8 + lane * 8;
+          store_pairs(dst, hi, live);
+          store_pairs(dst + 32 * DK, lo, live);
         }
       }
       operand_ready(sy->sr, lane);
@@ -434,10 +433,9 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             split2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), hi[i], lo[i]);
-          __nv_bfloat16* dst =
-              p.um + (slot * 2 * p.V + v0) * kChunk + t0 * channels + cl * 8;
-          store_pairs(dst, channels, hi, live);
-          store_pairs(dst + int64_t(p.V) * kChunk, channels, lo, live);
+          __nv_bfloat16* dst = p.um + (slot * p.V + group0) * 2 * kChunk + t0 * 32 + lane * 8;
+          store_pairs(dst, hi, live);
+          store_pairs(dst + 32 * kChunk, lo, live);
         }
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
@@ -567,7 +565,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
     walk_load<DK>(D, p.dfinal == nullptr ? nullptr : p.dfinal + state_at, p.V, live);
     uint32_t vr[32], hi[16], lo[16];
     const uint32_t dostep = uint32_t(p.do_st * 2), dvstep = uint32_t(p.HV * p.V * 2);
-    const int channels = min(p.V, 128), cl = ch - v0;
+    const int group0 = v0 + 32 * (warp & 3);
     auto rows_of = [&](int cc) { return int(min(int64_t(32), s.len - int64_t(cc) * kChunk - t0)); };
     auto fetch_do = [&](int c) {  // c counts from the end
       const int cc = chunks - 1 - c;
@@ -607,10 +605,10 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
 #pragma unroll
         for (int i = 0; i < 32; ++i) w[i] = D[32 * x + i];
         split_to_tmem(w, lanes + cS + half * (DK / 4) + 16 * x, sStep, hi, lo);
-        __nv_bfloat16* dst = p.dm + (slot * 2 * p.V + v0) * DK +
-                             (half * (DK / 16) + 4 * x) * channels * 8 + cl * 8;
-        store_pairs(dst, channels, hi, live);
-        store_pairs(dst + int64_t(p.V) * DK, channels, lo, live);
+        __nv_bfloat16* dst = p.dm + (slot * p.V + group0) * 2 * DK +
+                             (half * (DK / 16) + 4 * x) * 32 * 8 + lane * 8;
+        store_pairs(dst, hi, live);
+        store_pairs(dst + 32 * DK, lo, live);
       }
       operand_ready(sy->sr, lane);
       // gam dO beside the chain (its region's last reader was the last chunk's update)
@@ -673,9 +671,9 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           split2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), hi[i], lo[i]);
-        __nv_bfloat16* dst = p.xm + (slot * 2 * p.V + v0) * kChunk + t0 * channels + cl * 8;
-        store_pairs(dst, channels, hi, live);
-        store_pairs(dst + int64_t(p.V) * kChunk, channels, lo, live);
+        __nv_bfloat16* dst = p.xm + (slot * p.V + group0) * 2 * kChunk + t0 * 32 + lane * 8;
+        store_pairs(dst, hi, live);
+        store_pairs(dst + 32 * kChunk, lo, live);
 #pragma unroll
         for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
         walk_put<E>(dv + (int64_t(cc) * kChunk + t0) * p.HV * p.V, dvstep, x, rows_of(cc), live);

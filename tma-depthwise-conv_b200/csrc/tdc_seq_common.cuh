@@ -149,14 +149,14 @@ __device__ __forceinline__ void cp_async_wait() {
 // so the C fragments of two neighbouring 8-column tiles are, once packed, the
 // A fragment of a 16-deep step: products chain in registers.
 __device__ __forceinline__ void mma_bf16(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_f16(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -169,13 +169,13 @@ __device__ __forceinline__ void mma_elem(float c[4], const uint32_t a[4], uint32
   else mma_f16(c, a, b0, b1);
 }
 
-__device__ __forceinline__ void ldsm4(uint32_t r[4], uint32_t addr) {
+__device__ __forceinline__ void ldsm4(uint32_t* r, uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr)
                : "memory");
 }
-__device__ __forceinline__ void ldsm4_t(uint32_t r[4], uint32_t addr) {
+__device__ __forceinline__ void ldsm4_t(uint32_t* r, uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr)
@@ -242,6 +242,50 @@ __device__ __forceinline__ void mma_split(float c[4], const uint32_t ah[4], cons
   mma_bf16(c, ah, bh0, bh1);
   mma_bf16(c, al, bh0, bh1);
   mma_bf16(c, ah, bl0, bl1);
+}
+
+// The same for N accumulators side by side, product by product rather than
+// accumulator by accumulator: neighbouring instructions are independent (one
+// that waits for the one before it takes 20 cycles instead of 8).
+template <int N>
+__device__ __forceinline__ void mma_split_n(float (*c)[4], const uint32_t ah[4], const uint32_t al[4],
+                                            const uint32_t* bh, const uint32_t* bl) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) mma_bf16(c[i], ah, bh[2 * i], bh[2 * i + 1]);
+#pragma unroll
+  for (int i = 0; i < N; ++i) mma_bf16(c[i], al, bh[2 * i], bh[2 * i + 1]);
+#pragma unroll
+  for (int i = 0; i < N; ++i) mma_bf16(c[i], ah, bl[2 * i], bl[2 * i + 1]);
+}
+// A exact in the element type (ah, and al for fp16), B split.
+template <class E, int N>
+__device__ __forceinline__ void mma_elem_split_n(float (*c)[4], const uint32_t ah[4],
+                                                 const uint32_t al[4], const uint32_t* bh,
+                                                 const uint32_t* bl) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) mma_bf16(c[i], ah, bh[2 * i], bh[2 * i + 1]);
+#pragma unroll
+  for (int i = 0; i < N; ++i) mma_bf16(c[i], ah, bl[2 * i], bl[2 * i + 1]);
+  if constexpr (!std::is_same_v<E, BF16>) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) mma_bf16(c[i], al, bh[2 * i], bh[2 * i + 1]);
+  }
+}
+// A split, B exact in the element type.
+template <class E, int N>
+__device__ __forceinline__ void mma_split_elem_n(float (*c)[4], const uint32_t ah[4],
+                                                 const uint32_t al[4], const uint32_t* b) {
+  uint32_t bh[2 * N], bl[2 * N];
+#pragma unroll
+  for (int i = 0; i < 2 * N; ++i) split_elem<E>(b[i], bh[i], bl[i]);
+#pragma unroll
+  for (int i = 0; i < N; ++i) mma_bf16(c[i], ah, bh[2 * i], bh[2 * i + 1]);
+#pragma unroll
+  for (int i = 0; i < N; ++i) mma_bf16(c[i], al, bh[2 * i], bh[2 * i + 1]);
+  if constexpr (!std::is_same_v<E, BF16>) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) mma_bf16(c[i], ah, bl[2 * i], bl[2 * i + 1]);
+  }
 }
 
 // Addresses for ldmatrix.x4 over a row-major 16-bit tile with `ld` elements a
