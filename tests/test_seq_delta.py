@@ -123,6 +123,37 @@ def test_every_block_size_of_the_walk(walks):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,T,H,HV,K,V", [(1, 1601, 1, 1, 64, 64), (2, 2048, 1, 2, 128, 128),
+                                          (1, 1537, 2, 2, 64, 256), (1, 4000, 1, 1, 128, 64),
+                                          (1, 1984, 16, 32, 64, 64)])
+@pytest.mark.parametrize("state,dtype", [(True, "bf16"), (False, "fp16")])
+def test_long_sequences_in_segments(B, T, H, HV, K, V, state, dtype):
+    c = _case(B, T, H, HV, K, V, dtype, state=state, seed=T)
+    c["g"] *= 0.05                                   # states that last over several segments
+    args = [c[k] for k in ("q", "k", "v", "g", "beta")]
+    o, f = S.gated_delta_rule(*(t.cuda() for t in args), None,
+                              c["state"].cuda() if state else None, None, True)
+    # the recurrence in fp64 (on the GPU: thousands of tokens)
+    d = [t.double().cuda() for t in args]
+    q, k = (t.repeat_interleave(HV // H, 2) for t in d[:2])
+    s = (c["state"].double().cuda() if state else torch.zeros(B, HV, K, V, dtype=torch.float64).cuda())
+    rows = []
+    for t in range(T):
+        s = s * d[3][:, t].exp()[..., None, None]
+        u = (d[2][:, t] - torch.einsum("bhkv,bhk->bhv", s, k[:, t])) * d[4][:, t][..., None]
+        s = s + k[:, t][..., None] * u[:, :, None, :]
+        rows.append(torch.einsum("bhkv,bhk->bhv", s, q[:, t]) * K ** -0.5)
+    want = torch.stack(rows, 1)
+    R.close(o, want, CHUNKED * want.abs().max().item(), "o")
+    R.close(f, s, CHUNKED * s.abs().max().item(), "final")
+    # the same without segments: a packed batch of the sequences
+    cu = torch.arange(B + 1).cuda() * T
+    o2, f2 = S.gated_delta_rule(*(t.cuda().flatten(0, 1)[None] for t in args), None,
+                                c["state"].cuda() if state else None, cu, True)
+    assert (f2 - f).abs().max().item() <= 2 * CHUNKED * s.abs().max().item()
+
+
+@pytest.mark.gpu
 def test_no_rows_gives_the_state_back():
     c = _case(2, 0, 1, 2, 64, 64, "bf16", state=True)
     got = _run(c)

@@ -45,6 +45,10 @@ struct DeltaParams {
   int64_t* seq_chunk;     // [N + 1] first chunk of each sequence
   bool beta_f32;
   float scale;
+  // the forward in segments (segments > 1, batch form): see delta_walk_kernel
+  int segments, segment_chunks, pass;
+  float* seg_s;           // [N][HV][segments][K][V]: state before each
+  float* seg_m;           // [N][HV][segments][K][K]: what a segment makes of a state
   // workspace of all chunks, [chunk][HV] each
   // (tiles in the order of WalkTiles; 8 x 8 blocks, see tdc_tc.cuh)
   __nv_bfloat16* tp;      // T and P, high parts and remainders: [4][64 x 64]

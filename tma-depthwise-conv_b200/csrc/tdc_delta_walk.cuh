@@ -260,8 +260,93 @@ __device__ __forceinline__ void store_pairs(__nv_bfloat16* dst, const uint32_t (
         make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
 }
 
+// What a block of the forward walks.
+struct Segment {
+  enum { kWhole, kFromZero, kMap };  // as it is, from a state of 0, the identity with V = 0
+  int64_t n;
+  int index, role, v0, channels;
+};
+__device__ __forceinline__ Segment segment_of(const DeltaParams& p, int tiles, int DK) {
+  Segment r{int64_t(blockIdx.x) / tiles, 0, Segment::kWhole, int(blockIdx.x % tiles) * 128, p.V};
+  if (p.segments <= 1) return r;
+  // pass 1: tiles of the first segment, of the inner ones, the inner ones' maps;
+  // pass 2: tiles of all but the first
+  const int inner = p.segments - 2;
+  const int per = p.pass == 1 ? tiles * (1 + inner) + inner : tiles * (p.segments - 1);
+  int j = int(blockIdx.x % per);
+  r.n = blockIdx.x / per;
+  if (p.pass == 1 && j >= tiles * (1 + inner)) {
+    r.index = 1 + j - tiles * (1 + inner);
+    r.role = Segment::kMap;
+    r.v0 = 0;
+    r.channels = DK;
+    return r;
+  }
+  r.index = j / tiles + (p.pass == 1 ? 0 : 1);
+  r.v0 = j % tiles * 128;
+  if (p.pass == 1 && r.index > 0) r.role = Segment::kFromZero;
+  return r;
+}
+__device__ __forceinline__ float* segment_state(const DeltaParams& p, float* base, int64_t n, int hv,
+                                                int index, int K, int columns) {
+  return base + ((n * p.HV + hv) * p.segments + index) * int64_t(K) * columns;
+}
+
+// The states between the segments, S_(i+1) = M_i S_i + N_i (N_i is in S_(i+1)'s
+// place), in fp32: a block has 32 columns of a head's state, one a lane, a warp
+// DK / 8 of its rows.  M comes through shared memory, in whole lines.
+template <int DK>
+__global__ void __launch_bounds__(256) delta_join_kernel(const DeltaParams p) {
+  constexpr int R = DK / 8;
+  extern __shared__ __align__(16) float sh[];  // M [DK][DK], S [DK][32]
+  float* S = sh + DK * DK;
+  const int tid = threadIdx.x, lane = tid & 31, k0 = (tid >> 5) * R, v0 = blockIdx.y * 32;
+  const int64_t n = blockIdx.x / p.HV;
+  const int hv = int(blockIdx.x % p.HV);
+  float acc[R];
+  for (int i = 1; i < p.segments; ++i) {
+    float* at = segment_state(p, p.seg_s, n, hv, i, DK, p.V) + int64_t(k0) * p.V + v0 + lane;
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[r] = at[int64_t(r) * p.V];
+    if (i > 1) {
+      const float4* m = reinterpret_cast<const float4*>(
+          segment_state(p, p.seg_m, n, hv, i - 1, DK, DK));
+#pragma unroll 4
+      for (int e = tid; e < DK * DK / 4; e += 256) reinterpret_cast<float4*>(sh)[e] = m[e];
+      __syncthreads();
+      for (int x = 0; x < DK; x += 4) {
+        float s[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) s[u] = S[(x + u) * 32 + lane];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float4 w = *reinterpret_cast<const float4*>(sh + (k0 + r) * DK + x);
+          acc[r] = fmaf(w.x, s[0], acc[r]);
+          acc[r] = fmaf(w.y, s[1], acc[r]);
+          acc[r] = fmaf(w.z, s[2], acc[r]);
+          acc[r] = fmaf(w.w, s[3], acc[r]);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) at[int64_t(r) * p.V] = acc[r];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) S[(k0 + r) * 32 + lane] = acc[r];
+    __syncthreads();
+  }
+}
+
 // MODE 0: the forward (o and the final state).  MODE 1: the forward once more
 // for the gradients: U of each chunk and the state before it.
+//
+// A long sequence with few heads leaves most SMs idle, so MODE 0 can walk its
+// segments side by side.  A segment maps the state before it to M S + N: pass 1
+// walks the first segment as it is and each inner one twice, from a state of 0
+// (its end is N) and with V = 0 from the identity (its end is M, whose K columns
+// stand in the channels' place); delta_join_kernel makes the states between the
+// segments; pass 2 walks all but the first from them.  Two passes of a
+// segment's length replace one of the whole.
 template <class E, int DK, int MODE>
 __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const DeltaParams p) {
   extern __shared__ __align__(1024) unsigned char raw[];
@@ -271,9 +356,17 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int hv = blockIdx.y, h = hv / p.group;
   const int tiles = (p.V + 127) / 128;
-  const int64_t n = blockIdx.x / tiles;
-  const int v0 = int(blockIdx.x % tiles) * 128;
-  const SeqAt s = seq_at(p, n);
+  const Segment sg = MODE == 0 ? segment_of(p, tiles, DK) : Segment{};
+  const int64_t n = MODE == 0 ? sg.n : blockIdx.x / tiles;
+  const int v0 = MODE == 0 ? sg.v0 : int(blockIdx.x % tiles) * 128;
+  const int V = MODE == 0 ? sg.channels : p.V;  // of the state that is walked
+  SeqAt s = seq_at(p, n);
+  if (MODE == 0 && p.segments > 1) {
+    const int64_t from = int64_t(sg.index) * p.segment_chunks;
+    s.chunk0 += from;
+    s.lo += from * kChunk;
+    s.len = max(int64_t(0), min(s.len - from * kChunk, int64_t(p.segment_chunks) * kChunk));
+  }
   const int chunks = int((s.len + kChunk - 1) / kChunk);
   walk_setup(sy, tid, warp);
   const Waiter wait{&sy->abort, p.timeout_ns, p.status_words, p.status_host, int(blockIdx.x)};
@@ -333,19 +426,35 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWalkRegs));
     const uint32_t lanes = tm + (uint32_t(warp & 3) << 21);  // 32 lanes a quadrant
     const int half = warp >> 2, ch = v0 + 32 * (warp & 3) + lane, t0 = 32 * half;
-    const bool live = ch < p.V;
-    const int64_t state_at = ((n * p.HV + hv) * DK + half * (DK / 2)) * int64_t(p.V) + ch;
+    const bool live = ch < V;
+    const bool real = MODE != 0 || sg.role != Segment::kMap;  // V is read
+    const bool out = MODE != 0 || sg.role == Segment::kWhole;  // o is written
+    const int64_t state_at = ((n * p.HV + hv) * DK + half * (DK / 2)) * int64_t(V) + ch;
     const uint16_t* v = static_cast<const uint16_t*>(p.v) + s.b * p.v_sb + s.lo * p.v_st + hv * p.v_sh + ch;
     uint16_t* o = static_cast<uint16_t*>(p.o) + ((s.b * p.T + s.lo) * p.HV + hv) * p.V + ch;
     float S[DK / 2];
-    walk_load<DK>(S, p.init == nullptr ? nullptr : p.init + state_at, p.V, live);
+    if (MODE == 0 && p.segments > 1) {
+      if (sg.role == Segment::kMap) {
+#pragma unroll
+        for (int i = 0; i < DK / 2; ++i) S[i] = half * (DK / 2) + i == ch ? 1.f : 0.f;
+      } else {
+        const float* from = sg.role == Segment::kFromZero ? nullptr
+                            : sg.index == 0
+                                ? (p.init == nullptr ? nullptr : p.init + state_at)
+                                : segment_state(p, p.seg_s, n, hv, sg.index, DK, V) +
+                                      int64_t(half * (DK / 2)) * V + ch;
+        walk_load<DK>(S, from, V, live);
+      }
+    } else {
+      walk_load<DK>(S, p.init == nullptr ? nullptr : p.init + state_at, p.V, live);
+    }
     uint32_t vr[32], hi[16], lo[16];
     const uint32_t vstep = uint32_t(p.v_st * 2), ostep = uint32_t(p.HV * p.V * 2);
     const int group0 = v0 + 32 * (warp & 3);  // first of the warp's channels
     auto rows_of = [&](int c) {  // of this thread's 32 tokens
       return int(min(int64_t(32), s.len - int64_t(c) * kChunk - t0));
     };
-    walk_column(vr, v + t0 * p.v_st, vstep, rows_of(0), live);
+    walk_column(vr, v + t0 * p.v_st, vstep, rows_of(0), live && real);
     float qs[32];     // scale gam S^T Q^T of the chunk
     float last = 1.f; // gam_63 of the chunk before
     bool ok = true;
@@ -358,7 +467,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
       tmem_ld(lanes + cO + t0, r);
 #pragma unroll
       for (int i = 0; i < 32; ++i) qs[i] += __uint_as_float(r[i]);
-      walk_put<E>(o + (int64_t(c) * kChunk + t0) * p.HV * p.V, ostep, qs, rows_of(c), live);
+      walk_put<E>(o + (int64_t(c) * kChunk + t0) * p.HV * p.V, ostep, qs, rows_of(c), live && out);
     };
     // The state after the chunk before: gam_63 S + its update.
     auto advance = [&](int c) {
@@ -419,7 +528,8 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
       }
       operand_ready(sy->xr, lane);
       if (c + 1 < chunks)
-        walk_column(vr, v + (int64_t(c + 1) * kChunk + t0) * p.v_st, vstep, rows_of(c + 1), live);
+        walk_column(vr, v + (int64_t(c + 1) * kChunk + t0) * p.v_st, vstep, rows_of(c + 1),
+                    live && real);
       // V' = beta U and w V'
       ok = warp_wait(wait, sy->u, c);
       if (!ok) break;
@@ -475,8 +585,16 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
       advance(chunks - 1);
       if (MODE == 0 && ok) put_out(chunks - 1);
     }
-    if (MODE == 0 && ok && p.final_state != nullptr)
-      walk_store<DK>(p.final_state + state_at, S, p.V, live);
+    if (MODE == 0 && ok) {
+      float* to = nullptr;
+      if (p.segments <= 1 || sg.index == p.segments - 1)
+        to = p.final_state == nullptr ? nullptr : p.final_state + state_at;
+      else if (sg.role == Segment::kMap)
+        to = segment_state(p, p.seg_m, n, hv, sg.index, DK, DK) + int64_t(half * (DK / 2)) * DK + ch;
+      else if (p.pass == 1)  // the state behind the first segment, N of an inner one
+        to = segment_state(p, p.seg_s, n, hv, sg.index + 1, DK, V) + int64_t(half * (DK / 2)) * V + ch;
+      if (to != nullptr) walk_store<DK>(to, S, V, live);
+    }
   }
   __syncwarp();
   tc_fence_before();

@@ -318,6 +318,24 @@ int64_t delta_chunks(const tdc_delta_args* a) {
                                   : a->B * ceil_div(a->T, tdc::kChunk);
 }
 
+// Segments that the forward walks side by side (1: none): as many as give every
+// block of both passes an SM of its own, if two passes over a segment (and about
+// 6 chunks' time for the second launch and the join) are shorter than one over
+// the whole.  Packed batches' lengths are not known here: they are walked whole.
+int delta_segments(const tdc_delta_args* a) {
+  if (a->cu_seqlens != nullptr) return 1;
+  const int64_t chunks = ceil_div(a->T, tdc::kChunk), heads = a->B * a->HV;
+  const int64_t walks = heads * ceil_div(a->V, 128);
+  int best = 1;
+  int64_t cost = chunks;
+  for (int p = 3; p <= 16; ++p) {
+    if (walks + (p - 2) * (walks + heads) > 148 || walks * (p - 1) > 148) break;
+    const int64_t c = 2 * ceil_div(chunks, p) + 6;
+    if (c < cost) best = p, cost = c;
+  }
+  return best;
+}
+
 // Lays the workspace out (base may be null: only the size is wanted).
 int64_t delta_layout(const tdc_delta_args* a, bool grads, unsigned char* base, tdc::DeltaParams* p) {
   int64_t at = 0;
@@ -333,6 +351,12 @@ int64_t delta_layout(const tdc_delta_args* a, bool grads, unsigned char* base, t
   unsigned char* kq = take(delta_chunks(a) * a->H * 2 * parts * tdc::kChunk * a->K * 2);
   unsigned char* coef = take(slots * 3 * tdc::kChunk * 4);
   unsigned char *um = nullptr, *xm = nullptr, *sm = nullptr, *dm = nullptr;
+  unsigned char *seg_s = nullptr, *seg_m = nullptr;
+  const int segments = grads ? 1 : delta_segments(a);
+  if (segments > 1) {
+    seg_s = take(a->B * a->HV * segments * a->K * a->V * 4);
+    seg_m = take(a->B * a->HV * segments * a->K * a->K * 4);
+  }
   if (grads) {
     um = take(slots * 2 * a->V * tdc::kChunk * 2);
     xm = take(slots * 2 * a->V * tdc::kChunk * 2);
@@ -344,6 +368,10 @@ int64_t delta_layout(const tdc_delta_args* a, bool grads, unsigned char* base, t
     p->seq_chunk = p->seq_lo + delta_seqs(a) + 1;
     p->tp = reinterpret_cast<__nv_bfloat16*>(tp);
     p->kq = kq;
+    p->segments = segments;
+    p->segment_chunks = int(ceil_div(ceil_div(a->T, tdc::kChunk), segments));
+    p->seg_s = reinterpret_cast<float*>(seg_s);
+    p->seg_m = reinterpret_cast<float*>(seg_m);
     p->coef = reinterpret_cast<float*>(coef);
     p->um = reinterpret_cast<__nv_bfloat16*>(um);
     p->xm = reinterpret_cast<__nv_bfloat16*>(xm);
@@ -393,28 +421,44 @@ int delta_prepare(const tdc::DeltaParams& p, cudaStream_t st) {
   return launched();
 }
 
-// One block for 128 value channels of a head of a sequence.
+// `blocks` blocks for each head: 128 value channels of a sequence (or segment) each.
 template <class E, int DK, class Kernel>
-int delta_walk(Kernel* k, const tdc::DeltaParams& p, cudaStream_t st) {
+int delta_walk(Kernel* k, const tdc::DeltaParams& p, int64_t blocks, cudaStream_t st) {
   if (p.seq.n == 0) return TDC_OK;
   const size_t smem = 2 * tdc::WalkTiles<E, DK>::stage + sizeof(tdc::WalkSync);
   const int rc = allow_smem(k, smem);
   if (rc != TDC_OK) return rc;
-  k<<<dim3(unsigned(p.seq.n * ceil_div(p.V, 128)), unsigned(p.HV)), tdc::kWalkThreads, smem, st>>>(p);
+  k<<<dim3(unsigned(blocks), unsigned(p.HV)), tdc::kWalkThreads, smem, st>>>(p);
   return launched();
 }
 
 template <class E, int DK>
-int delta_fwd_t(const tdc::DeltaParams& p, cudaStream_t st) {
-  const int rc = delta_prepare<E, DK>(p, st);
-  return rc != TDC_OK ? rc : delta_walk<E, DK>(&tdc::delta_walk_kernel<E, DK, 0>, p, st);
+int delta_fwd_t(tdc::DeltaParams& p, cudaStream_t st) {
+  int rc = delta_prepare<E, DK>(p, st);
+  if (rc != TDC_OK) return rc;
+  auto* k = &tdc::delta_walk_kernel<E, DK, 0>;
+  const int64_t tiles = ceil_div(p.V, 128);
+  if (p.segments <= 1) return delta_walk<E, DK>(k, p, p.seq.n * tiles, st);
+  const int64_t inner = p.segments - 2;
+  p.pass = 1;
+  rc = delta_walk<E, DK>(k, p, p.seq.n * (tiles * (1 + inner) + inner), st);
+  if (rc != TDC_OK) return rc;
+  const size_t smem = (DK * DK + DK * 32) * sizeof(float);
+  rc = allow_smem(&tdc::delta_join_kernel<DK>, smem);
+  if (rc != TDC_OK) return rc;
+  tdc::delta_join_kernel<DK>
+      <<<dim3(unsigned(p.seq.n * p.HV), unsigned(p.V / 32)), 256, smem, st>>>(p);
+  rc = launched();
+  p.pass = 2;
+  return rc != TDC_OK ? rc : delta_walk<E, DK>(k, p, p.seq.n * tiles * (p.segments - 1), st);
 }
 
 template <class E, int DK>
 int delta_bwd_t(const tdc::DeltaParams& p, cudaStream_t st) {
   int rc = delta_prepare<E, DK>(p, st);
-  if (rc == TDC_OK) rc = delta_walk<E, DK>(&tdc::delta_walk_kernel<E, DK, 1>, p, st);
-  if (rc == TDC_OK) rc = delta_walk<E, DK>(&tdc::delta_walk_back_kernel<E, DK>, p, st);
+  if (rc == TDC_OK) rc = delta_walk<E, DK>(&tdc::delta_walk_kernel<E, DK, 1>, p, p.seq.n * ceil_div(p.V, 128), st);
+  if (rc == TDC_OK)
+    rc = delta_walk<E, DK>(&tdc::delta_walk_back_kernel<E, DK>, p, p.seq.n * ceil_div(p.V, 128), st);
   if (rc != TDC_OK || p.max_chunks == 0) return rc;
   auto* k = &tdc::delta_grad_kernel<E, DK>;
   const size_t smem = tdc::GradSmem<DK>::bytes;
