@@ -128,6 +128,24 @@ def test_inputs_far_behind_32_bits():
     assert torch.equal(S.causal_conv1d(x, w), S.causal_conv1d(x.contiguous(), w))
 
 
+def test_nan_outside_the_sequences_and_in_a_neighbour():
+    cu = [3, 40, 70, 90]
+    c = _case(1, 100, 16, 4, "bf16", True, True, cu)
+    want = _run(c, "silu")
+    bad = {k: t.detach().clone() if isinstance(t, torch.Tensor) else t for k, t in c.items()}
+    for k in ("x", "dy"):
+        bad[k][0, :3] = float("nan")
+        bad[k][0, 90:] = float("nan")
+    got = _run(bad, "silu")                      # rows that no sequence owns are not used
+    for k in want:
+        assert torch.equal(got[k], want[k]), k
+    bad["x"][0, 40:70] = float("nan")
+    got = _run(bad, "silu")
+    for lo, hi in ((0, 40), (70, 100)):          # a sequence's NaN stays its own
+        assert torch.equal(got["y"][0, lo:hi], want["y"][0, lo:hi])
+        assert torch.equal(got["dx"][0, lo:hi], want["dx"][0, lo:hi])
+
+
 def test_infinities_stay_in_their_channel_and_reach():
     x = torch.randn(1, 40, 16, generator=torch.Generator().manual_seed(0)).bfloat16().cuda()
     w = torch.rand(4, 16).bfloat16().cuda() + 0.5

@@ -7,6 +7,10 @@ one after another; unit keys keep their sums from growing, and a factor of 2
 allows for cancellation: 8 * 2^-17 * 2 = 2^-13 of the tensor's largest value,
 plus the output's own rounding.  The recurrent form works in fp32 throughout:
 its sums over K = 128 and a few tokens stay below 2^-18."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -236,6 +240,58 @@ def test_nan_stays_in_its_sequence_and_head():
     clean[0, :, 1, 7] = False                                    # value channels do not mix
     assert torch.equal(got[clean.cuda()], want[clean.cuda()])
     assert torch.isnan(got[0, 64:, 1, 7]).all()
+
+
+@pytest.mark.gpu
+def test_nan_outside_the_sequences_and_in_a_neighbour():
+    # rows that no sequence owns are not read; one sequence's NaN stays its own, also
+    # where it ends inside the next one's first chunk
+    cu = [7, 40, 110, 131]
+    c = _case(1, 140, 1, 2, 64, 64, "bf16", state=True, cu=cu)
+    want = _run(c)
+    bad = {k: t.detach().clone() if isinstance(t, torch.Tensor) else t for k, t in c.items()}
+    for k in ("q", "k", "v", "g", "beta", "do"):
+        bad[k][0, :7] = float("nan")
+        bad[k][0, 131:] = float("nan")
+        bad[k][0, 40:110] = float("nan")
+    got = _run(bad)
+    for k in ("o", "dq", "dk", "dv", "dg", "dbeta"):
+        a, b = got[k][0], want[k][0]
+        for lo, hi in ((0, 40), (110, 140)):
+            assert torch.equal(a[lo:hi], b[lo:hi]), k
+    for k in ("final", "dstate"):
+        assert torch.equal(got[k][[0, 2]], want[k][[0, 2]]), k
+
+
+@pytest.mark.gpu
+def test_first_call_of_a_process_inside_a_capture():
+    code = """
+import sys; sys.path.insert(0, %r)
+import torch, tdc_sequence as S
+q = torch.randn(1, 100, 1, 64, device="cuda").bfloat16() / 8
+v = torch.randn(1, 100, 1, 64, device="cuda").bfloat16()
+g, b = -torch.rand(1, 100, 1, device="cuda"), torch.rand(1, 100, 1, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    o = S.gated_delta_rule(q, q, v, g, b)
+    x = S.causal_conv1d(v.flatten(2), torch.ones(4, 64, device="cuda").bfloat16(), activation="silu")
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(o, S.gated_delta_rule(q, q, v, g, b)) and torch.isfinite(x).all()
+""" % os.path.dirname(S.__file__)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.gpu
+def test_no_second_derivatives():
+    c = _case(1, 20, 1, 1, 64, 64)
+    q, k, v, g, b = (c[n].cuda().requires_grad_() for n in ("q", "k", "v", "g", "beta"))
+    o = S.gated_delta_rule(q, k, v, g, b)
+    d, = torch.autograd.grad(o.float().square().sum(), v, create_graph=True)
+    with pytest.raises(RuntimeError):
+        d.float().sum().backward()
 
 
 @pytest.mark.gpu

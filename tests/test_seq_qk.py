@@ -75,7 +75,7 @@ def test_head_sizes(D, rotary, interleaved):
 
 
 @pytest.mark.parametrize("B,T,H,HK", [(1, 1, 1, 1), (3, 1, 32, 8), (1, 300, 4, 4), (2, 9, 5, 0),
-                                      (2, 9, 0, 7), (1, 1300, 1, 1)])
+                                      (2, 9, 0, 7), (1, 1300, 1, 1), (2, 3, 0, 0)])
 def test_heads_and_lengths(B, T, H, HK):
     c = _case(B, T, H, HK, 64, 32, "bf16", True, None, seed=T)
     _check(_run(c, "rms", False), _want(c, "rms", False))

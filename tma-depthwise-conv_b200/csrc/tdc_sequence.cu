@@ -230,7 +230,7 @@ int qk_lanes(int64_t D) { return D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32;
 // does once (places, the angle) is spread over several.
 int qk_threads(const tdc_qk_args* a, int64_t heads) {
   const int64_t want = ceil_div(a->Hq + a->Hk, heads) * qk_lanes(a->D);
-  return int(std::min<int64_t>(256, ceil_div(want, 32) * 32));
+  return int(std::min<int64_t>(256, std::max<int64_t>(1, ceil_div(want, 32)) * 32));
 }
 
 // Blocks of the gradient kernel: 4 on each of 148 SMs, or one for each row.

@@ -35,6 +35,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor, nn
+from torch.autograd.function import once_differentiable
 
 import _tma_dwconv_C as _C  # type: ignore
 
@@ -78,6 +79,7 @@ class _Conv1dFunction(torch.autograd.Function):
         return y, final
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dfinal):
         x, w, bias, initial_state, cu = ctx.saved_tensors
         if dy is None:
@@ -249,6 +251,7 @@ class _QkFunction(torch.autograd.Function):
         return qo, ko
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dqo, dko):
         q, k, qw, kw, cos, sin, positions = ctx.saved_tensors
         if dqo is None and dko is None:
@@ -350,6 +353,7 @@ class _DeltaFunction(torch.autograd.Function):
         return o, final
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_o, dfinal):
         q, k, v, g, beta, initial_state, cu = ctx.saved_tensors
         if d_o is None:
