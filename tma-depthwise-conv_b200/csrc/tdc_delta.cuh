@@ -61,6 +61,7 @@ struct DeltaParams {
   // (32 channels together: [V / 32][2 parts][columns / 8][32][8])
   __nv_bfloat16* um;      // U^T, 64 columns
   __nv_bfloat16* xm;      // dX^T
+  __nv_bfloat16* om;      // dO^T (bf16: one part)
   __nv_bfloat16* sm;      // S^T before the chunk, K columns
   __nv_bfloat16* dm;      // dS^T behind the chunk
   const void* d_o;
@@ -345,7 +346,7 @@ __device__ __forceinline__ void store_keys(unsigned char* dst, const unsigned ch
 
 template <class E, int DK>
 __global__ void __launch_bounds__(128) delta_prepare_kernel(const DeltaParams p) {
-  extern __shared__ __align__(16) unsigned char raw[];
+  extern __shared__ __align__(1024) unsigned char raw[];
   using Sm = PrepareSmem<DK>;
   constexpr int ld = Sm::ld, part = Sm::part;
   const int64_t chunk = blockIdx.x;
@@ -469,404 +470,6 @@ __global__ void __launch_bounds__(128) delta_prepare_kernel(const DeltaParams p)
     if (warp < 2) join_inverse<32>(sb + Sm::a, sb + Sm::t, 0, 16 * warp, lane);
     __syncthreads();
     store_lower(p.tp + slot * 4 * kSq, raw + Sm::t, tid, 128);
-  }
-}
-
-// ---- gradients of a chunk ------------------------------------------------------------
-// One block a chunk and key head, all chunks at once.  With D = dO U^T and
-// M = dX U^T (lower parts):
-//   dQ = scale gam (dO S^T) + Dt K                     Dt = scale Gam beta_j D
-//   dK = -gam (dX S^T) + w beta (U dS^T) + Dt^T Q + (N + N^T) K,  N = -M beta_j Gam
-//   dbeta_j = sum_i (P_ij D_ij - M_ij L_ij) + w_j k_j.(U dS^T)_j
-// The decay of row t stands in front of everything that reaches from before t to
-// t or behind it, so with E_ij = beta_j (P_ij D_ij - M_ij L_ij), i > j,
-//   dg_t = sum_{i >= t} (scale gam q.(dO S^T) - gam k.(dX S^T))_i
-//        + sum_{j < t} (w beta k.(U dS^T))_j + sum_{i >= t > j} E_ij + gam_63 <dS, S>:
-// no terms that cancel (a first token without a state gets exactly 0); the
-// double sum grows by the column sum of E and falls by its row sum from row to row.
-// 8 warps: 4 groups of 16 rows by 2 halves of the columns.  The value channels
-// are walked in tiles of 32, of which the next is on its way while one is used,
-// also from one head to the next, as bulk copies (through the load unit,
-// cp.async, their issue took half of the kernel's time).
-constexpr int kTile = 32;
-template <int DK>
-struct GradSmem {
-  static constexpr int ld = DK + 8;
-  static constexpr int ldo = kTile + 8;
-  static constexpr int q = 0;
-  static constexpr int k = q + kChunk * ld * 2;
-  // a stage: S^T, dS^T, U^T, dX^T in two parts each, [columns / 8][32][8] as in the
-  // workspace, and dO
-  static constexpr int stages = k + kChunk * ld * 2;
-  static constexpr int part = kTile * DK * 2, upart = kTile * kChunk * 2;
-  static constexpr int s = 0;
-  static constexpr int d = s + 2 * part;
-  static constexpr int u = d + 2 * part;
-  static constexpr int x = u + 2 * upart;
-  static constexpr int o = x + 2 * upart;                 // [64][ldo]
-  static constexpr int stage = o + kChunk * ldo * 2;
-  static constexpr int dt = stages + 2 * stage;           // [2][64][72]
-  static constexpr int nn = dt + 2 * kChunk * kLdT * 2;   // [2][64][72]
-  static constexpr int G = nn + 2 * kChunk * kLdT * 2;    // Far [64]
-  static constexpr int coef = G + 64 * 8;                 // [3][64]
-  static constexpr int rows = coef + 3 * 64 * 4;          // [2][4][64]: row sums of both halves
-  static constexpr int cols = rows + 2 * 4 * 64 * 4;      // [4][64]: column sums of the row groups
-  static constexpr int diag = cols + 4 * 64 * 4;          // [64]
-  static constexpr int dot = diag + 64 * 4;               // [8]
-  static constexpr int dg = dot + 8 * 4;                  // [2][64]
-  static constexpr int full = dg + 2 * 64 * 4;            // uint64 [2]
-  static constexpr int bytes = full + 2 * 8;
-};
-
-// Addresses in a [columns / 8][32][8] tile: a B fragment pair with the channels as
-// contraction, and an A fragment (both with .trans); 8 x 8 blocks of 128
-// contiguous bytes, so no bank is hit twice.
-__device__ __forceinline__ uint32_t addr_bt_blocks(uint32_t base, int n0, int k0, int lane) {
-  return base + (n0 / 8 + (lane >> 4)) * (kTile * 16) + (k0 + (lane & 7) + ((lane >> 3) & 1) * 8) * 16;
-}
-__device__ __forceinline__ uint32_t addr_at_blocks(uint32_t base, int m0, int k0, int lane) {
-  return base + (m0 / 8 + ((lane >> 3) & 1)) * (kTile * 16) + (k0 + (lane & 7) + (lane >> 4) * 8) * 16;
-}
-
-template <class E, int DK>
-__global__ void __launch_bounds__(256, 1) delta_grad_kernel(const DeltaParams p) {
-  extern __shared__ __align__(16) unsigned char raw[];
-  using Sm = GradSmem<DK>;
-  constexpr int ld = Sm::ld, NT = DK / 16;  // 8-column tiles of a half of K
-  const int64_t chunk = blockIdx.x;
-  const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int rg = warp & 3, ch = warp >> 2;
-  const ChunkAt at = chunk_at(p, chunk);
-  if (at.rows == 0) return;
-  const uint32_t sb = smem_addr(raw);
-  Far* G = reinterpret_cast<Far*>(raw + Sm::G);
-  float* coef = reinterpret_cast<float*>(raw + Sm::coef);
-  float* rows = reinterpret_cast<float*>(raw + Sm::rows);
-  float* cols = reinterpret_cast<float*>(raw + Sm::cols);
-  float* dot = reinterpret_cast<float*>(raw + Sm::dot);
-  float* diag = reinterpret_cast<float*>(raw + Sm::diag);
-  float* dgs = reinterpret_cast<float*>(raw + Sm::dg);
-  const uint16_t* q = static_cast<const uint16_t*>(p.q) + at.b * p.q_sb + at.t0 * p.q_st + h * p.q_sh;
-  const uint16_t* k = static_cast<const uint16_t*>(p.k) + at.b * p.k_sb + at.t0 * p.k_st + h * p.k_sh;
-  copy_rows(sb + Sm::q, ld, q, p.q_st, kChunk, at.rows, DK / 8, tid, 256);
-  copy_rows(sb + Sm::k, ld, k, p.k_st, kChunk, at.rows, DK / 8, tid, 256);
-  const int g = lane >> 2, t2 = (lane & 3) * 2;
-  const int i0 = 16 * rg + g;        // this thread's rows: i0, i0 + 8
-  const int kc0 = ch * (DK / 2);     // its half of K's columns
-  float dq[NT][4] = {}, dk[NT][4] = {};
-
-  const int per_head = p.V / kTile, tiles = p.group * per_head;
-  uint64_t* full = reinterpret_cast<uint64_t*>(raw + Sm::full);
-  if (tid == 0) {
-    mbar_init(smem_addr(&full[0]), 1);
-    mbar_init(smem_addr(&full[1]), 1);
-    fence_mbar_init();
-  }
-  // Tiles come as four bulk copies, dO's rows through the load unit (one piece a
-  // thread; rows behind the sequence's end become zeros).
-  auto fetch = [&](int tile) {
-    const int head = tile / per_head, v0 = (tile - head * per_head) * kTile;
-    const int hv = h * p.group + head;
-    const uint32_t st = sb + Sm::stages + (tile & 1) * Sm::stage, bar = smem_addr(&full[tile & 1]);
-    if (tid == 0) {
-      const int64_t at32 = ((chunk * p.HV + hv) * p.V + v0) / kTile;
-      mbar_arrive_expect_tx(bar, 4 * Sm::part + 4 * Sm::upart);
-      bulk_load(st + Sm::s, p.sm + at32 * Sm::part, 2 * Sm::part, bar);
-      bulk_load(st + Sm::d, p.dm + at32 * Sm::part, 2 * Sm::part, bar);
-      bulk_load(st + Sm::u, p.um + at32 * Sm::upart, 2 * Sm::upart, bar);
-      bulk_load(st + Sm::x, p.xm + at32 * Sm::upart, 2 * Sm::upart, bar);
-    }
-    const uint16_t* d_o = static_cast<const uint16_t*>(p.d_o) + at.b * p.do_sb + at.t0 * p.do_st +
-                          hv * p.do_sh + v0;
-    copy_rows(st + Sm::o, Sm::ldo, d_o, p.do_st, kChunk, at.rows, kTile / 8, tid, 256);
-    cp_async_commit();
-  };
-  __syncthreads();
-  fetch(0);  // (Q and K go with its group)
-
-  for (int gi = 0; gi < p.group; ++gi) {
-    const int hv = h * p.group + gi;
-    const int64_t slot = chunk * p.HV + hv;
-    float os[NT][4] = {}, xs[NT][4] = {}, us[NT][4] = {}, D[4][4] = {}, M[4][4] = {};
-    float dsum = 0.f;
-    for (int vt = 0; vt < per_head; ++vt) {
-      const int tile = gi * per_head + vt;
-      __syncthreads();  // the other stage (and with a new head what is kept for one) is free
-      if (tile + 1 < tiles) fetch(tile + 1);
-      if (vt == 0) {
-        if (warp == 0) chunk_decay(load_decay(p, at, hv, lane), G, lane);
-        const float* src = p.coef + slot * 3 * kChunk;
-        if (tid >= 64) coef[tid - 64] = src[tid - 64];
-      }
-      if (tile + 1 < tiles) cp_async_wait<1>(); else cp_async_wait<0>();
-      // A copy that does not come ends the block (all its threads together).
-      const bool ok = mbar_wait_bounded(smem_addr(&full[tile & 1]), uint32_t(tile >> 1) & 1u, nullptr,
-                                        false, p.timeout_ns);
-      if (!ok && tid == 0)
-        record_wait_failure(p.status_words, p.status_host, TDC_DEVICE_FULL_TIMEOUT, int(blockIdx.x),
-                            tile & 1, tile);
-      if (!__syncthreads_and(ok)) {
-        // the next tile's copies, if any are on their way, come to rest first
-        if (tile + 1 < tiles)
-          mbar_wait_bounded(smem_addr(&full[(tile + 1) & 1]), uint32_t((tile + 1) >> 1) & 1u, nullptr,
-                            false, p.timeout_ns);
-        return;
-      }
-      const unsigned char* stage = raw + Sm::stages + (tile & 1) * Sm::stage;
-      const uint32_t st = smem_addr(stage);
-      // <dS, S>
-      for (int e = tid; e < kTile * DK / 8; e += 256) {  // 8 values at the same place of all four
-        float a[2][8], b[2][8];
-#pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          const int off = part * Sm::part + 16 * e;
-          unpack8<BF16>(*reinterpret_cast<const uint4*>(stage + Sm::s + off), a[part]);
-          unpack8<BF16>(*reinterpret_cast<const uint4*>(stage + Sm::d + off), b[part]);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) dsum = fmaf(a[0][i] + a[1][i], b[0][i] + b[1][i], dsum);
-      }
-#pragma unroll 1
-      for (int ks = 0; ks < kTile / 16; ++ks) {
-        uint32_t a[4], oh[4], ol[4], xh[4], xl[4], uh[4], ul[4];
-        ldsm4(a, addr_a(st + Sm::o, Sm::ldo, 16 * rg, 16 * ks, lane));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) split_elem<E>(a[i], oh[i], ol[i]);
-        ldsm4_t(xh, addr_at_blocks(st + Sm::x, 16 * rg, 16 * ks, lane));
-        ldsm4_t(xl, addr_at_blocks(st + Sm::x + Sm::upart, 16 * rg, 16 * ks, lane));
-        ldsm4_t(uh, addr_at_blocks(st + Sm::u, 16 * rg, 16 * ks, lane));
-        ldsm4_t(ul, addr_at_blocks(st + Sm::u + Sm::upart, 16 * rg, 16 * ks, lane));
-        // D and M: columns are tokens 32 ch .. + 31, from U^T [channel][token]
-        {
-          uint32_t bh[8], bl[8];
-#pragma unroll
-          for (int np = 0; np < 2; ++np) {
-            ldsm4_t(bh + 4 * np, addr_bt_blocks(st + Sm::u, 32 * ch + 16 * np, 16 * ks, lane));
-            ldsm4_t(bl + 4 * np, addr_bt_blocks(st + Sm::u + Sm::upart, 32 * ch + 16 * np, 16 * ks, lane));
-          }
-          if (32 * ch + 16 <= 16 * rg) {  // all four tiles reach below the diagonal
-            mma_elem_split_n<E, 4>(D, oh, ol, bh, bl);
-            mma_split_n<4>(M, xh, xl, bh, bl);
-          } else if (32 * ch <= 16 * rg) {
-            mma_elem_split_n<E, 2>(D, oh, ol, bh, bl);
-            mma_split_n<2>(M, xh, xl, bh, bl);
-          }
-        }
-        // dO S^T, dX S^T, U dS^T: columns kc0 .. of K, from S^T [channel][K], 32 at a time
-#pragma unroll
-        for (int nq = 0; nq < NT / 4; ++nq) {
-          uint32_t bh[8], bl[8];
-#pragma unroll
-          for (int np = 0; np < 2; ++np) {
-            ldsm4_t(bh + 4 * np, addr_bt_blocks(st + Sm::s, kc0 + 32 * nq + 16 * np, 16 * ks, lane));
-            ldsm4_t(bl + 4 * np, addr_bt_blocks(st + Sm::s + Sm::part, kc0 + 32 * nq + 16 * np, 16 * ks, lane));
-          }
-          mma_elem_split_n<E, 4>(os + 4 * nq, oh, ol, bh, bl);
-          mma_split_n<4>(xs + 4 * nq, xh, xl, bh, bl);
-#pragma unroll
-          for (int np = 0; np < 2; ++np) {
-            ldsm4_t(bh + 4 * np, addr_bt_blocks(st + Sm::d, kc0 + 32 * nq + 16 * np, 16 * ks, lane));
-            ldsm4_t(bl + 4 * np, addr_bt_blocks(st + Sm::d + Sm::part, kc0 + 32 * nq + 16 * np, 16 * ks, lane));
-          }
-          mma_split_n<4>(us + 4 * nq, uh, ul, bh, bl);
-        }
-      }
-    }
-    // Row sums with q and k, and the three products into dq and dk.
-    float r[2][3] = {};  // [row i0 / i0 + 8][q.dOS, k.dXS, k.UdS]
-    const float ga[2] = {coef[i0], coef[i0 + 8]};
-    const float wb[2] = {coef[64 + i0] * coef[128 + i0], coef[64 + i0 + 8] * coef[128 + i0 + 8]};
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int off = 2 * ((i0 + 8 * half) * ld + kc0 + 8 * nt + t2);
-        float qv[2], kv[2];
-        unpack2<E>(*reinterpret_cast<const uint32_t*>(raw + Sm::q + off), qv[0], qv[1]);
-        unpack2<E>(*reinterpret_cast<const uint32_t*>(raw + Sm::k + off), kv[0], kv[1]);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int e = 2 * half + u;
-          r[half][0] = fmaf(qv[u], os[nt][e], r[half][0]);
-          r[half][1] = fmaf(kv[u], xs[nt][e], r[half][1]);
-          r[half][2] = fmaf(kv[u], us[nt][e], r[half][2]);
-          dq[nt][e] = fmaf(p.scale * ga[half], os[nt][e], dq[nt][e]);
-          dk[nt][e] += wb[half] * us[nt][e] - ga[half] * xs[nt][e];
-        }
-      }
-    // Q K^T and K K^T once more, for this warp's 16 x 32 part.
-    float qk[4][4] = {}, kk[4][4] = {};
-#pragma unroll 2
-    for (int ks = 0; ks < DK / 16; ++ks) {
-      uint32_t aq[4], ak[4];
-      ldsm4(aq, addr_a(sb + Sm::q, ld, 16 * rg, 16 * ks, lane));
-      ldsm4(ak, addr_a(sb + Sm::k, ld, 16 * rg, 16 * ks, lane));
-#pragma unroll
-      for (int np = 0; np < 2; ++np) {
-        uint32_t b[4];
-        ldsm4(b, addr_b(sb + Sm::k, ld, 32 * ch + 16 * np, 16 * ks, lane));
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          mma_elem<E>(qk[2 * np + i], aq, b[2 * i], b[2 * i + 1]);
-          mma_elem<E>(kk[2 * np + i], ak, b[2 * i], b[2 * i + 1]);
-        }
-      }
-    }
-    float re[2] = {};  // row sums of E below the diagonal
-#pragma unroll
-    for (int nt = 0; nt < 4; ++nt) {
-      float cs[2] = {};  // column sums of P D - M L below the diagonal, this thread's two rows
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int i = i0 + 8 * half, j = 32 * ch + 8 * nt + t2;
-        float dt[2], nn[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int e = 2 * half + u;
-          const float gam = i >= j + u ? __expf(minus(G[i], G[j + u])) : 0.f;
-          const float be = coef[128 + j + u];
-          const float dv = i >= j + u ? D[nt][e] : 0.f, mv = i > j + u ? M[nt][e] : 0.f;
-          const float pd = p.scale * gam * qk[nt][e] * dv, ml = gam * kk[nt][e] * mv;
-          if (i > j + u) {
-            cs[u] += pd - ml;
-            re[half] = fmaf(be, pd - ml, re[half]);
-          } else if (i == j + u) {
-            diag[i] = pd;
-          }
-          dt[u] = p.scale * gam * be * dv;
-          nn[u] = -mv * be * gam;
-        }
-        uint32_t hi, lo;
-        const int off = 2 * (i * kLdT + j);
-        split2(dt[0], dt[1], hi, lo);
-        *reinterpret_cast<uint32_t*>(raw + Sm::dt + off) = hi;
-        *reinterpret_cast<uint32_t*>(raw + Sm::dt + 64 * kLdT * 2 + off) = lo;
-        split2(nn[0], nn[1], hi, lo);
-        *reinterpret_cast<uint32_t*>(raw + Sm::nn + off) = hi;
-        *reinterpret_cast<uint32_t*>(raw + Sm::nn + 64 * kLdT * 2 + off) = lo;
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) {
-          cs[u] += __shfl_xor_sync(0xffffffffu, cs[u], d);
-        }
-        if (g == 0) cols[rg * 64 + 32 * ch + 8 * nt + t2 + u] = cs[u];
-      }
-    }
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-#pragma unroll
-      for (int d = 1; d < 4; d <<= 1) {
-        re[half] += __shfl_xor_sync(0xffffffffu, re[half], d);
-#pragma unroll
-        for (int j = 0; j < 3; ++j) r[half][j] += __shfl_xor_sync(0xffffffffu, r[half][j], d);
-      }
-      if ((lane & 3) == 0) {
-#pragma unroll
-        for (int j = 0; j < 3; ++j) rows[(ch * 4 + j) * 64 + i0 + 8 * half] = r[half][j];
-        rows[(ch * 4 + 3) * 64 + i0 + 8 * half] = re[half];
-      }
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) dsum += __shfl_xor_sync(0xffffffffu, dsum, d);
-    if (lane == 0) dot[warp] = dsum;
-    __syncthreads();
-    // dq += Dt K; dk += Dt^T Q + (N + N^T) K
-#pragma unroll 1
-    for (int ks = 0; ks < 4; ++ks) {
-      uint32_t ah[4], al[4], nh[4], nl[4];
-      constexpr int part = kChunk * kLdT * 2;
-      if (ks <= rg) {
-        ldsm4(ah, addr_a(sb + Sm::dt, kLdT, 16 * rg, 16 * ks, lane));
-        ldsm4(al, addr_a(sb + Sm::dt + part, kLdT, 16 * rg, 16 * ks, lane));
-        ldsm4(nh, addr_a(sb + Sm::nn, kLdT, 16 * rg, 16 * ks, lane));
-        ldsm4(nl, addr_a(sb + Sm::nn + part, kLdT, 16 * rg, 16 * ks, lane));
-#pragma unroll
-        for (int nq = 0; nq < NT / 4; ++nq) {
-          uint32_t b[8];
-#pragma unroll
-          for (int np = 0; np < 2; ++np)
-            ldsm4_t(b + 4 * np, addr_bt(sb + Sm::k, ld, kc0 + 32 * nq + 16 * np, 16 * ks, lane));
-          mma_split_elem_n<E, 4>(dq + 4 * nq, ah, al, b);
-          mma_split_elem_n<E, 4>(dk + 4 * nq, nh, nl, b);
-        }
-      }
-      if (ks >= rg) {
-        ldsm4_t(ah, addr_at(sb + Sm::dt, kLdT, 16 * rg, 16 * ks, lane));
-        ldsm4_t(al, addr_at(sb + Sm::dt + part, kLdT, 16 * rg, 16 * ks, lane));
-        ldsm4_t(nh, addr_at(sb + Sm::nn, kLdT, 16 * rg, 16 * ks, lane));
-        ldsm4_t(nl, addr_at(sb + Sm::nn + part, kLdT, 16 * rg, 16 * ks, lane));
-#pragma unroll
-        for (int nq = 0; nq < NT / 4; ++nq) {
-          uint32_t b[8], c[8];
-#pragma unroll
-          for (int np = 0; np < 2; ++np) {
-            ldsm4_t(b + 4 * np, addr_bt(sb + Sm::q, ld, kc0 + 32 * nq + 16 * np, 16 * ks, lane));
-            ldsm4_t(c + 4 * np, addr_bt(sb + Sm::k, ld, kc0 + 32 * nq + 16 * np, 16 * ks, lane));
-          }
-          mma_split_elem_n<E, 4>(dk + 4 * nq, ah, al, b);
-          mma_split_elem_n<E, 4>(dk + 4 * nq, nh, nl, c);
-        }
-      }
-    }
-    // dbeta and dg
-    if (tid < 64) {
-      const int i = tid;
-      const float ga1 = coef[i], w1 = coef[64 + i], be = coef[128 + i];
-      float s0[4], c0 = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s0[j] = rows[j * 64 + i] + rows[(4 + j) * 64 + i];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) c0 += cols[j * 64 + i];
-      if (i < at.rows) {
-        const int64_t o = (at.b * p.T + at.t0 + i) * p.HV + hv;
-        const float db = c0 + diag[i] + w1 * s0[2];
-        if (p.beta_f32) static_cast<float*>(p.dbeta)[o] = db;
-        else store_float<E>(p.dbeta, o, db);
-      }
-      dgs[i] = p.scale * ga1 * s0[0] - ga1 * s0[1];
-      dgs[64 + i] = be * c0 - s0[3] + w1 * be * s0[2];
-    }
-    __syncthreads();
-    if (warp == 0) {
-      float ds = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ds += dot[i];
-      ds *= coef[63];
-      // sums from the row to the end, and over the rows before it
-      const float a0 = dgs[2 * lane], a1 = dgs[2 * lane + 1];
-      const float f0 = dgs[64 + 2 * lane], f1 = dgs[64 + 2 * lane + 1];
-      float up = a0 + a1, down = f0 + f1;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const float x = __shfl_down_sync(0xffffffffu, up, d);
-        const float y = __shfl_up_sync(0xffffffffu, down, d);
-        if (lane + d < 32) up += x;
-        if (lane >= d) down += y;
-      }
-      const float above = __shfl_down_sync(0xffffffffu, up, 1);
-      float before = __shfl_up_sync(0xffffffffu, down, 1);
-      if (lane == 0) before = 0.f;
-      const int64_t o = (at.b * p.T + at.t0 + 2 * lane) * p.HV + hv;
-      if (2 * lane < at.rows) p.dg[o] = up + before + ds;
-      if (2 * lane + 1 < at.rows)
-        p.dg[o + p.HV] = a1 + (lane < 31 ? above : 0.f) + before + f0 + ds;
-    }
-  }
-  // dq and dk rows
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int i = i0 + 8 * half;
-    if (i >= at.rows) continue;
-    const int64_t o = ((at.b * p.T + at.t0 + i) * p.H + h) * DK + kc0 + t2;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.dq) + o + 8 * nt) =
-          pack2_rn<E>(dq[nt][2 * half], dq[nt][2 * half + 1]);
-      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.dk) + o + 8 * nt) =
-          pack2_rn<E>(dk[nt][2 * half], dk[nt][2 * half + 1]);
-    }
   }
 }
 

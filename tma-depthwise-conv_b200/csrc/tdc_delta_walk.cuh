@@ -379,48 +379,48 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
     if (warp == 9 && lane == 0) walk_fetch<E, DK, MODE == 1>(p, raw, sy, wait, s, chunks, h, hv, false);
     if (warp == 8) {
-    for (int c = 0; c < chunks; ++c) {
-      const uint32_t st = smem_addr(raw) + (c & 1) * W::stage;
-      if (!warp_wait(wait, sy->full[c & 1], c >> 1) || !warp_wait(wait, sy->sr, c)) break;
-      tc_fence_after();
-      if (elect_one()) {
-        issue_product<DK, 64, false, KP>(tm + cY, tm + cS, sStep, st + W::k, W::keys, false);
-        tc_commit(smem_addr(&sy->y));
-      }
-      __syncwarp();
-      if (!warp_wait(wait, sy->xr, c)) break;
-      tc_fence_after();
-      if (elect_one()) {
-        issue_lower<false, 2>(tm + cY, tm + cX, xStep, st + W::t, false);
-        tc_commit(smem_addr(&sy->u));
-        if constexpr (MODE == 0) {
-          issue_product<DK, 64, false, KP>(tm + cO, tm + cS, sStep, st + W::q, W::keys, false);
-          tc_commit(smem_addr(&sy->q));
-        }
-      }
-      __syncwarp();
-      if (!warp_wait(wait, sy->vr, c)) break;
-      tc_fence_after();
-      if (elect_one()) {
-        issue_product<kChunk, DK, true, KP>(tm + cS, tm + cX, xStep, st + W::k, W::keys, false);
-        tc_commit(smem_addr(&sy->s));
-        if constexpr (MODE == 1) tc_commit(smem_addr(&sy->free[c & 1]));
-      }
-      __syncwarp();
-      if constexpr (MODE == 0) {
-        if (!warp_wait(wait, sy->qr, c)) break;
+      for (int c = 0; c < chunks; ++c) {
+        const uint32_t st = smem_addr(raw) + (c & 1) * W::stage;
+        if (!warp_wait(wait, sy->full[c & 1], c >> 1) || !warp_wait(wait, sy->sr, c)) break;
         tc_fence_after();
         if (elect_one()) {
-          issue_lower<false, 2>(tm + cO, tm + cV, xStep, st + W::p, false);
-          tc_commit(smem_addr(&sy->o));
-          tc_commit(smem_addr(&sy->free[c & 1]));
+          issue_product<DK, 64, false, KP>(tm + cY, tm + cS, sStep, st + W::k, W::keys, false);
+          tc_commit(smem_addr(&sy->y));
         }
         __syncwarp();
+        if (!warp_wait(wait, sy->xr, c)) break;
+        tc_fence_after();
+        if (elect_one()) {
+          issue_lower<false, 2>(tm + cY, tm + cX, xStep, st + W::t, false);
+          tc_commit(smem_addr(&sy->u));
+          if constexpr (MODE == 0) {
+            issue_product<DK, 64, false, KP>(tm + cO, tm + cS, sStep, st + W::q, W::keys, false);
+            tc_commit(smem_addr(&sy->q));
+          }
+        }
+        __syncwarp();
+        if (!warp_wait(wait, sy->vr, c)) break;
+        tc_fence_after();
+        if (elect_one()) {
+          issue_product<kChunk, DK, true, KP>(tm + cS, tm + cX, xStep, st + W::k, W::keys, false);
+          tc_commit(smem_addr(&sy->s));
+          if constexpr (MODE == 1) tc_commit(smem_addr(&sy->free[c & 1]));
+        }
+        __syncwarp();
+        if constexpr (MODE == 0) {
+          if (!warp_wait(wait, sy->qr, c)) break;
+          tc_fence_after();
+          if (elect_one()) {
+            issue_lower<false, 2>(tm + cO, tm + cV, xStep, st + W::p, false);
+            tc_commit(smem_addr(&sy->o));
+            tc_commit(smem_addr(&sy->free[c & 1]));
+          }
+          __syncwarp();
+        }
       }
-    }
-    if (elect_one()) tc_commit(smem_addr(&sy->drain));
-    __syncwarp();
-    mbar_wait_bounded(smem_addr(&sy->drain), 0, wait.abort, false, wait.timeout_ns);
+      if (elect_one()) tc_commit(smem_addr(&sy->drain));
+      __syncwarp();
+      mbar_wait_bounded(smem_addr(&sy->drain), 0, wait.abort, false, wait.timeout_ns);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWalkRegs));
@@ -605,7 +605,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
 // The walk back:
 //   dV' = P^T dO + w (K dS)        dX = T^T (beta dV')  (= dV)
 //   dS <- gam_63 dS + scale Q^T (gam dO) - K^T (gam dX)
-// with dS^T in the lanes.  dS behind each chunk and dX go to the workspace.
+// with dS^T in the lanes.  dS behind each chunk, dX and dO^T go to the workspace.
 template <class E, int DK>
 __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const DeltaParams p) {
   extern __shared__ __align__(1024) unsigned char raw[];
@@ -631,44 +631,44 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
     if (warp == 9 && lane == 0) walk_fetch<E, DK, false>(p, raw, sy, wait, s, chunks, h, hv, true);
     if (warp == 8) {
-    for (int c = 0; c < chunks; ++c) {
-      const uint32_t st = smem_addr(raw) + (c & 1) * W::stage;
-      if (!warp_wait(wait, sy->full[c & 1], c >> 1) || !warp_wait(wait, sy->gr, c)) break;
-      tc_fence_after();
-      if (elect_one()) issue_lower<true, KP>(tm + cP, tm + cO, xStep, st + W::p, false);
-      __syncwarp();
-      if (!warp_wait(wait, sy->sr, c)) break;
-      tc_fence_after();
-      if (elect_one()) {
-        issue_product<DK, 64, false, KP>(tm + cY, tm + cS, sStep, st + W::k, W::keys, false);
-        tc_commit(smem_addr(&sy->y));
+      for (int c = 0; c < chunks; ++c) {
+        const uint32_t st = smem_addr(raw) + (c & 1) * W::stage;
+        if (!warp_wait(wait, sy->full[c & 1], c >> 1) || !warp_wait(wait, sy->gr, c)) break;
+        tc_fence_after();
+        if (elect_one()) issue_lower<true, KP>(tm + cP, tm + cO, xStep, st + W::p, false);
+        __syncwarp();
+        if (!warp_wait(wait, sy->sr, c)) break;
+        tc_fence_after();
+        if (elect_one()) {
+          issue_product<DK, 64, false, KP>(tm + cY, tm + cS, sStep, st + W::k, W::keys, false);
+          tc_commit(smem_addr(&sy->y));
+        }
+        __syncwarp();
+        // (K dS comes first and has read dS^T's parts: the update may take their place)
+        if (!warp_wait(wait, sy->y, c) || !warp_wait(wait, sy->qr, c)) break;
+        tc_fence_after();
+        if (elect_one())
+          issue_product<kChunk, DK, true, KP>(tm + cS, tm + cG, xStep, st + W::q, W::keys, false);
+        __syncwarp();
+        if (!warp_wait(wait, sy->xr, c)) break;
+        tc_fence_after();
+        if (elect_one()) {
+          issue_lower<true, 2>(tm + cY, tm + cX, xStep, st + W::t, false);
+          tc_commit(smem_addr(&sy->u));
+        }
+        __syncwarp();
+        if (!warp_wait(wait, sy->vr, c)) break;
+        tc_fence_after();
+        if (elect_one()) {
+          issue_product<kChunk, DK, true, KP>(tm + cS, tm + cX, xStep, st + W::k, W::keys, true);
+          tc_commit(smem_addr(&sy->s));
+          tc_commit(smem_addr(&sy->free[c & 1]));
+        }
+        __syncwarp();
       }
+      if (elect_one()) tc_commit(smem_addr(&sy->drain));
       __syncwarp();
-      // (K dS comes first and has read dS^T's parts: the update may take their place)
-      if (!warp_wait(wait, sy->y, c) || !warp_wait(wait, sy->qr, c)) break;
-      tc_fence_after();
-      if (elect_one())
-        issue_product<kChunk, DK, true, KP>(tm + cS, tm + cG, xStep, st + W::q, W::keys, false);
-      __syncwarp();
-      if (!warp_wait(wait, sy->xr, c)) break;
-      tc_fence_after();
-      if (elect_one()) {
-        issue_lower<true, 2>(tm + cY, tm + cX, xStep, st + W::t, false);
-        tc_commit(smem_addr(&sy->u));
-      }
-      __syncwarp();
-      if (!warp_wait(wait, sy->vr, c)) break;
-      tc_fence_after();
-      if (elect_one()) {
-        issue_product<kChunk, DK, true, KP>(tm + cS, tm + cX, xStep, st + W::k, W::keys, true);
-        tc_commit(smem_addr(&sy->s));
-        tc_commit(smem_addr(&sy->free[c & 1]));
-      }
-      __syncwarp();
-    }
-    if (elect_one()) tc_commit(smem_addr(&sy->drain));
-    __syncwarp();
-    mbar_wait_bounded(smem_addr(&sy->drain), 0, wait.abort, false, wait.timeout_ns);
+      mbar_wait_bounded(smem_addr(&sy->drain), 0, wait.abort, false, wait.timeout_ns);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWalkRegs));
@@ -712,6 +712,11 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
       tmem_st(lanes + cO + t0 / 2, hi);
       if constexpr (KP == 2) tmem_st(lanes + cO + xStep + t0 / 2, lo);
       operand_ready(sy->gr, lane);
+      {
+        __nv_bfloat16* dst = p.om + (slot * p.V + group0) * KP * kChunk + t0 * 32 + lane * 8;
+        store_pairs(dst, hi, live);
+        if constexpr (KP == 2) store_pairs(dst + 32 * kChunk, lo, live);
+      }
       if (c > 0) {
         advance(c - 1);
         if (!ok) break;

@@ -220,23 +220,8 @@ __device__ __forceinline__ void split_frag(const float c0[4], const float c1[4],
   split2(c1[2], c1[3], hi[3], lo[3]);
 }
 
-// c += A B with A split and B exact in the element type.
-template <class E>
-__device__ __forceinline__ void mma_split_elem(float c[4], const uint32_t ah[4],
-                                               const uint32_t al[4], uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same_v<E, BF16>) {
-    mma_bf16(c, ah, b0, b1);
-    mma_bf16(c, al, b0, b1);
-  } else {
-    uint32_t h0, l0, h1, l1;
-    split_elem<E>(b0, h0, l0);
-    split_elem<E>(b1, h1, l1);
-    mma_bf16(c, ah, h0, h1);
-    mma_bf16(c, al, h0, h1);
-    mma_bf16(c, ah, l0, l1);
-  }
-}
-// Both split (the product of the two remainders is below the others' rounding).
+// c += A B, both split (the product of the two remainders is below the others'
+// rounding).
 __device__ __forceinline__ void mma_split(float c[4], const uint32_t ah[4], const uint32_t al[4],
                                           uint32_t bh0, uint32_t bh1, uint32_t bl0, uint32_t bl1) {
   mma_bf16(c, ah, bh0, bh1);

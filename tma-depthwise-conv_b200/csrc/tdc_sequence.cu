@@ -8,6 +8,7 @@
 
 #include "tdc_sequence.h"
 #include "tdc_conv1d.cuh"
+#include "tdc_delta_grad.cuh"
 #include "tdc_delta_walk.cuh"
 #include "tdc_host.h"
 #include "tdc_qknorm.cuh"
@@ -350,7 +351,7 @@ int64_t delta_layout(const tdc_delta_args* a, bool grads, unsigned char* base, t
   const int64_t parts = a->dtype == TDC_BF16 ? 1 : 2;
   unsigned char* kq = take(delta_chunks(a) * a->H * 2 * parts * tdc::kChunk * a->K * 2);
   unsigned char* coef = take(slots * 3 * tdc::kChunk * 4);
-  unsigned char *um = nullptr, *xm = nullptr, *sm = nullptr, *dm = nullptr;
+  unsigned char *um = nullptr, *xm = nullptr, *om = nullptr, *sm = nullptr, *dm = nullptr;
   unsigned char *seg_s = nullptr, *seg_m = nullptr;
   const int segments = grads ? 1 : delta_segments(a);
   if (segments > 1) {
@@ -360,6 +361,7 @@ int64_t delta_layout(const tdc_delta_args* a, bool grads, unsigned char* base, t
   if (grads) {
     um = take(slots * 2 * a->V * tdc::kChunk * 2);
     xm = take(slots * 2 * a->V * tdc::kChunk * 2);
+    om = take(slots * parts * a->V * tdc::kChunk * 2);
     sm = take(slots * 2 * a->V * a->K * 2);
     dm = take(slots * 2 * a->V * a->K * 2);
   }
@@ -375,6 +377,7 @@ int64_t delta_layout(const tdc_delta_args* a, bool grads, unsigned char* base, t
     p->coef = reinterpret_cast<float*>(coef);
     p->um = reinterpret_cast<__nv_bfloat16*>(um);
     p->xm = reinterpret_cast<__nv_bfloat16*>(xm);
+    p->om = reinterpret_cast<__nv_bfloat16*>(om);
     p->sm = reinterpret_cast<__nv_bfloat16*>(sm);
     p->dm = reinterpret_cast<__nv_bfloat16*>(dm);
   }
@@ -461,7 +464,7 @@ int delta_bwd_t(const tdc::DeltaParams& p, cudaStream_t st) {
     rc = delta_walk<E, DK>(&tdc::delta_walk_back_kernel<E, DK>, p, p.seq.n * ceil_div(p.V, 128), st);
   if (rc != TDC_OK || p.max_chunks == 0) return rc;
   auto* k = &tdc::delta_grad_kernel<E, DK>;
-  const size_t smem = tdc::GradSmem<DK>::bytes;
+  const size_t smem = tdc::GradSmem<E, DK>::sync + sizeof(tdc::GradSync);
   rc = allow_smem(k, smem);
   if (rc != TDC_OK) return rc;
   k<<<dim3(unsigned(p.max_chunks), unsigned(p.H)), 256, smem, st>>>(p);

@@ -96,10 +96,19 @@ __device__ __forceinline__ uint32_t tile_desc(uint32_t addr, bool n_major) {
 __host__ __device__ constexpr uint32_t tile_desc_high(bool n_major) {
   return ((n_major ? kColBlock : kRowBlock) >> 4) | 1u << 14;
 }
+// The same for tiles whose 8 x 8 blocks lie `lead` (along the contraction; K-major)
+// and `stride` (along M or N) bytes apart; N-major (or M-major) the other way round
+// in what a block's rows are, not in the words: lead is along the contraction.
+__device__ __forceinline__ uint32_t block_desc(uint32_t addr, uint32_t lead) {
+  return (addr >> 4) | (lead >> 4) << 16;
+}
+__host__ __device__ constexpr uint32_t block_desc_high(uint32_t stride) {
+  return (stride >> 4) | 1u << 14;
+}
 // bf16 operands, fp32 accumulators, M = 128.
-__device__ __forceinline__ uint32_t mma_desc(uint32_t n, bool n_major) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(n_major) << 16) | ((n >> 3) << 17) |
-         ((128u >> 4) << 24);
+__device__ __forceinline__ uint32_t mma_desc(uint32_t n, bool n_major, bool m_major = false) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(m_major) << 15) | (uint32_t(n_major) << 16) |
+         ((n >> 3) << 17) | ((128u >> 4) << 24);
 }
 // d[128 x N] (+)= a[128 x 16] b[16 x N]; one thread issues it.
 __device__ __forceinline__ void tc_mma(uint32_t d, uint32_t a, uint32_t b_low, uint32_t b_high,
@@ -114,6 +123,25 @@ __device__ __forceinline__ void tc_mma(uint32_t d, uint32_t a, uint32_t b_low, u
       "}\n" ::"r"(d),
       "r"(a), "r"(b_low), "r"(b_high), "r"(desc), "r"(uint32_t(accumulate))
       : "memory");
+}
+// The same with A in shared memory.
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint32_t a_low, uint32_t a_high, uint32_t b_low,
+                                          uint32_t b_high, uint32_t desc, bool accumulate) {
+  asm volatile(
+      "{\n"
+      " .reg .pred p;\n"
+      " .reg .b64 a, b;\n"
+      " setp.ne.b32 p, %6, 0;\n"
+      " mov.b64 a, {%1, %2};\n"
+      " mov.b64 b, {%3, %4};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n"
+      "}\n" ::"r"(d),
+      "r"(a_low), "r"(a_high), "r"(b_low), "r"(b_high), "r"(desc), "r"(uint32_t(accumulate))
+      : "memory");
+}
+// What this thread wrote to shared memory, before the products read it.
+__device__ __forceinline__ void fence_proxy_async() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 // One lane of a converged warp, the same one every time.  The products are
 // issued under it in code that the whole warp runs: then their operands stay in
