@@ -27,6 +27,7 @@ namespace tdc {
 constexpr int kChunk = 64;
 constexpr int kLdT = kChunk + 8;     // row of a [64][64] tile in shared memory
 constexpr int kSq = kChunk * kChunk;  // elements of such a tile in the workspace
+constexpr int kTile = 16;  // value channels that lie together in the gradients' workspace
 
 struct DeltaParams {
   const void *q, *k, *v, *beta;
@@ -58,7 +59,7 @@ struct DeltaParams {
   int64_t withhold;       // first chunk of a sequence whose copies never come (-1: none)
   int *status_words, *status_host;
   // gradients
-  // (32 channels together: [V / 32][2 parts][columns / 8][32][8])
+  // (kTile channels together: [V / kTile][2 parts][columns / 8][kTile][8])
   __nv_bfloat16* um;      // U^T, 64 columns
   __nv_bfloat16* xm;      // dX^T
   __nv_bfloat16* om;      // dO^T (bf16: one part)

@@ -47,6 +47,7 @@ struct WalkSync {
   uint64_t full[2], free[2];
   uint64_t y, u, q, s, o;                 // products done
   uint64_t sr, xr, vr, qr, gr;            // operands ready (or results read)
+  uint64_t all;                           // the computing warps are there
   uint64_t drain;
   uint32_t tmem;
   int abort;
@@ -99,11 +100,15 @@ __device__ __forceinline__ void operand_ready(uint64_t& bar, int lane) {
   if (lane == 0) mbar_arrive(smem_addr(&bar));
 }
 
-// The 8 computing warps, between one's TMEM loads and another's stores.
-__device__ __forceinline__ void compute_sync() {
+// The 8 computing warps, between one's TMEM loads and another's stores (a bounded
+// wait as the others: a warp that gave up elsewhere does not come).
+__device__ __forceinline__ bool compute_sync(const Waiter& wait, uint64_t& bar, int phase, int lane) {
   tc_fence_before();
-  asm volatile("bar.sync 1, 256;" ::: "memory");
+  __syncwarp();
+  if (lane == 0) mbar_arrive(smem_addr(&bar));
+  const bool ok = warp_wait(wait, bar, phase);
   tc_fence_after();
+  return ok;
 }
 
 // d[128 x N] (+)= A B; A split in two parts at a, a + astep (columns), B a tile
@@ -154,7 +159,7 @@ __device__ __forceinline__ void walk_setup(WalkSync* sy, int tid, int warp) {
     for (uint64_t* b : {&sy->full[0], &sy->full[1], &sy->free[0], &sy->free[1], &sy->y, &sy->u,
                         &sy->q, &sy->s, &sy->o, &sy->drain})
       mbar_init(smem_addr(b), 1);
-    for (uint64_t* b : {&sy->sr, &sy->xr, &sy->vr, &sy->qr, &sy->gr}) mbar_init(smem_addr(b), 8);
+    for (uint64_t* b : {&sy->sr, &sy->xr, &sy->vr, &sy->qr, &sy->gr, &sy->all}) mbar_init(smem_addr(b), 8);
     sy->abort = 0;
     fence_mbar_init();
   }
@@ -249,14 +254,20 @@ __device__ __forceinline__ float widen(uint32_t raw) {
   else return __half2float(__ushort_as_half(static_cast<unsigned short>(raw)));
 }
 
-// 16 packed pairs (32 tokens or keys) of a channel to the workspace, where 8
-// columns of the warp's 32 channels lie together (16 bytes a channel): its
-// stores are whole lines.
+// Where column `col` (a multiple of 8) of a channel (of all slots') lies in the
+// gradients' workspace: 8 columns of kTile channels together, 16 bytes a channel.
+__device__ __forceinline__ __nv_bfloat16* channel_at(__nv_bfloat16* base, int64_t channel, int parts,
+                                                     int columns, int col) {
+  return base + (channel & ~int64_t(kTile - 1)) * (parts * columns) + (channel & (kTile - 1)) * 8 +
+         col * kTile;
+}
+// 16 packed pairs (32 tokens or keys) of a channel there: a warp's stores are
+// whole lines.
 __device__ __forceinline__ void store_pairs(__nv_bfloat16* dst, const uint32_t (&r)[16], bool live) {
   if (!live) return;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    *reinterpret_cast<uint4*>(dst + i * 32 * 8) =
+    *reinterpret_cast<uint4*>(dst + i * kTile * 8) =
         make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
 }
 
@@ -450,7 +461,6 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
     }
     uint32_t vr[32], hi[16], lo[16];
     const uint32_t vstep = uint32_t(p.v_st * 2), ostep = uint32_t(p.HV * p.V * 2);
-    const int group0 = v0 + 32 * (warp & 3);  // first of the warp's channels
     auto rows_of = [&](int c) {  // of this thread's 32 tokens
       return int(min(int64_t(32), s.len - int64_t(c) * kChunk - t0));
     };
@@ -486,7 +496,9 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
       if (c > 0) {
         advance(c - 1);
         if (!ok) break;
-        compute_sync();  // the update lies where S^T's parts go: everyone has read it first
+        // the update lies where S^T's parts go: everyone has read it first
+        ok = compute_sync(wait, sy->all, c - 1, lane);
+        if (!ok) break;
       }
 #pragma unroll
       for (int x = 0; x < DK / 64; ++x) {
@@ -495,10 +507,9 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         for (int i = 0; i < 32; ++i) w[i] = S[32 * x + i];
         split_to_tmem(w, lanes + cS + half * (DK / 4) + 16 * x, sStep, hi, lo);
         if constexpr (MODE == 1) {
-          __nv_bfloat16* dst = p.sm + (slot * p.V + group0) * 2 * DK +
-                               (half * (DK / 16) + 4 * x) * 32 * 8 + lane * 8;
+          __nv_bfloat16* dst = channel_at(p.sm, slot * p.V + ch, 2, DK, half * (DK / 2) + 32 * x);
           store_pairs(dst, hi, live);
-          store_pairs(dst + 32 * DK, lo, live);
+          store_pairs(dst + kTile * DK, lo, live);
         }
       }
       operand_ready(sy->sr, lane);
@@ -543,9 +554,9 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             split2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), hi[i], lo[i]);
-          __nv_bfloat16* dst = p.um + (slot * p.V + group0) * 2 * kChunk + t0 * 32 + lane * 8;
+          __nv_bfloat16* dst = channel_at(p.um, slot * p.V + ch, 2, kChunk, t0);
           store_pairs(dst, hi, live);
-          store_pairs(dst + 32 * kChunk, lo, live);
+          store_pairs(dst + kTile * kChunk, lo, live);
         }
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
@@ -683,7 +694,6 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
     walk_load<DK>(D, p.dfinal == nullptr ? nullptr : p.dfinal + state_at, p.V, live);
     uint32_t vr[32], hi[16], lo[16];
     const uint32_t dostep = uint32_t(p.do_st * 2), dvstep = uint32_t(p.HV * p.V * 2);
-    const int group0 = v0 + 32 * (warp & 3);
     auto rows_of = [&](int cc) { return int(min(int64_t(32), s.len - int64_t(cc) * kChunk - t0)); };
     auto fetch_do = [&](int c) {  // c counts from the end
       const int cc = chunks - 1 - c;
@@ -713,14 +723,15 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
       if constexpr (KP == 2) tmem_st(lanes + cO + xStep + t0 / 2, lo);
       operand_ready(sy->gr, lane);
       {
-        __nv_bfloat16* dst = p.om + (slot * p.V + group0) * KP * kChunk + t0 * 32 + lane * 8;
+        __nv_bfloat16* dst = channel_at(p.om, slot * p.V + ch, KP, kChunk, t0);
         store_pairs(dst, hi, live);
-        if constexpr (KP == 2) store_pairs(dst + 32 * kChunk, lo, live);
+        if constexpr (KP == 2) store_pairs(dst + kTile * kChunk, lo, live);
       }
       if (c > 0) {
         advance(c - 1);
         if (!ok) break;
-        compute_sync();
+        ok = compute_sync(wait, sy->all, c - 1, lane);
+        if (!ok) break;
       }
 #pragma unroll
       for (int x = 0; x < DK / 64; ++x) {
@@ -728,10 +739,9 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
 #pragma unroll
         for (int i = 0; i < 32; ++i) w[i] = D[32 * x + i];
         split_to_tmem(w, lanes + cS + half * (DK / 4) + 16 * x, sStep, hi, lo);
-        __nv_bfloat16* dst = p.dm + (slot * p.V + group0) * 2 * DK +
-                             (half * (DK / 16) + 4 * x) * 32 * 8 + lane * 8;
+        __nv_bfloat16* dst = channel_at(p.dm, slot * p.V + ch, 2, DK, half * (DK / 2) + 32 * x);
         store_pairs(dst, hi, live);
-        store_pairs(dst + 32 * DK, lo, live);
+        store_pairs(dst + kTile * DK, lo, live);
       }
       operand_ready(sy->sr, lane);
       // gam dO beside the chain (its region's last reader was the last chunk's update)
@@ -794,9 +804,9 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           split2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), hi[i], lo[i]);
-        __nv_bfloat16* dst = p.xm + (slot * p.V + group0) * 2 * kChunk + t0 * 32 + lane * 8;
+        __nv_bfloat16* dst = channel_at(p.xm, slot * p.V + ch, 2, kChunk, t0);
         store_pairs(dst, hi, live);
-        store_pairs(dst + 32 * kChunk, lo, live);
+        store_pairs(dst + kTile * kChunk, lo, live);
 #pragma unroll
         for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
         walk_put<E>(dv + (int64_t(cc) * kChunk + t0) * p.HV * p.V, dvstep, x, rows_of(cc), live);

@@ -319,6 +319,8 @@ int64_t delta_chunks(const tdc_delta_args* a) {
                                   : a->B * ceil_div(a->T, tdc::kChunk);
 }
 
+constexpr int kSms = 148;  // a B200's
+
 // Segments that the forward walks side by side (1: none): as many as give every
 // block of both passes an SM of its own, if two passes over a segment (and about
 // 6 chunks' time for the second launch and the join) are shorter than one over
@@ -330,7 +332,7 @@ int delta_segments(const tdc_delta_args* a) {
   int best = 1;
   int64_t cost = chunks;
   for (int p = 3; p <= 16; ++p) {
-    if (walks + (p - 2) * (walks + heads) > 148 || walks * (p - 1) > 148) break;
+    if (walks + (p - 2) * (walks + heads) > kSms || walks * (p - 1) > kSms) break;
     const int64_t c = 2 * ceil_div(chunks, p) + 6;
     if (c < cost) best = p, cost = c;
   }
@@ -467,7 +469,7 @@ int delta_bwd_t(const tdc::DeltaParams& p, cudaStream_t st) {
   const size_t smem = tdc::GradSmem<E, DK>::sync + sizeof(tdc::GradSync);
   rc = allow_smem(k, smem);
   if (rc != TDC_OK) return rc;
-  k<<<dim3(unsigned(p.max_chunks), unsigned(p.H)), 256, smem, st>>>(p);
+  k<<<unsigned(std::min<int64_t>(kSms, p.max_chunks * p.H)), tdc::kWalkThreads, smem, st>>>(p);
   return launched();
 }
 
