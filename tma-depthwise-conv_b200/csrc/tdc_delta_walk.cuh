@@ -47,7 +47,6 @@ struct WalkSync {
   uint64_t full[2], free[2];
   uint64_t y, u, q, s, o;                 // products done
   uint64_t sr, xr, vr, qr, gr;            // operands ready (or results read)
-  uint64_t all;                           // the computing warps are there
   uint64_t drain;
   uint32_t tmem;
   int abort;
@@ -100,21 +99,12 @@ __device__ __forceinline__ void operand_ready(uint64_t& bar, int lane) {
   if (lane == 0) mbar_arrive(smem_addr(&bar));
 }
 
-// The 8 computing warps, between one's TMEM loads and another's stores (a bounded
-// wait as the others: a warp that gave up elsewhere does not come).
-__device__ __forceinline__ bool compute_sync(const Waiter& wait, uint64_t& bar, int phase, int lane) {
-  tc_fence_before();
-  __syncwarp();
-  if (lane == 0) mbar_arrive(smem_addr(&bar));
-  const bool ok = warp_wait(wait, bar, phase);
-  tc_fence_after();
-  return ok;
-}
-
-// d[128 x N] (+)= A B; A split in two parts at a, a + astep (columns), B a tile
-// at b in BP parts bstep bytes apart, its rows (n_major false) or its columns as
-// N, DEPTH elements of the contraction.  The remainders' product is left out.
-template <int DEPTH, int N, bool N_MAJOR, int BP>
+// d[128 x N] (+)= A B; A split in two parts, B a tile at b in BP parts bstep bytes
+// apart, its rows (n_major false) or its columns as N, DEPTH elements of the
+// contraction.  The remainders' product is left out.  A's parts start at a and
+// a + astep (columns); the state's (STATE) lie in halves, high parts and remainders
+// of each in the columns of the update that the same threads read before.
+template <int DEPTH, int N, bool N_MAJOR, int BP, bool STATE>
 __device__ __forceinline__ void issue_product(uint32_t d, uint32_t a, uint32_t astep, uint32_t b,
                                               uint32_t bstep, bool accumulate) {
   const uint32_t low = tile_desc(b, N_MAJOR);
@@ -126,8 +116,9 @@ __device__ __forceinline__ void issue_product(uint32_t d, uint32_t a, uint32_t a
       if (i + j > 1) continue;
 #pragma unroll
       for (int ks = 0; ks < DEPTH / 16; ++ks)
-        tc_mma(d, a + i * astep + 8 * ks, low + j * (bstep / 16) + ks * kstep, tile_desc_high(N_MAJOR),
-               mma_desc(N, N_MAJOR), accumulate || i + j + ks > 0);
+        tc_mma(d, a + i * astep + 8 * ks + (STATE ? ks / (DEPTH / 32) * (DEPTH / 4) : 0),
+               low + j * (bstep / 16) + ks * kstep, tile_desc_high(N_MAJOR), mma_desc(N, N_MAJOR),
+               accumulate || i + j + ks > 0);
     }
 }
 
@@ -159,7 +150,7 @@ __device__ __forceinline__ void walk_setup(WalkSync* sy, int tid, int warp) {
     for (uint64_t* b : {&sy->full[0], &sy->full[1], &sy->free[0], &sy->free[1], &sy->y, &sy->u,
                         &sy->q, &sy->s, &sy->o, &sy->drain})
       mbar_init(smem_addr(b), 1);
-    for (uint64_t* b : {&sy->sr, &sy->xr, &sy->vr, &sy->qr, &sy->gr, &sy->all}) mbar_init(smem_addr(b), 8);
+    for (uint64_t* b : {&sy->sr, &sy->xr, &sy->vr, &sy->qr, &sy->gr}) mbar_init(smem_addr(b), 8);
     sy->abort = 0;
     fence_mbar_init();
   }
@@ -384,7 +375,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
   const uint32_t tm = sy->tmem;
   // TMEM columns: Y, then U; O; S^T parts, then the state's update; X, then w V'; V'
   constexpr uint32_t cY = 0, cO = 64, cS = 128, cX = 320, cV = 416;
-  constexpr uint32_t sStep = DK / 2, xStep = 32;
+  constexpr uint32_t sStep = DK / 4, xStep = 32;
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
@@ -395,7 +386,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         if (!warp_wait(wait, sy->full[c & 1], c >> 1) || !warp_wait(wait, sy->sr, c)) break;
         tc_fence_after();
         if (elect_one()) {
-          issue_product<DK, 64, false, KP>(tm + cY, tm + cS, sStep, st + W::k, W::keys, false);
+          issue_product<DK, 64, false, KP, true>(tm + cY, tm + cS, sStep, st + W::k, W::keys, false);
           tc_commit(smem_addr(&sy->y));
         }
         __syncwarp();
@@ -405,7 +396,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
           issue_lower<false, 2>(tm + cY, tm + cX, xStep, st + W::t, false);
           tc_commit(smem_addr(&sy->u));
           if constexpr (MODE == 0) {
-            issue_product<DK, 64, false, KP>(tm + cO, tm + cS, sStep, st + W::q, W::keys, false);
+            issue_product<DK, 64, false, KP, true>(tm + cO, tm + cS, sStep, st + W::q, W::keys, false);
             tc_commit(smem_addr(&sy->q));
           }
         }
@@ -413,7 +404,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         if (!warp_wait(wait, sy->vr, c)) break;
         tc_fence_after();
         if (elect_one()) {
-          issue_product<kChunk, DK, true, KP>(tm + cS, tm + cX, xStep, st + W::k, W::keys, false);
+          issue_product<kChunk, DK, true, KP, false>(tm + cS, tm + cX, xStep, st + W::k, W::keys, false);
           tc_commit(smem_addr(&sy->s));
           if constexpr (MODE == 1) tc_commit(smem_addr(&sy->free[c & 1]));
         }
@@ -496,16 +487,13 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
       if (c > 0) {
         advance(c - 1);
         if (!ok) break;
-        // the update lies where S^T's parts go: everyone has read it first
-        ok = compute_sync(wait, sy->all, c - 1, lane);
-        if (!ok) break;
       }
 #pragma unroll
       for (int x = 0; x < DK / 64; ++x) {
         float w[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) w[i] = S[32 * x + i];
-        split_to_tmem(w, lanes + cS + half * (DK / 4) + 16 * x, sStep, hi, lo);
+        split_to_tmem(w, lanes + cS + half * (DK / 2) + 16 * x, sStep, hi, lo);
         if constexpr (MODE == 1) {
           __nv_bfloat16* dst = channel_at(p.sm, slot * p.V + ch, 2, DK, half * (DK / 2) + 32 * x);
           store_pairs(dst, hi, live);
@@ -636,7 +624,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
   // TMEM columns: K dS, then dX; dS^T parts, then the state's update; P^T dO; dO (exact);
   // gam dO; beta dV', then -gam dX
   constexpr uint32_t cY = 0, cS = 64, cP = 192, cO = 256, cG = 320, cX = 384;
-  constexpr uint32_t sStep = DK / 2, xStep = 32;
+  constexpr uint32_t sStep = DK / 4, xStep = 32;
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
@@ -651,7 +639,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
         if (!warp_wait(wait, sy->sr, c)) break;
         tc_fence_after();
         if (elect_one()) {
-          issue_product<DK, 64, false, KP>(tm + cY, tm + cS, sStep, st + W::k, W::keys, false);
+          issue_product<DK, 64, false, KP, true>(tm + cY, tm + cS, sStep, st + W::k, W::keys, false);
           tc_commit(smem_addr(&sy->y));
         }
         __syncwarp();
@@ -659,7 +647,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
         if (!warp_wait(wait, sy->y, c) || !warp_wait(wait, sy->qr, c)) break;
         tc_fence_after();
         if (elect_one())
-          issue_product<kChunk, DK, true, KP>(tm + cS, tm + cG, xStep, st + W::q, W::keys, false);
+          issue_product<kChunk, DK, true, KP, false>(tm + cS, tm + cG, xStep, st + W::q, W::keys, false);
         __syncwarp();
         if (!warp_wait(wait, sy->xr, c)) break;
         tc_fence_after();
@@ -671,7 +659,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
         if (!warp_wait(wait, sy->vr, c)) break;
         tc_fence_after();
         if (elect_one()) {
-          issue_product<kChunk, DK, true, KP>(tm + cS, tm + cX, xStep, st + W::k, W::keys, true);
+          issue_product<kChunk, DK, true, KP, false>(tm + cS, tm + cX, xStep, st + W::k, W::keys, true);
           tc_commit(smem_addr(&sy->s));
           tc_commit(smem_addr(&sy->free[c & 1]));
         }
@@ -730,15 +718,13 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
       if (c > 0) {
         advance(c - 1);
         if (!ok) break;
-        ok = compute_sync(wait, sy->all, c - 1, lane);
-        if (!ok) break;
       }
 #pragma unroll
       for (int x = 0; x < DK / 64; ++x) {
         float w[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) w[i] = D[32 * x + i];
-        split_to_tmem(w, lanes + cS + half * (DK / 4) + 16 * x, sStep, hi, lo);
+        split_to_tmem(w, lanes + cS + half * (DK / 2) + 16 * x, sStep, hi, lo);
         __nv_bfloat16* dst = channel_at(p.dm, slot * p.V + ch, 2, DK, half * (DK / 2) + 32 * x);
         store_pairs(dst, hi, live);
         store_pairs(dst + kTile * DK, lo, live);
