@@ -27,7 +27,27 @@ namespace tdc {
 constexpr int kChunk = 64;
 constexpr int kLdT = kChunk + 8;     // row of a [64][64] tile in shared memory
 constexpr int kSq = kChunk * kChunk;  // elements of such a tile in the workspace
-constexpr int kTile = 16;  // value channels that lie together in the gradients' workspace
+
+// The gradients' workspace: for kTile value channels of a slot, transposed, what
+// the gradients of a chunk need of them, in the order of a stage in shared memory
+// (so that one copy brings it).  Each part is [columns / 8][kTile][8]; hi is the
+// high parts, lo the remainders.  In bf16 dO has none: the workspace starts behind
+// that place, which holds zeros in shared memory.
+constexpr int kTile = 16;
+template <int KP, int DK>
+struct GradTile {
+  static constexpr int part = kTile * DK * 2, upart = kTile * kChunk * 2;  // bytes
+  static constexpr int olo = 0;             // dO^T, dX^T: remainders
+  static constexpr int xlo = olo + upart;
+  static constexpr int s = xlo + upart;     // S^T before the chunk: hi, lo
+  static constexpr int d = s + 2 * part;    // dS^T behind it: hi, lo
+  static constexpr int u = d + 2 * part;    // U^T: hi, lo
+  static constexpr int ohi = u + 2 * upart;
+  static constexpr int xhi = ohi + upart;
+  static constexpr int stage = xhi + upart;
+  static constexpr int skip = KP == 1 ? upart : 0;
+  static constexpr int bytes = stage - skip;
+};
 
 struct DeltaParams {
   const void *q, *k, *v, *beta;
@@ -54,17 +74,12 @@ struct DeltaParams {
   // (tiles in the order of WalkTiles; 8 x 8 blocks, see tdc_tc.cuh)
   __nv_bfloat16* tp;      // T and P, high parts and remainders: [4][64 x 64]
   float* coef;            // [3][64]: gam, w, beta
-  unsigned char* kq;      // [chunk][H]: K and Q, [2][parts][64 x K]
+  unsigned char* kq;      // [chunk][H]: [parts][K / 8][Q's 64 rows, K's 64 rows][8]
   uint64_t timeout_ns;    // of the bounded waits
   int64_t withhold;       // first chunk of a sequence whose copies never come (-1: none)
   int *status_words, *status_host;
   // gradients
-  // (kTile channels together: [V / kTile][2 parts][columns / 8][kTile][8])
-  __nv_bfloat16* um;      // U^T, 64 columns
-  __nv_bfloat16* xm;      // dX^T
-  __nv_bfloat16* om;      // dO^T (bf16: one part)
-  __nv_bfloat16* sm;      // S^T before the chunk, K columns
-  __nv_bfloat16* dm;      // dS^T behind the chunk
+  unsigned char* tiles;   // [chunk][HV][V / kTile] GradTile
   const void* d_o;
   int64_t do_sb, do_st, do_sh;
   const float* dfinal;
@@ -323,14 +338,15 @@ __device__ __forceinline__ void store_lower(__nv_bfloat16* dst, const unsigned c
   }
 }
 
-// A [64][DK] tile of the element type to its parts in 8 x 8 blocks.
+// Rows of K or Q to their parts, 8 columns of the rows of both together.
+constexpr int kKeyBlock = 2 * kChunk * 16;  // bytes of 8 columns
 template <class E, int DK>
 __device__ __forceinline__ void store_keys(unsigned char* dst, const unsigned char* tile, int tid,
                                            int threads) {
   for (int e = tid; e < kChunk * (DK / 8); e += threads) {
     const int r = e & 63, c = e >> 6;
     const uint4 v = *reinterpret_cast<const uint4*>(tile + 2 * (r * (DK + 8) + 8 * c));
-    uint4* d = reinterpret_cast<uint4*>(dst + 2 * block_offset(r, c));
+    uint4* d = reinterpret_cast<uint4*>(dst + c * kKeyBlock + r * 16);
     if constexpr (std::is_same_v<E, BF16>) {
       *d = v;
     } else {
@@ -340,7 +356,7 @@ __device__ __forceinline__ void store_keys(unsigned char* dst, const unsigned ch
       split_elem<E>(v.z, hi.z, lo.z);
       split_elem<E>(v.w, hi.w, lo.w);
       *d = hi;
-      d[kChunk * DK / 8] = lo;
+      d[DK / 8 * kKeyBlock / 16] = lo;
     }
   }
 }
@@ -398,8 +414,8 @@ __global__ void __launch_bounds__(128) delta_prepare_kernel(const DeltaParams p)
   {
     constexpr int64_t bytes = int64_t(std::is_same_v<E, BF16> ? 1 : 2) * kChunk * DK * 2;
     unsigned char* kq = p.kq + (chunk * p.H + h) * 2 * bytes;
-    store_keys<E, DK>(kq, raw + Sm::k, tid, 128);
-    store_keys<E, DK>(kq + bytes, raw + Sm::q, tid, 128);
+    store_keys<E, DK>(kq, raw + Sm::q, tid, 128);
+    store_keys<E, DK>(kq + kChunk * 16, raw + Sm::k, tid, 128);
   }
   const int g = lane >> 2, t2 = (lane & 3) * 2;
   for (int gi = 0; gi < p.group; ++gi) {

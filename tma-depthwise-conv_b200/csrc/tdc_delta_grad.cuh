@@ -41,16 +41,11 @@ template <class E, int DK>
 struct GradSmem {
   static constexpr int KP = std::is_same_v<E, BF16> ? 1 : 2;
   // rows of Q, then of K: [parts][DK / 8][128][8]
-  static constexpr int qk = 0, qkpart = 2 * kChunk * DK * 2;
+  using Tile = GradTile<KP, DK>;
+  static constexpr int qk = 0, qkpart = DK / 8 * kKeyBlock;
   // rows of Dt, then of N: [2 parts][8][128][8]
-  static constexpr int dn = qk + KP * qkpart, dnpart = 2 * kChunk * kChunk * 2;
-  static constexpr int stages = dn + 2 * dnpart;
-  static constexpr int part = kTile * DK * 2, upart = kTile * kChunk * 2;
-  static constexpr int s = 0;               // S^T, high parts and remainders
-  static constexpr int d = s + 2 * part;    // dS^T
-  static constexpr int u = d + 2 * part;    // U^T
-  static constexpr int a = u + 2 * upart;   // dO^T and dX^T, then their remainders (dO's: 0 in bf16)
-  static constexpr int stage = a + 4 * upart;
+  static constexpr int dn = qk + KP * qkpart, dnpart = kChunk / 8 * kKeyBlock;
+  static constexpr int stages = dn + 2 * dnpart, stage = Tile::stage;
   static constexpr int kMaxBytes = 232448 - 7168;  // of a block, less GradSync
   static constexpr int count = (kMaxBytes - stages) / stage < 6 ? (kMaxBytes - stages) / stage : 6;
   static constexpr int sync = stages + count * stage;
@@ -105,7 +100,7 @@ __device__ __forceinline__ void load_key_row(float (&f)[32], const unsigned char
   using Sm = GradSmem<E, DK>;
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    const unsigned char* src = qk + (c0 / 8 + c) * 2048 + l * 16;
+    const unsigned char* src = qk + (c0 / 8 + c) * kKeyBlock + l * 16;
     unpack8<BF16>(*reinterpret_cast<const uint4*>(src), f + 8 * c);
     if constexpr (Sm::KP == 2) {
       float lo[8];
@@ -137,36 +132,19 @@ __device__ __forceinline__ void grad_fetch(const DeltaParams& p, unsigned char* 
       if (t == min(NS, tiles)) {
         if (done > 0) ok = wait(sy->next, uint32_t(done * p.group - 1), TDC_DEVICE_EMPTY_TIMEOUT, n);
         if (!ok) break;
-        // 8 columns a copy: the two halves of the rows beside each other
-        constexpr int bytes = kChunk * DK * 2;
-        const unsigned char* src = p.kq + (chunk * p.H + h) * (2 * KP * bytes);
-        mbar_arrive_expect_tx(smem_addr(&sy->keys), 2 * KP * bytes);
+        constexpr int bytes = KP * Sm::qkpart;
+        mbar_arrive_expect_tx(smem_addr(&sy->keys), bytes);
         ++sent;
-#pragma unroll 1
-        for (int which = 0; which < 2 * KP; ++which) {  // K's parts, then Q's
-          const uint32_t dst =
-              sb + Sm::qk + (which % KP) * Sm::qkpart + (which < KP ? 1024 : 0);
-#pragma unroll 4
-          for (int c = 0; c < DK / 8; ++c)
-            bulk_load(dst + c * 2048, src + which * bytes + c * 1024, 1024, smem_addr(&sy->keys));
-        }
+        bulk_load(sb + Sm::qk, p.kq + (chunk * p.H + h) * bytes, bytes, smem_addr(&sy->keys));
       }
       if (t == tiles) break;
       const int x = n % NS;
       if (n >= NS) ok = wait(sy->used[x], uint32_t(n / NS - 1), TDC_DEVICE_EMPTY_TIMEOUT, n);
       if (!ok) break;
-      const int64_t tile = tile0 + t;
-      const uint32_t st = sb + Sm::stages + x * Sm::stage, bar = smem_addr(&sy->full[x]);
-      mbar_arrive_expect_tx(bar, 4 * Sm::part + (4 + KP) * Sm::upart);
-      bulk_load(st + Sm::s, p.sm + tile * Sm::part, 2 * Sm::part, bar);
-      bulk_load(st + Sm::d, p.dm + tile * Sm::part, 2 * Sm::part, bar);
-      bulk_load(st + Sm::u, p.um + tile * Sm::upart, 2 * Sm::upart, bar);
-      const __nv_bfloat16* dx = p.xm + tile * Sm::upart;
-      bulk_load(st + Sm::a + Sm::upart, dx, Sm::upart, bar);
-      bulk_load(st + Sm::a + 3 * Sm::upart, dx + Sm::upart / 2, Sm::upart, bar);
-      const __nv_bfloat16* o = p.om + tile * (KP * Sm::upart / 2);
-      bulk_load(st + Sm::a, o, Sm::upart, bar);
-      if constexpr (KP == 2) bulk_load(st + Sm::a + 2 * Sm::upart, o + Sm::upart / 2, Sm::upart, bar);
+      constexpr int bytes = Sm::Tile::bytes;
+      const uint32_t bar = smem_addr(&sy->full[x]);
+      mbar_arrive_expect_tx(bar, bytes);
+      bulk_load(sb + Sm::stages + x * Sm::stage + Sm::Tile::skip, p.tiles + (tile0 + t) * bytes, bytes, bar);
       ++n;
     }
   }
@@ -184,7 +162,7 @@ __device__ __forceinline__ void grad_issue(const DeltaParams& p, uint32_t sb, Gr
                                            const Waiter& wait, uint32_t tm) {
   using Sm = GradSmem<E, DK>;
   constexpr int KP = Sm::KP, NS = Sm::count;
-  constexpr uint32_t khigh = block_desc_high(2048), rhigh = block_desc_high(kRowBlock);
+  constexpr uint32_t khigh = block_desc_high(kKeyBlock), rhigh = block_desc_high(kRowBlock);
   const GradItems items(p);
   const int per_head = p.V / kTile;
   int x = 0, phase = 0, heads = 0, done = 0;
@@ -196,15 +174,16 @@ __device__ __forceinline__ void grad_issue(const DeltaParams& p, uint32_t sb, Gr
         tc_fence_after();
         const uint32_t st = sb + Sm::stages + x * Sm::stage;
         if (elect_one()) {
-          const uint32_t a = st + Sm::a, b = a + 2 * Sm::upart, u = st + Sm::u;
-          grad_product<DK>(tm + kGradOX, a, st + Sm::s, vt > 0);
-          grad_product<DK>(tm + kGradOX, b, st + Sm::s, true);
-          grad_product<DK>(tm + kGradOX, a, st + Sm::s + Sm::part, true);
+          using T = typename Sm::Tile;
+          const uint32_t a = st + T::ohi, b = st + T::olo, u = st + T::u;
+          grad_product<DK>(tm + kGradOX, a, st + T::s, vt > 0);
+          grad_product<DK>(tm + kGradOX, b, st + T::s, true);
+          grad_product<DK>(tm + kGradOX, a, st + T::s + T::part, true);
           grad_product<64>(tm + kGradDM, a, u, vt > 0);
           grad_product<64>(tm + kGradDM, b, u, true);
-          grad_product<64>(tm + kGradDM, a, u + Sm::upart, true);
-          grad_product<DK>(tm + kGradUS, u, st + Sm::d, vt > 0);
-          grad_product<DK>(tm + kGradUS, u, st + Sm::d + Sm::part, true);
+          grad_product<64>(tm + kGradDM, a, u + T::upart, true);
+          grad_product<DK>(tm + kGradUS, u, st + T::d, vt > 0);
+          grad_product<DK>(tm + kGradUS, u, st + T::d + T::part, true);
           tc_commit(smem_addr(&sy->used[x]));
         }
         __syncwarp();
@@ -220,8 +199,8 @@ __device__ __forceinline__ void grad_issue(const DeltaParams& p, uint32_t sb, Gr
             for (int z = 0; z < KP - y; ++z)
 #pragma unroll
               for (int ks = 0; ks < DK / 16; ++ks)
-                tc_mma_ss(tm + kGradGram, block_desc(sb + Sm::qk + y * Sm::qkpart + ks * 4096, 2048), rhigh,
-                          block_desc(sb + Sm::qk + z * Sm::qkpart + 1024 + ks * 4096, 2048), rhigh,
+                tc_mma_ss(tm + kGradGram, block_desc(sb + Sm::qk + y * Sm::qkpart + ks * 2 * kKeyBlock, kKeyBlock), rhigh,
+                          block_desc(sb + Sm::qk + z * Sm::qkpart + 1024 + ks * 2 * kKeyBlock, kKeyBlock), rhigh,
                           mma_desc(64, false, false), y + z + ks > 0);
         }
         __syncwarp();
@@ -239,7 +218,7 @@ __device__ __forceinline__ void grad_issue(const DeltaParams& p, uint32_t sb, Gr
             if (y + z > 1) continue;
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
-              tc_mma_ss(tm + kGradOX, block_desc(sb + Sm::dn + y * Sm::dnpart + ks * 4096, 2048), rhigh,
+              tc_mma_ss(tm + kGradOX, block_desc(sb + Sm::dn + y * Sm::dnpart + ks * 2 * kKeyBlock, kKeyBlock), rhigh,
                         block_desc(sb + Sm::qk + z * Sm::qkpart + 1024 + ks * 2 * kRowBlock, kRowBlock),
                         khigh, mma_desc(DK, true, false), true);
           }
@@ -292,9 +271,9 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_grad_kernel(const Delta
   }
   if (warp == 8) tmem_alloc(smem_addr(&sy->tmem), kTmemColumns);
   if constexpr (KP == 1) {  // dO has no remainders
-    for (int e = 16 * tid; e < NS * Sm::upart; e += 16 * kWalkThreads)
-      *reinterpret_cast<uint4*>(raw + Sm::stages + e / Sm::upart * Sm::stage + Sm::a + 2 * Sm::upart +
-                                e % Sm::upart) = make_uint4(0, 0, 0, 0);
+    constexpr int skip = Sm::Tile::skip;
+    for (int e = 16 * tid; e < NS * skip; e += 16 * kWalkThreads)
+      *reinterpret_cast<uint4*>(raw + Sm::stages + e / skip * Sm::stage + e % skip) = make_uint4(0, 0, 0, 0);
     fence_proxy_async();
   }
   tc_fence_before();
@@ -364,9 +343,9 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_grad_kernel(const Delta
             float f[2][8], g[2][8];
 #pragma unroll
             for (int part = 0; part < 2; ++part) {
-              const int off = part * Sm::part + 16 * e;
-              unpack8<BF16>(*reinterpret_cast<const uint4*>(stage + Sm::s + off), f[part]);
-              unpack8<BF16>(*reinterpret_cast<const uint4*>(stage + Sm::d + off), g[part]);
+              const int off = part * Sm::Tile::part + 16 * e;
+              unpack8<BF16>(*reinterpret_cast<const uint4*>(stage + Sm::Tile::s + off), f[part]);
+              unpack8<BF16>(*reinterpret_cast<const uint4*>(stage + Sm::Tile::d + off), g[part]);
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) dsum = fmaf(f[0][j] + f[1][j], g[0][j] + g[1][j], dsum);
@@ -408,7 +387,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_grad_kernel(const Delta
           const Far Gi = sy->G[i];
           const float sign = upper ? -1.f : p.scale;
           const int low = upper ? i : i + 1;  // columns below this are kept
-          float row = 0.f, cs[32];
+          float row = 0.f, own = 0.f, cs[32];
 #pragma unroll
           for (int y = 0; y < 32; y += 2) {
             const float4 far2 = *reinterpret_cast<const float4*>(sy->G + 32 * hc + y);
@@ -421,20 +400,21 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_grad_kernel(const Delta
               const bool in = j < low;
               const float v = in ? sign * __expf(minus(Gi, Gj)) * __uint_as_float(r[y + z]) : 0.f;
               const float t = in ? v * __uint_as_float(g[y + z]) : 0.f;
-              if (j == i && !upper) sy->diag[i] = t;
+              own = j == i ? t : own;
               cs[y + z] = j < i ? t : 0.f;
               row = fmaf(bj, cs[y + z], row);
               r[y + z] = __float_as_uint(in ? bj * v : 0.f);
             }
           }
           sy->sums[kSumE][hc][l] = row;
+          if (!upper && (i >> 5) == hc) sy->diag[i] = own;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int m = 0; m < 4; ++m)
               split2(__uint_as_float(r[8 * c + 2 * m]), __uint_as_float(r[8 * c + 2 * m + 1]), hi[m], lo[m]);
-            unsigned char* dst = raw + Sm::dn + (4 * hc + c) * 2048 + l * 16;
+            unsigned char* dst = raw + Sm::dn + (4 * hc + c) * kKeyBlock + l * 16;
             *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             *reinterpret_cast<uint4*>(dst + Sm::dnpart) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
           }

@@ -33,10 +33,10 @@ namespace tdc {
 template <class E, int DK>
 struct WalkTiles {
   static constexpr int KP = std::is_same_v<E, BF16> ? 1 : 2;
-  static constexpr int keys = kChunk * DK * 2;        // one part of K or Q
-  static constexpr int k = 0;
-  static constexpr int q = k + KP * keys;
-  static constexpr int t = q + KP * keys;
+  static constexpr int keys = DK / 8 * kKeyBlock;     // one part of Q and K
+  static constexpr int q = 0;
+  static constexpr int k = kChunk * 16;
+  static constexpr int t = KP * keys;
   static constexpr int p = t + 2 * kSq * 2;
   static constexpr int coef = p + 2 * kSq * 2;
   static constexpr int stage = coef + 3 * kChunk * 4;
@@ -99,16 +99,17 @@ __device__ __forceinline__ void operand_ready(uint64_t& bar, int lane) {
   if (lane == 0) mbar_arrive(smem_addr(&bar));
 }
 
-// d[128 x N] (+)= A B; A split in two parts, B a tile at b in BP parts bstep bytes
-// apart, its rows (n_major false) or its columns as N, DEPTH elements of the
-// contraction.  The remainders' product is left out.  A's parts start at a and
+// d[128 x N] (+)= A B; A split in two parts, B the rows of Q or K at b in BP parts
+// bstep bytes apart, their tokens (n_major false) or their columns as N, DEPTH
+// elements of the contraction.  The remainders' product is left out.  A's parts start at a and
 // a + astep (columns); the state's (STATE) lie in halves, high parts and remainders
 // of each in the columns of the update that the same threads read before.
 template <int DEPTH, int N, bool N_MAJOR, int BP, bool STATE>
 __device__ __forceinline__ void issue_product(uint32_t d, uint32_t a, uint32_t astep, uint32_t b,
                                               uint32_t bstep, bool accumulate) {
-  const uint32_t low = tile_desc(b, N_MAJOR);
-  constexpr uint32_t kstep = (N_MAJOR ? 2 * kRowBlock : 2 * kColBlock) / 16;
+  const uint32_t low = block_desc(b, N_MAJOR ? kRowBlock : kKeyBlock);
+  constexpr uint32_t high = block_desc_high(N_MAJOR ? kKeyBlock : kRowBlock);
+  constexpr uint32_t kstep = (N_MAJOR ? 2 * kRowBlock : 2 * kKeyBlock) / 16;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -117,7 +118,7 @@ __device__ __forceinline__ void issue_product(uint32_t d, uint32_t a, uint32_t a
 #pragma unroll
       for (int ks = 0; ks < DEPTH / 16; ++ks)
         tc_mma(d, a + i * astep + 8 * ks + (STATE ? ks / (DEPTH / 32) * (DEPTH / 4) : 0),
-               low + j * (bstep / 16) + ks * kstep, tile_desc_high(N_MAJOR), mma_desc(N, N_MAJOR),
+               low + j * (bstep / 16) + ks * kstep, high, mma_desc(N, N_MAJOR),
                accumulate || i + j + ks > 0);
     }
 }
@@ -160,7 +161,7 @@ __device__ __forceinline__ void walk_setup(WalkSync* sy, int tid, int warp) {
 }
 
 // Warp 9, one thread: the tiles of each chunk in turn.
-template <class E, int DK, bool KEYS_ONLY>
+template <class E, int DK, bool T_ONLY>
 __device__ __forceinline__ void walk_fetch(const DeltaParams& p, unsigned char* raw, WalkSync* sy,
                                            const Waiter& wait, const SeqAt& s, int chunks, int h,
                                            int hv, bool back) {
@@ -171,11 +172,11 @@ __device__ __forceinline__ void walk_fetch(const DeltaParams& p, unsigned char* 
     if (c >= 2 && !wait(sy->free[st], uint32_t((c >> 1) - 1), TDC_DEVICE_EMPTY_TIMEOUT, c)) break;
     const int64_t chunk = s.chunk0 + (back ? chunks - 1 - c : c), slot = chunk * p.HV + hv;
     const uint32_t dst = smem_addr(raw) + st * W::stage, bar = smem_addr(&sy->full[st]);
-    const unsigned char* keys = p.kq + (chunk * p.H + h) * (2 * W::KP * W::keys);
-    constexpr uint32_t kbytes = KEYS_ONLY ? W::KP * W::keys : 2 * W::KP * W::keys;
-    constexpr uint32_t tbytes = KEYS_ONLY ? 2 * kSq * 2 : 4 * kSq * 2;
+    const unsigned char* keys = p.kq + (chunk * p.H + h) * (W::KP * W::keys);
+    constexpr uint32_t kbytes = W::KP * W::keys;
+    constexpr uint32_t tbytes = T_ONLY ? 2 * kSq * 2 : 4 * kSq * 2;
     mbar_arrive_expect_tx(bar, kbytes + tbytes + 3 * kChunk * 4);
-    bulk_load(dst + W::k, keys, kbytes, bar);
+    bulk_load(dst + W::q, keys, kbytes, bar);
     bulk_load(dst + W::t, p.tp + slot * (4 * kSq), tbytes, bar);
     bulk_load(dst + W::coef, p.coef + slot * 3 * kChunk, 3 * kChunk * 4, bar);
     issued = c + 1;
@@ -246,19 +247,19 @@ __device__ __forceinline__ float widen(uint32_t raw) {
 }
 
 // Where column `col` (a multiple of 8) of a channel (of all slots') lies in the
-// gradients' workspace: 8 columns of kTile channels together, 16 bytes a channel.
-__device__ __forceinline__ __nv_bfloat16* channel_at(__nv_bfloat16* base, int64_t channel, int parts,
-                                                     int columns, int col) {
-  return base + (channel & ~int64_t(kTile - 1)) * (parts * columns) + (channel & (kTile - 1)) * 8 +
-         col * kTile;
+// gradients' workspace, in the part at `off` of its tile.
+template <int KP, int DK>
+__device__ __forceinline__ unsigned char* channel_at(unsigned char* base, int64_t channel, int off, int col) {
+  using G = GradTile<KP, DK>;
+  return base + channel / kTile * G::bytes + (off - G::skip) + int(channel % kTile) * 16 + col * (2 * kTile);
 }
 // 16 packed pairs (32 tokens or keys) of a channel there: a warp's stores are
 // whole lines.
-__device__ __forceinline__ void store_pairs(__nv_bfloat16* dst, const uint32_t (&r)[16], bool live) {
+__device__ __forceinline__ void store_pairs(unsigned char* dst, const uint32_t (&r)[16], bool live) {
   if (!live) return;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    *reinterpret_cast<uint4*>(dst + i * kTile * 8) =
+    *reinterpret_cast<uint4*>(dst + i * kTile * 16) =
         make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
 }
 
@@ -354,6 +355,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
   extern __shared__ __align__(1024) unsigned char raw[];
   using W = WalkTiles<E, DK>;
   constexpr int KP = W::KP;
+  using GT = GradTile<KP, DK>;
   WalkSync* sy = reinterpret_cast<WalkSync*>(raw + 2 * W::stage);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int hv = blockIdx.y, h = hv / p.group;
@@ -495,9 +497,9 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         for (int i = 0; i < 32; ++i) w[i] = S[32 * x + i];
         split_to_tmem(w, lanes + cS + half * (DK / 2) + 16 * x, sStep, hi, lo);
         if constexpr (MODE == 1) {
-          __nv_bfloat16* dst = channel_at(p.sm, slot * p.V + ch, 2, DK, half * (DK / 2) + 32 * x);
+          unsigned char* dst = channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::s, half * (DK / 2) + 32 * x);
           store_pairs(dst, hi, live);
-          store_pairs(dst + kTile * DK, lo, live);
+          store_pairs(dst + GT::part, lo, live);
         }
       }
       operand_ready(sy->sr, lane);
@@ -542,9 +544,9 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             split2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), hi[i], lo[i]);
-          __nv_bfloat16* dst = channel_at(p.um, slot * p.V + ch, 2, kChunk, t0);
+          unsigned char* dst = channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::u, t0);
           store_pairs(dst, hi, live);
-          store_pairs(dst + kTile * kChunk, lo, live);
+          store_pairs(dst + GT::upart, lo, live);
         }
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
@@ -610,6 +612,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
   extern __shared__ __align__(1024) unsigned char raw[];
   using W = WalkTiles<E, DK>;
   constexpr int KP = W::KP;
+  using GT = GradTile<KP, DK>;
   WalkSync* sy = reinterpret_cast<WalkSync*>(raw + 2 * W::stage);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int hv = blockIdx.y, h = hv / p.group;
@@ -711,9 +714,9 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
       if constexpr (KP == 2) tmem_st(lanes + cO + xStep + t0 / 2, lo);
       operand_ready(sy->gr, lane);
       {
-        __nv_bfloat16* dst = channel_at(p.om, slot * p.V + ch, KP, kChunk, t0);
-        store_pairs(dst, hi, live);
-        if constexpr (KP == 2) store_pairs(dst + kTile * kChunk, lo, live);
+        store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::ohi, t0), hi, live);
+        if constexpr (KP == 2)
+          store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::olo, t0), lo, live);
       }
       if (c > 0) {
         advance(c - 1);
@@ -725,9 +728,9 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
 #pragma unroll
         for (int i = 0; i < 32; ++i) w[i] = D[32 * x + i];
         split_to_tmem(w, lanes + cS + half * (DK / 2) + 16 * x, sStep, hi, lo);
-        __nv_bfloat16* dst = channel_at(p.dm, slot * p.V + ch, 2, DK, half * (DK / 2) + 32 * x);
+        unsigned char* dst = channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::d, half * (DK / 2) + 32 * x);
         store_pairs(dst, hi, live);
-        store_pairs(dst + kTile * DK, lo, live);
+        store_pairs(dst + GT::part, lo, live);
       }
       operand_ready(sy->sr, lane);
       // gam dO beside the chain (its region's last reader was the last chunk's update)
@@ -790,9 +793,8 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           split2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), hi[i], lo[i]);
-        __nv_bfloat16* dst = channel_at(p.xm, slot * p.V + ch, 2, kChunk, t0);
-        store_pairs(dst, hi, live);
-        store_pairs(dst + kTile * kChunk, lo, live);
+        store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::xhi, t0), hi, live);
+        store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::xlo, t0), lo, live);
 #pragma unroll
         for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
         walk_put<E>(dv + (int64_t(cc) * kChunk + t0) * p.HV * p.V, dvstep, x, rows_of(cc), live);

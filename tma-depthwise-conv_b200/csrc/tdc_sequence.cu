@@ -353,7 +353,7 @@ int64_t delta_layout(const tdc_delta_args* a, bool grads, unsigned char* base, t
   const int64_t parts = a->dtype == TDC_BF16 ? 1 : 2;
   unsigned char* kq = take(delta_chunks(a) * a->H * 2 * parts * tdc::kChunk * a->K * 2);
   unsigned char* coef = take(slots * 3 * tdc::kChunk * 4);
-  unsigned char *um = nullptr, *xm = nullptr, *om = nullptr, *sm = nullptr, *dm = nullptr;
+  unsigned char* tiles = nullptr;
   unsigned char *seg_s = nullptr, *seg_m = nullptr;
   const int segments = grads ? 1 : delta_segments(a);
   if (segments > 1) {
@@ -361,11 +361,8 @@ int64_t delta_layout(const tdc_delta_args* a, bool grads, unsigned char* base, t
     seg_m = take(a->B * a->HV * segments * a->K * a->K * 4);
   }
   if (grads) {
-    um = take(slots * 2 * a->V * tdc::kChunk * 2);
-    xm = take(slots * 2 * a->V * tdc::kChunk * 2);
-    om = take(slots * parts * a->V * tdc::kChunk * 2);
-    sm = take(slots * 2 * a->V * a->K * 2);
-    dm = take(slots * 2 * a->V * a->K * 2);
+    // (GradTile: S, dS, U and dX in two parts, dO in `parts`)
+    tiles = take(slots * a->V * 2 * (4 * a->K + (4 + parts) * tdc::kChunk));
   }
   if (p != nullptr) {
     p->seq_lo = reinterpret_cast<int64_t*>(plan);
@@ -377,11 +374,7 @@ int64_t delta_layout(const tdc_delta_args* a, bool grads, unsigned char* base, t
     p->seg_s = reinterpret_cast<float*>(seg_s);
     p->seg_m = reinterpret_cast<float*>(seg_m);
     p->coef = reinterpret_cast<float*>(coef);
-    p->um = reinterpret_cast<__nv_bfloat16*>(um);
-    p->xm = reinterpret_cast<__nv_bfloat16*>(xm);
-    p->om = reinterpret_cast<__nv_bfloat16*>(om);
-    p->sm = reinterpret_cast<__nv_bfloat16*>(sm);
-    p->dm = reinterpret_cast<__nv_bfloat16*>(dm);
+    p->tiles = tiles;
   }
   return at;
 }
