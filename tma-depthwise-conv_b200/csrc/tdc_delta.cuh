@@ -39,9 +39,10 @@ struct GradTile {
   static constexpr int part = kTile * DK * 2, upart = kTile * kChunk * 2;  // bytes
   static constexpr int olo = 0;             // dO^T, dX^T: remainders
   static constexpr int xlo = olo + upart;
-  static constexpr int s = xlo + upart;     // S^T before the chunk: hi, lo
-  static constexpr int d = s + 2 * part;    // dS^T behind it: hi, lo
-  static constexpr int u = d + 2 * part;    // U^T: hi, lo
+  static constexpr int d = xlo + upart;     // dS^T behind the chunk: hi, lo
+  static constexpr int slo = d + 2 * part;  // S^T before it
+  static constexpr int shi = slo + part;
+  static constexpr int u = shi + part;      // U^T: hi, lo
   static constexpr int ohi = u + 2 * upart;
   static constexpr int xhi = ohi + upart;
   static constexpr int stage = xhi + upart;

@@ -55,6 +55,7 @@ struct GradSync {
   uint64_t keys;               // Q and K are there
   uint64_t gates;              // G and coef are
   uint64_t ready;              // products over the channels done
+  uint64_t gram;               // products of Q and K with K done
   uint64_t dn;                 // Dt and N are stored
   uint64_t done;               // products with them done
   uint64_t swap;               // dK's parts of lanes 0-63 stored
@@ -70,7 +71,8 @@ struct GradSync {
   float dot[8];
 };
 enum { kSumState = 0, kSumKey = 1, kSumE = 2 };
-constexpr uint32_t kGradOX = 0, kGradDM = 128, kGradUS = 192, kGradGram = 320;
+// TMEM columns; D and M stand behind the products with S (DK columns).
+constexpr uint32_t kGradOX = 0, kGradUS = 192, kGradGram = 320;
 
 // What a block works on: chunk and key head of item x, and of the next that has rows.
 struct GradItems {
@@ -162,6 +164,7 @@ __device__ __forceinline__ void grad_issue(const DeltaParams& p, uint32_t sb, Gr
                                            const Waiter& wait, uint32_t tm) {
   using Sm = GradSmem<E, DK>;
   constexpr int KP = Sm::KP, NS = Sm::count;
+  constexpr uint32_t kGradDM = kGradOX + DK;
   constexpr uint32_t khigh = block_desc_high(kKeyBlock), rhigh = block_desc_high(kRowBlock);
   const GradItems items(p);
   const int per_head = p.V / kTile;
@@ -176,11 +179,10 @@ __device__ __forceinline__ void grad_issue(const DeltaParams& p, uint32_t sb, Gr
         if (elect_one()) {
           using T = typename Sm::Tile;
           const uint32_t a = st + T::ohi, b = st + T::olo, u = st + T::u;
-          grad_product<DK>(tm + kGradOX, a, st + T::s, vt > 0);
-          grad_product<DK>(tm + kGradOX, b, st + T::s, true);
-          grad_product<DK>(tm + kGradOX, a, st + T::s + T::part, true);
-          grad_product<64>(tm + kGradDM, a, u, vt > 0);
-          grad_product<64>(tm + kGradDM, b, u, true);
+          // by S and U together, where their parts lie beside each other
+          grad_product<DK + 64>(tm + kGradOX, a, st + T::shi, vt > 0);
+          grad_product<DK + 64>(tm + kGradOX, b, st + T::shi, true);
+          grad_product<DK>(tm + kGradOX, a, st + T::slo, true);
           grad_product<64>(tm + kGradDM, a, u + T::upart, true);
           grad_product<DK>(tm + kGradUS, u, st + T::d, vt > 0);
           grad_product<DK>(tm + kGradUS, u, st + T::d + T::part, true);
@@ -189,6 +191,8 @@ __device__ __forceinline__ void grad_issue(const DeltaParams& p, uint32_t sb, Gr
         __syncwarp();
         if (++x == NS) x = 0, ++phase;
       }
+      if (elect_one()) tc_commit(smem_addr(&sy->ready));
+      __syncwarp();
       if (gi == 0) {
         if (!warp_wait(wait, sy->keys, done)) return;
         tc_fence_after();
@@ -202,11 +206,10 @@ __device__ __forceinline__ void grad_issue(const DeltaParams& p, uint32_t sb, Gr
                 tc_mma_ss(tm + kGradGram, block_desc(sb + Sm::qk + y * Sm::qkpart + ks * 2 * kKeyBlock, kKeyBlock), rhigh,
                           block_desc(sb + Sm::qk + z * Sm::qkpart + 1024 + ks * 2 * kKeyBlock, kKeyBlock), rhigh,
                           mma_desc(64, false, false), y + z + ks > 0);
+          tc_commit(smem_addr(&sy->gram));
         }
         __syncwarp();
       }
-      if (elect_one()) tc_commit(smem_addr(&sy->ready));
-      __syncwarp();
       if (!warp_wait(wait, sy->dn, heads)) return;
       tc_fence_after();
       if (elect_one()) {
@@ -263,7 +266,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_grad_kernel(const Delta
       mbar_init(smem_addr(&sy->full[x]), 1);
       mbar_init(smem_addr(&sy->used[x]), 9);
     }
-    for (uint64_t* one : {&sy->keys, &sy->gates, &sy->ready, &sy->done, &sy->drain})
+    for (uint64_t* one : {&sy->keys, &sy->gates, &sy->ready, &sy->gram, &sy->done, &sy->drain})
       mbar_init(smem_addr(one), 1);
     for (uint64_t* all : {&sy->dn, &sy->swap, &sy->next}) mbar_init(smem_addr(all), 8);
     sy->abort = 0;
@@ -344,7 +347,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_grad_kernel(const Delta
 #pragma unroll
             for (int part = 0; part < 2; ++part) {
               const int off = part * Sm::Tile::part + 16 * e;
-              unpack8<BF16>(*reinterpret_cast<const uint4*>(stage + Sm::Tile::s + off), f[part]);
+              unpack8<BF16>(*reinterpret_cast<const uint4*>(stage + Sm::Tile::slo + off), f[part]);
               unpack8<BF16>(*reinterpret_cast<const uint4*>(stage + Sm::Tile::d + off), g[part]);
             }
 #pragma unroll
@@ -379,10 +382,15 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_grad_kernel(const Delta
           sy->sums[kSumState][hc][l] = own;
           sy->sums[kSumKey][hc][l] = key;
         }
+        if (gi == 0) {
+          ok = all_wait(sy->gram, done);
+          if (!ok) break;
+          tc_fence_after();
+        }
         // Dt and N, and the sums of E.
         {
           uint32_t r[32], g[32];
-          tmem_ld(lanes + kGradDM + 32 * hc, r);
+          tmem_ld(lanes + kGradOX + DK + 32 * hc, r);
           tmem_ld(lanes + kGradGram + 32 * hc, g);
           const Far Gi = sy->G[i];
           const float sign = upper ? -1.f : p.scale;
@@ -397,13 +405,14 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_grad_kernel(const Delta
               const int j = 32 * hc + y + z;
               const float bj = z ? be2.y : be2.x;
               const Far Gj = z ? Far{far2.z, far2.w} : Far{far2.x, far2.y};
+              // (what is masked is replaced before it is used: no branches)
               const bool in = j < low;
-              const float v = in ? sign * __expf(minus(Gi, Gj)) * __uint_as_float(r[y + z]) : 0.f;
-              const float t = in ? v * __uint_as_float(g[y + z]) : 0.f;
+              const float v = sign * __expf(in ? minus(Gi, Gj) : 0.f) * __uint_as_float(in ? r[y + z] : 0u);
+              const float t = v * __uint_as_float(in ? g[y + z] : 0u);
               own = j == i ? t : own;
               cs[y + z] = j < i ? t : 0.f;
               row = fmaf(bj, cs[y + z], row);
-              r[y + z] = __float_as_uint(in ? bj * v : 0.f);
+              r[y + z] = in ? __float_as_uint(bj * v) : 0u;
             }
           }
           sy->sums[kSumE][hc][l] = row;
