@@ -99,8 +99,9 @@ struct ChunkAt {
 __device__ __forceinline__ ChunkAt chunk_at(const DeltaParams& p, int64_t c) {
   ChunkAt r;
   if (p.seq.cu == nullptr) {
-    r.n = r.b = c / p.chunks_per_b;
-    r.t0 = (c % p.chunks_per_b) * kChunk;
+    const uint32_t n = uint32_t(c) / uint32_t(p.chunks_per_b);  // (both below 2^31)
+    r.n = r.b = n;
+    r.t0 = (c - n * p.chunks_per_b) * kChunk;
     r.rows = int(min(int64_t(kChunk), p.T - r.t0));
     return r;
   }

@@ -74,17 +74,28 @@ enum { kSumState = 0, kSumKey = 1, kSumE = 2 };
 // TMEM columns; D and M stand behind the products with S (DK columns).
 constexpr uint32_t kGradOX = 0, kGradUS = 192, kGradGram = 320;
 
-// What a block works on: chunk and key head of item x, and of the next that has rows.
-struct GradItems {
-  const DeltaParams& p;
-  int64_t count;
-  __device__ __forceinline__ explicit GradItems(const DeltaParams& q) : p(q), count(q.max_chunks * q.H) {}
-  __device__ __forceinline__ int64_t from(int64_t x) const {
-    while (x < count && chunk_at(p, x % p.max_chunks).rows == 0) x += gridDim.x;
-    return x;
+// What a block works on: a chunk that has rows, and a key head; every gridDim.x-th.
+struct GradItem {
+  int64_t chunk;
+  int head;
+  ChunkAt at;
+
+  __device__ __forceinline__ explicit GradItem(const DeltaParams& p) : chunk(blockIdx.x), head(0) {
+    settle(p);
   }
-  __device__ __forceinline__ int64_t chunk(int64_t x) const { return x % p.max_chunks; }
-  __device__ __forceinline__ int head(int64_t x) const { return int(x / p.max_chunks); }
+  __device__ __forceinline__ bool here(const DeltaParams& p) const { return head < p.H; }
+  __device__ __forceinline__ void next(const DeltaParams& p) {
+    chunk += gridDim.x;
+    settle(p);
+  }
+  __device__ __forceinline__ void settle(const DeltaParams& p) {
+    for (;; chunk += gridDim.x) {
+      while (chunk >= p.max_chunks) chunk -= p.max_chunks, ++head;
+      if (head >= p.H) return;
+      at = chunk_at(p, chunk);
+      if (at.rows > 0) return;
+    }
+  }
 };
 
 // d[128 x N] (+)= A B over 16 contraction rows; the operands are tiles
@@ -121,14 +132,12 @@ __device__ __forceinline__ void grad_fetch(const DeltaParams& p, unsigned char* 
   using Sm = GradSmem<E, DK>;
   constexpr int KP = Sm::KP, NS = Sm::count;
   const uint32_t sb = smem_addr(raw);
-  const GradItems items(p);
   const int per_head = p.V / kTile, tiles = p.group * per_head;
   int n = 0, done = 0, sent = 0;  // tiles, items, and those whose Q and K are on their way
   bool ok = true;
-  for (int64_t item = items.from(blockIdx.x); item < items.count && ok;
-       item = items.from(item + gridDim.x), ++done) {
-    const int64_t chunk = items.chunk(item);
-    const int h = items.head(item);
+  for (GradItem item(p); item.here(p) && ok; item.next(p), ++done) {
+    const int64_t chunk = item.chunk;
+    const int h = item.head;
     const int64_t tile0 = (chunk * p.HV + h * p.group) * per_head;
     for (int t = 0; t <= tiles && ok; ++t) {
       if (t == min(NS, tiles)) {
@@ -165,11 +174,11 @@ __device__ __forceinline__ void grad_issue(const DeltaParams& p, uint32_t sb, Gr
   using Sm = GradSmem<E, DK>;
   constexpr int KP = Sm::KP, NS = Sm::count;
   constexpr uint32_t kGradDM = kGradOX + DK;
+  const uint32_t q = sb + Sm::qk, k = q + 1024, dn = sb + Sm::dn;
   constexpr uint32_t khigh = block_desc_high(kKeyBlock), rhigh = block_desc_high(kRowBlock);
-  const GradItems items(p);
   const int per_head = p.V / kTile;
   int x = 0, phase = 0, heads = 0, done = 0;
-  for (int64_t item = items.from(blockIdx.x); item < items.count; item = items.from(item + gridDim.x), ++done) {
+  for (GradItem item(p); item.here(p); item.next(p), ++done) {
     for (int gi = 0; gi < p.group; ++gi, ++heads) {
       if (heads > 0 && !warp_wait(wait, sy->next, heads - 1)) return;
       for (int vt = 0; vt < per_head; ++vt) {
@@ -203,8 +212,8 @@ __device__ __forceinline__ void grad_issue(const DeltaParams& p, uint32_t sb, Gr
             for (int z = 0; z < KP - y; ++z)
 #pragma unroll
               for (int ks = 0; ks < DK / 16; ++ks)
-                tc_mma_ss(tm + kGradGram, block_desc(sb + Sm::qk + y * Sm::qkpart + ks * 2 * kKeyBlock, kKeyBlock), rhigh,
-                          block_desc(sb + Sm::qk + z * Sm::qkpart + 1024 + ks * 2 * kKeyBlock, kKeyBlock), rhigh,
+                tc_mma_ss(tm + kGradGram, block_desc(q + y * Sm::qkpart + ks * 2 * kKeyBlock, kKeyBlock),
+                          rhigh, block_desc(k + z * Sm::qkpart + ks * 2 * kKeyBlock, kKeyBlock), rhigh,
                           mma_desc(64, false, false), y + z + ks > 0);
           tc_commit(smem_addr(&sy->gram));
         }
@@ -221,9 +230,9 @@ __device__ __forceinline__ void grad_issue(const DeltaParams& p, uint32_t sb, Gr
             if (y + z > 1) continue;
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
-              tc_mma_ss(tm + kGradOX, block_desc(sb + Sm::dn + y * Sm::dnpart + ks * 2 * kKeyBlock, kKeyBlock), rhigh,
-                        block_desc(sb + Sm::qk + z * Sm::qkpart + 1024 + ks * 2 * kRowBlock, kRowBlock),
-                        khigh, mma_desc(DK, true, false), true);
+              tc_mma_ss(tm + kGradOX, block_desc(dn + y * Sm::dnpart + ks * 2 * kKeyBlock, kKeyBlock), rhigh,
+                        block_desc(k + z * Sm::qkpart + ks * 2 * kRowBlock, kRowBlock), khigh,
+                        mma_desc(DK, true, false), true);
           }
 #pragma unroll
         for (int z = 0; z < KP; ++z)
@@ -232,9 +241,8 @@ __device__ __forceinline__ void grad_issue(const DeltaParams& p, uint32_t sb, Gr
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
               tc_mma_ss(tm + kGradUS,
-                        block_desc(sb + Sm::dn + rows * 1024 + ks * 2 * kRowBlock, kRowBlock), khigh,
-                        block_desc(sb + Sm::qk + z * Sm::qkpart + rows * 1024 + ks * 2 * kRowBlock,
-                                   kRowBlock),
+                        block_desc(dn + rows * 1024 + ks * 2 * kRowBlock, kRowBlock), khigh,
+                        block_desc(q + z * Sm::qkpart + rows * 1024 + ks * 2 * kRowBlock, kRowBlock),
                         khigh, mma_desc(DK, true, true), true);
         tc_commit(smem_addr(&sy->done));
       }
@@ -284,7 +292,6 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_grad_kernel(const Delta
   tc_fence_after();
   const uint32_t tm = sy->tmem;
   const Waiter wait{&sy->abort, p.timeout_ns, p.status_words, p.status_host, int(blockIdx.x)};
-  const GradItems items(p);
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
     if (warp == 8) {
@@ -297,14 +304,12 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_grad_kernel(const Delta
     } else if (warp == 10) {
       int heads = 0;
       bool ok = true;
-      for (int64_t item = items.from(blockIdx.x); item < items.count && ok;
-           item = items.from(item + gridDim.x)) {
-        const ChunkAt at = chunk_at(p, items.chunk(item));
+      for (GradItem item(p); item.here(p) && ok; item.next(p)) {
         for (int gi = 0; gi < p.group && ok; ++gi, ++heads) {
-          const int hv = items.head(item) * p.group + gi;
-          const float2 g = load_decay(p, at, hv, lane);
+          const int hv = item.head * p.group + gi;
+          const float2 g = load_decay(p, item.at, hv, lane);
           const float2* src =
-              reinterpret_cast<const float2*>(p.coef + (items.chunk(item) * p.HV + hv) * 3 * kChunk);
+              reinterpret_cast<const float2*>(p.coef + (item.chunk * p.HV + hv) * 3 * kChunk);
           const float2 c[3] = {src[lane], src[32 + lane], src[64 + lane]};
           if (heads > 0) ok = warp_wait(wait, sy->next, heads - 1);
           chunk_decay(g, sy->G, lane);
@@ -330,10 +335,9 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_grad_kernel(const Delta
     };
     bool ok = true;
     int x = 0, phase = 0, heads = 0, done = 0;
-    for (int64_t item = items.from(blockIdx.x); item < items.count && ok;
-         item = items.from(item + gridDim.x), ++done) {
-      const ChunkAt at = chunk_at(p, items.chunk(item));
-      const int h = items.head(item);
+    for (GradItem item(p); item.here(p) && ok; item.next(p), ++done) {
+      const ChunkAt& at = item.at;
+      const int h = item.head;
       float acc[DK / 2] = {};  // dQ (lanes 0-63) or dK of the lane's token
       for (int gi = 0; gi < p.group; ++gi, ++heads) {
         const int hv = h * p.group + gi;
@@ -407,7 +411,8 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_grad_kernel(const Delta
               const Far Gj = z ? Far{far2.z, far2.w} : Far{far2.x, far2.y};
               // (what is masked is replaced before it is used: no branches)
               const bool in = j < low;
-              const float v = sign * __expf(in ? minus(Gi, Gj) : 0.f) * __uint_as_float(in ? r[y + z] : 0u);
+              const float v =
+                  sign * __expf(in ? minus(Gi, Gj) : 0.f) * __uint_as_float(in ? r[y + z] : 0u);
               const float t = v * __uint_as_float(in ? g[y + z] : 0u);
               own = j == i ? t : own;
               cs[y + z] = j < i ? t : 0.f;
@@ -451,7 +456,9 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_grad_kernel(const Delta
 #pragma unroll
           for (int z = 0; z < 2; ++z) {
             const int t = 2 * lane + z;
-            auto sum = [&](int which, int from) { return sy->sums[which][0][from] + sy->sums[which][1][from]; };
+            auto sum = [&](int which, int from) {
+              return sy->sums[which][0][from] + sy->sums[which][1][from];
+            };
             const float ga = coef[t], w = coef[kChunk + t], bt = coef[2 * kChunk + t];
             const float key = sum(kSumKey, t) + sum(kSumKey, 64 + t);
             const float col = (sy->cols[0][t] + sy->cols[1][t]) + (sy->cols[2][t] + sy->cols[3][t]);

@@ -497,7 +497,8 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         for (int i = 0; i < 32; ++i) w[i] = S[32 * x + i];
         split_to_tmem(w, lanes + cS + half * (DK / 2) + 16 * x, sStep, hi, lo);
         if constexpr (MODE == 1) {
-          unsigned char* dst = channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::shi, half * (DK / 2) + 32 * x);
+          unsigned char* dst =
+              channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::shi, half * (DK / 2) + 32 * x);
           store_pairs(dst, hi, live);
           store_pairs(dst - GT::part, lo, live);
         }
