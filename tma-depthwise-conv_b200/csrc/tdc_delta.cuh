@@ -340,15 +340,14 @@ __device__ __forceinline__ void store_lower(__nv_bfloat16* dst, const unsigned c
   }
 }
 
-// Rows of K or Q to their parts, 8 columns of the rows of both together.
+// Q's rows (threads 0-63) and K's to their parts, 8 columns of all rows together.
 constexpr int kKeyBlock = 2 * kChunk * 16;  // bytes of 8 columns
 template <class E, int DK>
-__device__ __forceinline__ void store_keys(unsigned char* dst, const unsigned char* tile, int tid,
-                                           int threads) {
-  for (int e = tid; e < kChunk * (DK / 8); e += threads) {
-    const int r = e & 63, c = e >> 6;
-    const uint4 v = *reinterpret_cast<const uint4*>(tile + 2 * (r * (DK + 8) + 8 * c));
-    uint4* d = reinterpret_cast<uint4*>(dst + c * kKeyBlock + r * 16);
+__device__ __forceinline__ void store_keys(unsigned char* dst, const unsigned char* row, int tid) {
+#pragma unroll
+  for (int c = 0; c < DK / 8; ++c) {
+    const uint4 v = *reinterpret_cast<const uint4*>(row + 16 * c);
+    uint4* d = reinterpret_cast<uint4*>(dst + c * kKeyBlock + tid * 16);
     if constexpr (std::is_same_v<E, BF16>) {
       *d = v;
     } else {
@@ -364,7 +363,7 @@ __device__ __forceinline__ void store_keys(unsigned char* dst, const unsigned ch
 }
 
 template <class E, int DK>
-__global__ void __launch_bounds__(128) delta_prepare_kernel(const DeltaParams p) {
+__global__ void __launch_bounds__(128, 4) delta_prepare_kernel(const DeltaParams p) {
   extern __shared__ __align__(1024) unsigned char raw[];
   using Sm = PrepareSmem<DK>;
   constexpr int ld = Sm::ld, part = Sm::part;
@@ -416,8 +415,7 @@ __global__ void __launch_bounds__(128) delta_prepare_kernel(const DeltaParams p)
   {
     constexpr int64_t bytes = int64_t(std::is_same_v<E, BF16> ? 1 : 2) * kChunk * DK * 2;
     unsigned char* kq = p.kq + (chunk * p.H + h) * 2 * bytes;
-    store_keys<E, DK>(kq, raw + Sm::q, tid, 128);
-    store_keys<E, DK>(kq + kChunk * 16, raw + Sm::k, tid, 128);
+    store_keys<E, DK>(kq, raw + (tid < kChunk ? Sm::q : Sm::k) + 2 * (tid & 63) * ld, tid);
   }
   const int g = lane >> 2, t2 = (lane & 3) * 2;
   for (int gi = 0; gi < p.group; ++gi) {
