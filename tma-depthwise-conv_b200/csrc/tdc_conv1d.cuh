@@ -125,21 +125,28 @@ __global__ void __launch_bounds__(256, 2) conv1d_fwd_kernel(const Conv1dParams p
   const int64_t xbase = b * p.x_sb;
   const uint16_t* x = static_cast<const uint16_t*>(p.x) + xbase + t0 * p.x_st + c;
   uint16_t* y = static_cast<uint16_t*>(p.y) + (b * p.T + t0) * p.C + c;
-  SeqSpan s{b, 0, p.T, true};
-  if (PACKED) s = span_at(p.seq, b, t0);
-
-  // win: the K-1 inputs before the first of 4 rows, then those rows.
+  // win: the K-1 inputs before the first of 4 rows, then those rows.  What does not
+  // depend on the sequences is on its way before they are looked up.
   uint4 win[K + 3], next[4], w[K];
 #pragma unroll
   for (int u = 0; u < 4; ++u)
     if (u < rows) next[u] = ld16(x, u * p.x_st);
 #pragma unroll
   for (int j = 0; j < K - 1; ++j)
-    win[j] = s.covered ? conv_input(p, K, s, xbase, t0 - (K - 1) + j, c) : make_uint4(0, 0, 0, 0);
+    if (t0 >= K - 1 - j) win[j] = ld16(x, (j - (K - 1)) * p.x_st);
 #pragma unroll
   for (int j = 0; j < K; ++j) w[j] = ld16(p.w, j * p.C + c);
-  float bias[8] = {};
-  if (p.bias != nullptr) unpack8<E>(ld16(p.bias, c), bias);
+  uint4 b8 = make_uint4(0, 0, 0, 0);
+  if (p.bias != nullptr) b8 = ld16(p.bias, c);
+  SeqSpan s{b, 0, p.T, true};
+  if (PACKED) s = span_at(p.seq, b, t0);
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j) {
+    if (!s.covered) win[j] = make_uint4(0, 0, 0, 0);
+    else if (t0 - (K - 1) + j < s.lo) win[j] = conv_input(p, K, s, xbase, t0 - (K - 1) + j, c);
+  }
+  float bias[8];
+  unpack8<E>(b8, bias);
 
   for (int t = 0; t < rows; t += 4) {
 #pragma unroll
@@ -148,27 +155,36 @@ __global__ void __launch_bounds__(256, 2) conv1d_fwd_kernel(const Conv1dParams p
 #pragma unroll
     for (int u = 0; u < 4; ++u)
       if (t + 4 + u < rows) next[u] = ld16(x, u * p.x_st);
+    auto put = [&](int u, bool covered) {
+      float z[8];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (t + u < rows) {
-        if (PACKED && t0 + t + u >= s.hi) {  // the next sequence (or gap) starts here
-          s = span_from(p.seq, s.n, t0 + t + u);
-          if (s.covered) {
+      for (int i = 0; i < 8; ++i) z[i] = bias[i];
+      conv_dot<E, K>(z, win + u, w);
+      if constexpr (SILU) {
 #pragma unroll
-            for (int j = 0; j < K - 1; ++j)
-              win[u + j] = conv_input(p, K, s, xbase, s.lo - (K - 1) + j, c);
+        for (int i = 0; i < 8; ++i) z[i] *= sigmoid_f(z[i]);
+      }
+      st16(y, 0, covered ? pack8<E>(z) : make_uint4(0, 0, 0, 0));
+      y += p.C;
+    };
+    if (t + 4 <= rows && (!PACKED || (s.covered && t0 + t + 4 <= s.hi))) {
+      // in the inside of a run and a sequence: no tests between the rows
+#pragma unroll
+      for (int u = 0; u < 4; ++u) put(u, true);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (t + u < rows) {
+          if (PACKED && t0 + t + u >= s.hi) {  // the next sequence (or gap) starts here
+            s = span_from(p.seq, s.n, t0 + t + u);
+            if (s.covered) {
+#pragma unroll
+              for (int j = 0; j < K - 1; ++j)
+                win[u + j] = conv_input(p, K, s, xbase, s.lo - (K - 1) + j, c);
+            }
           }
+          put(u, s.covered);
         }
-        float z[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) z[i] = bias[i];
-        conv_dot<E, K>(z, win + u, w);
-        if constexpr (SILU) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) z[i] *= sigmoid_f(z[i]);
-        }
-        st16(y, 0, !PACKED || s.covered ? pack8<E>(z) : make_uint4(0, 0, 0, 0));
-        y += p.C;
       }
     }
 #pragma unroll
