@@ -7,6 +7,9 @@
 // that fma.rn.f32.{f16,bf16} takes without conversion; consecutive threads own
 // consecutive channels, so every access of a warp is whole 128-byte lines and
 // needs no shared memory.  Four rows are loaded ahead of their use.
+// Measured (K = 4, SiLU): 8192 rows of 8192 channels in bf16 (268 MB) 50 us,
+// 5.3 TB/s of the 6.46 that a copy reaches; 5003 packed rows of 2560 in fp16
+// (51 MB) about 13 us, the latency of one wave of blocks.
 #pragma once
 
 #include "tdc_seq_common.cuh"
@@ -204,6 +207,9 @@ __global__ void __launch_bounds__(256, 2) conv1d_fwd_kernel(const Conv1dParams p
 // The K-1 values of dz behind the run are recomputed.  The runs of a block are
 // added in shared memory and one partial sum per block goes to the workspace,
 // which conv1d_wsum_kernel adds in a fixed order.
+// Measured (K = 4, SiLU, bf16, 8192 rows of 8192 channels, 403 MB): 101 us,
+// 4.0 TB/s; what is left is latency, with the 512 threads an SM that the taps'
+// sums leave room for.  conv1d_wsum_kernel: 5.6 us.
 constexpr int kGradVec = 4;
 
 struct Quad {  // 4 channels
@@ -437,7 +443,8 @@ __global__ void __launch_bounds__(128) conv1d_dinit_kernel(const Conv1dParams p)
 // ---- running sequences ---------------------------------------------------------
 // One thread takes 8 channels of one request: K-1 state rows in, T inputs
 // through the window, K-1 rows out.  Bound by latency at the usual sizes: all
-// loads of a thread are independent.
+// loads of a thread are independent.  4 requests of 8192 channels: 4.7 us with
+// cold caches, less than the call takes on the host.
 template <class E, int K, bool SILU>
 __global__ void __launch_bounds__(128) conv1d_step_kernel(const Conv1dParams p) {
   const int64_t b = blockIdx.x;

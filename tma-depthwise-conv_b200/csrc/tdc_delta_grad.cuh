@@ -31,6 +31,13 @@
 // go through shuffles.  It puts the products with the states back scaled, so that
 // the last products add to them in place.  Warp 8 issues the products, warp 9 the
 // copies (also the next chunk's), warp 10 brings the decays.
+//
+// 8192 tokens of 16 key and 32 value heads of 128 x 128 (bf16): 852 MB of workspace
+// in 265 us, 3.2 TB/s.  A head's 8 tiles take about 8000 cycles, in which shared
+// memory (copies, the products' operands and <dS, S> share its 128 bytes a cycle)
+// and memory are both near their rates; finishing a head takes 9000 more, in which
+// only the copies go on: TMEM has no room for the sums of two heads.  With warp
+// matrix instructions and accumulators in registers it took 500 us.
 #pragma once
 
 #include "tdc_delta_walk.cuh"

@@ -1,6 +1,6 @@
 // tdc_tc.cuh — thin wrappers of the 5th-generation tensor core instructions:
-// TMEM allocation, loads and stores, tcgen05.mma with A in TMEM and B in shared
-// memory, and untiled bulk copies.  Every instruction is spelled out.
+// TMEM allocation, loads and stores, tcgen05.mma with A in TMEM or shared memory and
+// B in shared memory, and untiled bulk copies.  Every instruction is spelled out.
 #pragma once
 
 #include "tdc_ptx.cuh"
@@ -96,9 +96,8 @@ __device__ __forceinline__ uint32_t tile_desc(uint32_t addr, bool n_major) {
 __host__ __device__ constexpr uint32_t tile_desc_high(bool n_major) {
   return ((n_major ? kColBlock : kRowBlock) >> 4) | 1u << 14;
 }
-// The same for tiles whose 8 x 8 blocks lie `lead` (along the contraction; K-major)
-// and `stride` (along M or N) bytes apart; N-major (or M-major) the other way round
-// in what a block's rows are, not in the words: lead is along the contraction.
+// The same for any tile of 8 x 8 blocks of 128 bytes: `lead` bytes from one to the
+// next along the contraction, `stride` along M or N.
 __device__ __forceinline__ uint32_t block_desc(uint32_t addr, uint32_t lead) {
   return (addr >> 4) | (lead >> 4) << 16;
 }
