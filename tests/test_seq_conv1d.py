@@ -87,6 +87,18 @@ def test_packed(cu, state, dtype):
     _check(_run(c, "silu", cu_dtype=torch.int64 if state else torch.int32), _want(c, "silu"))
 
 
+@pytest.mark.parametrize("B,T,C,cu", [(1, 5000, 1024, None), (3, 1700, 1024, None),
+                                      (1, 5000, 1024, [2, 3, 9, 9, 17, 40, 1000, 1001, 1007, 2500, 4321, 4990]),
+                                      (1, 5000, 1024, [0, 8, 12, 16, 20, 21, 22, 23, 24, 36, 4996, 5000])])
+@pytest.mark.parametrize("K,dtype,state", [(2, "bf16", True), (4, "fp16", False), (8, "bf16", True)])
+def test_forward_in_runs_of_several_rows(B, T, C, cu, K, dtype, state):
+    c = _case(B, T, C, K, dtype, True, state, cu, seed=K)
+    got = _run(c, "silu", grads=False)
+    y, f = R.conv(*(None if c[n] is None else c[n].double() for n in ("x", "w", "bias")), "silu",
+                  None if c["state"] is None else c["state"].double(), cu)
+    _check(got, {"y": y, "final": f})
+
+
 def test_no_rows_gives_the_state_back():
     c = _case(2, 0, 16, 4, "fp16", True, True, None)
     got = _run(c, "silu")

@@ -158,6 +158,19 @@ def test_long_sequences_in_segments(B, T, H, HV, K, V, state, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,T,H,HV,K,V,dtype,cu", [
+    (3, 200, 14, 28, 64, 64, "bf16", None),               # 168 chunks and key heads
+    (2, 640, 16, 16, 128, 64, "fp16", None),              # 320, several a block
+    (1, 330, 30, 30, 128, 256, "bf16", None),             # 180, 16 tiles of channels a head
+    (1, 260, 31, 31, 64, 128, "fp16", [0, 1, 1, 70, 200, 200, 255]),
+    (1, 40, 8, 16, 64, 64, "bf16", [min(i, 40) for i in range(60)]),  # most have no rows
+    (1, 64, 1, 8, 128, 128, "fp16", None)])               # one of 8 heads
+def test_gradients_of_more_chunks_and_heads_than_blocks(B, T, H, HV, K, V, dtype, cu):
+    c = _case(B, T, H, HV, K, V, dtype, state=True, cu=cu, seed=T)
+    _check(_run(c), _want(c))
+
+
+@pytest.mark.gpu
 def test_no_rows_gives_the_state_back():
     c = _case(2, 0, 1, 2, 64, 64, "bf16", state=True)
     got = _run(c)

@@ -77,6 +77,7 @@ struct GradSync {
   float diag[kChunk];          // P D on it
   float dot[8];
 };
+static_assert(sizeof(GradSync) <= 7168, "see kMaxBytes");
 enum { kSumState = 0, kSumKey = 1, kSumE = 2 };
 // TMEM columns; D and M stand behind the products with S (DK columns).
 constexpr uint32_t kGradOX = 0, kGradUS = 192, kGradGram = 320;

@@ -525,14 +525,12 @@ TDC_API int tdc_conv1d_fwd(const tdc_conv1d_args* a, void* stream) {
   // with several equal ones if they were longer than 128 rows.  Against the shortest
   // runs that give each SM 1024 threads (at most 32 rows), K = 4: 1500 rows of 2560
   // channels 14.1 -> 11.4 us, 5003 rows 20.5 -> 16.4, 9000 rows of 8192 61.4 -> 57.8.
-  // (The blocks behind them that copy final states belong to the wave.)
-  const int64_t tail = a->final_state != nullptr ? p.seq.n * (a->K - 1) * vecs : 0;
-  const int64_t wave = 2 * kSms * 256 - std::min<int64_t>(ceil_div(tail, 256), kSms) * 256;
-  const int64_t work = a->B * a->T * vecs;
+  const int64_t wave = 2 * kSms * 256, work = a->B * a->T * vecs;
   const int64_t waves = std::max<int64_t>(1, ceil_div(work, wave * 128));
   p.runs_per_b = ceil_div(a->T, std::max<int64_t>(1, ceil_div(work, wave * waves)));
   p.run = int(std::min<int64_t>(ceil_div(a->T, std::max<int64_t>(1, p.runs_per_b)), 1 << 30));
   p.main_threads = a->B * p.runs_per_b * vecs;
+  const int64_t tail = a->final_state != nullptr ? p.seq.n * (a->K - 1) * vecs : 0;
   const int64_t blocks = ceil_div(p.main_threads + tail, 256);
   if (blocks > 0x7fffffff) return TDC_ERR_TOO_LARGE;
   rc = prepare_device();
