@@ -302,33 +302,48 @@ __device__ __forceinline__ float* segment_state(const DeltaParams& p, float* bas
 // The states between the segments, S_(i+1) = M_i S_i + N_i (N_i is in S_(i+1)'s
 // place), in fp32: a block has 32 columns of a head's state, one a lane, a warp
 // DK / 8 of its rows.  M comes through shared memory, in whole lines.  Bound by
-// the latency of the segments one after another: 12 us for 3 segments of 32 heads.
+// the latency of the segments one after another: 11 us for 3 segments of 32 heads
+// (12 without the next one's M on its way).
 template <int DK>
 __global__ void __launch_bounds__(256) delta_join_kernel(const DeltaParams p) {
   constexpr int R = DK / 8;
-  extern __shared__ __align__(16) float sh[];  // M [DK][DK], S [DK][32]
-  float* S = sh + DK * DK;
+  extern __shared__ __align__(16) float sh[];  // M [2][DK][DK], S [DK][32]
+  float* S = sh + 2 * DK * DK;
   const int tid = threadIdx.x, lane = tid & 31, k0 = (tid >> 5) * R, v0 = blockIdx.y * 32;
   const int64_t n = blockIdx.x / p.HV;
   const int hv = int(blockIdx.x % p.HV);
-  float acc[R];
-  for (int i = 1; i < p.segments; ++i) {
-    float* at = segment_state(p, p.seg_s, n, hv, i, DK, p.V) + int64_t(k0) * p.V + v0 + lane;
+  auto state = [&](int i) {
+    return segment_state(p, p.seg_s, n, hv, i, DK, p.V) + int64_t(k0) * p.V + v0 + lane;
+  };
+  auto fetch = [&](int i) {  // M of inner segment i, one ahead
+    const float* m = segment_state(p, p.seg_m, n, hv, i, DK, DK);
+    const uint32_t dst = smem_addr(sh + (i & 1) * DK * DK);
+    for (int e = 4 * tid; e < DK * DK; e += 4 * 256) cp_async16(dst + 4 * e, m + e, true);
+    cp_async_commit();
+  };
+  float acc[R], next[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) acc[r] = at[int64_t(r) * p.V];
+  for (int r = 0; r < R; ++r) next[r] = state(1)[int64_t(r) * p.V];
+  for (int i = 1; i < p.segments; ++i) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[r] = next[r];
+    const bool more = i + 1 < p.segments;
+    if (more) {
+      fetch(i);
+#pragma unroll
+      for (int r = 0; r < R; ++r) next[r] = state(i + 1)[int64_t(r) * p.V];
+    }
     if (i > 1) {
-      const float4* m = reinterpret_cast<const float4*>(
-          segment_state(p, p.seg_m, n, hv, i - 1, DK, DK));
-#pragma unroll 4
-      for (int e = tid; e < DK * DK / 4; e += 256) reinterpret_cast<float4*>(sh)[e] = m[e];
+      if (more) cp_async_wait<1>(); else cp_async_wait<0>();
       __syncthreads();
+      const float* m = sh + ((i - 1) & 1) * DK * DK;
       for (int x = 0; x < DK; x += 4) {
         float s[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) s[u] = S[(x + u) * 32 + lane];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const float4 w = *reinterpret_cast<const float4*>(sh + (k0 + r) * DK + x);
+          const float4 w = *reinterpret_cast<const float4*>(m + (k0 + r) * DK + x);
           acc[r] = fmaf(w.x, s[0], acc[r]);
           acc[r] = fmaf(w.y, s[1], acc[r]);
           acc[r] = fmaf(w.z, s[2], acc[r]);
@@ -336,7 +351,7 @@ __global__ void __launch_bounds__(256) delta_join_kernel(const DeltaParams p) {
         }
       }
 #pragma unroll
-      for (int r = 0; r < R; ++r) at[int64_t(r) * p.V] = acc[r];
+      for (int r = 0; r < R; ++r) state(i)[int64_t(r) * p.V] = acc[r];
     }
     __syncthreads();
 #pragma unroll
@@ -355,7 +370,7 @@ __global__ void __launch_bounds__(256) delta_join_kernel(const DeltaParams p) {
 // stand in the channels' place); delta_join_kernel makes the states between the
 // segments; pass 2 walks all but the first from them.  Two passes of a
 // segment's length replace one of the whole: one sequence of 8192 tokens with 32
-// heads takes 138 + 12 + 140 us instead of 420.
+// heads takes 138 + 11 + 140 us instead of 420.
 template <class E, int DK, int MODE>
 __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const DeltaParams p) {
   extern __shared__ __align__(1024) unsigned char raw[];

@@ -325,7 +325,7 @@ int64_t delta_chunks(const tdc_delta_args* a) {
 // block of both passes an SM of its own, if two passes over a segment (and about
 // 6 chunks' time for the second launch and the join) are shorter than one over
 // the whole.  Packed batches' lengths are not known here: they are walked whole.
-// One sequence of 8192 tokens with 32 heads: 348 us in 3 segments, 500 whole.
+// One sequence of 8192 tokens with 32 heads: 344 us in 3 segments, 500 whole.
 int delta_segments(const tdc_delta_args* a) {
   if (a->cu_seqlens != nullptr) return 1;
   const int64_t chunks = ceil_div(a->T, tdc::kChunk), heads = a->B * a->HV;
@@ -442,7 +442,7 @@ int delta_fwd_t(tdc::DeltaParams& p, cudaStream_t st) {
   p.pass = 1;
   rc = delta_walk<E, DK>(k, p, p.seq.n * (tiles * (1 + inner) + inner), st);
   if (rc != TDC_OK) return rc;
-  const size_t smem = (DK * DK + DK * 32) * sizeof(float);
+  const size_t smem = (2 * DK * DK + DK * 32) * sizeof(float);
   rc = allow_smem(&tdc::delta_join_kernel<DK>, smem);
   if (rc != TDC_OK) return rc;
   tdc::delta_join_kernel<DK>
@@ -455,9 +455,9 @@ int delta_fwd_t(tdc::DeltaParams& p, cudaStream_t st) {
 template <class E, int DK>
 int delta_bwd_t(const tdc::DeltaParams& p, cudaStream_t st) {
   int rc = delta_prepare<E, DK>(p, st);
-  if (rc == TDC_OK) rc = delta_walk<E, DK>(&tdc::delta_walk_kernel<E, DK, 1>, p, p.seq.n * ceil_div(p.V, 128), st);
-  if (rc == TDC_OK)
-    rc = delta_walk<E, DK>(&tdc::delta_walk_back_kernel<E, DK>, p, p.seq.n * ceil_div(p.V, 128), st);
+  const int64_t blocks = p.seq.n * ceil_div(p.V, 128);
+  if (rc == TDC_OK) rc = delta_walk<E, DK>(&tdc::delta_walk_kernel<E, DK, 1>, p, blocks, st);
+  if (rc == TDC_OK) rc = delta_walk<E, DK>(&tdc::delta_walk_back_kernel<E, DK>, p, blocks, st);
   if (rc != TDC_OK || p.max_chunks == 0) return rc;
   auto* k = &tdc::delta_grad_kernel<E, DK>;
   const size_t smem = tdc::GradSmem<E, DK>::sync + sizeof(tdc::GradSync);
