@@ -12,13 +12,12 @@
 // in a third file.
 //
 // Precision: states, decays, sums and all accumulators are fp32.  An fp32
-// operand of a matrix instruction is split into two bf16 parts (16 bits of
-// mantissa or more; fp16 inputs are split as well, exactly), since one bf16
-// rounding (2^-9) at each of the chain's operands would put about 3e-3 on
-// every output, more than the output's own rounding, and the final state is
-// fp32: with the split it is off by 4e-6, dg by 7e-6 (relative to the norm; fp32
-// throughout gives 2e-7).  Two fp16 parts would reach that, but fp16's range
-// would turn the products of keys with a norm far above 1 into infinities.
+// operand of a matrix instruction is split into three bf16 parts, which hold it
+// exactly (fp16 inputs into two, exactly too): one bf16 rounding (2^-9) at each of the
+// chain's operands would put about 3e-3 on every output, and two parts 4e-6 on the
+// fp32 final state, twenty times what fp32 throughout gives.  Two fp16 parts have
+// nearly fp32's bits, but fp16's range would turn the products of keys with a norm far
+// above 1 into infinities.
 #pragma once
 
 #include "tdc_dwconv.h"
@@ -76,7 +75,7 @@ struct DeltaParams {
   float* seg_m;           // [N][HV][segments][K][K]: what a segment makes of a state
   // workspace of all chunks, [chunk][HV] each
   // (tiles in the order of WalkTiles; 8 x 8 blocks, see tdc_tc.cuh)
-  __nv_bfloat16* tp;      // T and P, high parts and remainders: [4][64 x 64]
+  __nv_bfloat16* tp;      // T in its three parts, then P: [6][64 x 64]
   float* coef;            // [3][64]: gam, w, beta
   unsigned char* kq;      // [chunk][H]: [parts][K / 8][Q's 64 rows, K's 64 rows][8]
   uint64_t timeout_ns;    // of the bounded waits
@@ -268,12 +267,12 @@ template <int DK>
 struct PrepareSmem {
   static constexpr int ld = DK + 8;
   static constexpr int part = kChunk * kLdT * 2;       // one [64][72] tile
-  static constexpr int q = 0;                          // [64][ld], later T hi, lo and P hi
+  static constexpr int q = 0;                          // [64][ld]
   static constexpr int k = kChunk * ld * 2;            // [64][ld]
-  static constexpr int t = 0;
-  static constexpr int p = 2 * part;
-  static constexpr int a = 2 * kChunk * ld * 2 > 4 * part ? 2 * kChunk * ld * 2 : 4 * part;
-  static constexpr int G = a + 2 * part;               // Far [64]
+  static constexpr int t = 0;                          // T and A by parts, once Q and K are used
+  static constexpr int a = 3 * part;
+  static constexpr int G = a + 3 * part;               // Far [64]
+  static_assert(2 * kChunk * ld * 2 <= G, "Q and K");
   static constexpr int beta = G + 64 * 8;
   static constexpr int bytes = beta + 64 * 4;
 };
@@ -287,45 +286,45 @@ __device__ __forceinline__ void join_inverse(uint32_t a, uint32_t t, int o, int 
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
     if (16 * ks < c0) continue;  // P' is lower triangular: nothing is stored above
-    uint32_t ph[4], pl[4];
-    ldsm4_t(ph, addr_at(t, kLdT, o + c0, o + 16 * ks, lane));
-    ldsm4_t(pl, addr_at(t + part, kLdT, o + c0, o + 16 * ks, lane));
+    uint32_t pp[3][4];
+#pragma unroll
+    for (int y = 0; y < 3; ++y)
+      ldsm4_t(pp[y], addr_at(t + y * part, kLdT, o + c0, o + 16 * ks, lane));
 #pragma unroll
     for (int np = 0; np < NT / 2; ++np) {
-      uint32_t bh[4], bl[4];
-      ldsm4(bh, addr_b(a, kLdT, o + n + 16 * np, o + 16 * ks, lane));
-      ldsm4(bl, addr_b(a + part, kLdT, o + n + 16 * np, o + 16 * ks, lane));
+      uint32_t b[3][4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        mma_split(w[2 * np + i], ph, pl, bh[2 * i], bh[2 * i + 1], bl[2 * i], bl[2 * i + 1]);
+      for (int y = 0; y < 3; ++y)
+        ldsm4(b[y], addr_b(a + y * part, kLdT, o + n + 16 * np, o + 16 * ks, lane));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) mma_split(w[2 * np + i], pp, b, 2 * i);
     }
   }
   float x[NT][4] = {};
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
-    uint32_t wh[4], wl[4];
-    split_frag(w[2 * ks], w[2 * ks + 1], wh, wl);
+    uint32_t wp[3][4];
+    split_frag(w[2 * ks], w[2 * ks + 1], wp);
 #pragma unroll
     for (int np = ks; np < NT / 2; ++np) {
-      uint32_t rh[4], rl[4];
-      ldsm4(rh, addr_b(t, kLdT, o + n + 16 * np, o + n + 16 * ks, lane));
-      ldsm4(rl, addr_b(t + part, kLdT, o + n + 16 * np, o + n + 16 * ks, lane));
+      uint32_t r[3][4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        mma_split(x[2 * np + i], wh, wl, rh[2 * i], rh[2 * i + 1], rl[2 * i], rl[2 * i + 1]);
+      for (int y = 0; y < 3; ++y)
+        ldsm4(r[y], addr_b(t + y * part, kLdT, o + n + 16 * np, o + n + 16 * ks, lane));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) mma_split(x[2 * np + i], wp, r, 2 * i);
     }
   }
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {  // X^T's tiles into rows o + n .. of T
-    uint32_t hi[4], lo[4];
+    float v[2][4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float* v = x[2 * ks + i];
-      split2(-v[0], -v[1], hi[2 * i], lo[2 * i]);
-      split2(-v[2], -v[3], hi[2 * i + 1], lo[2 * i + 1]);
-    }
-    stsm4_t(addr_at(t, kLdT, o + c0, o + n + 16 * ks, lane), hi);
-    stsm4_t(addr_at(t + part, kLdT, o + c0, o + n + 16 * ks, lane), lo);
+    for (int i = 0; i < 8; ++i) v[i / 4][i % 4] = -x[2 * ks + i / 4][i % 4];
+    uint32_t xp[3][4];
+    split_frag(v[0], v[1], xp);
+#pragma unroll
+    for (int y = 0; y < 3; ++y)
+      stsm4_t(addr_at(t + y * part, kLdT, o + c0, o + n + 16 * ks, lane), xp[y]);
   }
 }
 
@@ -335,10 +334,10 @@ __device__ __forceinline__ int block_offset(int r, int c) {
   return c * (kChunk * 8) + r * 8;
 }
 
-// Blocks on and below the diagonal of a split [64][64] tile, to [2][64 x 64].
+// Blocks on and below the diagonal of a split [64][64] tile, to [3][64 x 64].
 __device__ __forceinline__ void store_lower(__nv_bfloat16* dst, const unsigned char* tile, int tid,
                                             int threads) {
-  for (int e = tid; e < 2 * kChunk * 8; e += threads) {
+  for (int e = tid; e < 3 * kChunk * 8; e += threads) {
     const int r = e & 63, c = (e >> 6) & 7, part = e >> 9;
     if (c < 2 * (r / 16 + 1))
       *reinterpret_cast<uint4*>(dst + part * kSq + block_offset(r, c)) =
@@ -427,6 +426,7 @@ __global__ void __launch_bounds__(128, 4) delta_prepare_kernel(const DeltaParams
   for (int gi = 0; gi < p.group; ++gi) {
     const int hv = h * p.group + gi;
     const int64_t slot = chunk * p.HV + hv;
+    __nv_bfloat16* tp = p.tp + slot * 6 * kSq;
     __syncthreads();  // q and k, or the last head's tiles, are free
     if (warp == 0) chunk_decay(decay, G, lane);
     if (tid >= 64) sB[tid - 64] = beta;
@@ -459,14 +459,14 @@ __global__ void __launch_bounds__(128, 4) delta_prepare_kernel(const DeltaParams
         if (nt >= 2 * warp)
           *reinterpret_cast<float2*>(raw + Sm::t + diag_offset(warp, g + 8 * half) +
                                      4 * (j - 16 * warp)) = make_float2(av[0], av[1]);
-        uint32_t hi, lo;
-        const int off = 2 * (i * kLdT + j);
-        split2(pv[0], pv[1], hi, lo);
-        *reinterpret_cast<uint32_t*>(raw + Sm::p + off) = hi;
-        *reinterpret_cast<uint32_t*>(raw + Sm::p + part + off) = lo;
-        split2(av[0], av[1], hi, lo);
-        *reinterpret_cast<uint32_t*>(raw + Sm::a + off) = hi;
-        *reinterpret_cast<uint32_t*>(raw + Sm::a + part + off) = lo;
+        uint32_t pp[3], ap[3];
+        split3(pv[0], pv[1], pp);
+        split3(av[0], av[1], ap);
+#pragma unroll
+        for (int y = 0; y < 3; ++y) {  // (a warp's 8 rows of P are a whole line)
+          *reinterpret_cast<uint32_t*>(tp + (3 + y) * kSq + block_offset(i, nt) + t2) = pp[y];
+          *reinterpret_cast<uint32_t*>(raw + Sm::a + y * part + 2 * (i * kLdT + j)) = ap[y];
+        }
       }
     }
     __syncwarp();
@@ -479,20 +479,22 @@ __global__ void __launch_bounds__(128, 4) delta_prepare_kernel(const DeltaParams
 #pragma unroll
         for (int m = 0; m < i; ++m) v = fmaf(-d[m], x[m], v);
         x[i] = v;
-        const __nv_bfloat16 hi = __float2bfloat16_rn(v);
         __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(raw + Sm::t) +
                              (16 * warp + i) * kLdT + 16 * warp + lane;
-        dst[0] = hi;
-        dst[part / 2] = __float2bfloat16_rn(v - __bfloat162float(hi));
+#pragma unroll
+        for (int y = 0; y < 3; ++y) {
+          const __nv_bfloat16 r = __float2bfloat16_rn(v);
+          dst[y * (part / 2)] = r;
+          v -= __bfloat162float(r);
+        }
       }
     }
     __syncthreads();
     if (warp < 2) join_inverse<16>(sb + Sm::a, sb + Sm::t, 32 * warp, 0, lane);
-    else store_lower(p.tp + slot * 4 * kSq + 2 * kSq, raw + Sm::p, tid - 64, 64);
     __syncthreads();
     if (warp < 2) join_inverse<32>(sb + Sm::a, sb + Sm::t, 0, 16 * warp, lane);
     __syncthreads();
-    store_lower(p.tp + slot * 4 * kSq, raw + Sm::t, tid, 128);
+    store_lower(tp, raw + Sm::t, tid, 128);
   }
 }
 

@@ -41,8 +41,8 @@ struct WalkTiles {
   static constexpr int q = 0;
   static constexpr int k = kChunk * 16;
   static constexpr int t = KP * keys;
-  static constexpr int p = t + 2 * kSq * 2;
-  static constexpr int coef = p + 2 * kSq * 2;
+  static constexpr int p = t + 3 * kSq * 2;
+  static constexpr int coef = p + 3 * kSq * 2;
   static constexpr int stage = coef + 3 * kChunk * 4;
 };
 
@@ -55,6 +55,7 @@ struct WalkSync {
   uint32_t tmem;
   int abort;
 };
+static_assert(2 * WalkTiles<F16, 128>::stage + sizeof(WalkSync) <= 232448, "a block's shared memory");
 
 // Three warpgroups; the third (products, copies) hands registers to the two that
 // compute: 2 x 128 x 216 + 128 x 72 = 384 x 168, what the block starts with.
@@ -79,14 +80,24 @@ struct Waiter {
   }
 };
 
-// v as bf16 high parts and remainders, 16 packed columns each, to TMEM columns
-// at and at + step; both are left in hi and lo.
-__device__ __forceinline__ void split_to_tmem(const float (&v)[32], uint32_t at, uint32_t step,
-                                              uint32_t (&hi)[16], uint32_t (&lo)[16]) {
+// v as three bf16 parts (split3), 16 packed columns each: keep(part, columns) gets them
+// one after another.  v is used up.
+template <class Keep>
+__device__ __forceinline__ void split_parts(float (&v)[32], Keep keep) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) split2(v[2 * i], v[2 * i + 1], hi[i], lo[i]);
-  tmem_st(at, hi);
-  tmem_st(at + step, lo);
+  for (int part = 0; part < 3; ++part) {
+    uint32_t r[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      r[i] = pack2_rn<BF16>(v[2 * i], v[2 * i + 1]);
+      if (part < 2) fma2<BF16>(r[i], 0xBF80BF80u, v[2 * i], v[2 * i + 1]);
+    }
+    keep(part, r);
+  }
+}
+// The parts to TMEM columns at, at + step, at + 2 step.
+__device__ __forceinline__ void split_to_tmem(float (&v)[32], uint32_t at, uint32_t step) {
+  split_parts(v, [&](int part, const uint32_t (&r)[16]) { tmem_st(at + part * step, r); });
 }
 
 // For whole warps: all lanes go on, or none does.
@@ -103,50 +114,65 @@ __device__ __forceinline__ void operand_ready(uint64_t& bar, int lane) {
   if (lane == 0) mbar_arrive(smem_addr(&bar));
 }
 
-// d[128 x N] (+)= A B; A split in two parts, B the rows of Q or K at b in BP parts
-// bstep bytes apart, their tokens (n_major false) or their columns as N, DEPTH
-// elements of the contraction.  The remainders' product is left out.  A's parts start at a and
-// a + astep (columns); the state's (STATE) lie in halves, high parts and remainders
-// of each in the columns of the update that the same threads read before.
-template <int DEPTH, int N, bool N_MAJOR, int BP, bool STATE>
-__device__ __forceinline__ void issue_product(uint32_t d, uint32_t a, uint32_t astep, uint32_t b,
-                                              uint32_t bstep, bool accumulate) {
+// Where the three parts of an A operand lie in TMEM, 8 columns a step of 16 of the
+// contraction.  Of tokens: 32 columns a part.  The state's, in halves by the threads that
+// own them: the first two parts of each in the columns of the update that the same
+// threads read before, the third behind all of them.  Of tokens in halves: 48 columns a
+// half.
+struct TokenParts {
+  static __device__ __forceinline__ constexpr uint32_t at(int part, int ks) { return 32 * part + 8 * ks; }
+};
+template <int DK>
+struct StateParts {
+  static __device__ __forceinline__ constexpr uint32_t at(int part, int ks) {
+    constexpr int half = DK / 32;  // steps
+    return part == 2 ? DK + 8 * ks : ks / half * (DK / 2) + part * (DK / 4) + ks % half * 8;
+  }
+};
+struct HalfParts {
+  static __device__ __forceinline__ constexpr uint32_t at(int part, int ks) {
+    return ks / 2 * 48 + part * 16 + ks % 2 * 8;
+  }
+};
+
+// d[128 x N] (+)= A B; A in three parts at a (Parts), B the rows of Q or K at b in BP
+// parts bstep bytes apart, their tokens (n_major false) or their columns as N, DEPTH
+// elements of the contraction.  Products of 2^-24 and below are left out, and the
+// small ones come first: a sum that is still small rounds off less.
+template <class Parts, int DEPTH, int N, bool N_MAJOR, int BP>
+__device__ __forceinline__ void issue_product(uint32_t d, uint32_t a, uint32_t b, uint32_t bstep,
+                                              bool accumulate) {
   const uint32_t low = block_desc(b, N_MAJOR ? kRowBlock : kKeyBlock);
   constexpr uint32_t high = block_desc_high(N_MAJOR ? kKeyBlock : kRowBlock);
   constexpr uint32_t kstep = (N_MAJOR ? 2 * kRowBlock : 2 * kKeyBlock) / 16;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int sum = 2; sum >= 0; --sum)
 #pragma unroll
-    for (int j = 0; j < BP; ++j) {
-      if (i + j > 1) continue;
+    for (int j = 0; j < BP && j <= sum; ++j)
 #pragma unroll
       for (int ks = 0; ks < DEPTH / 16; ++ks)
-        tc_mma(d, a + i * astep + 8 * ks + (STATE ? ks / (DEPTH / 32) * (DEPTH / 4) : 0),
-               low + j * (bstep / 16) + ks * kstep, high, mma_desc(N, N_MAJOR),
-               accumulate || i + j + ks > 0);
-    }
+        tc_mma(d, a + Parts::at(sum - j, ks), low + j * (bstep / 16) + ks * kstep, high,
+               mma_desc(N, N_MAJOR), accumulate || sum < 2 || j + ks > 0);
 }
 
-// d = A M^T (back: A M) for a lower triangular split [64][64] tile M: only the
-// blocks on and below the diagonal are read.  AP: parts of A.
+// d = A M^T (back: A M) for a lower triangular [64][64] tile M in three parts: only the
+// blocks on and below the diagonal are read.  AP: parts of A, 32 columns each.
 template <bool BACK, int AP>
-__device__ __forceinline__ void issue_lower(uint32_t d, uint32_t a, uint32_t astep, uint32_t m,
-                                            bool accumulate) {
+__device__ __forceinline__ void issue_lower(uint32_t d, uint32_t a, uint32_t m) {
   const uint32_t low = tile_desc(m, BACK);
 #pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    const int ks = BACK ? 3 - x : x;  // the step that fills all columns first
-    const uint32_t n = BACK ? 16 * (ks + 1) : 64 - 16 * ks;
-    const uint32_t from = BACK ? ks * 2 * kRowBlock : ks * (2 * kRowBlock + 2 * kColBlock);
+  for (int sum = 2; sum >= 0; --sum)
 #pragma unroll
-    for (int i = 0; i < AP; ++i)
+    for (int i = 0; i < AP && i <= sum; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if (i + j > 1) continue;
-        tc_mma(BACK ? d : d + 16 * ks, a + i * astep + 8 * ks, low + (from + j * kSq * 2) / 16,
-               tile_desc_high(BACK), mma_desc(n, BACK), accumulate || x + i + j > 0);
+      for (int x = 0; x < 4; ++x) {
+        const int ks = BACK ? 3 - x : x;  // the step that fills all columns first
+        const uint32_t n = BACK ? 16 * (ks + 1) : 64 - 16 * ks;
+        const uint32_t from = BACK ? ks * 2 * kRowBlock : ks * (2 * kRowBlock + 2 * kColBlock);
+        tc_mma(BACK ? d : d + 16 * ks, a + TokenParts::at(i, ks),
+               low + (from + (sum - i) * kSq * 2) / 16, tile_desc_high(BACK), mma_desc(n, BACK),
+               sum < 2 || i + x > 0);
       }
-  }
 }
 
 __device__ __forceinline__ void walk_setup(WalkSync* sy, int tid, int warp) {
@@ -178,10 +204,10 @@ __device__ __forceinline__ void walk_fetch(const DeltaParams& p, unsigned char* 
     const uint32_t dst = smem_addr(raw) + st * W::stage, bar = smem_addr(&sy->full[st]);
     const unsigned char* keys = p.kq + (chunk * p.H + h) * (W::KP * W::keys);
     constexpr uint32_t kbytes = W::KP * W::keys;
-    constexpr uint32_t tbytes = T_ONLY ? 2 * kSq * 2 : 4 * kSq * 2;
+    constexpr uint32_t tbytes = T_ONLY ? 3 * kSq * 2 : 6 * kSq * 2;
     mbar_arrive_expect_tx(bar, kbytes + tbytes + 3 * kChunk * 4);
     bulk_load(dst + W::q, keys, kbytes, bar);
-    bulk_load(dst + W::t, p.tp + slot * (4 * kSq), tbytes, bar);
+    bulk_load(dst + W::t, p.tp + slot * (6 * kSq), tbytes, bar);
     bulk_load(dst + W::coef, p.coef + slot * 3 * kChunk, 3 * kChunk * 4, bar);
     issued = c + 1;
   }
@@ -396,9 +422,11 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
   walk_setup(sy, tid, warp);
   const Waiter wait{&sy->abort, p.timeout_ns, p.status_words, p.status_host, int(blockIdx.x)};
   const uint32_t tm = sy->tmem;
-  // TMEM columns: Y, then U; O; S^T parts, then the state's update; X, then w V'; V'
+  // TMEM columns: Y, then U; O; S^T parts, the first two then the state's update; X, then
+  // w V'; V'
   constexpr uint32_t cY = 0, cO = 64, cS = 128, cX = 320, cV = 416;
   constexpr uint32_t sStep = DK / 4, xStep = 32;
+  using SP = StateParts<DK>;
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
@@ -409,17 +437,17 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         if (!warp_wait(wait, sy->full[c & 1], c >> 1) || !warp_wait(wait, sy->sr, c)) break;
         tc_fence_after();
         if (elect_one()) {
-          issue_product<DK, 64, false, KP, true>(tm + cY, tm + cS, sStep, st + W::k, W::keys, false);
+          issue_product<SP, DK, 64, false, KP>(tm + cY, tm + cS, st + W::k, W::keys, false);
           tc_commit(smem_addr(&sy->y));
         }
         __syncwarp();
         if (!warp_wait(wait, sy->xr, c)) break;
         tc_fence_after();
         if (elect_one()) {
-          issue_lower<false, 2>(tm + cY, tm + cX, xStep, st + W::t, false);
+          issue_lower<false, 3>(tm + cY, tm + cX, st + W::t);
           tc_commit(smem_addr(&sy->u));
           if constexpr (MODE == 0) {
-            issue_product<DK, 64, false, KP, true>(tm + cO, tm + cS, sStep, st + W::q, W::keys, false);
+            issue_product<SP, DK, 64, false, KP>(tm + cO, tm + cS, st + W::q, W::keys, false);
             tc_commit(smem_addr(&sy->q));
           }
         }
@@ -427,7 +455,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         if (!warp_wait(wait, sy->vr, c)) break;
         tc_fence_after();
         if (elect_one()) {
-          issue_product<kChunk, DK, true, KP, false>(tm + cS, tm + cX, xStep, st + W::k, W::keys, false);
+          issue_product<TokenParts, kChunk, DK, true, KP>(tm + cS, tm + cX, st + W::k, W::keys, false);
           tc_commit(smem_addr(&sy->s));
           if constexpr (MODE == 1) tc_commit(smem_addr(&sy->free[c & 1]));
         }
@@ -436,7 +464,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
           if (!warp_wait(wait, sy->qr, c)) break;
           tc_fence_after();
           if (elect_one()) {
-            issue_lower<false, 2>(tm + cO, tm + cV, xStep, st + W::p, false);
+            issue_lower<false, 3>(tm + cO, tm + cV, st + W::p);
             tc_commit(smem_addr(&sy->o));
             tc_commit(smem_addr(&sy->free[c & 1]));
           }
@@ -473,7 +501,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
     } else {
       walk_load<DK>(S, p.init == nullptr ? nullptr : p.init + state_at, p.V, live);
     }
-    uint32_t vr[32], hi[16], lo[16];
+    uint32_t vr[32];
     const uint32_t vstep = uint32_t(p.v_st * 2), ostep = uint32_t(p.HV * p.V * 2);
     auto rows_of = [&](int c) {  // of this thread's 32 tokens
       return int(min(int64_t(32), s.len - int64_t(c) * kChunk - t0));
@@ -516,13 +544,12 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         float w[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) w[i] = S[32 * x + i];
-        split_to_tmem(w, lanes + cS + half * (DK / 2) + 16 * x, sStep, hi, lo);
-        if constexpr (MODE == 1) {
-          unsigned char* dst =
-              channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::shi, half * (DK / 2) + 32 * x);
-          store_pairs(dst, hi, live);
-          store_pairs(dst - GT::part, lo, live);
-        }
+        split_parts(w, [&](int part, const uint32_t (&r)[16]) {
+          tmem_st(lanes + cS + 16 * x + (part == 2 ? DK + half * sStep : half * (DK / 2) + part * sStep), r);
+          if (MODE == 1 && part < 2)
+            store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::shi - part * GT::part,
+                                           half * (DK / 2) + 32 * x), r, live);
+        });
       }
       operand_ready(sy->sr, lane);
       if (MODE == 0 && c > 0) {
@@ -547,7 +574,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
           x[i + 2] = widen<E>(vr[i + 2]) - gam.z * __uint_as_float(r[i + 2]);
           x[i + 3] = widen<E>(vr[i + 3]) - gam.w * __uint_as_float(r[i + 3]);
         }
-        split_to_tmem(x, lanes + cX + t0 / 2, xStep, hi, lo);
+        split_to_tmem(x, lanes + cX + t0 / 2, xStep);
       }
       operand_ready(sy->xr, lane);
       if (c + 1 < chunks)
@@ -564,11 +591,11 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         float u[32], x[32];
         if constexpr (MODE == 1) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            split2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), hi[i], lo[i]);
-          unsigned char* dst = channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::u, t0);
-          store_pairs(dst, hi, live);
-          store_pairs(dst + GT::upart, lo, live);
+          for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
+          split_parts(x, [&](int part, const uint32_t (&b)[16]) {
+            if (part < 2)
+              store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::u + part * GT::upart, t0), b, live);
+          });
         }
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
@@ -583,11 +610,11 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
           x[i + 2] = w.z * u[i + 2];
           x[i + 3] = w.w * u[i + 3];
         }
-        split_to_tmem(x, lanes + cX + t0 / 2, xStep, hi, lo);
+        split_to_tmem(x, lanes + cX + t0 / 2, xStep);
         operand_ready(sy->vr, lane);
         if constexpr (MODE == 0) {
           // beside the chain: V' for the output, and Q's product
-          split_to_tmem(u, lanes + cV + t0 / 2, xStep, hi, lo);
+          split_to_tmem(u, lanes + cV + t0 / 2, xStep);
           ok = warp_wait(wait, sy->q, c);
           if (!ok) break;
           tc_fence_after();
@@ -647,10 +674,11 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
   walk_setup(sy, tid, warp);
   const Waiter wait{&sy->abort, p.timeout_ns, p.status_words, p.status_host, int(blockIdx.x)};
   const uint32_t tm = sy->tmem;
-  // TMEM columns: K dS, then dX; dS^T parts, then the state's update; P^T dO; dO (exact);
-  // gam dO; beta dV', then -gam dX
-  constexpr uint32_t cY = 0, cS = 64, cP = 192, cO = 256, cG = 320, cX = 384;
+  // TMEM columns: K dS, then dX; dS^T parts, the first two then the state's update; P^T dO
+  // and, once a half of it is read, that half of gam dO; dO (exact); beta dV', then -gam dX
+  constexpr uint32_t cY = 0, cS = 64, cG = 256, cP = cG + 16, cO = 352, cX = 416;
   constexpr uint32_t sStep = DK / 4, xStep = 32;
+  using SP = StateParts<DK>;
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
@@ -660,32 +688,32 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
         const uint32_t st = smem_addr(raw) + (c & 1) * W::stage;
         if (!warp_wait(wait, sy->full[c & 1], c >> 1) || !warp_wait(wait, sy->gr, c)) break;
         tc_fence_after();
-        if (elect_one()) issue_lower<true, KP>(tm + cP, tm + cO, xStep, st + W::p, false);
+        if (elect_one()) issue_lower<true, KP>(tm + cP, tm + cO, st + W::p);
         __syncwarp();
         if (!warp_wait(wait, sy->sr, c)) break;
         tc_fence_after();
         if (elect_one()) {
-          issue_product<DK, 64, false, KP, true>(tm + cY, tm + cS, sStep, st + W::k, W::keys, false);
+          issue_product<SP, DK, 64, false, KP>(tm + cY, tm + cS, st + W::k, W::keys, false);
           tc_commit(smem_addr(&sy->y));
         }
-        __syncwarp();
-        // (K dS comes first and has read dS^T's parts: the update may take their place)
-        if (!warp_wait(wait, sy->y, c) || !warp_wait(wait, sy->qr, c)) break;
-        tc_fence_after();
-        if (elect_one())
-          issue_product<kChunk, DK, true, KP, false>(tm + cS, tm + cG, xStep, st + W::q, W::keys, false);
         __syncwarp();
         if (!warp_wait(wait, sy->xr, c)) break;
         tc_fence_after();
         if (elect_one()) {
-          issue_lower<true, 2>(tm + cY, tm + cX, xStep, st + W::t, false);
+          issue_lower<true, 3>(tm + cY, tm + cX, st + W::t);
           tc_commit(smem_addr(&sy->u));
         }
+        __syncwarp();
+        // (xr stands behind y: K dS has read dS^T's parts, the update may take their place)
+        if (!warp_wait(wait, sy->qr, c)) break;
+        tc_fence_after();
+        if (elect_one())
+          issue_product<HalfParts, kChunk, DK, true, KP>(tm + cS, tm + cG, st + W::q, W::keys, false);
         __syncwarp();
         if (!warp_wait(wait, sy->vr, c)) break;
         tc_fence_after();
         if (elect_one()) {
-          issue_product<kChunk, DK, true, KP, false>(tm + cS, tm + cX, xStep, st + W::k, W::keys, true);
+          issue_product<TokenParts, kChunk, DK, true, KP>(tm + cS, tm + cX, st + W::k, W::keys, true);
           tc_commit(smem_addr(&sy->s));
           tc_commit(smem_addr(&sy->free[c & 1]));
         }
@@ -750,30 +778,17 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
         float w[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) w[i] = D[32 * x + i];
-        split_to_tmem(w, lanes + cS + half * (DK / 2) + 16 * x, sStep, hi, lo);
-        unsigned char* dst = channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::d, half * (DK / 2) + 32 * x);
-        store_pairs(dst, hi, live);
-        store_pairs(dst + GT::part, lo, live);
+        split_parts(w, [&](int part, const uint32_t (&r)[16]) {
+          tmem_st(lanes + cS + 16 * x + (part == 2 ? DK + half * sStep : half * (DK / 2) + part * sStep), r);
+          if (part < 2)
+            store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::d + part * GT::part,
+                                           half * (DK / 2) + 32 * x), r, live);
+        });
       }
       operand_ready(sy->sr, lane);
-      // gam dO beside the chain (its region's last reader was the last chunk's update)
-      ok = warp_wait(wait, sy->full[c & 1], c >> 1);
-      if (!ok) break;
-      {
-        float x[32];
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          const float4 gam = *reinterpret_cast<const float4*>(coef + t0 + i);
-          x[i] = p.scale * gam.x * widen<E>(vr[i]);
-          x[i + 1] = p.scale * gam.y * widen<E>(vr[i + 1]);
-          x[i + 2] = p.scale * gam.z * widen<E>(vr[i + 2]);
-          x[i + 3] = p.scale * gam.w * widen<E>(vr[i + 3]);
-        }
-        split_to_tmem(x, lanes + cG + t0 / 2, xStep, hi, lo);
-        operand_ready(sy->qr, lane);
-      }
-      if (c + 1 < chunks) fetch_do(c + 1);
       // beta dV'
+      ok = warp_wait(wait, sy->full[c & 1], c >> 1);  // (the coefficients)
+      if (!ok) break;
       ok = warp_wait(wait, sy->y, c);
       if (!ok) break;
       tc_fence_after();
@@ -791,9 +806,23 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
           x[i + 2] = be.z * fmaf(w.z, __uint_as_float(r[i + 2]), __uint_as_float(r2[i + 2]));
           x[i + 3] = be.w * fmaf(w.w, __uint_as_float(r[i + 3]), __uint_as_float(r2[i + 3]));
         }
-        split_to_tmem(x, lanes + cX + t0 / 2, xStep, hi, lo);
+        split_to_tmem(x, lanes + cX + t0 / 2, xStep);
       }
       operand_ready(sy->xr, lane);
+      {  // gam dO beside the chain, where this thread has just read P^T dO
+        float x[32];
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 gam = *reinterpret_cast<const float4*>(coef + t0 + i);
+          x[i] = p.scale * gam.x * widen<E>(vr[i]);
+          x[i + 1] = p.scale * gam.y * widen<E>(vr[i + 1]);
+          x[i + 2] = p.scale * gam.z * widen<E>(vr[i + 2]);
+          x[i + 3] = p.scale * gam.w * widen<E>(vr[i + 3]);
+        }
+        split_to_tmem(x, lanes + cG + half * 48, 16);
+        operand_ready(sy->qr, lane);
+      }
+      if (c + 1 < chunks) fetch_do(c + 1);
       // dX
       ok = warp_wait(wait, sy->u, c);
       if (!ok) break;
@@ -811,16 +840,15 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
           x[i + 2] = -gam.z * __uint_as_float(r[i + 2]);
           x[i + 3] = -gam.w * __uint_as_float(r[i + 3]);
         }
-        split_to_tmem(x, lanes + cX + t0 / 2, xStep, hi, lo);
+        split_to_tmem(x, lanes + cX + t0 / 2, xStep);
         operand_ready(sy->vr, lane);
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          split2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), hi[i], lo[i]);
-        store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::xhi, t0), hi, live);
-        store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::xlo, t0), lo, live);
 #pragma unroll
         for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
         walk_put<E>(dv + (int64_t(cc) * kChunk + t0) * p.HV * p.V, dvstep, x, rows_of(cc), live);
+        split_parts(x, [&](int part, const uint32_t (&b)[16]) {
+          if (part < 2)
+            store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, part ? GT::xlo : GT::xhi, t0), b, live);
+        });
       }
     }
     if (ok && chunks > 0) advance(chunks - 1);

@@ -187,10 +187,19 @@ __device__ __forceinline__ void stsm4_t(uint32_t addr, const uint32_t r[4]) {
                : "memory");
 }
 
-// An fp32 pair as bf16 high parts plus bf16 remainders: together 16 bits of
-// mantissa or more, so a product with an exact bf16 operand costs two matrix
-// instructions and is off by about 2^-18 of its size (against 2^-9 with the
-// high parts alone).
+// An fp32 pair as three bf16 parts, each the remainder of those before it: 3 x 8
+// bits hold fp32's 24, so nothing is lost (but what is below bf16's smallest values).
+// A product with an exact bf16 operand costs three matrix instructions; one of two such
+// operands six, without those of 2^-24 of its size and below.
+__device__ __forceinline__ void split3(float x, float y, uint32_t r[3]) {
+  r[0] = pack2_rn<BF16>(x, y);
+  fma2<BF16>(r[0], 0xBF80BF80u, x, y);  // x - its part, exact (times -1, no unpacking)
+  r[1] = pack2_rn<BF16>(x, y);
+  fma2<BF16>(r[1], 0xBF80BF80u, x, y);
+  r[2] = pack2_rn<BF16>(x, y);
+}
+
+// The first two of them: 16 bits of mantissa or more.
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
   hi = pack2_rn<BF16>(x, y);
   fma2<BF16>(hi, 0xBF80BF80u, x, y);  // x - high part, exact (times -1, no unpacking)
@@ -212,21 +221,25 @@ __device__ __forceinline__ void split_elem(uint32_t v, uint32_t& hi, uint32_t& l
 }
 
 // The A fragment of step `ks` from the C fragments of tiles 2ks, 2ks+1, split.
-__device__ __forceinline__ void split_frag(const float c0[4], const float c1[4], uint32_t hi[4],
-                                           uint32_t lo[4]) {
-  split2(c0[0], c0[1], hi[0], lo[0]);
-  split2(c0[2], c0[3], hi[1], lo[1]);
-  split2(c1[0], c1[1], hi[2], lo[2]);
-  split2(c1[2], c1[3], hi[3], lo[3]);
+__device__ __forceinline__ void split_frag(const float c0[4], const float c1[4], uint32_t a[3][4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float* c = i < 2 ? c0 : c1;
+    uint32_t r[3];
+    split3(c[2 * (i & 1)], c[2 * (i & 1) + 1], r);
+#pragma unroll
+    for (int x = 0; x < 3; ++x) a[x][i] = r[x];
+  }
 }
 
-// c += A B, both split (the product of the two remainders is below the others'
-// rounding).
-__device__ __forceinline__ void mma_split(float c[4], const uint32_t ah[4], const uint32_t al[4],
-                                          uint32_t bh0, uint32_t bh1, uint32_t bl0, uint32_t bl1) {
-  mma_bf16(c, ah, bh0, bh1);
-  mma_bf16(c, al, bh0, bh1);
-  mma_bf16(c, ah, bl0, bl1);
+// c += A B, both split (b: registers at, at + 1 of each part), the small products first:
+// an accumulator that is still small rounds off less.
+__device__ __forceinline__ void mma_split(float c[4], const uint32_t a[3][4], const uint32_t b[3][4],
+                                          int at) {
+#pragma unroll
+  for (int sum = 2; sum >= 0; --sum)
+#pragma unroll
+    for (int i = 0; i <= sum; ++i) mma_bf16(c, a[i], b[sum - i][at], b[sum - i][at + 1]);
 }
 
 // The same for N accumulators side by side, product by product rather than

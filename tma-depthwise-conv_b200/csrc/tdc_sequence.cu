@@ -350,7 +350,7 @@ int64_t delta_layout(const tdc_delta_args* a, bool grads, unsigned char* base, t
   };
   const int64_t slots = delta_chunks(a) * a->HV;
   unsigned char* plan = take(2 * (delta_seqs(a) + 1) * 8);
-  unsigned char* tp = take(slots * 4 * tdc::kSq * 2);
+  unsigned char* tp = take(slots * 6 * tdc::kSq * 2);
   const int64_t parts = a->dtype == TDC_BF16 ? 1 : 2;
   unsigned char* kq = take(delta_chunks(a) * a->H * 2 * parts * tdc::kChunk * a->K * 2);
   unsigned char* coef = take(slots * 3 * tdc::kChunk * 4);
