@@ -1,5 +1,5 @@
 """The fp32 outputs of the chunked gated delta rule (final states, gradients of the
-initial states) have fp32's exactness.
+decays, of fp32 betas and of the initial states) have fp32's exactness.
 
 Tolerance, of the 2-norm of the error over that of the result in fp64.  A sum of 128
 products takes 8 steps of the tensor core, each off by at most 2^-23 of the partial sum;
@@ -15,7 +15,7 @@ import tdc_sequence as S
 from test_seq_delta import _case, _run, _want
 
 TOL = 2 ** -20
-FP32 = ("final", "dstate")
+FP32 = ("final", "dg", "dbeta", "dstate")
 
 
 def _off(got, want):
@@ -26,7 +26,6 @@ def _off(got, want):
 def _exact(name, got, want):
     assert got.dtype == torch.float32, name
     off = _off(got, want)
-    print(f"{name}: {off:.3g}")
     assert off <= TOL, f"{name}: {off:.3g} of the norm"
 
 
@@ -37,6 +36,7 @@ def _exact(name, got, want):
     (1, 200, 1, 2, 64, 64, "bf16", None),
     (1, 200, 1, 2, 64, 64, "fp16", None),
     (1, 150, 2, 2, 128, 256, "bf16", [3, 20, 20, 101, 148]),
+    (1, 150, 2, 2, 128, 256, "fp16", [3, 20, 20, 101, 148]),
     (1, 130, 1, 1, 64, 128, "fp16", [0, 64, 130])])
 def test_fp32_outputs(B, T, H, HV, K, V, dtype, cu):
     c = _case(B, T, H, HV, K, V, dtype, state=True, cu=cu, beta_f32=True, seed=T)

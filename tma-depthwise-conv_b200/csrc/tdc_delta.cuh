@@ -32,24 +32,30 @@ constexpr int kSq = kChunk * kChunk;  // elements of such a tile in the workspac
 
 // The gradients' workspace: for kTile value channels of a slot, transposed, what
 // the gradients of a chunk need of them, in the order of a stage in shared memory
-// (so that one copy brings it).  Each part is [columns / 8][kTile][8]; hi is the
-// high parts, lo the remainders.  In bf16 dO has none: the workspace starts behind
-// that place, which holds zeros in shared memory.
+// (so that two copies bring it).  Each part is [columns / 8][kTile][8]; S, dS, U and dX
+// have three parts (split3), dO what its type needs.  Two places of a stage hold zeros and
+// are not in the workspace: bf16's second part of dO, and one between U's last
+// part and dX's, which serves both as the other 64 rows of an operand.
 constexpr int kTile = 16;
 template <int KP, int DK>
 struct GradTile {
   static constexpr int part = kTile * DK * 2, upart = kTile * kChunk * 2;  // bytes
-  static constexpr int olo = 0;             // dO^T, dX^T: remainders
-  static constexpr int xlo = olo + upart;
-  static constexpr int d = xlo + upart;     // dS^T behind the chunk: hi, lo
-  static constexpr int slo = d + 2 * part;  // S^T before it
-  static constexpr int shi = slo + part;
-  static constexpr int u = shi + part;      // U^T: hi, lo
-  static constexpr int ohi = u + 2 * upart;
-  static constexpr int xhi = ohi + upart;
-  static constexpr int stage = xhi + upart;
+  static constexpr int om = 0;              // dO^T, dX^T: second parts
+  static constexpr int xm = om + upart;
+  static constexpr int d = xm + upart;      // dS^T behind the chunk
+  static constexpr int s = d + 5 * part;    // S^T before it: part i at s - i part
+  static constexpr int u = s + part;        // U^T
+  static constexpr int zero = u + 3 * upart;
+  static constexpr int xl = zero + upart;   // dX^T: last part
+  static constexpr int oh = xl + upart;     // dO^T, dX^T: first parts
+  static constexpr int xh = oh + upart;
+  static constexpr int stage = xh + upart;
   static constexpr int skip = KP == 1 ? upart : 0;
-  static constexpr int bytes = stage - skip;
+  static constexpr int front = zero - skip, back = stage - xl;  // the two copies
+  static constexpr int bytes = front + back;
+  static __host__ __device__ constexpr int x(int part) { return part == 0 ? xh : part == 1 ? xm : xl; }
+  // where `off` of a stage lies in the workspace's tile
+  static __host__ __device__ constexpr int at(int off) { return off - skip - (off > zero ? upart : 0); }
 };
 
 struct DeltaParams {

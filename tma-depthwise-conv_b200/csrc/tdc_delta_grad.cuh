@@ -17,10 +17,12 @@
 // 0-63 of TMEM are the tokens of dO (and of what becomes dQ), lanes 64-127 those
 // of dX (dK), so with M = 128
 //   [dO; dX] S^T and [dO; dX] U^T      both halves at once,
-//   [U_hi; U_lo] dS^T                  the two parts of U in the halves, added later,
+//   [U_1; U_2] dS^T, [U_3; 0] dS^T     parts of U in the halves, added later,
 //   [Q; K] K^T                         once a block,
 //   [Dt; N] K                          into dQ and dK,
-//   [Dt_hi; Dt_lo]^T Q + [N_hi; N_lo]^T K   into dK, again by parts.
+//   [Dt_1; Dt_2]^T Q + [N_1; N_2]^T K  into dK, again by parts: the halves are added, so
+//                                      with [Dt_2; Dt_3] too the second part counts twice
+//                                      and is kept halved.
 // The walks left U, dX, dO, S and dS transposed, as [kTile channels][8 columns]
 // blocks that serve as A with the tokens and as B with the keys along them.  The
 // channels are the contraction and come in tiles of kTile by bulk copies, as many
@@ -50,12 +52,13 @@ struct GradSmem {
   // rows of Q, then of K: [parts][DK / 8][128][8]
   using Tile = GradTile<KP, DK>;
   static constexpr int qk = 0, qkpart = DK / 8 * kKeyBlock;
-  // rows of Dt, then of N: [2 parts][8][128][8]
+  // rows of Dt, then of N: [3 parts][8][128][8], half of the second part
   static constexpr int dn = qk + KP * qkpart, dnpart = kChunk / 8 * kKeyBlock;
-  static constexpr int stages = dn + 2 * dnpart, stage = Tile::stage;
+  static constexpr int stages = dn + 3 * dnpart, stage = Tile::stage;
   static constexpr int kMaxBytes = 232448 - 7168;  // of a block, less GradSync
   static constexpr int count = (kMaxBytes - stages) / stage < 6 ? (kMaxBytes - stages) / stage : 6;
   static constexpr int sync = stages + count * stage;
+  static_assert(count >= 2, "one stage is read while another is filled");
 };
 struct GradSync {
   uint64_t full[6], used[6];   // stages: copied; read by the products and the 8 warps
@@ -79,8 +82,11 @@ struct GradSync {
 };
 static_assert(sizeof(GradSync) <= 7168, "see kMaxBytes");
 enum { kSumState = 0, kSumKey = 1, kSumE = 2 };
-// TMEM columns; D and M stand behind the products with S (DK columns).
-constexpr uint32_t kGradOX = 0, kGradUS = 192, kGradGram = 320;
+// TMEM columns; D and M stand behind the products with S (DK columns).  The tensor core
+// cuts a sum's low bits off at each product it adds, so U dS's small products have a sum
+// of their own (dbeta of 256 value channels: 1.1e-6 -> 6.7e-7 of the norm); there is
+// no room for the others'.
+constexpr uint32_t kGradOX = 0, kGradUS = 192, kGradGram = 320, kGradUS2 = 384;
 
 // What a block works on: a chunk that has rows, and a key head; every gridDim.x-th.
 struct GradItem {
@@ -162,8 +168,11 @@ __device__ __forceinline__ void grad_fetch(const DeltaParams& p, unsigned char* 
       if (!ok) break;
       constexpr int bytes = Sm::Tile::bytes;
       const uint32_t bar = smem_addr(&sy->full[x]);
+      const uint32_t dst = sb + Sm::stages + x * Sm::stage;
+      const unsigned char* src = p.tiles + (tile0 + t) * bytes;
       mbar_arrive_expect_tx(bar, bytes);
-      bulk_load(sb + Sm::stages + x * Sm::stage + Sm::Tile::skip, p.tiles + (tile0 + t) * bytes, bytes, bar);
+      bulk_load(dst + Sm::Tile::skip, src, Sm::Tile::front, bar);
+      bulk_load(dst + Sm::Tile::xl, src + Sm::Tile::front, Sm::Tile::back, bar);
       ++n;
     }
   }
@@ -195,14 +204,24 @@ __device__ __forceinline__ void grad_issue(const DeltaParams& p, uint32_t sb, Gr
         const uint32_t st = sb + Sm::stages + x * Sm::stage;
         if (elect_one()) {
           using T = typename Sm::Tile;
-          const uint32_t a = st + T::ohi, b = st + T::olo, u = st + T::u;
-          // by S and U together, where their parts lie beside each other
-          grad_product<DK + 64>(tm + kGradOX, a, st + T::shi, vt > 0);
-          grad_product<DK + 64>(tm + kGradOX, b, st + T::shi, true);
-          grad_product<DK>(tm + kGradOX, a, st + T::slo, true);
+          const uint32_t a = st + T::oh, b = st + T::om, c = st + T::zero;  // [dO; dX] by parts
+          const uint32_t u = st + T::u, s = st + T::s, d = st + T::d;
+          // by S and U together, where their parts lie beside each other; without the
+          // products of 2^-24 and below
+          grad_product<DK + 64>(tm + kGradOX, c, s, vt > 0);
+          grad_product<DK>(tm + kGradOX, b, s - T::part, true);
+          grad_product<64>(tm + kGradDM, b, u + T::upart, true);
+          grad_product<DK>(tm + kGradOX, a, s - 2 * T::part, true);
+          grad_product<64>(tm + kGradDM, a, u + 2 * T::upart, true);
+          grad_product<DK + 64>(tm + kGradOX, b, s, true);
+          grad_product<DK>(tm + kGradOX, a, s - T::part, true);
           grad_product<64>(tm + kGradDM, a, u + T::upart, true);
-          grad_product<DK>(tm + kGradUS, u, st + T::d, vt > 0);
-          grad_product<DK>(tm + kGradUS, u, st + T::d + T::part, true);
+          grad_product<DK + 64>(tm + kGradOX, a, s, true);
+          // [U's last part; 0], then its first two
+          grad_product<DK>(tm + kGradUS2, u + 2 * T::upart, d, vt > 0);
+          grad_product<DK>(tm + kGradUS2, u, d + 2 * T::part, true);
+          grad_product<DK>(tm + kGradUS2, u, d + T::part, true);
+          grad_product<DK>(tm + kGradUS, u, d, vt > 0);
           tc_commit(smem_addr(&sy->used[x]));
         }
         __syncwarp();
@@ -215,14 +234,14 @@ __device__ __forceinline__ void grad_issue(const DeltaParams& p, uint32_t sb, Gr
         tc_fence_after();
         if (elect_one()) {  // the rows of Q and K by those of K
 #pragma unroll
-          for (int y = 0; y < KP; ++y)
+          for (int y = KP - 1; y >= 0; --y)
 #pragma unroll
-            for (int z = 0; z < KP - y; ++z)
+            for (int z = KP - 1; z >= 0; --z)
 #pragma unroll
               for (int ks = 0; ks < DK / 16; ++ks)
                 tc_mma_ss(tm + kGradGram, block_desc(q + y * Sm::qkpart + ks * 2 * kKeyBlock, kKeyBlock),
                           rhigh, block_desc(k + z * Sm::qkpart + ks * 2 * kKeyBlock, kKeyBlock), rhigh,
-                          mma_desc(64, false, false), y + z + ks > 0);
+                          mma_desc(64, false, false), y + z < 2 * KP - 2 || ks > 0);
           tc_commit(smem_addr(&sy->gram));
         }
         __syncwarp();
@@ -230,28 +249,32 @@ __device__ __forceinline__ void grad_issue(const DeltaParams& p, uint32_t sb, Gr
       if (!warp_wait(wait, sy->dn, heads)) return;
       tc_fence_after();
       if (elect_one()) {
-        // [Dt; N] K onto the first, [Dt_hi; Dt_lo]^T Q + [N_hi; N_lo]^T K onto the last
+        // [Dt; N] K onto the first (half of the second part twice), then two parts at a
+        // time, the last two and the first two, [Dt; Dt]^T Q + [N; N]^T K onto the last
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
+        for (int sum = 2; sum >= 0; --sum)
 #pragma unroll
-          for (int z = 0; z < KP; ++z) {
-            if (y + z > 1) continue;
+          for (int z = 0; z < KP && z <= sum; ++z)
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-              tc_mma_ss(tm + kGradOX, block_desc(dn + y * Sm::dnpart + ks * 2 * kKeyBlock, kKeyBlock), rhigh,
-                        block_desc(k + z * Sm::qkpart + ks * 2 * kRowBlock, kRowBlock), khigh,
-                        mma_desc(DK, true, false), true);
-          }
+            for (int twice = 0; twice < (sum - z == 1 ? 2 : 1); ++twice)
 #pragma unroll
-        for (int z = 0; z < KP; ++z)
+              for (int ks = 0; ks < 4; ++ks)
+                tc_mma_ss(tm + kGradOX,
+                          block_desc(dn + (sum - z) * Sm::dnpart + ks * 2 * kKeyBlock, kKeyBlock), rhigh,
+                          block_desc(k + z * Sm::qkpart + ks * 2 * kRowBlock, kRowBlock), khigh,
+                          mma_desc(DK, true, false), true);
 #pragma unroll
-          for (int rows = 0; rows < 2; ++rows)  // of Dt and Q, of N and K
+        for (int z = KP - 1; z >= 0; --z)
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-              tc_mma_ss(tm + kGradUS,
-                        block_desc(dn + rows * 1024 + ks * 2 * kRowBlock, kRowBlock), khigh,
-                        block_desc(q + z * Sm::qkpart + rows * 1024 + ks * 2 * kRowBlock, kRowBlock),
-                        khigh, mma_desc(DK, true, true), true);
+          for (int y = 1; y >= 0; --y)
+#pragma unroll
+            for (int rows = 0; rows < 2; ++rows)  // of Dt and Q, of N and K
+#pragma unroll
+              for (int ks = 0; ks < 4; ++ks)
+                tc_mma_ss(tm + kGradUS,
+                          block_desc(dn + y * Sm::dnpart + rows * 1024 + ks * 2 * kRowBlock, kRowBlock), khigh,
+                          block_desc(q + z * Sm::qkpart + rows * 1024 + ks * 2 * kRowBlock, kRowBlock),
+                          khigh, mma_desc(DK, true, true), true);
         tc_commit(smem_addr(&sy->done));
       }
       __syncwarp();
@@ -289,10 +312,13 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_grad_kernel(const Delta
     fence_mbar_init();
   }
   if (warp == 8) tmem_alloc(smem_addr(&sy->tmem), kTmemColumns);
-  if constexpr (KP == 1) {  // dO has no remainders
-    constexpr int skip = Sm::Tile::skip;
-    for (int e = 16 * tid; e < NS * skip; e += 16 * kWalkThreads)
-      *reinterpret_cast<uint4*>(raw + Sm::stages + e / skip * Sm::stage + e % skip) = make_uint4(0, 0, 0, 0);
+  {  // the stages' places of zeros
+    constexpr int upart = Sm::Tile::upart;
+    for (int e = 16 * tid; e < NS * upart; e += 16 * kWalkThreads) {
+      unsigned char* at = raw + Sm::stages + e / upart * Sm::stage + e % upart;
+      *reinterpret_cast<uint4*>(at + Sm::Tile::zero) = make_uint4(0, 0, 0, 0);
+      if (KP == 1) *reinterpret_cast<uint4*>(at + Sm::Tile::om) = make_uint4(0, 0, 0, 0);
+    }
     fence_proxy_async();
   }
   tc_fence_before();
@@ -354,16 +380,18 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_grad_kernel(const Delta
           ok = all_wait(sy->full[x], phase);
           if (!ok) break;
           const unsigned char* stage = raw + Sm::stages + x * Sm::stage;
-          for (int e = tid; e < kTile * DK / 8; e += 256) {  // 8 values at the same place of all four
-            float f[2][8], g[2][8];
+          for (int e = tid; e < kTile * DK / 8; e += 256) {  // 8 values at the same place of all six
+            float f[8] = {}, g[8] = {};
 #pragma unroll
-            for (int part = 0; part < 2; ++part) {
-              const int off = part * Sm::Tile::part + 16 * e;
-              unpack8<BF16>(*reinterpret_cast<const uint4*>(stage + Sm::Tile::slo + off), f[part]);
-              unpack8<BF16>(*reinterpret_cast<const uint4*>(stage + Sm::Tile::d + off), g[part]);
+            for (int part = 2; part >= 0; --part) {
+              float a[8], b[8];
+              unpack8<BF16>(*reinterpret_cast<const uint4*>(stage + Sm::Tile::s - part * Sm::Tile::part + 16 * e), a);
+              unpack8<BF16>(*reinterpret_cast<const uint4*>(stage + Sm::Tile::d + part * Sm::Tile::part + 16 * e), b);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) f[j] += a[j], g[j] += b[j];
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) dsum = fmaf(f[0][j] + f[1][j], g[0][j] + g[1][j], dsum);
+            for (int j = 0; j < 8; ++j) dsum = fmaf(f[j], g[j], dsum);
           }
           arrive(sy->used[x]);
           if (++x == NS) x = 0, ++phase;
@@ -386,6 +414,13 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_grad_kernel(const Delta
             for (int j = 0; j < 32; ++j) own = fmaf(f[j], __uint_as_float(r[j]), own);
             put_scaled(lanes + kGradOX + kc0 + 32 * y, r, by);
             tmem_ld(lanes + kGradUS + kc0 + 32 * y, r);
+            {  // and the small products' sum
+              uint32_t r2[32];
+              tmem_ld(lanes + kGradUS2 + kc0 + 32 * y, r2);
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(r2[j]));
+            }
             if (!upper) load_key_row<E, DK>(f, raw + Sm::qk, 64 + l, kc0 + 32 * y);
 #pragma unroll
             for (int j = 0; j < 32; ++j) key = fmaf(f[j], __uint_as_float(r[j]), key);
@@ -432,13 +467,20 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_grad_kernel(const Delta
           if (!upper && (i >> 5) == hc) sy->diag[i] = own;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            uint32_t hi[4], lo[4];
+            uint32_t w[3][4];
 #pragma unroll
-            for (int m = 0; m < 4; ++m)
-              split2(__uint_as_float(r[8 * c + 2 * m]), __uint_as_float(r[8 * c + 2 * m + 1]), hi[m], lo[m]);
+            for (int m = 0; m < 4; ++m) {
+              float v0 = __uint_as_float(r[8 * c + 2 * m]), v1 = __uint_as_float(r[8 * c + 2 * m + 1]);
+              w[0][m] = pack2_rn<BF16>(v0, v1);
+              fma2<BF16>(w[0][m], 0xBF80BF80u, v0, v1);  // less the part
+              w[1][m] = pack2_rn<BF16>(0.5f * v0, 0.5f * v1);
+              fma2<BF16>(w[1][m], 0xC000C000u, v0, v1);  // less twice its half
+              w[2][m] = pack2_rn<BF16>(v0, v1);
+            }
             unsigned char* dst = raw + Sm::dn + (4 * hc + c) * kKeyBlock + l * 16;
-            *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4*>(dst + Sm::dnpart) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+            for (int m = 0; m < 3; ++m)
+              *reinterpret_cast<uint4*>(dst + m * Sm::dnpart) = make_uint4(w[m][0], w[m][1], w[m][2], w[m][3]);
           }
           fence_proxy_async();
           // column sums over the warp's lanes: lane j ends with column j

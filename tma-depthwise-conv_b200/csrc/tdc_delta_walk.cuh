@@ -281,7 +281,7 @@ __device__ __forceinline__ float widen(uint32_t raw) {
 template <int KP, int DK>
 __device__ __forceinline__ unsigned char* channel_at(unsigned char* base, int64_t channel, int off, int col) {
   using G = GradTile<KP, DK>;
-  return base + channel / kTile * G::bytes + (off - G::skip) + int(channel % kTile) * 16 + col * (2 * kTile);
+  return base + channel / kTile * G::bytes + G::at(off) + int(channel % kTile) * 16 + col * (2 * kTile);
 }
 // 16 packed pairs (32 tokens or keys) of a channel there: a warp's stores are
 // whole lines.
@@ -546,8 +546,8 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         for (int i = 0; i < 32; ++i) w[i] = S[32 * x + i];
         split_parts(w, [&](int part, const uint32_t (&r)[16]) {
           tmem_st(lanes + cS + 16 * x + (part == 2 ? DK + half * sStep : half * (DK / 2) + part * sStep), r);
-          if (MODE == 1 && part < 2)
-            store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::shi - part * GT::part,
+          if constexpr (MODE == 1)
+            store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::s - part * GT::part,
                                            half * (DK / 2) + 32 * x), r, live);
         });
       }
@@ -593,8 +593,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
 #pragma unroll
           for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
           split_parts(x, [&](int part, const uint32_t (&b)[16]) {
-            if (part < 2)
-              store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::u + part * GT::upart, t0), b, live);
+            store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::u + part * GT::upart, t0), b, live);
           });
         }
 #pragma unroll
@@ -765,9 +764,9 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
       if constexpr (KP == 2) tmem_st(lanes + cO + xStep + t0 / 2, lo);
       operand_ready(sy->gr, lane);
       {
-        store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::ohi, t0), hi, live);
+        store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::oh, t0), hi, live);
         if constexpr (KP == 2)
-          store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::olo, t0), lo, live);
+          store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::om, t0), lo, live);
       }
       if (c > 0) {
         advance(c - 1);
@@ -780,9 +779,8 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
         for (int i = 0; i < 32; ++i) w[i] = D[32 * x + i];
         split_parts(w, [&](int part, const uint32_t (&r)[16]) {
           tmem_st(lanes + cS + 16 * x + (part == 2 ? DK + half * sStep : half * (DK / 2) + part * sStep), r);
-          if (part < 2)
-            store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::d + part * GT::part,
-                                           half * (DK / 2) + 32 * x), r, live);
+          store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::d + part * GT::part,
+                                         half * (DK / 2) + 32 * x), r, live);
         });
       }
       operand_ready(sy->sr, lane);
@@ -846,8 +844,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
         for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
         walk_put<E>(dv + (int64_t(cc) * kChunk + t0) * p.HV * p.V, dvstep, x, rows_of(cc), live);
         split_parts(x, [&](int part, const uint32_t (&b)[16]) {
-          if (part < 2)
-            store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, part ? GT::xlo : GT::xhi, t0), b, live);
+          store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::x(part), t0), b, live);
         });
       }
     }

@@ -362,8 +362,8 @@ int64_t delta_layout(const tdc_delta_args* a, bool grads, unsigned char* base, t
     seg_m = take(a->B * a->HV * segments * a->K * a->K * 4);
   }
   if (grads) {
-    // (GradTile: S, dS, U and dX in two parts, dO in `parts`)
-    tiles = take(slots * a->V * 2 * (4 * a->K + (4 + parts) * tdc::kChunk));
+    // (GradTile: S, dS, U and dX in three parts, dO in `parts`)
+    tiles = take(slots * a->V * 2 * (6 * a->K + (6 + parts) * tdc::kChunk));
   }
   if (p != nullptr) {
     p->seq_lo = reinterpret_cast<int64_t*>(plan);
