@@ -15,6 +15,7 @@ what is older than its sources.
 from __future__ import annotations
 
 import os
+import re
 import subprocess
 import sys
 import sysconfig
@@ -48,19 +49,24 @@ def _run(cmd: list[str]) -> str:
     return r.stdout + r.stderr
 
 
-#: The library's translation units with the headers each is built from.
-UNITS = {
-    "tdc_capi.cu": ["tdc_dgrad_s2.cuh", "tdc_host.h", "tdc_kernels.cuh", "tdc_plain.cuh",
-                    "tdc_ptx.cuh", "tdc_wgrad.cuh"],
-    "tdc_sequence.cu": ["tdc_conv1d.cuh", "tdc_delta.cuh", "tdc_delta_walk.cuh", "tdc_host.h",
-                        "tdc_ptx.cuh", "tdc_qknorm.cuh", "tdc_seq_common.cuh", "tdc_tc.cuh"],
-}
+#: The library's translation units.
+UNITS = ("tdc_capi.cu", "tdc_sequence.cu")
 EXT_SOURCES = ("bindings.cpp", "bindings_sequence.cpp")
 
 
 def _deps(*names: str) -> list[str]:
-    return ([os.path.join(CSRC, n) for n in names]
-            + [os.path.join(INCLUDE, h) for h in ("tdc_dwconv.h", "tdc_sequence.h")])
+    """The sources `names` and every file of this repository that they include,
+    directly or through one another."""
+    found, todo = {}, list(names)
+    while todo:
+        name = todo.pop()
+        if name in found:
+            continue
+        found[name] = next(p for p in (os.path.join(d, name) for d in (CSRC, INCLUDE))
+                           if os.path.exists(p))
+        with open(found[name]) as f:
+            todo += re.findall(r'^[ \t]*#[ \t]*include[ \t]*"([^"]+)"', f.read(), re.M)
+    return sorted(found.values())
 
 
 def _tmp(path: str) -> str:
@@ -73,7 +79,7 @@ def _tmp(path: str) -> str:
 def _build_unit(nvcc: str, name: str, force: bool) -> str:
     """Object file of one .cu source, with its ptxas report beside it."""
     obj = os.path.join(HERE, name.replace(".cu", ".o"))
-    if force or _stale(obj, _deps(name, *UNITS[name])):
+    if force or _stale(obj, _deps(name)):
         tmp = _tmp(obj)
         out = _run([nvcc, *NVCC_FLAGS, "-c", f"-I{INCLUDE}", f"-I{CSRC}",
                     os.path.join(CSRC, name), "-o", tmp])
@@ -84,8 +90,7 @@ def _build_unit(nvcc: str, name: str, force: bool) -> str:
 
 
 def build_lib(force: bool = False) -> str:
-    deps = _deps(*UNITS, *{h for hs in UNITS.values() for h in hs})
-    if force or _stale(LIB, deps):
+    if force or _stale(LIB, _deps(*UNITS)):
         nvcc = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "bin", "nvcc")
         with ThreadPoolExecutor(len(UNITS)) as pool:  # one nvcc process for each source
             objs = list(pool.map(lambda n: _build_unit(nvcc, n, force), UNITS))
@@ -96,7 +101,7 @@ def build_lib(force: bool = False) -> str:
 
 
 def build_ext(force: bool = False) -> str:
-    deps = _deps(*EXT_SOURCES, "bindings_common.h") + [LIB]
+    deps = _deps(*EXT_SOURCES) + [LIB]
     if force or _stale(EXT, deps):
         import torch
         import torch.utils.cpp_extension as ce
@@ -109,7 +114,7 @@ def build_ext(force: bool = False) -> str:
 
         def unit(name: str) -> str:
             obj = os.path.join(HERE, name.replace(".cpp", ".o"))
-            if force or _stale(obj, _deps(name, "bindings_common.h")):
+            if force or _stale(obj, _deps(name)):
                 _run(["g++", "-c", *flags, os.path.join(CSRC, name), "-o", _tmp(obj)])
                 os.replace(_tmp(obj), obj)
             return obj
