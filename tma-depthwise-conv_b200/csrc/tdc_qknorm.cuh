@@ -253,8 +253,9 @@ __global__ void __launch_bounds__(256) qk_norm_rope_bwd_kernel(const QkParams p)
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const float dw = d[j] * f[j];
+            // (a spare group's row of zeros may have 0 * inf here)
             dqw[j] += is_q ? dw : 0.f;
-            dkw[j] += is_q ? 0.f : dw;
+            dkw[j] += is_q || h >= heads ? 0.f : dw;
             d[j] *= w[j];
           }
         }
