@@ -16,3 +16,25 @@ def test_weight_gradients_without_eps(H, HK, dim, norm):
     # totals of heads that leave some lanes of a warp without one: what they hold counts nowhere
     c = Q._case(2, 5, H, HK, dim, 16, "bf16", True, "batch", seed=H)
     Q._check(Q._run(c, norm, False, 0.0), Q._want(c, norm, False, 0.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["q", "k", "v", "g", "beta"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("T,t", [(100, 1), (100, 37), (100, 63), (100, 64), (100, 99), (1700, 901)])
+@pytest.mark.parametrize("K,V,dtype", [(64, 64, "bf16"), (128, 256, "fp16")])
+def test_what_is_not_finite_reaches_no_token_before_it(name, bad, T, t, K, V, dtype):
+    # as in the recurrence: a padded batch may hold anything behind its last token.
+    # (1700 tokens are walked in segments; a decay is never +inf)
+    bad = float("nan") if name == "g" else bad
+    c = D._case(2, T, 1, 2, K, V, dtype, state=True, beta_f32=True)
+    a = {n: c[n].detach().clone().cuda() for n in ("q", "k", "v", "g", "beta")}
+    run = lambda: S.gated_delta_rule(*a.values(), initial_state=c["state"].cuda())  # noqa: E731
+    want = run()
+    a[name][(0, t) + {"q": (0, 5), "k": (0, 5), "v": (1, 7), "g": (1,), "beta": (1,)}[name]] = bad
+    got = run()
+    reached = torch.zeros_like(got, dtype=torch.bool)    # head 0 shares q and k with head 1
+    heads, channels = {"q": (slice(None),) * 2, "k": (slice(None),) * 2}.get(name, (1, slice(None)))
+    reached[0, slice(t, t + 1 if name == "q" else None), heads, 7 if name == "v" else channels] = True
+    assert torch.equal(got[~reached], want[~reached])
+    assert not torch.isfinite(got[reached]).any()

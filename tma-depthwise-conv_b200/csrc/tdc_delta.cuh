@@ -20,6 +20,8 @@
 // above 1 into infinities.
 #pragma once
 
+#include <cfloat>
+
 #include "tdc_dwconv.h"
 #include "tdc_seq_common.cuh"
 #include "tdc_tc.cuh"
@@ -29,6 +31,7 @@ namespace tdc {
 constexpr int kChunk = 64;
 constexpr int kLdT = kChunk + 8;     // row of a [64][64] tile in shared memory
 constexpr int kSq = kChunk * kChunk;  // elements of such a tile in the workspace
+constexpr int kCoef = 3 * kChunk + 4;  // a slot's coefficients
 
 // The gradients' workspace: for kTile value channels of a slot, transposed, what
 // the gradients of a chunk need of them, in the order of a stage in shared memory
@@ -82,7 +85,7 @@ struct DeltaParams {
   // workspace of all chunks, [chunk][HV] each
   // (tiles in the order of WalkTiles; 8 x 8 blocks, see tdc_tc.cuh)
   __nv_bfloat16* tp;      // T in its three parts, then P: [6][64 x 64]
-  float* coef;            // [3][64]: gam, w, beta
+  float* coef;            // kCoef: gam, w, beta [64] each, and whether a key or a gate is not finite
   unsigned char* kq;      // [chunk][H]: [parts][K / 8][Q's 64 rows, K's 64 rows][8]
   uint64_t timeout_ns;    // of the bounded waits
   int64_t withhold;       // first chunk of a sequence whose copies never come (-1: none)
@@ -250,8 +253,10 @@ __device__ __forceinline__ void chunk_decay(const float2& g, Far* G, int lane) {
     const double o = __shfl_up_sync(0xffffffffu, sum, d);
     if (lane >= d) sum += o;
   }
+  double before = __shfl_up_sync(0xffffffffu, sum, 1);
+  if (lane == 0) before = 0.0;
   G[2 * lane + 1] = to_far(sum);
-  G[2 * lane] = to_far(sum - double(g.y));
+  G[2 * lane] = to_far(before + double(g.x));  // (not sum - g.y: a NaN reaches no token before it)
 }
 
 // ---- T and P of every chunk -------------------------------------------------------
@@ -429,6 +434,12 @@ __global__ void __launch_bounds__(128, 4) delta_prepare_kernel(const DeltaParams
     store_keys<E, DK>(kq, raw + (tid < kChunk ? Sm::q : Sm::k) + 2 * (tid & 63) * ld, tid);
   }
   const int g = lane >> 2, t2 = (lane & 3) * 2;
+  bool odd_key = false;  // a key of this thread's that is not finite: k.k is not
+#pragma unroll
+  for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (8 * nt + t2 + (e & 1) == 16 * warp + g + 8 * (e >> 1)) odd_key |= !(fabsf(kk[nt][e]) <= FLT_MAX);
   for (int gi = 0; gi < p.group; ++gi) {
     const int hv = h * p.group + gi;
     const int64_t slot = chunk * p.HV + hv;
@@ -438,8 +449,10 @@ __global__ void __launch_bounds__(128, 4) delta_prepare_kernel(const DeltaParams
     if (tid >= 64) sB[tid - 64] = beta;
     if (gi + 1 < p.group) fetch_gates(hv + 1);
     __syncthreads();
+    float* coef = p.coef + slot * kCoef;
+    bool odd = odd_key;
     if (tid < kChunk) {
-      float* coef = p.coef + slot * 3 * kChunk;
+      odd |= !(fabsf(sB[tid]) <= FLT_MAX) || !(fabsf(G[tid].hi) <= FLT_MAX);
       coef[tid] = expf(G[tid].hi + G[tid].lo);
       coef[kChunk + tid] = expf(minus(G[kChunk - 1], G[tid]));
       coef[2 * kChunk + tid] = sB[tid];
@@ -460,7 +473,11 @@ __global__ void __launch_bounds__(128, 4) delta_prepare_kernel(const DeltaParams
         for (int u = 0; u < 2; ++u) {
           const float gam = __expf(minus(Gi[half], Gj[u]));
           pv[u] = i >= j + u ? p.scale * gam * qk[nt][2 * half + u] : 0.f;
-          av[u] = i > j + u ? kk[nt][2 * half + u] * gam * (u ? be.y : be.x) : 0.f;
+          // A row of T multiplies with the zeros behind its diagonal: what a NaN or infinite
+          // key or decay leaves here would reach the rows before it.  Its own and later
+          // rows get their NaN from X (delta_walk_kernel).
+          const float l = kk[nt][2 * half + u] * gam;
+          av[u] = i > j + u ? (fabsf(l) <= FLT_MAX ? l : 0.f) * (u ? be.y : be.x) : 0.f;
         }
         if (nt >= 2 * warp)
           *reinterpret_cast<float2*>(raw + Sm::t + diag_offset(warp, g + 8 * half) +
@@ -495,7 +512,8 @@ __global__ void __launch_bounds__(128, 4) delta_prepare_kernel(const DeltaParams
         }
       }
     }
-    __syncthreads();
+    odd = __syncthreads_or(odd);
+    if (tid == 127) coef[3 * kChunk] = odd ? 1.f : 0.f;
     if (warp < 2) join_inverse<16>(sb + Sm::a, sb + Sm::t, 32 * warp, 0, lane);
     __syncthreads();
     if (warp < 2) join_inverse<32>(sb + Sm::a, sb + Sm::t, 0, 16 * warp, lane);

@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_grad_kernel(const Delta
           const int hv = item.head * p.group + gi;
           const float2 g = load_decay(p, item.at, hv, lane);
           const float2* src =
-              reinterpret_cast<const float2*>(p.coef + (item.chunk * p.HV + hv) * 3 * kChunk);
+              reinterpret_cast<const float2*>(p.coef + (item.chunk * p.HV + hv) * kCoef);
           const float2 c[3] = {src[lane], src[32 + lane], src[64 + lane]};
           if (heads > 0) ok = warp_wait(wait, sy->next, heads - 1);
           chunk_decay(g, sy->G, lane);

@@ -43,7 +43,7 @@ struct WalkTiles {
   static constexpr int t = KP * keys;
   static constexpr int p = t + 3 * kSq * 2;
   static constexpr int coef = p + 3 * kSq * 2;
-  static constexpr int stage = coef + 3 * kChunk * 4;
+  static constexpr int stage = coef + kCoef * 4;
 };
 
 // Shared memory behind the two stages.
@@ -54,6 +54,8 @@ struct WalkSync {
   uint64_t drain;
   uint32_t tmem;
   int abort;
+  int bad[128];                // last chunk in which a channel's first 32 tokens spoil those behind
+  unsigned char odd[2][128];   // whether a half of a channel's tokens ever did, or its state may
 };
 static_assert(2 * WalkTiles<F16, 128>::stage + sizeof(WalkSync) <= 232448, "a block's shared memory");
 
@@ -185,6 +187,10 @@ __device__ __forceinline__ void walk_setup(WalkSync* sy, int tid, int warp) {
     sy->abort = 0;
     fence_mbar_init();
   }
+  if (tid < 256) {
+    sy->bad[tid & 127] = -1;
+    sy->odd[tid >> 7][tid & 127] = 0;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -205,10 +211,10 @@ __device__ __forceinline__ void walk_fetch(const DeltaParams& p, unsigned char* 
     const unsigned char* keys = p.kq + (chunk * p.H + h) * (W::KP * W::keys);
     constexpr uint32_t kbytes = W::KP * W::keys;
     constexpr uint32_t tbytes = T_ONLY ? 3 * kSq * 2 : 6 * kSq * 2;
-    mbar_arrive_expect_tx(bar, kbytes + tbytes + 3 * kChunk * 4);
+    mbar_arrive_expect_tx(bar, kbytes + tbytes + kCoef * 4);
     bulk_load(dst + W::q, keys, kbytes, bar);
     bulk_load(dst + W::t, p.tp + slot * (6 * kSq), tbytes, bar);
-    bulk_load(dst + W::coef, p.coef + slot * 3 * kChunk, 3 * kChunk * 4, bar);
+    bulk_load(dst + W::coef, p.coef + slot * kCoef, kCoef * 4, bar);
     issued = c + 1;
   }
   // No copy is in flight when the block ends.
@@ -268,6 +274,41 @@ __device__ __forceinline__ void walk_put(void* dst, uint32_t stride, const float
       *reinterpret_cast<uint16_t*>(at + uint64_t(uint32_t(i)) * stride) = uint16_t(pack2_rn<E>(v, 0.f));
     }
   }
+}
+
+// T's and P's rows multiply with the zeros behind their diagonals, so a NaN or an infinity
+// in a row of X or V' would reach the tokens before its own.  It becomes 0 as an operand,
+// and the results from its token on become NaN, as they are in the recurrence.  It comes
+// from a value, from the chunk's keys and gates (delta_prepare looks at them) or from a
+// state, so X and V' need a look only where one of these is odd.
+template <int N, class At>
+__device__ __forceinline__ bool all_finite(At at) {
+  float s[4] = {};
+#pragma unroll
+  for (int i = 0; i < N; ++i) s[i & 3] = fmaf(at(i), 0.f, s[i & 3]);  // 0 or NaN
+  return (s[0] + s[1]) + (s[2] + s[3]) == 0.f;
+}
+// The first place of a thread's 32 that is not finite, 32 if none is; zeros in such places.
+__device__ __forceinline__ int first_bad(float (&x)[32]) {
+  int first = 32;
+#pragma unroll
+  for (int i = 31; i >= 0; --i) {
+    if (fabsf(x[i]) <= FLT_MAX) continue;
+    first = i;
+    x[i] = 0.f;
+  }
+  return first;
+}
+// NaN from place `first` on.
+template <class T>
+__device__ __forceinline__ void spoil(T (&r)[32], int first) {
+  if (__all_sync(0xffffffffu, first >= 32)) return;
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (i >= first) {
+      if constexpr (std::is_same_v<T, float>) r[i] = __int_as_float(0x7fc00000);
+      else r[i] = 0x7fc00000u;
+    }
 }
 
 template <class E>
@@ -509,9 +550,18 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
     walk_column(vr, v + t0 * p.v_st, vstep, rows_of(0), live && real);
     float qs[32];     // scale gam S^T Q^T of the chunk
     float last = 1.f; // gam_63 of the chunk before
+    const int own = 32 * (warp & 3) + lane;
+    int bad = 32, bad_out = 32;  // first of this thread's tokens that are spoiled, and outputs
+    bool odd = !all_finite<DK / 2>([&](int i) { return S[i]; });
+    if (odd) sy->odd[half][own] = 1;
     bool ok = true;
     // Output of a chunk: qs plus P's product.
     auto put_out = [&](int c) {
+      if (half) {  // (the other half's tokens come first)
+        ok = warp_wait(wait, sy->qr, c);
+        if (!ok) return;
+        if (sy->bad[own] == c) bad_out = 0;
+      }
       ok = warp_wait(wait, sy->o, c);
       if (!ok) return;
       tc_fence_after();
@@ -519,6 +569,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
       tmem_ld(lanes + cO + t0, r);
 #pragma unroll
       for (int i = 0; i < 32; ++i) qs[i] += __uint_as_float(r[i]);
+      spoil(qs, bad_out);
       walk_put<E>(o + (int64_t(c) * kChunk + t0) * p.HV * p.V, ostep, qs, rows_of(c), live && out);
     };
     // The state after the chunk before: gam_63 S + its update.
@@ -557,8 +608,13 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         if (!ok) break;
       }
       // X = V - gam Y
-      ok = warp_wait(wait, sy->full[c & 1], c >> 1);  // (the coefficients)
+      ok = warp_wait(wait, sy->full[c & 1], c >> 1) &&  // (the coefficients)
+           warp_wait(wait, sy->sr, c);                  // (the other half's word on the state)
       if (!ok) break;
+      if (coef[3 * kChunk] != 0.f && !odd) odd = true, sy->odd[half][own] = 1;
+      const bool look = __any_sync(0xffffffffu, odd || sy->odd[half ^ 1][own] ||
+                                                    !all_finite<32>([&](int i) { return widen<E>(vr[i]); }));
+      bad = 32;
       ok = warp_wait(wait, sy->y, c);
       if (!ok) break;
       tc_fence_after();
@@ -574,6 +630,14 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
           x[i + 2] = widen<E>(vr[i + 2]) - gam.z * __uint_as_float(r[i + 2]);
           x[i + 3] = widen<E>(vr[i + 3]) - gam.w * __uint_as_float(r[i + 3]);
         }
+        if (look) {
+          bad = first_bad(x);
+          if (bad < 32) {
+            odd = true;
+            sy->odd[half][own] = 1;
+            if (!half) sy->bad[own] = c;
+          }
+        }
         split_to_tmem(x, lanes + cX + t0 / 2, xStep);
       }
       operand_ready(sy->xr, lane);
@@ -581,6 +645,11 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         walk_column(vr, v + (int64_t(c + 1) * kChunk + t0) * p.v_st, vstep, rows_of(c + 1),
                     live && real);
       // V' = beta U and w V'
+      if (half) {
+        ok = warp_wait(wait, sy->xr, c);
+        if (!ok) break;
+        if (sy->bad[own] == c) bad = 0;
+      }
       ok = warp_wait(wait, sy->u, c);
       if (!ok) break;
       tc_fence_after();
@@ -588,6 +657,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
       {
         uint32_t r[32];
         tmem_ld(lanes + cY + t0, r);
+        spoil(r, bad);
         float u[32], x[32];
         if constexpr (MODE == 1) {
 #pragma unroll
@@ -613,6 +683,11 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         operand_ready(sy->vr, lane);
         if constexpr (MODE == 0) {
           // beside the chain: V' for the output, and Q's product
+          bad_out = 32;
+          if (__any_sync(0xffffffffu, look || bad < 32)) {
+            bad_out = first_bad(u);  // (U's NaN among them)
+            if (!half && bad_out < 32) sy->bad[own] = c;
+          }
           split_to_tmem(u, lanes + cV + t0 / 2, xStep);
           ok = warp_wait(wait, sy->q, c);
           if (!ok) break;

@@ -353,7 +353,7 @@ int64_t delta_layout(const tdc_delta_args* a, bool grads, unsigned char* base, t
   unsigned char* tp = take(slots * 6 * tdc::kSq * 2);
   const int64_t parts = a->dtype == TDC_BF16 ? 1 : 2;
   unsigned char* kq = take(delta_chunks(a) * a->H * 2 * parts * tdc::kChunk * a->K * 2);
-  unsigned char* coef = take(slots * 3 * tdc::kChunk * 4);
+  unsigned char* coef = take(slots * tdc::kCoef * 4);
   unsigned char* tiles = nullptr;
   unsigned char *seg_s = nullptr, *seg_m = nullptr;
   const int segments = grads ? 1 : delta_segments(a);
