@@ -38,3 +38,26 @@ def test_what_is_not_finite_reaches_no_token_before_it(name, bad, T, t, K, V, dt
     reached[0, slice(t, t + 1 if name == "q" else None), heads, 7 if name == "v" else channels] = True
     assert torch.equal(got[~reached], want[~reached])
     assert not torch.isfinite(got[reached]).any()
+
+
+@pytest.mark.gpu
+def test_states_saved_for_a_backward_pass_and_stepped_since():
+    # as after any in-place operation: the backward pass refuses instead of using the new state
+    x = torch.randn(2, 5, 64, device="cuda").half()
+    w = torch.randn(4, 64, device="cuda").half().requires_grad_()
+    pool = torch.randn(2, 3, 64, device="cuda").half()
+    y = S.causal_conv1d(x, w, initial_state=pool)
+    with torch.no_grad():
+        S.causal_conv1d_step(x[:, :1], w, None, pool)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        y.sum().backward()
+    c = D._case(2, 5, 1, 1, 64, 64)
+    a = [c[n].cuda() for n in ("q", "k", "v", "g", "beta")]
+    pool = torch.randn(2, 1, 64, 64, device="cuda")
+    o = S.gated_delta_rule(*(t.clone().requires_grad_() for t in a), initial_state=pool)
+    S.gated_delta_step(*(t[:, :1] for t in a), pool)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        o.sum().backward()
+    with torch.inference_mode():
+        pool = torch.randn(2, 1, 64, 64, device="cuda")
+    S.gated_delta_step(*(t[:, :1] for t in a), pool)          # (has no version)

@@ -72,6 +72,12 @@ torch::Tensor bytes_on(const torch::Tensor& x, int64_t n) {
   return torch::empty({n}, torch::TensorOptions().dtype(torch::kByte).device(x.device()));
 }
 
+// `t` was written in place: a tensor that a backward pass saved before raises there, as
+// after any in-place operation of torch (inference tensors have no versions).
+void written(const torch::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void check_cu(const OptTensor& cu, const torch::Tensor& x) {
   if (!cu) return;
   is_index64(*cu, x, "cu_seqlens");
@@ -209,6 +215,7 @@ torch::Tensor causal_conv1d_step(torch::Tensor x, torch::Tensor w, OptTensor bia
   s.indices_are_64 = idx && idx->scalar_type() == torch::kLong;
   s.dtype = c.a.dtype, s.act = act;
   check_status(tdc_conv1d_step(&s, stream_of(x)), "causal_conv1d_step");
+  written(state);
   return y;
 }
 
@@ -467,6 +474,7 @@ torch::Tensor gated_delta_step(torch::Tensor q, torch::Tensor k, torch::Tensor v
   check_status(tdc_delta_step(&c.a, state.data_ptr<float>(), state.size(0), ptr(idx),
                               idx && idx->scalar_type() == torch::kLong, stream_of(q)),
                "gated_delta_step");
+  written(state);
   return o;
 }
 
