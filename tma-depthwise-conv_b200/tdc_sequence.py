@@ -22,10 +22,11 @@ Inputs are fp16 or bf16 CUDA tensors; states and decays are fp32, and every sum
 is.  Wrong arguments raise ``ValueError`` or ``RuntimeError`` before anything
 runs.  The functions run on torch's current stream of their tensors' device,
 take their workspaces from torch's allocator (so they can be captured into CUDA
-graphs) and give the same bits every run.  Under ``torch.compile`` they are the
-custom ops ``torch.ops.tdc.causal_conv1d``, ``tdc.qk_norm_rope`` and
-``tdc.gated_delta_rule``; in eager mode lighter autograd Functions call the
-same kernels.
+graphs) and give the same bits every run.  They have first derivatives in
+reverse mode; second and forward-mode ones raise ``RuntimeError``.  Under
+``torch.compile`` they are the custom ops ``torch.ops.tdc.causal_conv1d``,
+``tdc.qk_norm_rope`` and ``tdc.gated_delta_rule``; in eager mode lighter
+autograd Functions call the same kernels.
 """
 from __future__ import annotations
 
@@ -35,6 +36,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor, nn
+from torch.autograd import forward_ad as fwAD
 from torch.autograd.function import once_differentiable
 
 import _tma_dwconv_C as _C  # type: ignore
@@ -50,6 +52,9 @@ NORMS = {"none": 0, "rms": 1, "l2": 2}
 
 
 def _needs_grad(*tensors: Optional[Tensor]) -> bool:
+    if fwAD._current_level >= 0 and any(t is not None and fwAD.unpack_dual(t).tangent is not None
+                                        for t in tensors):
+        raise RuntimeError("the sequence operators have no forward-mode derivatives")
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
