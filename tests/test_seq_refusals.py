@@ -27,3 +27,23 @@ def test_forward_mode_derivatives():
                 call()
         with pytest.raises(RuntimeError, match="CUDA"):       # others go on to their checks
             S.causal_conv1d(x, w)
+
+
+def test_rotated_layer_without_positions():
+    # its states hold keys turned by their positions: 0 .. T-1 cannot be right for more tokens
+    m = S.GatedDeltaMixer(64, 1, key_dim=64, value_dim=64, rotary_dim=32, max_positions=100)
+    x, state = torch.randn(2, 3, 64).bfloat16(), m.new_state(2)
+    with pytest.raises(ValueError, match="positions"):
+        m.step(x, state)
+    with pytest.raises(ValueError, match="positions"):
+        m(x, state)
+    with pytest.raises(ValueError, match="positions"):
+        m(x[:1], cu_seqlens=torch.tensor([0, 1, 3]), output_state=True)
+    for call in (lambda: m.step(x, state, positions=torch.arange(3)),
+                 lambda: m(x, output_state=True),
+                 lambda: m(x[:1], cu_seqlens=torch.tensor([0, 1, 3]))):
+        with pytest.raises(RuntimeError, match="CUDA"):       # go on to the operators
+            call()
+    plain = S.GatedDeltaMixer(64, 1, key_dim=64, value_dim=64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        plain.step(x, plain.new_state(2))

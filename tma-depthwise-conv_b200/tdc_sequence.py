@@ -578,7 +578,13 @@ class GatedDeltaMixer(nn.Module):
                 output_state: bool = False):
         """y [B, T, hidden]; with ``output_state`` also the ``MixerState`` behind
         the last tokens, one slot a sequence.  ``state`` continues earlier tokens.
-        ``positions`` ([T] or [B, T], for the rotation) default to 0 .. T-1."""
+        ``positions`` ([T] or [B, T], for the rotation) default to 0 .. T-1, the row
+        of a packed batch too; with ``rotary_dim`` they have to be given where that
+        cannot be right: with a ``state``, and for the states of a packed batch."""
+        if self.rotary_dim and positions is None and (
+                state is not None or (output_state and cu_seqlens is not None)):
+            raise ValueError("a rotated layer needs positions with a state, and for the states of "
+                             "a packed batch")
         mixed, gate, g, beta = self._project(x)
         conv_state, delta_state = (None, None) if state is None else (state.conv, state.delta)
         out = causal_conv1d(mixed, self.conv_weight, activation="silu", initial_state=conv_state,
@@ -596,7 +602,10 @@ class GatedDeltaMixer(nn.Module):
              positions: Optional[Tensor] = None) -> Tensor:
         """The next tokens x [B, T, hidden] (T usually 1) of B running sequences,
         whose slots are updated in place (``causal_conv1d_step`` says how slots
-        are picked)."""
+        are picked).  With ``rotary_dim`` the tokens' ``positions`` ([B, T], or [T]
+        for all alike) have to be given."""
+        if self.rotary_dim and positions is None:
+            raise ValueError("a rotated layer needs the tokens' positions")
         mixed, gate, g, beta = self._project(x)
         mixed = causal_conv1d_step(mixed, self.conv_weight, None, state.conv, activation="silu",
                                    state_indices=state_indices)
