@@ -15,7 +15,6 @@ def test_blend_of_kept_and_divided_frequencies(dim, base, length, factor):
     half, size = dim // 2, 0.1 * math.log(factor) + 1
     at = lambda turns: half * math.log(length / (2 * math.pi * turns)) / math.log(base)  # noqa: E731
     low, high = max(math.floor(at(32.0)), 0), math.ceil(at(1.0))
-    assert high <= dim - 1
     for i in range(half):
         freq = base ** (-i / half)
         share = min(max((i - low) / max(high - low, 1e-3), 0.0), 1.0)   # of the divided one

@@ -238,9 +238,8 @@ def rotary_table(rotary_dim: int, length: int, base: float = 10000.0, scaling: s
         # index of the frequency as a real number at which `beta` turns happen
         at = [half * math.log(original_length / (b * 2 * math.pi)) / math.log(base)
               for b in (beta_fast, beta_slow)]
-        # (the blend may end behind the last pair, where that one still turns beta_slow times
-        # or more; the published method's bound is rotary_dim - 1)
-        low, high = max(math.floor(at[0]), 0), min(math.ceil(at[1]), rotary_dim - 1)
+        # (the blend may end behind the last pair, where that one still turns beta_slow times)
+        low, high = max(math.floor(at[0]), 0), math.ceil(at[1])
         ramp = ((i - low) / max(high - low, 1e-3)).clamp(0, 1)
         freq = freq * (1 - ramp) + freq / factor * ramp
         size = 0.1 * math.log(factor) + 1.0
