@@ -61,3 +61,22 @@ def test_states_saved_for_a_backward_pass_and_stepped_since():
     with torch.inference_mode():
         pool = torch.randn(2, 1, 64, 64, device="cuda")
     S.gated_delta_step(*(t[:, :1] for t in a), pool)          # (has no version)
+
+
+@pytest.mark.gpu
+def test_views_without_rows():
+    # strides of a view that has no element are no reason to refuse it
+    odd = lambda *s: torch.randn(*s, 68, device="cuda").half()[..., :64]  # noqa: E731
+    w, state = torch.randn(4, 64, device="cuda").half(), torch.randn(2, 3, 64, device="cuda").half()
+    y, last = S.causal_conv1d(odd(2, 5)[:, :0], w, initial_state=state, output_final_state=True)
+    assert y.shape == (2, 0, 64) and torch.equal(last, state)
+    assert S.causal_conv1d_step(odd(2, 5)[:, :0], w, None, state).shape == (2, 0, 64)
+    q, k = S.qk_norm_rope(odd(2, 5, 3)[:, :0], odd(2, 5, 1)[:, :0])
+    assert q.shape == (2, 0, 3, 64) and k.shape == (2, 0, 1, 64)
+    q, k = S.qk_norm_rope(torch.randn(2, 5, 1, 64, device="cuda").half(), odd(2, 5, 3)[:, :, :0])
+    assert k.shape == (2, 5, 0, 64)
+    q, g = odd(2, 5, 2)[:, :0], torch.rand(2, 5, 2, device="cuda")[:, :0]
+    pool = torch.randn(2, 2, 64, 64, device="cuda")
+    o, last = S.gated_delta_rule(q, q, q, g, g, initial_state=pool, output_final_state=True)
+    assert o.shape == q.shape and torch.equal(last, pool)
+    assert S.gated_delta_step(q, q, q, g, g, pool).shape == q.shape

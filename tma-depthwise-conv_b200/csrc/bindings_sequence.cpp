@@ -64,7 +64,10 @@ torch::Tensor aligned(const torch::Tensor& t) {
                                                              : c.clone(at::MemoryFormat::Contiguous);
 }
 
-int64_t stride_of(const torch::Tensor& t, int64_t dim) { return t.size(dim) <= 1 ? 0 : t.stride(dim); }
+// (strides without an element do not matter either)
+int64_t stride_of(const torch::Tensor& t, int64_t dim) {
+  return t.size(dim) <= 1 || t.numel() == 0 ? 0 : t.stride(dim);
+}
 
 const void* ptr(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }
 
