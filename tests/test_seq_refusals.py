@@ -1,4 +1,6 @@
 """Calls that the sequence operators refuse, without a GPU: nothing runs before the refusal."""
+import os
+
 import pytest
 import torch
 from torch.autograd import forward_ad as fwAD
@@ -47,3 +49,26 @@ def test_rotated_layer_without_positions():
     plain = S.GatedDeltaMixer(64, 1, key_dim=64, value_dim=64)
     with pytest.raises(RuntimeError, match="CUDA"):
         plain.step(x, plain.new_state(2))
+
+
+def test_sizes_whose_workspace_has_no_number():
+    # products of sizes that pass 64 bits: refused, not a small or negative size
+    import test_seq_host as H
+    import ctypes as C
+    lib = C.CDLL(os.path.join(H.REPO, "tma-depthwise-conv_b200", "libtdc_sm100.so"))
+    sizes = ("tdc_conv1d_bwd_workspace", "tdc_delta_fwd_workspace", "tdc_delta_bwd_workspace")
+    for f in sizes:
+        getattr(lib, f).restype = C.c_int64
+    large, p = H.CODES["TDC_ERR_TOO_LARGE"], C.c_void_p(H.P)
+    big = 1 << 40
+    for over in (dict(B=big, T=big), dict(B=1 << 20, T=1 << 20, C=1 << 20),
+                 dict(B=1, cu_seqlens=H.P, num_seqs=1 << 62)):
+        a = H._conv(**over)
+        assert lib.tdc_conv1d_bwd_workspace(C.byref(a)) == large
+        assert lib.tdc_conv1d_fwd(C.byref(a), None) == large
+    for over in (dict(B=1 << 24, T=1 << 36, HV=65534, V=256, K=128, v_sb=0, v_st=0),
+                 dict(B=1 << 24, T=1, HV=65534, V=256), dict(B=1 << 20, T=1 << 30)):
+        a = H._delta(**over)
+        for f in sizes[1:]:
+            assert getattr(lib, f)(C.byref(a)) == large
+        assert lib.tdc_delta_fwd(C.byref(a), p, C.c_int64(1 << 40), None) == large

@@ -20,6 +20,10 @@ using tdc::host::prepare_device;
 
 constexpr int64_t kMaxDim = int64_t(1) << 40;
 constexpr int64_t kMaxRow = int64_t(1) << 31;  // elements of 2 bytes
+constexpr int64_t kMaxSize = int64_t(1) << 46;  // elements of a tensor, channels of all chunks
+
+// a * b > limit, without the product (all at least 0)
+bool exceeds(int64_t a, int64_t b, int64_t limit) { return b > 0 && a > limit / b; }
 
 bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
 bool bad_stride(int64_t s) { return s % 8 != 0; }
@@ -48,6 +52,8 @@ int check_conv(int64_t B, int64_t T, int64_t C, int64_t K, int64_t dtype, int64_
   if (K < 2 || K > 8) return TDC_ERR_FILTER_SHAPE;
   if (C % 8 != 0) return TDC_ERR_CHANNELS;
   if (B > kMaxDim || T > kMaxDim || C > kMaxDim) return TDC_ERR_TOO_LARGE;
+  if (exceeds(B, T, kMaxDim) || exceeds(B, C, kMaxSize) || exceeds(B * T, C, kMaxSize))
+    return TDC_ERR_TOO_LARGE;
   if (bad_stride(x_sb) || bad_stride(x_st)) return TDC_ERR_ALIGNMENT;
   return TDC_OK;
 }
@@ -57,6 +63,8 @@ int check_conv_args(const tdc_conv1d_args* a) {
   const int rc = check_conv(a->B, a->T, a->C, a->K, a->dtype, a->act, a->x_sb, a->x_st);
   if (rc != TDC_OK) return rc;
   if (a->cu_seqlens != nullptr && (a->B != 1 || a->num_seqs < 1)) return TDC_ERR_BAD_SHAPE;
+  if (a->cu_seqlens != nullptr && exceeds(a->num_seqs, std::max<int64_t>(1, a->C), kMaxSize))
+    return TDC_ERR_TOO_LARGE;
   return TDC_OK;
 }
 
@@ -287,6 +295,12 @@ int qk_bwd_e(const tdc::QkParams& p, int threads, int64_t blocks, void* dqw, voi
 }
 
 // ---- gated delta rule -------------------------------------------------------------
+int64_t delta_seqs(const tdc_delta_args* a) { return a->cu_seqlens != nullptr ? a->num_seqs : a->B; }
+int64_t delta_chunks(const tdc_delta_args* a) {
+  return a->cu_seqlens != nullptr ? a->T / tdc::kChunk + a->num_seqs
+                                  : a->B * ceil_div(a->T, tdc::kChunk);
+}
+
 int check_delta(const tdc_delta_args* a) {
   if (a == nullptr) return TDC_ERR_NULL_POINTER;
   if (a->dtype != TDC_F16 && a->dtype != TDC_BF16) return TDC_ERR_UNSUPPORTED;
@@ -297,6 +311,8 @@ int check_delta(const tdc_delta_args* a) {
     return TDC_ERR_TOO_LARGE;
   if (a->cu_seqlens != nullptr && (a->B != 1 || a->num_seqs < 1)) return TDC_ERR_BAD_SHAPE;
   if (a->num_seqs > (int64_t(1) << 24)) return TDC_ERR_TOO_LARGE;
+  // The workspace's size, at most 2.6 KB a value channel of a chunk, fits 64 bits.
+  if (exceeds(delta_chunks(a), a->HV * a->V, kMaxSize)) return TDC_ERR_TOO_LARGE;
   for (int64_t s : {a->q_sb, a->q_st, a->q_sh, a->k_sb, a->k_st, a->k_sh, a->v_sb, a->v_st, a->v_sh})
     if (bad_stride(s)) return TDC_ERR_ALIGNMENT;
   // rows of v and o are addressed by 32-bit byte strides in a chunk
@@ -313,12 +329,6 @@ int delta_wait_record(tdc::DeltaParams* p) {
   p->status_words = r.words;
   p->status_host = r.host;
   return TDC_OK;
-}
-
-int64_t delta_seqs(const tdc_delta_args* a) { return a->cu_seqlens != nullptr ? a->num_seqs : a->B; }
-int64_t delta_chunks(const tdc_delta_args* a) {
-  return a->cu_seqlens != nullptr ? a->T / tdc::kChunk + a->num_seqs
-                                  : a->B * ceil_div(a->T, tdc::kChunk);
 }
 
 // Segments that the forward walks side by side (1: none): as many as give every
