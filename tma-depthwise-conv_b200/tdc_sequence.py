@@ -534,7 +534,8 @@ class GatedDeltaMixer(nn.Module):
         self.out_proj = nn.Linear(inner, hidden, bias=False, **make)
         self.rotary_dim = rotary_dim
         if rotary_dim:
-            cos, sin = rotary_table(rotary_dim, max_positions, rotary_base, device=device)
+            self.table_args = (rotary_dim, max_positions, rotary_base)
+            cos, sin = rotary_table(*self.table_args, device=device)
             self.register_buffer("cos", cos, persistent=False)
             self.register_buffer("sin", sin, persistent=False)
 
@@ -543,7 +544,10 @@ class GatedDeltaMixer(nn.Module):
         tables = {n: getattr(self, n) for n in ("cos", "sin") if self.rotary_dim}
         super()._apply(fn, *args, **kwargs)
         for n, t in tables.items():
-            setattr(self, n, t.to(getattr(self, n).device))
+            device = getattr(self, n).device
+            if t.is_meta and device.type != "meta":   # (to_empty: they are in no state dict)
+                t = rotary_table(*self.table_args, device=device)[n == "sin"]
+            setattr(self, n, t.to(device))
         return self
 
     def new_state(self, slots: int) -> MixerState:
