@@ -59,7 +59,7 @@ extern "C" {
 #define TDC_ERR_DEVICE_TIMEOUT  -11  /* an earlier launch gave up waiting on its pipeline  */
 #define TDC_ERR_NO_DEVICE       -12  /* no usable sm_100 device is current                   */
 #define TDC_ERR_ACT             -13  /* unknown activation code (tdc_dwconv3x3_fwd)          */
-#define TDC_ERR_WORKSPACE       -14  /* workspace too small (tdc_dwconv3x3_bwd_weight)       */
+#define TDC_ERR_WORKSPACE       -14  /* workspace smaller than the operation's query says    */
 #define TDC_ERR_SCRATCH_LIMIT   -15  /* C beyond the static scratch (..._bwd_weight_noalloc) */
 #define TDC_ERR_STRIDE          -16  /* stride not 1 or 2 (tdc_dwconv_fwd)                  */
 #define TDC_ERR_UNSUPPORTED     -17  /* no kernel for this request (e.g. an unknown plan kind) */

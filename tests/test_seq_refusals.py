@@ -72,3 +72,12 @@ def test_sizes_whose_workspace_has_no_number():
         for f in sizes[1:]:
             assert getattr(lib, f)(C.byref(a)) == large
         assert lib.tdc_delta_fwd(C.byref(a), p, C.c_int64(1 << 40), None) == large
+
+
+def test_workspace_error_names_no_other_operation():
+    import test_seq_host as H
+    import ctypes as C
+    lib = C.CDLL(os.path.join(H.REPO, "tma-depthwise-conv_b200", "libtdc_sm100.so"))
+    lib.tdc_strerror.restype = C.c_char_p
+    text = lib.tdc_strerror(H.CODES["TDC_ERR_WORKSPACE"]).decode()
+    assert "workspace" in text and "dwconv3x3" not in text

@@ -1737,7 +1737,7 @@ TDC_API const char* tdc_strerror(int code) {
     case TDC_ERR_TMA_ENCODE: return "cuTensorMapEncodeTiled failed";
     case TDC_ERR_DEVICE_TIMEOUT: return "an earlier launch on this device gave up waiting on a pipeline barrier and left its output incomplete; tdc_device_status(1, info) (tma_dwconv.device_status) reports and clears the record";
     case TDC_ERR_NO_DEVICE: return "no sm_100 CUDA device is current";
-    case TDC_ERR_WORKSPACE: return "workspace smaller than tdc_dwconv3x3_bwd_weight_workspace reports";
+    case TDC_ERR_WORKSPACE: return "workspace smaller than the operation's workspace query reports";
     case TDC_ERR_SCRATCH_LIMIT: return "C too large for the 16 MiB static scratch of tdc_dwconv3x3_bwd_weight_noalloc (C <= 116508)";
     case TDC_ERR_STRIDE: return "stride must be 1 or 2";
     case TDC_ERR_UNSUPPORTED: return "not implemented for this geometry";
