@@ -242,60 +242,12 @@ __device__ __forceinline__ void mma_split(float c[4], const uint32_t a[3][4], co
     for (int i = 0; i <= sum; ++i) mma_bf16(c, a[i], b[sum - i][at], b[sum - i][at + 1]);
 }
 
-// The same for N accumulators side by side, product by product rather than
-// accumulator by accumulator: neighbouring instructions are independent (one
-// that waits for the one before it takes 20 cycles instead of 8).
-template <int N>
-__device__ __forceinline__ void mma_split_n(float (*c)[4], const uint32_t ah[4], const uint32_t al[4],
-                                            const uint32_t* bh, const uint32_t* bl) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) mma_bf16(c[i], ah, bh[2 * i], bh[2 * i + 1]);
-#pragma unroll
-  for (int i = 0; i < N; ++i) mma_bf16(c[i], al, bh[2 * i], bh[2 * i + 1]);
-#pragma unroll
-  for (int i = 0; i < N; ++i) mma_bf16(c[i], ah, bl[2 * i], bl[2 * i + 1]);
-}
-// A exact in the element type (ah, and al for fp16), B split.
-template <class E, int N>
-__device__ __forceinline__ void mma_elem_split_n(float (*c)[4], const uint32_t ah[4],
-                                                 const uint32_t al[4], const uint32_t* bh,
-                                                 const uint32_t* bl) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) mma_bf16(c[i], ah, bh[2 * i], bh[2 * i + 1]);
-#pragma unroll
-  for (int i = 0; i < N; ++i) mma_bf16(c[i], ah, bl[2 * i], bl[2 * i + 1]);
-  if constexpr (!std::is_same_v<E, BF16>) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) mma_bf16(c[i], al, bh[2 * i], bh[2 * i + 1]);
-  }
-}
-// A split, B exact in the element type.
-template <class E, int N>
-__device__ __forceinline__ void mma_split_elem_n(float (*c)[4], const uint32_t ah[4],
-                                                 const uint32_t al[4], const uint32_t* b) {
-  uint32_t bh[2 * N], bl[2 * N];
-#pragma unroll
-  for (int i = 0; i < 2 * N; ++i) split_elem<E>(b[i], bh[i], bl[i]);
-#pragma unroll
-  for (int i = 0; i < N; ++i) mma_bf16(c[i], ah, bh[2 * i], bh[2 * i + 1]);
-#pragma unroll
-  for (int i = 0; i < N; ++i) mma_bf16(c[i], al, bh[2 * i], bh[2 * i + 1]);
-  if constexpr (!std::is_same_v<E, BF16>) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) mma_bf16(c[i], ah, bl[2 * i], bl[2 * i + 1]);
-  }
-}
-
 // Addresses for ldmatrix.x4 over a row-major 16-bit tile with `ld` elements a
 // row (ld * 2 bytes an odd multiple of 16, so that 8 rows hit all banks).
 // B fragments of two 8-column tiles from a tile stored [n][k]:
 //   r0,r1 = b0,b1 of columns n0..n0+7, r2,r3 of n0+8..n0+15.
 __device__ __forceinline__ uint32_t addr_b(uint32_t base, int ld, int n0, int k0, int lane) {
   return base + 2 * ((n0 + (lane & 7) + ((lane >> 4) << 3)) * ld + k0 + ((lane >> 3) & 1) * 8);
-}
-// The same from a tile stored [k][n] (with .trans).
-__device__ __forceinline__ uint32_t addr_bt(uint32_t base, int ld, int n0, int k0, int lane) {
-  return base + 2 * ((k0 + (lane & 7) + ((lane >> 3) & 1) * 8) * ld + n0 + ((lane >> 4) << 3));
 }
 // An A fragment from a tile stored [m][k].
 __device__ __forceinline__ uint32_t addr_a(uint32_t base, int ld, int m0, int k0, int lane) {
