@@ -80,3 +80,16 @@ def test_views_without_rows():
     o, last = S.gated_delta_rule(q, q, q, g, g, initial_state=pool, output_final_state=True)
     assert o.shape == q.shape and torch.equal(last, pool)
     assert S.gated_delta_step(q, q, q, g, g, pool).shape == q.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("B,T,H,HV,K,V", [(4, 1, 2, 4, 128, 128), (2, 3, 1, 2, 64, 256)])
+def test_steps_with_fp32_betas(B, T, H, HV, K, V, dtype):
+    c = D._case(B, T, H, HV, K, V, dtype, state=True, beta_f32=True, seed=T)
+    pool = c["state"].clone().cuda()
+    names = ("q", "k", "v", "g", "beta")
+    o = S.gated_delta_step(*(c[n].cuda() for n in names), pool)
+    want, final = R.delta(*(c[n].double() for n in names), K ** -0.5, c["state"].double(), None)
+    R.close(o, want, D.STEP * want.abs().max().item(), "o")
+    R.close(pool, final, D.STEP * final.abs().max().item(), "state")
