@@ -82,8 +82,9 @@ struct Waiter {
   }
 };
 
-// v as three bf16 parts (split3), 16 packed columns each: keep(part, columns) gets them
-// one after another.  v is used up.
+// v as three bf16 parts, 16 packed columns each: keep(part, columns) gets them one after
+// another.  v is used up.  A part is the upper half of a value, cut and not rounded: 3 x 8
+// bits hold it exactly all the same, and it takes one instruction instead of two slots.
 template <class Keep>
 __device__ __forceinline__ void split_parts(float (&v)[32], Keep keep) {
 #pragma unroll
@@ -91,7 +92,7 @@ __device__ __forceinline__ void split_parts(float (&v)[32], Keep keep) {
     uint32_t r[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      r[i] = pack2_rn<BF16>(v[2 * i], v[2 * i + 1]);
+      r[i] = __byte_perm(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]), 0x7632);
       if (part < 2) fma2<BF16>(r[i], 0xBF80BF80u, v[2 * i], v[2 * i + 1]);
     }
     keep(part, r);
@@ -582,7 +583,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
 #pragma unroll
       for (int i = 0; i < DK / 2; ++i) S[i] = fmaf(last, S[i], __uint_as_float(r[i]));
     };
-    for (int c = 0; c < chunks; ++c) {
+    for (int c = 0; chunks > 0; ++c) {  // (behind the last chunk: its state and output)
       const float* coef =
           reinterpret_cast<const float*>(raw + (c & 1) * W::stage + W::coef);
       const int64_t slot = (s.chunk0 + c) * p.HV + hv;
@@ -590,6 +591,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         advance(c - 1);
         if (!ok) break;
       }
+      if (MODE == 1 && c == chunks) break;
 #pragma unroll
       for (int x = 0; x < DK / 64; ++x) {
         float w[32];
@@ -607,6 +609,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         put_out(c - 1);
         if (!ok) break;
       }
+      if (c == chunks) break;
       // X = V - gam Y
       ok = warp_wait(wait, sy->full[c & 1], c >> 1) &&  // (the coefficients)
            warp_wait(wait, sy->sr, c);                  // (the other half's word on the state)
@@ -659,13 +662,6 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         tmem_ld(lanes + cY + t0, r);
         spoil(r, bad);
         float u[32], x[32];
-        if constexpr (MODE == 1) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
-          split_parts(x, [&](int part, const uint32_t (&b)[16]) {
-            store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::u + part * GT::upart, t0), b, live);
-          });
-        }
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
           const float4 w = *reinterpret_cast<const float4*>(coef + kChunk + t0 + i);
@@ -681,6 +677,13 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         }
         split_to_tmem(x, lanes + cX + t0 / 2, xStep);
         operand_ready(sy->vr, lane);
+        if constexpr (MODE == 1) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
+          split_parts(x, [&](int part, const uint32_t (&b)[16]) {
+            store_pairs(channel_at<KP, DK>(p.tiles, slot * p.V + ch, GT::u + part * GT::upart, t0), b, live);
+          });
+        }
         if constexpr (MODE == 0) {
           // beside the chain: V' for the output, and Q's product
           bad_out = 32;
@@ -704,10 +707,6 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
           operand_ready(sy->qr, lane);
         }
       }
-    }
-    if (ok && chunks > 0) {
-      advance(chunks - 1);
-      if (MODE == 0 && ok) put_out(chunks - 1);
     }
     if (MODE == 0 && ok) {
       float* to = nullptr;
