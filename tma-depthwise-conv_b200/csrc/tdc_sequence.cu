@@ -332,19 +332,24 @@ int delta_wait_record(tdc::DeltaParams* p) {
 }
 
 // Segments that the forward walks side by side (1: none): as many as give every
-// block of both passes an SM of its own, if two passes over a segment (and about
-// 6 chunks' time for the second launch and the join) are shorter than one over
-// the whole.  Packed batches' lengths are not known here: they are walked whole.
-// One sequence of 8192 tokens with 32 heads: 344 us in 3 segments, 500 whole.
+// block of both passes an SM of its own, if two passes over a segment and what joins
+// them are shorter than one over the whole.  In chunks' times the second launch and
+// the join's start are 3, and each product of the join 5/3 with K = 128, 1/2 with K = 64.
+// Packed batches' lengths are not known here: they are walked whole.
+// Whole and split calls, us (bf16, K = V = 128, one sequence): 4 heads, 13 chunks whole 67,
+// 10 segments 104; 16 chunks 79 and 68; 40 chunks 177 and 104 (13 segments 129).
+// 32 heads, 16 chunks 86; 20 chunks 115 and 107; 40 chunks 212 and 181.  Two sequences of
+// 4 heads of 64 (fp16), 10 chunks 47 and 38; 40 chunks 153 and 68.
 int delta_segments(const tdc_delta_args* a) {
   if (a->cu_seqlens != nullptr) return 1;
   const int64_t chunks = ceil_div(a->T, tdc::kChunk), heads = a->B * a->HV;
   const int64_t walks = heads * ceil_div(a->V, 128);
+  const int64_t product = a->K == 128 ? 10 : 3;
   int best = 1;
-  int64_t cost = chunks;
+  int64_t cost = 6 * chunks;
   for (int p = 3; p <= 16; ++p) {
     if (walks + (p - 2) * (walks + heads) > kSms || walks * (p - 1) > kSms) break;
-    const int64_t c = 2 * ceil_div(chunks, p) + 6;
+    const int64_t c = 6 * (2 * ceil_div(chunks, p) + 3) + (p - 2) * product;
     if (c < cost) best = p, cost = c;
   }
   return best;
