@@ -17,11 +17,12 @@ def segments():
         return lib.tdc_delta_fwd_workspace(C.byref(H._delta(T=64 * chunks, dtype=H.CODES["TDC_BF16"], **o)))
 
     def count(chunks, B, HV, K, V):
-        o = dict(B=B, H=HV, HV=HV, K=K, V=V)
-        step = size(3, **o) - size(2, **o)
+        o, unit = dict(B=B, H=HV, HV=HV, K=K, V=V), B * HV * (K * V + K * K) * 4
+        # (every part is a multiple of 256 bytes: the step of four chunks from sizes never split)
+        step = (size(6, **o) - size(2, **o)) / 4
         extra = size(chunks, **o) - size(2, **o) - (chunks - 2) * step
-        assert extra % (B * HV * (K * V + K * K) * 4) == 0
-        return max(1, extra // (B * HV * (K * V + K * K) * 4))
+        assert abs(extra - round(extra / unit) * unit) < unit / 8
+        return max(1, round(extra / unit))
 
     return count
 
