@@ -191,7 +191,6 @@ __device__ __forceinline__ void grad_issue(const DeltaParams& p, uint32_t sb, Gr
   using Sm = GradSmem<E, DK>;
   constexpr int KP = Sm::KP, NS = Sm::count;
   constexpr uint32_t kGradDM = kGradOX + DK;
-  const uint32_t q = sb + Sm::qk, k = q + 1024, dn = sb + Sm::dn;
   constexpr uint32_t khigh = block_desc_high(kKeyBlock), rhigh = block_desc_high(kRowBlock);
   const int per_head = p.V / kTile;
   int x = 0, phase = 0, heads = 0, done = 0;
@@ -233,6 +232,9 @@ __device__ __forceinline__ void grad_issue(const DeltaParams& p, uint32_t sb, Gr
         if (!warp_wait(wait, sy->keys, done)) return;
         tc_fence_after();
         if (elect_one()) {  // the rows of Q and K by those of K
+          uint32_t q = sb + Sm::qk;
+          asm volatile("" : "+r"(q));
+          const uint32_t k = q + 1024;
 #pragma unroll
           for (int y = KP - 1; y >= 0; --y)
 #pragma unroll
@@ -249,6 +251,11 @@ __device__ __forceinline__ void grad_issue(const DeltaParams& p, uint32_t sb, Gr
       if (!warp_wait(wait, sy->dn, heads)) return;
       tc_fence_after();
       if (elect_one()) {
+        // (descriptors from an address of this turn: those of all products, kept over the
+        // turns, did not fit the warp's registers)
+        uint32_t q = sb + Sm::qk;
+        asm volatile("" : "+r"(q));
+        const uint32_t k = q + 1024, dn = q + (Sm::dn - Sm::qk);
         // [Dt; N] K onto the first (half of the second part twice), then two parts at a
         // time, the last two and the first two, [Dt; Dt]^T Q + [N; N]^T K onto the last
 #pragma unroll
@@ -414,14 +421,15 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_grad_kernel(const Delta
             for (int j = 0; j < 32; ++j) own = fmaf(f[j], __uint_as_float(r[j]), own);
             put_scaled(lanes + kGradOX + kc0 + 32 * y, r, by);
             tmem_ld(lanes + kGradUS + kc0 + 32 * y, r);
-            {  // and the small products' sum
-              uint32_t r2[32];
-              tmem_ld(lanes + kGradUS2 + kc0 + 32 * y, r2);
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(r2[j]));
+            for (int x = 0; x < 2; ++x) {  // and the small products' sum
+              uint32_t r2[16];
+              tmem_ld(lanes + kGradUS2 + kc0 + 32 * y + 16 * x, r2);
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                r[16 * x + j] = __float_as_uint(__uint_as_float(r[16 * x + j]) + __uint_as_float(r2[j]));
             }
-            if (!upper) load_key_row<E, DK>(f, raw + Sm::qk, 64 + l, kc0 + 32 * y);
+            load_key_row<E, DK>(f, raw + Sm::qk, 64 + i, kc0 + 32 * y);
 #pragma unroll
             for (int j = 0; j < 32; ++j) key = fmaf(f[j], __uint_as_float(r[j]), key);
             put_scaled(lanes + kGradUS + kc0 + 32 * y, r, wb);
