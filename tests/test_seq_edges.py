@@ -93,3 +93,21 @@ def test_steps_with_fp32_betas(B, T, H, HV, K, V, dtype):
     want, final = R.delta(*(c[n].double() for n in names), K ** -0.5, c["state"].double(), None)
     R.close(o, want, D.STEP * want.abs().max().item(), "o")
     R.close(pool, final, D.STEP * final.abs().max().item(), "state")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,t", [(100, 37), (200, 70), (200, 128)])
+@pytest.mark.parametrize("K,V,dtype", [(64, 64, "bf16"), (128, 256, "fp16")])
+def test_gradients_before_a_value_that_is_not_finite(T, t, K, V, dtype):
+    # a loss that takes nothing from token t on: what stands there does not reach the
+    # gradients before it (values enter no gradient of the state)
+    c = D._case(2, T, 1, 2, K, V, dtype, state=True, beta_f32=True)
+    c["do"][:, t:] = 0
+    want = D._run(c, final=False)
+    c["v"] = c["v"].detach().clone()
+    c["v"][0, t:, 1, 7] = float("nan")
+    c["v"][1, t:] = float("inf")
+    got = D._run(c, final=False)
+    for n in ("dq", "dk", "dv", "dg", "dbeta"):
+        assert torch.equal(got[n][:, :t], want[n][:, :t]), n
+    assert torch.equal(got["dstate"], want["dstate"])

@@ -54,8 +54,8 @@ struct WalkSync {
   uint64_t drain;
   uint32_t tmem;
   int abort;
-  int bad[128];                // last chunk in which a channel's first 32 tokens spoil those behind
-  unsigned char odd[2][128];   // whether a half of a channel's tokens ever did, or its state may
+  int bad[128];  // last chunk in which a channel's first 32 tokens spoil those behind
+  int odd;       // whether anything so far was not finite (set before a chunk's sr)
 };
 static_assert(2 * WalkTiles<F16, 128>::stage + sizeof(WalkSync) <= 232448, "a block's shared memory");
 
@@ -188,10 +188,8 @@ __device__ __forceinline__ void walk_setup(WalkSync* sy, int tid, int warp) {
     sy->abort = 0;
     fence_mbar_init();
   }
-  if (tid < 256) {
-    sy->bad[tid & 127] = -1;
-    sy->odd[tid >> 7][tid & 127] = 0;
-  }
+  if (tid < 128) sy->bad[tid] = -1;
+  if (tid == 0) sy->odd = 0;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -281,7 +279,8 @@ __device__ __forceinline__ void walk_put(void* dst, uint32_t stride, const float
 // in a row of X or V' would reach the tokens before its own.  It becomes 0 as an operand,
 // and the results from its token on become NaN, as they are in the recurrence.  It comes
 // from a value, from the chunk's keys and gates (delta_prepare looks at them) or from a
-// state, so X and V' need a look only where one of these is odd.
+// state, so X and V' are looked at only from a block's first chunk with one of these on;
+// values are while a thread waits for the state.
 template <int N, class At>
 __device__ __forceinline__ bool all_finite(At at) {
   float s[4] = {};
@@ -553,12 +552,13 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
     float last = 1.f; // gam_63 of the chunk before
     const int own = 32 * (warp & 3) + lane;
     int bad = 32, bad_out = 32;  // first of this thread's tokens that are spoiled, and outputs
-    bool odd = !all_finite<DK / 2>([&](int i) { return S[i]; });
-    if (odd) sy->odd[half][own] = 1;
+    bool look = false;
+    auto odd_values = [&] { return !all_finite<32>([&](int i) { return widen<E>(vr[i]); }); };
+    if (odd_values() || !all_finite<DK / 2>([&](int i) { return S[i]; })) sy->odd = 1;
     bool ok = true;
     // Output of a chunk: qs plus P's product.
     auto put_out = [&](int c) {
-      if (half) {  // (the other half's tokens come first)
+      if (look && half) {  // (the other half's tokens come first)
         ok = warp_wait(wait, sy->qr, c);
         if (!ok) return;
         if (sy->bad[own] == c) bad_out = 0;
@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
       tmem_ld(lanes + cO + t0, r);
 #pragma unroll
       for (int i = 0; i < 32; ++i) qs[i] += __uint_as_float(r[i]);
-      spoil(qs, bad_out);
+      if (look) spoil(qs, bad_out);
       walk_put<E>(o + (int64_t(c) * kChunk + t0) * p.HV * p.V, ostep, qs, rows_of(c), live && out);
     };
     // The state after the chunk before: gam_63 S + its update.
@@ -588,6 +588,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
           reinterpret_cast<const float*>(raw + (c & 1) * W::stage + W::coef);
       const int64_t slot = (s.chunk0 + c) * p.HV + hv;
       if (c > 0) {
+        if (c < chunks && odd_values()) sy->odd = 1;
         advance(c - 1);
         if (!ok) break;
       }
@@ -614,9 +615,8 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
       ok = warp_wait(wait, sy->full[c & 1], c >> 1) &&  // (the coefficients)
            warp_wait(wait, sy->sr, c);                  // (the other half's word on the state)
       if (!ok) break;
-      if (coef[3 * kChunk] != 0.f && !odd) odd = true, sy->odd[half][own] = 1;
-      const bool look = __any_sync(0xffffffffu, odd || sy->odd[half ^ 1][own] ||
-                                                    !all_finite<32>([&](int i) { return widen<E>(vr[i]); }));
+      look = *const_cast<volatile int*>(&sy->odd) != 0 || coef[3 * kChunk] != 0.f;  // (all threads)
+      if (look) sy->odd = 1;
       bad = 32;
       ok = warp_wait(wait, sy->y, c);
       if (!ok) break;
@@ -635,11 +635,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         }
         if (look) {
           bad = first_bad(x);
-          if (bad < 32) {
-            odd = true;
-            sy->odd[half][own] = 1;
-            if (!half) sy->bad[own] = c;
-          }
+          if (!half && bad < 32) sy->bad[own] = c;
         }
         split_to_tmem(x, lanes + cX + t0 / 2, xStep);
       }
@@ -648,7 +644,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         walk_column(vr, v + (int64_t(c + 1) * kChunk + t0) * p.v_st, vstep, rows_of(c + 1),
                     live && real);
       // V' = beta U and w V'
-      if (half) {
+      if (look && half) {
         ok = warp_wait(wait, sy->xr, c);
         if (!ok) break;
         if (sy->bad[own] == c) bad = 0;
@@ -660,7 +656,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
       {
         uint32_t r[32];
         tmem_ld(lanes + cY + t0, r);
-        spoil(r, bad);
+        if (look) spoil(r, bad);
         float u[32], x[32];
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
@@ -687,7 +683,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
         if constexpr (MODE == 0) {
           // beside the chain: V' for the output, and Q's product
           bad_out = 32;
-          if (__any_sync(0xffffffffu, look || bad < 32)) {
+          if (look) {
             bad_out = first_bad(u);  // (U's NaN among them)
             if (!half && bad_out < 32) sy->bad[own] = c;
           }
