@@ -153,7 +153,8 @@ TDC_API int tdc_qk_norm_rope_bwd(const tdc_qk_args* a, const tdc_qk_grad_args* g
  * K is 64 or 128, V is 64, 128 or 256, HV a multiple of H.  Keys are expected
  * to have a norm of about 1 and beta to lie in [0, 2): then the chunked form's
  * triangular systems are well conditioned, as the recurrence itself is.
- * g below -200 acts as -200 (a decay of 0 in fp32). */
+ * g below -200 acts as -200 (a decay of 0 in fp32).  A value that is not finite
+ * reaches no token before its own, in the chunked form as in the recurrence. */
 typedef struct tdc_delta_args {
   const void* q;
   const void* k;

@@ -1,5 +1,5 @@
-// tdc_delta.cuh — the gated delta rule: chunked forward and gradients with
-// warp matrix instructions, and the recurrence for running sequences.
+// tdc_delta.cuh — the gated delta rule: what a chunk needs that depends on no state (with
+// warp matrix instructions), and the recurrence for running sequences.
 //
 // Chunks of C = 64 tokens.  With G the running sum of g in the chunk (fp64),
 // gam = e^G, Gam_ij = e^(G_i - G_j) and w_i = e^(G_63 - G_i):
@@ -266,7 +266,7 @@ __device__ __forceinline__ void chunk_decay(const float2& g, Far* G, int lane) {
 // inv([[P, 0], [B, R]]) = [[P', 0], [-R' B P', R']].  Only the 16 x 16 blocks
 // on and below the diagonal of T and P are written, and none above is read.
 // Bound by the latency of the substitution and the two joins with 4 blocks an SM;
-// 8192 tokens of 16 key and 32 value heads (268 MB) take 70 us, 3.8 TB/s.
+// 8192 tokens of 16 key and 32 value heads (263 MB) take 78 us, 3.4 TB/s.
 //
 // The fp32 rows (16 floats) of the diagonal blocks of A lie in the unused
 // blocks above T's diagonal: row i of block w in row i or 16 + i of one part.

@@ -13,12 +13,15 @@
 // A thread owns one channel and half of the columns, so scaling, splitting and
 // the running state are thread-local; what a chunk costs is the chain of three
 // dependent products (the walk is bound by its latency, with few sequences and
-// heads, and by nothing else before the number of blocks passes the SMs).  Q's
-// and P's products and the output run beside the chain.  8192 tokens of 32 heads of
-// 128 x 128, as 4 sequences (128 blocks, 32 chunks each): 109 us forward, 137 when
-// it also stores U and S, 154 back, that is 3.4, 4.3 and 4.8 us a chunk.  Two
-// threads a channel measured best: with four (768 threads) one sequence of 8192
-// tokens took 504 us instead of 420, since every exchange then waits for more warps.
+// heads, and by nothing else before the number of blocks passes the SMs).  Q's and
+// P's products and the output run beside the chain.  8192 tokens of 32 heads of
+// 128 x 128, as 4 sequences (128 blocks, 32 chunks each): 168 us forward, 168 when
+// it stores U and S instead of making the output, 211 back, that is 5.2, 5.2 and 6.6 us
+// a chunk (32 blocks alone: 4.0 forward).  With operands in two parts instead of
+// three it took 109, 137 and 154, and was off by 4e-6 (see "Precision" in
+// tdc_delta.cuh).  Two threads a channel measured best: with four (768 threads) one
+// sequence of 8192 tokens took a fifth longer, since every exchange then waits for
+// more warps.
 //
 // Warps 0-7 compute (warp % 4 picks the lanes, warp / 4 the half of the
 // columns), warp 8 issues the products, warp 9 the bulk copies of the next
@@ -436,8 +439,8 @@ __global__ void __launch_bounds__(256) delta_join_kernel(const DeltaParams p) {
 // (its end is N) and with V = 0 from the identity (its end is M, whose K columns
 // stand in the channels' place); delta_join_kernel makes the states between the
 // segments; pass 2 walks all but the first from them.  Two passes of a
-// segment's length replace one of the whole: one sequence of 8192 tokens with 32
-// heads takes 138 + 11 + 140 us instead of 420.
+// segment's length replace one of the whole: a call for one sequence of 8192 tokens with
+// 32 heads takes 438 us (194 + 11 + 199 in these three launches) instead of 590.
 template <class E, int DK, int MODE>
 __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const DeltaParams p) {
   extern __shared__ __align__(1024) unsigned char raw[];
@@ -725,7 +728,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
 //   dV' = P^T dO + w (K dS)        dX = T^T (beta dV')  (= dV)
 //   dS <- gam_63 dS + scale Q^T (gam dO) - K^T (gam dX)
 // with dS^T in the lanes.  dS behind each chunk, dX and dO^T go to the workspace
-// (460 MB at 8192 tokens of 32 heads of 128 x 128: 3 TB/s beside the chain).
+// (671 MB at 8192 tokens of 32 heads of 128 x 128: 3.2 TB/s beside the chain).
 template <class E, int DK>
 __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const DeltaParams p) {
   extern __shared__ __align__(1024) unsigned char raw[];

@@ -1,6 +1,6 @@
 // tdc_seq_common.cuh — what the sequence kernels share: packed-batch lookups,
 // slot indices, 16-byte vectors of 16-bit elements, warp matrix instructions
-// and the split of an fp32 operand into two bf16 ones.
+// and the split of an fp32 operand into three bf16 ones.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -539,7 +539,8 @@ TDC_API int tdc_conv1d_fwd(const tdc_conv1d_args* a, void* stream) {
   // Runs that fill the SMs with one wave of blocks (2 of 256 threads on each), or
   // with several equal ones if they were longer than 128 rows.  Against the shortest
   // runs that give each SM 1024 threads (at most 32 rows), K = 4: 1500 rows of 2560
-  // channels 14.1 -> 11.4 us, 5003 rows 20.5 -> 16.4, 9000 rows of 8192 61.4 -> 57.8.
+  // channels 14.1 -> 11.4 us a call, 5003 rows 20.5 -> 16.4 (then 15 with loads before the
+  // sequences are looked up), 9000 rows of 8192 61.4 -> 57.8.
   const int64_t wave = 2 * kSms * 256, work = a->B * a->T * vecs;
   const int64_t waves = std::max<int64_t>(1, ceil_div(work, wave * 128));
   p.runs_per_b = ceil_div(a->T, std::max<int64_t>(1, ceil_div(work, wave * waves)));
