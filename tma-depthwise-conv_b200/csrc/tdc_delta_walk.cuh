@@ -496,7 +496,8 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_kernel(const Delta
           }
         }
         __syncwarp();
-        if (!warp_wait(wait, sy->vr, c)) break;
+        // (the update takes the place of the state's parts: Q's product is done with them)
+        if (!warp_wait(wait, sy->vr, c) || (MODE == 0 && !warp_wait(wait, sy->q, c))) break;
         tc_fence_after();
         if (elect_one()) {
           issue_product<TokenParts, kChunk, DK, true, KP>(tm + cS, tm + cX, st + W::k, W::keys, false);
@@ -758,7 +759,10 @@ __global__ void __launch_bounds__(kWalkThreads, 1) delta_walk_back_kernel(const 
     if (warp == 8) {
       for (int c = 0; c < chunks; ++c) {
         const uint32_t st = smem_addr(raw) + (c & 1) * W::stage;
-        if (!warp_wait(wait, sy->full[c & 1], c >> 1) || !warp_wait(wait, sy->gr, c)) break;
+        // (P^T dO takes the place of gam dO: the last chunk's products are done with it)
+        if (!warp_wait(wait, sy->full[c & 1], c >> 1) || !warp_wait(wait, sy->gr, c) ||
+            (c > 0 && !warp_wait(wait, sy->s, c - 1)))
+          break;
         tc_fence_after();
         if (elect_one()) issue_lower<true, KP>(tm + cP, tm + cO, st + W::p);
         __syncwarp();
